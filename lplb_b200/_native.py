@@ -52,6 +52,10 @@ SOURCES = [
     "count_noalloc.cu",
     "moe_binding.cpp",
     "moe_launch.cu",
+    "ops_binding.cpp",
+    "ops_status.cu",
+    "norm_fp8.cu",
+    "matmul_fp8.cu",
 ]
 
 NVCC_FLAGS = [

@@ -617,6 +617,7 @@ torch::Tensor debug_reciprocals(const torch::Tensor& x) {
 }  // namespace
 
 void bind_moe(py::module_& m);  // moe_binding.cpp
+void bind_ops(py::module_& m);  // ops_binding.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "lplb_b200 native runtime (sm_100a)";
@@ -661,6 +662,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("max_fused_ctas", &PlannerEngine::max_fused_ctas);
   m.def("debug_reciprocals", &debug_reciprocals);
   bind_moe(m);
+  bind_ops(m);
   m.attr("MAX_GROUP_SIZE") = lplb::kMaxGroupSize;
   m.attr("MAX_DUP") = lplb::kMaxDup;
   m.attr("MAX_LOGICAL_EXPERTS") = lplb::kMaxLogicalExperts;

@@ -1,0 +1,113 @@
+// Launcher of the block-scaled matrix product.
+#include "ops_api.h"
+
+#include <atomic>
+
+#include "matmul_fp8.cuh"
+#include "tensor_map.h"
+
+namespace lplb {
+namespace ops {
+
+namespace {
+
+constexpr uint32_t kRingBytes = 192 * 1024;
+constexpr int kFewSmem = 204 * 1024;  // ring, scales, barriers and the way to a 1024-byte boundary
+
+cudaError_t rows_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld};
+  const cuuint32_t box[2] = {(cuuint32_t)kKBytes, box_rows};
+  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 2, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename Kernel>
+cudaLaunchConfig_t cluster_config(cudaLaunchAttribute (&attrs)[2], int ctas, int split, uint32_t smem, cudaStream_t stream, Kernel) {
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = split;
+  attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(kFewThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attrs;
+  config.numAttrs = 2;
+  return config;
+}
+
+// Clusters of `split` CTAs that the device holds at once, one CTA per SM (GPCs of odd sizes leave SMs over).
+template <typename Kernel>
+cudaError_t resident_clusters(int device, int split, Kernel kernel, int* clusters) {
+  static std::atomic<int> known[kMaxDevices][kMaxSplit + 1];
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  *clusters = known[device][split].load(std::memory_order_relaxed);
+  if (*clusters > 0) return cudaSuccess;
+  cudaLaunchAttribute attrs[2]{};
+  cudaLaunchConfig_t config = cluster_config(attrs, split, split, kFewSmem, nullptr, kernel);
+  config.numAttrs = 1;
+  const cudaError_t err = cudaOccupancyMaxActiveClusters(clusters, kernel, &config);
+  if (err == cudaSuccess) known[device][split].store(*clusters, std::memory_order_relaxed);
+  return err;
+}
+
+template <typename Out>
+cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
+  auto kernel = few_rows_kernel<Out>;
+  static std::atomic<bool> prepared[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  cudaError_t err = cudaSuccess;
+  if (!prepared[device].load(std::memory_order_relaxed)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    if (err != cudaSuccess) return err;
+    prepared[device].store(true, std::memory_order_relaxed);
+  }
+  FewArgs a{};
+  if ((err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
+  a.a_scale = p.a_scale;
+  a.b_scale = p.b_scale;
+  a.out = p.out;
+  a.a_scale_ld = p.a_scale_ld;
+  a.out_ld = p.out_ld;
+  a.m = (int)p.m;
+  a.n = (int)p.n;
+  a.k_blocks = (int)((p.k + kKBytes - 1) / kKBytes);
+  a.cols = (a.m + 15) / 16 * 16;
+  a.scale_words = a.k_blocks % 4 == 0 && a.a_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.a_scale) & 3) == 0 &&
+                  (reinterpret_cast<uintptr_t>(a.b_scale) & 3) == 0;
+  const int tiles = (a.n + kTileRows - 1) / kTileRows;
+  // How many CTAs share a tile: the fewest rounds of k blocks over the SMs.
+  int split = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= kMaxSplit && s <= a.k_blocks; ++s) {
+    int fit = 0;
+    if ((err = resident_clusters(device, s, kernel, &fit)) != cudaSuccess) return err;
+    if (fit < 1) continue;
+    const int64_t rounds = (tiles + fit - 1) / fit, blocks = (a.k_blocks + s - 1) / s;
+    const int64_t cost = rounds * (blocks + 6) + (s > 1 ? 4 + a.cols / 32 : 0);
+    if (cost < least) least = cost, split = s;
+  }
+  const uint32_t stage = kWeightStage + a.cols * kKBytes;
+  a.stages = (int)(kRingBytes / stage);
+  if (a.stages > kMaxRingStages) a.stages = kMaxRingStages;
+  const int most = (a.k_blocks + split - 1) / split;
+  if (a.stages > most) a.stages = most;
+  CUtensorMap map_b, map_a;
+  if ((err = rows_map(&map_b, p.b, p.n, p.k, p.b_ld, kTileRows)) != cudaSuccess) return err;
+  if ((err = rows_map(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
+  cudaLaunchAttribute attrs[2]{};
+  const cudaLaunchConfig_t config = cluster_config(attrs, tiles * split, split, FewLayout(a.cols, a.stages).total + 1024, stream, kernel);
+  return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
+}
+
+}  // namespace
+
+cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream) {
+  if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.m > kFewMaxRows) return cudaErrorInvalidValue;
+  if (p.m == 0) return cudaSuccess;
+  return p.out_f32 ? launch_few<float>(p, device, stream) : launch_few<__nv_bfloat16>(p, device, stream);
+}
+
+}  // namespace ops
+}  // namespace lplb

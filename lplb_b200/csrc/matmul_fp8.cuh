@@ -1,0 +1,231 @@
+// C[m, n] = sum over blocks of 128 along k of sa[m, kb] * sb[n / 128, kb] * sum_k A[m, k] * B[n, k]
+// for few rows m: e4m3 operands, power-of-two scales that the tensor cores multiply in by themselves.
+//
+// Bound by reading B once.  A CTA computes 128 rows of B against all rows of A: the weights on the tensor core's M side, so that
+// few rows cost few cycles, and the k blocks of a tile are dealt out to the CTAs of a cluster, so
+// that a matrix with few tiles still occupies every SM.  The partial sums meet in distributed shared
+// memory, in rank order: no workspace, nothing to clear, the same bits every time.
+//
+// Roles (256 threads): warp 0 TMA producer, warp 1 matrix instructions, warp 2 scales, warps 4-7
+// epilogue; all of them add up the partial sums.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace lplb {
+namespace ops {
+
+enum OpsErr : int { kOpsTimeout = 21 };
+constexpr unsigned long long kWaitBudgetNs = 2000000000ull;
+
+constexpr int kTileRows = 128;                  // weight rows per CTA
+constexpr int kKBytes = 128;                    // bytes of a row per k block
+constexpr uint32_t kWeightStage = kTileRows * kKBytes;
+constexpr int kMaxRingStages = 12;
+constexpr int kScaleSlots = 4;
+constexpr uint32_t kScaleAtom = 512;            // 128 rows x 4 blocks
+constexpr int kFewThreads = 256;
+constexpr int kFewMaxRows = 256;
+constexpr int kMaxSplit = 8;                    // portable cluster size
+
+struct FewArgs {
+  const uint8_t* a_scale;  // [m, a_scale_ld]
+  const uint8_t* b_scale;  // [ceil(n / 128), k_blocks]
+  void* out;               // [m, out_ld]
+  int* error;              // the device's error word
+  int64_t a_scale_ld, out_ld;
+  int m, n, k_blocks;
+  int cols;                // m rounded up to 16
+  int stages;
+  int scale_words;         // scale rows start on 4-byte boundaries
+};
+
+struct FewLayout {  // shared memory from a 1024-byte boundary on
+  uint32_t stage, ring, scales, bars, total;
+  __host__ __device__ FewLayout(int cols, int stages) {
+    stage = kWeightStage + cols * kKBytes;
+    ring = 0;
+    scales = stage * stages;
+    const uint32_t partial = (uint32_t)cols * kTileRows * 4;  // over the ring, once it has been read
+    if (scales < partial) scales = partial;
+    bars = scales + kScaleSlots * 3 * kScaleAtom;
+    total = bars + (2 * kMaxRingStages + 2 * kScaleSlots + 1) * 8;
+  }
+};
+
+// Four scale bytes of blocks 4 * group ... of a row, 1 beyond the last block.
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int group, int k_blocks, bool words) {
+  if (words) return __ldcg(reinterpret_cast<const uint32_t*>(row) + group);
+  uint32_t w = 0x7F7F7F7Fu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (4 * group + i < k_blocks) w = (w & ~(0xFFu << (8 * i))) | ((uint32_t)__ldcg(row + 4 * group + i) << (8 * i));
+  return w;
+}
+
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename Out>
+__global__ void __launch_bounds__(kFewThreads, 1)
+few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, const FewArgs a) {
+  using namespace sm100;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const FewLayout at(a.cols, a.stages);
+  const uint32_t base = smem_u32(smem), bars = base + at.bars;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * kMaxRingStages;
+  const uint32_t bar_sfull = bars + 16 * kMaxRingStages, bar_sempty = bar_sfull + 8 * kScaleSlots;
+  const uint32_t bar_done = bar_sempty + 8 * kScaleSlots;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_cta_rank(), split = (int)(cluster_size());
+  const int tile = (int)blockIdx.x / split;
+  const int kb0 = (int)((int64_t)a.k_blocks * rank / split), kb1 = (int)((int64_t)a.k_blocks * (rank + 1) / split);
+  const uint32_t scale_cols = (uint32_t)(a.cols + 31) / 32 * 32;  // first column of the scales
+  const uint32_t tmem_cols = scale_cols + 16 <= 32 ? 32 : scale_cols + 16 <= 64 ? 64 : scale_cols + 16 <= 128 ? 128 : scale_cols + 16 <= 256 ? 256 : 512;
+  allow_successor();
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kMaxRingStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(bar_sfull + 8 * s, 1);
+      mbar_init(bar_sempty + 8 * s, 1);
+    }
+    mbar_init(bar_done, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&map_a);
+    tma_prefetch_desc(&map_b);
+  }
+  if (warp == 1) tmem_alloc_single(smem_u32(&tmem_slot), tmem_cols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abort = &abort_flag;
+  wait_predecessors();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t s = 0, ph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, kWaitBudgetNs)) break;
+        const uint32_t dst = base + s * at.stage;
+        mbar_expect_tx(bar_full + 8 * s, at.stage);
+        tma_load_2d(dst, &map_b, bar_full + 8 * s, kb * kKBytes, tile * kTileRows);
+        tma_load_2d(dst + kWeightStage, &map_a, bar_full + 8 * s, kb * kKBytes, 0);
+        if (++s == (uint32_t)a.stages) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = umma_idesc_mxf8(kTileRows, a.cols);
+      const uint32_t tmem_sa = tmem + scale_cols, tmem_sb = tmem_sa + 4;
+      uint32_t s = 0, ph = 0, ss = 0, sph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (kb == kb0 || (kb & 3) == 0) {
+          if (!mbar_wait(bar_sfull + 8 * ss, sph, abort, kWaitBudgetNs)) break;
+          tc_fence_after_sync();
+          const uint32_t src = base + at.scales + ss * 3 * kScaleAtom;
+          tmem_cp_scales(tmem_sa, src);
+          for (int i = 0; i * 128 < a.cols; ++i) tmem_cp_scales(tmem_sb + 4 * i, src + (1 + i) * kScaleAtom);
+          umma_commit(bar_sempty + 8 * ss);
+          if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+        }
+        if (!mbar_wait(bar_full + 8 * s, ph, abort, kWaitBudgetNs)) break;
+        tc_fence_after_sync();
+        const uint32_t src = base + s * at.stage;
+        const uint64_t dw = umma_desc_sw128(src), dt = umma_desc_sw128(src + kWeightStage);
+        const uint32_t id = umma_idesc_scale_byte(idesc, kb & 3);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 32 values = 32 bytes along k inside the swizzled row
+          umma_mxf8(tmem, dw + 2 * k, dt + 2 * k, id, tmem_sa, tmem_sb, kb != kb0 || k != 0);
+        umma_commit(bar_empty + 8 * s);
+        if (++s == (uint32_t)a.stages) s = 0, ph ^= 1;
+      }
+      umma_commit(bar_done);
+    }
+  } else if (warp == 2) {
+    const uint8_t* b_row = a.b_scale + (int64_t)tile * a.k_blocks;
+    uint32_t ss = 0, sph = 0;
+    for (int g = kb0 / 4; 4 * g < kb1; ++g) {
+      uint32_t t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = lane + 32 * j;
+        t[j] = r < a.m ? scale_word(a.a_scale + (int64_t)r * a.a_scale_ld, g, a.k_blocks, a.scale_words) : 0x7F7F7F7Fu;
+      }
+      const uint32_t w = scale_word(b_row, g, a.k_blocks, a.scale_words);
+      if (!mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs)) break;
+      uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
+      *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(t[0], t[1], t[2], t[3]);
+      *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(t[4], t[5], t[6], t[7]);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);
+      if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+    }
+  } else if (warp >= 4) {
+    const bool done = mbar_wait(bar_done, 0, abort, kWaitBudgetNs);
+    __syncwarp();
+    if (__all_sync(0xffffffffu, done)) {
+      tc_fence_after_sync();
+      const int row = (warp & 3) * 32 + lane, n = tile * kTileRows + row;
+      float* partial = reinterpret_cast<float*>(smem);
+      for (int c0 = 0; c0 < a.cols; c0 += 16) {
+        float v[16];
+        tmem_ld_32x16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
+        tmem_ld_wait();
+        if (split > 1) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) partial[(c0 + i) * kTileRows + row] = v[i];
+        } else if (n < a.n) {
+          Out* out = static_cast<Out*>(a.out) + (int64_t)c0 * a.out_ld + n;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c0 + i < a.m) store_out(out + i * a.out_ld, v[i]);
+        }
+      }
+      tc_fence_before_sync();
+    }
+  }
+  __syncthreads();
+  if (*abort) {  // a role gave up: copies in flight land before shared memory and tensor memory are released
+    const uint64_t t0 = timer_ns();
+    while (timer_ns() - t0 < 200000) __nanosleep(1000);
+    if (threadIdx.x == 0) atomicCAS(a.error, 0, kOpsTimeout);
+  }
+  if (split > 1) {
+    cluster_sync();
+    // 128 sums of a row of A are 32 x 4; the CTAs share the rows out among their threads
+    for (int i = rank * kFewThreads + threadIdx.x; i < a.m * 32; i += split * kFewThreads) {
+      const int m = i >> 5, c = (i & 31) * 4, n = tile * kTileRows + c;
+      const uint32_t mine = base + (uint32_t)i * 16;
+      float4 sum = ld_cluster_v4(map_to_rank(mine, 0));
+      for (int r = 1; r < split; ++r) {
+        const float4 f = ld_cluster_v4(map_to_rank(mine, r));
+        sum.x += f.x, sum.y += f.y, sum.z += f.z, sum.w += f.w;
+      }
+      Out* out = static_cast<Out*>(a.out) + (int64_t)m * a.out_ld + n;
+      if (n < a.n) store_out(out, sum.x);
+      if (n + 1 < a.n) store_out(out + 1, sum.y);
+      if (n + 2 < a.n) store_out(out + 2, sum.z);
+      if (n + 3 < a.n) store_out(out + 3, sum.w);
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc_single(tmem, tmem_cols);
+}
+
+}  // namespace ops
+}  // namespace lplb

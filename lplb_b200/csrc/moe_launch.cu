@@ -1,9 +1,8 @@
 // Launchers of the benchmark MoE layer kernels and the TMA descriptor builder.
 #include "moe_api.h"
 
-#include <cudaTypedefs.h>
-
 #include "moe_support.cuh"
+#include "tensor_map.h"
 
 namespace lplb {
 namespace moe {
@@ -11,21 +10,6 @@ namespace moe {
 size_t gemm_smem_bytes() { return kGemmSmem; }
 
 namespace {
-
-// The driver entry point is fetched at run time so that the library has no link-time
-// dependency on libcuda (it is imported on GPU-less build hosts too).
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }
-  return fn;
-}
 
 bool shape_ok(const LayerShape& sh) {
   return sh.n_ranks >= 1 && sh.n_ranks <= kMaxRanks && sh.my_rank >= 0 && sh.my_rank < sh.n_ranks &&
@@ -39,14 +23,7 @@ bool shape_ok(const LayerShape& sh) {
 namespace {
 int encode_map(CUtensorMap* out, const void* base, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
                const cuuint32_t* box) {
-  auto fn = encode_fn();
-  if (!fn) return -1;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || strides[0] % 16) return -2;
-  const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  const CUresult rc = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box,
-                         elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return rc == CUDA_SUCCESS ? 0 : (int)rc;
+  return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides, box);
 }
 int row_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
   const cuuint64_t dims[2] = {cols, rows};

@@ -1,0 +1,58 @@
+// Host-side launch interface of the 8-bit serving operators.  Plain C++ so that the CUDA
+// translation units need no torch headers.  The reference has no operators of this kind.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace lplb {
+namespace ops {
+
+enum class Type : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+// ---- rows in 8 bits -------------------------------------------------------------------------
+constexpr int kMaxRowLength = 32768;
+
+struct RowFp8 {
+  const void* x;         // [rows, cols], row stride x_ld elements
+  const void* residual;  // the same, or null
+  const void* weight;    // [cols] of the type `weight_type`, or null: no norm, only the conversion
+  void* sum;             // [rows, cols] of x's type: x + residual; null without a residual
+  void* normed;          // [rows, cols] of x's type: the normed rows, or null
+  uint8_t* q;            // [rows, cols] e4m3
+  uint8_t* scale;        // [rows, ceil(cols / 128)] e8m0
+  int64_t x_ld, residual_ld;
+  int64_t rows;
+  int cols;
+  float eps;
+  Type type, weight_type;
+};
+cudaError_t launch_row_fp8(const RowFp8& a, int n_sms, cudaStream_t stream);
+
+// w: [matrices, rows, cols] contiguous -> e4m3, with one scale per 128 x 128:
+// [matrices, ceil(rows / 128), ceil(cols / 128)]
+cudaError_t launch_weight_fp8(const void* w, Type type, int64_t matrices, int64_t rows, int64_t cols, uint8_t* q, uint8_t* scale,
+                              cudaStream_t stream);
+
+// ---- block-scaled product -------------------------------------------------------------------
+// out[m, n] = sum over k of a[m, k] * b[n, k], both e4m3, a with a scale per row and 128, b with one per 128 x 128.
+struct Product {
+  const void* a;           // [m, k], row stride a_ld
+  const void* b;           // [n, k], row stride b_ld
+  const uint8_t* a_scale;  // [m, ceil(k / 128)], row stride a_scale_ld
+  const uint8_t* b_scale;  // [ceil(n / 128), ceil(k / 128)]
+  void* out;               // [m, n], row stride out_ld, bf16 or float32
+  int64_t m, n, k, a_ld, b_ld, a_scale_ld, out_ld;
+  int out_f32;
+};
+cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream);
+
+// First error that a kernel of these operators has seen on the current device (0: none; 21: a wait inside a
+// kernel gave up, its results are not valid).  It stays until it is cleared; reading waits for the device.
+cudaError_t read_ops_error(int* code, bool clear);
+// Where the kernels put it.
+constexpr int kMaxDevices = 64;
+cudaError_t ops_error_word(int device, int** word);
+
+}  // namespace ops
+}  // namespace lplb

@@ -1,0 +1,232 @@
+// Python binding of the 8-bit serving operators: checks of the arguments, outputs, launches on the
+// current stream of the arguments' device.  The reference has no operators of this kind.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <pybind11/pybind11.h>
+#include <pybind11/stl.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <sstream>
+#include <stdexcept>
+#include <string>
+
+#include "ops_api.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+// A refused argument is a ValueError, a failed launch a RuntimeError.
+#define OPS_CHECK(cond, msg)                            \
+  do {                                                  \
+    if (!(cond)) {                                      \
+      std::ostringstream oss_;                          \
+      oss_ << "lplb_b200.ops." << msg;                  \
+      throw std::invalid_argument(oss_.str());          \
+    }                                                   \
+  } while (0)
+
+#define OPS_CUDA(expr)                                                                   \
+  do {                                                                                   \
+    cudaError_t err_ = (expr);                                                           \
+    if (err_ != cudaSuccess) {                                                           \
+      std::ostringstream oss_;                                                           \
+      oss_ << "lplb_b200.ops: " #expr " failed: " << cudaGetErrorName(err_) << ": "      \
+           << cudaGetErrorString(err_);                                                  \
+      throw std::runtime_error(oss_.str());                                              \
+    }                                                                                    \
+  } while (0)
+
+constexpr int64_t kBlock = 128;
+int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+lplb::ops::Type type_of(const Tensor& t, const char* who) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return lplb::ops::Type::kF32;
+    case torch::kBFloat16: return lplb::ops::Type::kBf16;
+    case torch::kFloat16: return lplb::ops::Type::kF16;
+    default: OPS_CHECK(false, who << " must be float32, bfloat16 or float16, not " << t.scalar_type());
+  }
+  return lplb::ops::Type::kF32;
+}
+
+void check_no_grad(const Tensor& t, const char* who) {
+  OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who << " requires a gradient: these operators have no backward pass (use torch.no_grad())");
+}
+
+int sm_count(int device) {
+  static int known[lplb::ops::kMaxDevices] = {};
+  if (device < 0 || device >= lplb::ops::kMaxDevices) return 1;
+  if (known[device] == 0) OPS_CUDA(cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device));
+  return known[device];
+}
+
+cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+
+// Rows of the last dimension as one matrix, without a copy wherever the strides allow it.
+Tensor as_rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+uint8_t* bytes(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
+  auto shape = t.sizes().vec();
+  shape.back() = last;
+  return shape;
+}
+
+struct RowsOut {
+  Tensor q, scale;
+};
+RowsOut make_rows(const Tensor& x) {
+  const int64_t cols = x.size(-1);
+  return {torch::empty(x.sizes(), x.options().dtype(torch::kFloat8_e4m3fn)),
+          torch::empty(with_last(x, blocks_of(cols)), x.options().dtype(torch::kFloat8_e8m0fnu))};
+}
+
+void check_rows(const Tensor& x, const char* who) {
+  OPS_CHECK(x.is_cuda(), who << " must be a CUDA tensor");
+  OPS_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= lplb::ops::kMaxRowLength,
+            who << " must have rows of 1 to " << lplb::ops::kMaxRowLength << " values");
+  OPS_CHECK(x.stride(-1) == 1 || x.size(-1) == 1 || x.numel() == 0, who << " must have the values of a row next to one another");
+  check_no_grad(x, who);
+}
+
+lplb::ops::RowFp8 row_args(const Tensor& x, const RowsOut& out, const char* who) {
+  lplb::ops::RowFp8 a{};
+  a.x = x.data_ptr();
+  a.x_ld = x.stride(0);
+  a.rows = x.size(0);
+  a.cols = (int)x.size(1);
+  a.q = bytes(out.q);
+  a.scale = bytes(out.scale);
+  a.type = type_of(x, who);
+  return a;
+}
+
+py::tuple quantize_fp8(const Tensor& x) {
+  check_rows(x, "quantize_fp8: x");
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto out = make_rows(x);
+  const Tensor rows = as_rows(x);
+  OPS_CUDA(lplb::ops::launch_row_fp8(row_args(rows, out, "quantize_fp8: x"), sm_count(x.get_device()), stream_of(x.get_device())));
+  return py::make_tuple(out.q, out.scale);
+}
+
+py::tuple rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, bool return_normed) {
+  check_rows(x, "rms_norm_fp8: x");
+  check_no_grad(weight, "rms_norm_fp8: weight");
+  OPS_CHECK(weight.is_cuda() && weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == x.size(-1) && weight.is_contiguous(),
+            "rms_norm_fp8: weight must be contiguous, on x's device, one value for each of a row");
+  OPS_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == torch::kFloat32, "rms_norm_fp8: weight must be float32 or of x's type");
+  OPS_CHECK(eps >= 0, "rms_norm_fp8: eps must not be negative");
+  c10::cuda::CUDAGuard guard(x.device());
+  const Tensor rows = as_rows(x);
+  const auto out = make_rows(x);
+  auto a = row_args(rows, out, "rms_norm_fp8: x");
+  a.weight = weight.data_ptr();
+  a.weight_type = type_of(weight, "rms_norm_fp8: weight");
+  a.eps = (float)eps;
+  Tensor sum = x, normed, other;
+  if (residual) {
+    check_rows(*residual, "rms_norm_fp8: residual");
+    OPS_CHECK(residual->device() == x.device() && residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
+              "rms_norm_fp8: residual must have x's shape, type and device");
+    other = as_rows(*residual);
+    sum = torch::empty(x.sizes(), x.options());
+    a.residual = other.data_ptr();
+    a.residual_ld = other.stride(0);
+    a.sum = sum.data_ptr();
+  }
+  if (return_normed) {
+    normed = torch::empty(x.sizes(), x.options());
+    a.normed = normed.data_ptr();
+  }
+  OPS_CUDA(lplb::ops::launch_row_fp8(a, sm_count(x.get_device()), stream_of(x.get_device())));
+  if (return_normed) return py::make_tuple(out.q, out.scale, sum, normed);
+  return py::make_tuple(out.q, out.scale, sum);
+}
+
+py::tuple quantize_weight_fp8(const Tensor& w) {
+  OPS_CHECK(w.is_cuda() && (w.dim() == 2 || w.dim() == 3) && w.is_contiguous(), "quantize_weight_fp8: w must be a contiguous CUDA tensor [rows, cols] or [matrices, rows, cols]");
+  check_no_grad(w, "quantize_weight_fp8: w");
+  const auto type = type_of(w, "quantize_weight_fp8: w");
+  c10::cuda::CUDAGuard guard(w.device());
+  const int64_t matrices = w.dim() == 3 ? w.size(0) : 1, rows = w.size(-2), cols = w.size(-1);
+  auto shape = w.sizes().vec();
+  shape[shape.size() - 2] = blocks_of(rows);
+  shape.back() = blocks_of(cols);
+  auto q = torch::empty(w.sizes(), w.options().dtype(torch::kFloat8_e4m3fn));
+  auto scale = torch::empty(shape, w.options().dtype(torch::kFloat8_e8m0fnu));
+  OPS_CUDA(lplb::ops::launch_weight_fp8(w.data_ptr(), type, matrices, rows, cols, bytes(q), bytes(scale), stream_of(w.get_device())));
+  return py::make_tuple(q, scale);
+}
+
+Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, const OptTensor& rows, const OptTensor& out,
+                  bool out_f32) {
+  const auto device = a.device();
+  OPS_CHECK(a.is_cuda() && a.dim() == 2 && a.scalar_type() == torch::kFloat8_e4m3fn, "matmul_fp8: a must be a CUDA tensor [rows, k] of float8_e4m3fn");
+  OPS_CHECK(b.device() == device && b.dim() == 2 && b.scalar_type() == torch::kFloat8_e4m3fn,
+            "matmul_fp8: b must be [n, k] of float8_e4m3fn on a's device");
+  OPS_CHECK(!rows, "matmul_fp8: rows");
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(0), kb = blocks_of(k);
+  OPS_CHECK(k >= 16 && k % 16 == 0 && b.size(-1) == k, "matmul_fp8: a and b must have the same k, a multiple of 16");
+  OPS_CHECK(n >= 1 && n < (1 << 28), "matmul_fp8: b has no rows, or too many");
+  OPS_CHECK(a.stride(1) == 1 && (m < 2 || (a.stride(0) % 16 == 0 && a.stride(0) >= k)) && reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0,
+            "matmul_fp8: rows of a must be contiguous, apart from one another and start on 16-byte boundaries");
+  OPS_CHECK(b.is_contiguous() && reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 == 0, "matmul_fp8: b must be contiguous and start on a 16-byte boundary");
+  OPS_CHECK(a_scale.device() == device && a_scale.scalar_type() == torch::kFloat8_e8m0fnu && a_scale.dim() == 2 && a_scale.size(0) == m &&
+                a_scale.size(1) == kb && (a_scale.stride(1) == 1 || kb == 1),
+            "matmul_fp8: a_scale must be [rows, ceil(k / 128)] of float8_e8m0fnu on a's device, rows contiguous");
+  OPS_CHECK(b_scale.device() == device && b_scale.scalar_type() == torch::kFloat8_e8m0fnu && b_scale.is_contiguous() && b_scale.dim() == 2 &&
+                b_scale.size(0) == blocks_of(n) && b_scale.size(1) == kb,
+            "matmul_fp8: b_scale must be contiguous [ceil(n / 128), ceil(k / 128)] of float8_e8m0fnu on a's device");
+  c10::cuda::CUDAGuard guard(device);
+  const auto type = out_f32 ? torch::kFloat32 : torch::kBFloat16;
+  Tensor result;
+  if (out) {
+    OPS_CHECK(out->device() == device && out->scalar_type() == type && out->dim() == 2 && out->size(0) == m && out->size(1) == n &&
+                  (out->stride(1) == 1 || n == 1) && (m < 2 || out->stride(0) >= n),
+              "matmul_fp8: out must be [rows, n] of the output type on a's device, rows contiguous and apart from one another");
+    result = *out;
+  } else {
+    result = torch::empty({m, n}, a.options().dtype(type));
+  }
+  lplb::ops::Product p{};
+  p.a = a.data_ptr();
+  p.b = b.data_ptr();
+  p.a_scale = bytes(a_scale);
+  p.b_scale = bytes(b_scale);
+  p.out = result.data_ptr();
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.a_ld = m < 2 ? k : a.stride(0);
+  p.b_ld = k;
+  p.a_scale_ld = m < 2 ? kb : a_scale.stride(0);
+  p.out_ld = result.stride(0);
+  p.out_f32 = out_f32;
+  OPS_CUDA(lplb::ops::launch_matmul_fp8(p, a.get_device(), stream_of(a.get_device())));
+  return result;
+}
+
+int ops_error(int device, bool clear) {
+  c10::cuda::CUDAGuard guard(device);
+  int code = 0;
+  OPS_CUDA(lplb::ops::read_ops_error(&code, clear));
+  return code;
+}
+
+}  // namespace
+
+void bind_ops(py::module_& m) {
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("quantize_weight_fp8", &quantize_weight_fp8);
+  m.def("rms_norm_fp8", &rms_norm_fp8);
+  m.def("matmul_fp8", &matmul_fp8);
+  m.def("ops_error", &ops_error);
+  m.attr("MAX_ROW_LENGTH") = lplb::ops::kMaxRowLength;
+}

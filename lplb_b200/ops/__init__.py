@@ -1,5 +1,26 @@
-"""Plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path)."""
+"""Operators: plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path), and
+the 8-bit serving operators that stand around a mixture-of-experts layer."""
 
-from .reference import count_reference, quotas_reference, redirect_reference, slice_bounds
+from .fp8 import check, matmul_fp8, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
+from .reference import (
+    count_reference,
+    dequantize_fp8,
+    dequantize_weight_fp8,
+    quotas_reference,
+    redirect_reference,
+    slice_bounds,
+)
 
-__all__ = ["count_reference", "quotas_reference", "redirect_reference", "slice_bounds"]
+__all__ = [
+    "count_reference",
+    "quotas_reference",
+    "redirect_reference",
+    "slice_bounds",
+    "quantize_fp8",
+    "quantize_weight_fp8",
+    "dequantize_fp8",
+    "dequantize_weight_fp8",
+    "rms_norm_fp8",
+    "matmul_fp8",
+    "check",
+]

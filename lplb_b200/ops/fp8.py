@@ -1,0 +1,93 @@
+"""Serving operators with values in 8 bits.
+
+Values are ``torch.float8_e4m3fn``; every block of 128 along a row shares one power-of-two scale,
+a ``torch.float8_e8m0fnu`` (weights: every block of 128 x 128).  That is the form whose scales the
+B200's tensor cores multiply in by themselves.  A block's scale is the smallest power of two that
+brings its largest finite magnitude to 448 or below, 2**-126 at least; infinities and NaN become NaN.
+
+* :func:`quantize_fp8`, :func:`quantize_weight_fp8` – to 8 bits
+* :func:`rms_norm_fp8` – residual's addition, root-mean-square norm and conversion in one pass
+* :func:`matmul_fp8` – the product of such rows with such weights, of one matrix or of many experts
+* :func:`moe_few_tokens` – a whole SwiGLU mixture-of-experts layer for up to 64 tokens
+
+CUDA tensors run on the native kernels, on the current stream of their device; CPU tensors on
+the plain statements in :mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph.  None has a
+backward pass; an argument that requires a gradient is refused.  Wrong arguments raise
+``ValueError``.  :func:`check` returns the first error that a kernel has seen.
+
+The reference has no operators of this kind.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import reference
+
+__all__ = ["quantize_fp8", "quantize_weight_fp8", "rms_norm_fp8", "matmul_fp8", "check"]
+
+
+def _native():
+    from .. import _native
+
+    return _native.load()
+
+
+def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(q, scale)`` of rows ``x`` ``[..., K]`` (float32, bfloat16 or float16; rows may be apart from one
+    another): ``q`` ``[..., K]`` and one scale per 128, ``[..., ceil(K / 128)]``, both contiguous."""
+    if x.is_cuda:
+        return _native().quantize_fp8(x)
+    return reference.quantize_fp8_reference(x)
+
+
+def quantize_weight_fp8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(q, scale)`` of contiguous weights ``[N, K]`` or ``[E, N, K]``: one scale per 128 x 128,
+    ``[..., ceil(N / 128), ceil(K / 128)]``."""
+    if w.is_cuda:
+        return _native().quantize_weight_fp8(w)
+    return reference.quantize_weight_fp8_reference(w)
+
+
+def rms_norm_fp8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    return_normed: bool = False,
+) -> tuple[torch.Tensor, ...]:
+    """``(q, scale, h)`` with ``h = x + residual`` rounded to ``x``'s type and ``(q, scale)`` the 8-bit form
+    of ``h / sqrt(mean(h**2) + eps) * weight`` over the last dimension, computed in 32 bits.  Without a
+    residual ``h`` is ``x`` itself.  ``weight`` is of ``x``'s type or float32.  ``return_normed`` adds the
+    normed rows in ``x``'s type, which a router reads."""
+    if x.is_cuda:
+        return _native().rms_norm_fp8(x, weight, residual, eps, return_normed)
+    return reference.rms_norm_fp8_reference(x, weight, residual, eps, return_normed)
+
+
+def matmul_fp8(
+    a: torch.Tensor,
+    a_scale: torch.Tensor,
+    b: torch.Tensor,
+    b_scale: torch.Tensor,
+    rows: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """``a @ b.T`` of the values that ``a`` ``[M, K]`` (scales ``[M, ceil(K / 128)]``) and ``b`` ``[N, K]``
+    (scales ``[ceil(N / 128), ceil(K / 128)]``) stand for, summed in 32 bits, in bfloat16 or float32.
+
+    ``K`` is a multiple of 16; rows of ``a`` and of ``out`` may be apart from one another."""
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
+    if a.is_cuda:
+        return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32)
+    result = reference.matmul_fp8_reference(a, a_scale, b, b_scale, rows).to(out_dtype)
+    return result if out is None else out.copy_(result)
+
+
+def check(device: torch.device | int | None = None, clear: bool = False) -> int:
+    """First error code that a kernel of these operators has raised on ``device`` (0: none; 21: a wait inside
+    a kernel gave up, its results are not valid).  Waits for the device; ``clear`` forgets the error."""
+    index = torch.device("cuda" if device is None else device).index if not isinstance(device, int) else device
+    return _native().ops_error(torch.cuda.current_device() if index is None else index, clear)

@@ -11,13 +11,27 @@ are what ``Planner`` executes when it is built on a CPU device.
   (kernel: ``redirect_kernel``).  Tokens of one expert are numbered in array order here;
   the kernels number them in an order that depends on atomics, so outputs agree as
   multisets per expert, not position by position.
+
+The 8-bit serving operators (``lplb_b200.ops.fp8``) are restated below in 32 bits, or in 64 where their
+inputs are: ``quantize_fp8_reference``, ``rms_norm_fp8_reference``, ``matmul_fp8_reference``.
 """
 
 from __future__ import annotations
 
 import torch
 
-__all__ = ["slice_bounds", "count_reference", "quotas_reference", "redirect_reference"]
+__all__ = [
+    "slice_bounds",
+    "count_reference",
+    "quotas_reference",
+    "redirect_reference",
+    "dequantize_fp8",
+    "dequantize_weight_fp8",
+    "quantize_fp8_reference",
+    "quantize_weight_fp8_reference",
+    "rms_norm_fp8_reference",
+    "matmul_fp8_reference",
+]
 
 _BLOCK = 256
 
@@ -78,3 +92,97 @@ def redirect_reference(
     out = torch.where(keep, phys[safe, 0], phys[safe, 1])
     out = torch.where(valid, out, torch.full_like(out, -1))
     return out.reshape(idx.shape).to(idx.dtype)
+
+
+# ---------------------------------------------------------------------------- values in 8 bits
+_SCALE_BLOCK = 128
+
+
+def _wide(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def _scale_exponents(amax: torch.Tensor) -> torch.Tensor:
+    """Biased exponent of the smallest power of two ``s`` with ``amax / s <= 448`` (``scale_exponent`` in
+    ``fp8.cuh``): 448 is 1.75 * 2**8, so it is amax's exponent less 8, one more above a mantissa of 1.75."""
+    mantissa, exponent = torch.frexp(amax)  # mantissa in [0.5, 1)
+    e = exponent - 1 - 8 + (mantissa > 0.875).to(exponent.dtype) + 127
+    return torch.where(amax > 0, e, torch.ones_like(e)).clamp_min(1).to(torch.uint8)
+
+
+def _powers(scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return torch.ldexp(torch.ones((), dtype=dtype, device=scale.device), scale.view(torch.uint8).to(dtype) - 127)
+
+
+def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that rows in 8 bits stand for."""
+    return q.to(dtype) * _powers(scale, dtype).repeat_interleave(_SCALE_BLOCK, -1)[..., : q.shape[-1]]
+
+
+def dequantize_weight_fp8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that weights in 8 bits stand for."""
+    s = _powers(scale, dtype).repeat_interleave(_SCALE_BLOCK, -1)[..., : q.shape[-1]]
+    return q.to(dtype) * s.repeat_interleave(_SCALE_BLOCK, -2)[..., : q.shape[-2], :]
+
+
+def _to_e4m3(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    x = torch.where(x.isfinite(), x, torch.full_like(x, float("nan")))
+    return (x / _powers(scale, x.dtype)).to(torch.float8_e4m3fn)
+
+
+def quantize_fp8_reference(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows to e4m3 with a scale per 128 (kernel: ``row_fp8_kernel`` in ``csrc/norm_fp8.cu``)."""
+    f = _wide(x)
+    k = f.shape[-1]
+    blocks = torch.nn.functional.pad(f, (0, -k % _SCALE_BLOCK)).unflatten(-1, (-1, _SCALE_BLOCK))
+    magnitude = torch.where(blocks.isfinite(), blocks.abs(), torch.zeros_like(blocks))
+    e = _scale_exponents(magnitude.amax(-1))
+    return _to_e4m3(blocks, e.unsqueeze(-1)).flatten(-2)[..., :k].contiguous(), e.view(torch.float8_e8m0fnu)
+
+
+def quantize_weight_fp8_reference(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights to e4m3 with a scale per 128 x 128 (kernel: ``weight_fp8_kernel``)."""
+    f = _wide(w)
+    n, k = f.shape[-2:]
+    padded = torch.nn.functional.pad(f, (0, -k % _SCALE_BLOCK, 0, -n % _SCALE_BLOCK))
+    blocks = padded.unflatten(-1, (-1, _SCALE_BLOCK)).unflatten(-3, (-1, _SCALE_BLOCK))
+    magnitude = torch.where(blocks.isfinite(), blocks.abs(), torch.zeros_like(blocks))
+    e = _scale_exponents(magnitude.amax((-3, -1)))
+    q = _to_e4m3(blocks, e.unsqueeze(-1).unsqueeze(-3)).flatten(-2).flatten(-3, -2)
+    return q[..., :n, :k].contiguous(), e.view(torch.float8_e8m0fnu)
+
+
+def rms_norm_fp8_reference(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    return_normed: bool = False,
+) -> tuple[torch.Tensor, ...]:
+    """Residual's addition, norm and conversion to 8 bits; the sum is rounded to ``x``'s type before its norm is taken."""
+    h = x if residual is None else (_wide(x) + _wide(residual)).to(x.dtype)
+    f = _wide(h)
+    n = f * torch.rsqrt((f * f).mean(-1, keepdim=True) + eps) * weight.to(f.dtype)
+    out = (*quantize_fp8_reference(n), h)
+    return (*out, n.to(x.dtype)) if return_normed else out
+
+
+def matmul_fp8_reference(
+    a: torch.Tensor,
+    a_scale: torch.Tensor,
+    b: torch.Tensor,
+    b_scale: torch.Tensor,
+    rows: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.float32,
+) -> torch.Tensor:
+    """``a @ b.T`` of the values they stand for; with ``rows`` the groups of ``a``'s rows, one after the other, each
+    with its own matrix of ``b`` (rows behind the last group are zero here)."""
+    af, bf = dequantize_fp8(a, a_scale, dtype), dequantize_weight_fp8(b, b_scale, dtype)
+    if rows is None:
+        return af @ bf.T
+    out = torch.zeros(a.shape[0], b.shape[1], dtype=dtype, device=a.device)
+    at = 0
+    for e, n in enumerate(rows.tolist()):
+        out[at : at + n] = af[at : at + n] @ bf[e].T
+        at += n
+    return out
