@@ -56,6 +56,7 @@ SOURCES = [
     "ops_status.cu",
     "norm_fp8.cu",
     "matmul_fp8.cu",
+    "moe_few.cu",
 ]
 
 NVCC_FLAGS = [

@@ -47,6 +47,37 @@ struct Product {
 };
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream);
 
+// ---- MoE layer for a few tokens ---------------------------------------------------------------
+constexpr int kMoeFewMaxTokens = 64, kMoeFewMaxTopk = 32, kMoeFewMaxExperts = 1024;
+
+// What the first kernel tells the second, in a workspace of the call.
+struct MoeFewPlan {
+  int* slots;        // number of experts that were chosen
+  int* ticket;       // shares taken
+  int* expert;       // [slots] their ids
+  uint64_t* tokens;  // [slots] bit t: token t chose it
+  float* weight;     // [slots, 64]
+  int* ready;        // [slots] finished tiles of `act`
+  int* tile_blocks;  // [slots * inter / 128] k blocks summed so far
+  int* out_blocks;   // [hidden / 256]
+};
+struct MoeFew {
+  const void* x;             // [tokens, hidden] bf16 (row stride x_ld) or e4m3 (with x_scale)
+  const uint8_t* x_scale;    // [tokens, hidden / 128], row stride x_scale_ld; null: x is bf16
+  const void* idx;           // [tokens, topk]
+  const float* weight;       // [tokens, topk]
+  const void* w13;           // [experts, 2 * inter, hidden] bf16 or e4m3, in blocks of 128 gate and 128 up rows
+  const void* w2;            // [experts, hidden, inter]
+  const uint8_t* w13_scale;  // null: bf16 weights
+  const uint8_t* w2_scale;
+  void* out;                 // [tokens, hidden] bf16
+  void* workspace;           // moe_few_workspace() bytes, 256-byte aligned
+  int64_t x_ld, x_scale_ld;
+  int idx_is64, tokens, topk, experts, hidden, inter;
+};
+size_t moe_few_workspace(const MoeFew& m, int device);
+cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream);
+
 // First error that a kernel of these operators has seen on the current device (0: none; 21: a wait inside a
 // kernel gave up, its results are not valid).  It stays until it is cleared; reading waits for the device.
 cudaError_t read_ops_error(int* code, bool clear);

@@ -213,6 +213,83 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   return result;
 }
 
+Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights, const Tensor& w13, const Tensor& w2, const OptTensor& x_scale,
+                      const OptTensor& w13_scale, const OptTensor& w2_scale) {
+  const auto device = x.device();
+  const bool fp8 = w13_scale.has_value();
+  OPS_CHECK(x.is_cuda() && x.dim() == 2, "moe_few_tokens: x must be a CUDA tensor [tokens, hidden]");
+  const int64_t tokens = x.size(0), hidden = x.size(1);
+  OPS_CHECK(tokens <= lplb::ops::kMoeFewMaxTokens, "moe_few_tokens: at most " << lplb::ops::kMoeFewMaxTokens << " tokens, not " << tokens);
+  OPS_CHECK(fp8 == w2_scale.has_value(), "moe_few_tokens: w13_scale and w2_scale come together");
+  OPS_CHECK(fp8 || !x_scale, "moe_few_tokens: x_scale needs weights in 8 bits");
+  const auto wtype = fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+  OPS_CHECK(w13.device() == device && w13.dim() == 3 && w13.scalar_type() == wtype && w13.is_contiguous() && w2.device() == device && w2.dim() == 3 &&
+                w2.scalar_type() == wtype && w2.is_contiguous(),
+            "moe_few_tokens: w13 and w2 must be contiguous, on x's device, " << wtype);
+  const int64_t experts = w13.size(0), inter = w13.size(1) / 2;
+  OPS_CHECK(experts >= 1 && experts <= lplb::ops::kMoeFewMaxExperts, "moe_few_tokens: 1 to " << lplb::ops::kMoeFewMaxExperts << " experts");
+  OPS_CHECK(hidden >= 256 && hidden % 256 == 0 && inter >= 128 && inter % 128 == 0 && hidden <= 16384 && inter <= 65536,
+            "moe_few_tokens: hidden must be a multiple of 256 (up to 16384), inter of 128 (up to 65536)");
+  OPS_CHECK(w13.size(1) == 2 * inter && w13.size(2) == hidden && w2.size(0) == experts && w2.size(1) == hidden && w2.size(2) == inter,
+            "moe_few_tokens: w13 must be [experts, 2 * inter, hidden], w2 [experts, hidden, inter]");
+  OPS_CHECK(experts * 2 * inter <= INT32_MAX && experts * hidden <= INT32_MAX, "moe_few_tokens: more than 2^31 weight rows");
+  const auto xtype = x_scale ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+  const int64_t xsize = x_scale ? 1 : 2;
+  OPS_CHECK(x.scalar_type() == xtype, "moe_few_tokens: x must be bfloat16, or float8_e4m3fn with x_scale");
+  OPS_CHECK(x.stride(1) == 1 && (tokens < 2 || (x.stride(0) * xsize % 16 == 0 && x.stride(0) >= hidden)) &&
+                reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
+            "moe_few_tokens: rows of x must be contiguous, apart from one another and start on 16-byte boundaries");
+  for (const Tensor* w : {&w13, &w2})
+    OPS_CHECK(reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0, "moe_few_tokens: weights must start on a 16-byte boundary");
+  OPS_CHECK(idx.device() == device && idx.dim() == 2 && idx.size(0) == tokens && (idx.scalar_type() == torch::kInt64 || idx.scalar_type() == torch::kInt32),
+            "moe_few_tokens: idx must be [tokens, topk] of int64 or int32 on x's device");
+  const int64_t topk = idx.size(1);
+  OPS_CHECK(topk >= 1 && topk <= lplb::ops::kMoeFewMaxTopk, "moe_few_tokens: 1 to " << lplb::ops::kMoeFewMaxTopk << " choices per token");
+  OPS_CHECK(weights.device() == device && weights.sizes() == idx.sizes() && weights.is_floating_point(),
+            "moe_few_tokens: weights must be floating point, of idx's shape, on x's device");
+  auto scales_ok = [&](const Tensor& s, const Tensor& w) {
+    return s.device() == device && s.scalar_type() == torch::kFloat8_e8m0fnu && s.is_contiguous() && s.dim() == 3 && s.size(0) == w.size(0) &&
+           s.size(1) == w.size(1) / kBlock && s.size(2) == w.size(2) / kBlock;
+  };
+  OPS_CHECK(!fp8 || (scales_ok(*w13_scale, w13) && scales_ok(*w2_scale, w2)),
+            "moe_few_tokens: scales of the weights must be contiguous [experts, rows / 128, cols / 128] of float8_e8m0fnu on x's device");
+  OPS_CHECK(!x_scale || (x_scale->device() == device && x_scale->scalar_type() == torch::kFloat8_e8m0fnu && x_scale->dim() == 2 &&
+                         x_scale->size(0) == tokens && x_scale->size(1) == hidden / kBlock && x_scale->stride(1) == 1),
+            "moe_few_tokens: x_scale must be [tokens, hidden / 128] of float8_e8m0fnu on x's device, rows contiguous");
+  check_no_grad(x, "moe_few_tokens: x");
+  check_no_grad(weights, "moe_few_tokens: weights");
+  check_no_grad(w13, "moe_few_tokens: w13");
+  check_no_grad(w2, "moe_few_tokens: w2");
+  c10::cuda::CUDAGuard guard(device);
+  const int index = x.get_device();
+  auto out = torch::empty({tokens, hidden}, x.options().dtype(torch::kBFloat16));
+  if (tokens == 0) return out;
+  const Tensor ids = idx.contiguous(), gate = weights.to(torch::kFloat32).contiguous();
+  lplb::ops::MoeFew m{};
+  m.x = x.data_ptr();
+  m.x_scale = x_scale ? bytes(*x_scale) : nullptr;
+  m.idx = ids.data_ptr();
+  m.weight = gate.data_ptr<float>();
+  m.w13 = w13.data_ptr();
+  m.w2 = w2.data_ptr();
+  m.w13_scale = fp8 ? bytes(*w13_scale) : nullptr;
+  m.w2_scale = fp8 ? bytes(*w2_scale) : nullptr;
+  m.out = out.data_ptr();
+  m.x_ld = tokens < 2 ? hidden : x.stride(0);
+  m.x_scale_ld = x_scale ? (tokens < 2 ? hidden / kBlock : x_scale->stride(0)) : 0;
+  m.idx_is64 = ids.scalar_type() == torch::kInt64;
+  m.tokens = (int)tokens;
+  m.topk = (int)topk;
+  m.experts = (int)experts;
+  m.hidden = (int)hidden;
+  m.inter = (int)inter;
+  // a workspace of this call alone: calls on two streams, or two captured graphs, share nothing
+  auto workspace = torch::empty({(int64_t)lplb::ops::moe_few_workspace(m, index)}, x.options().dtype(torch::kUInt8));
+  m.workspace = workspace.data_ptr();
+  OPS_CUDA(lplb::ops::launch_moe_few(m, index, stream_of(index)));
+  return out;
+}
+
 int ops_error(int device, bool clear) {
   c10::cuda::CUDAGuard guard(device);
   int code = 0;
@@ -227,6 +304,8 @@ void bind_ops(py::module_& m) {
   m.def("quantize_weight_fp8", &quantize_weight_fp8);
   m.def("rms_norm_fp8", &rms_norm_fp8);
   m.def("matmul_fp8", &matmul_fp8);
+  m.def("moe_few_tokens", &moe_few_tokens);
   m.def("ops_error", &ops_error);
+  m.attr("MOE_FEW_MAX_TOKENS") = lplb::ops::kMoeFewMaxTokens;
   m.attr("MAX_ROW_LENGTH") = lplb::ops::kMaxRowLength;
 }

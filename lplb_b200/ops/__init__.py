@@ -1,7 +1,7 @@
 """Operators: plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path), and
 the 8-bit serving operators that stand around a mixture-of-experts layer."""
 
-from .fp8 import check, matmul_fp8, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
+from .fp8 import check, matmul_fp8, moe_few_tokens, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
 from .reference import (
     count_reference,
     dequantize_fp8,
@@ -22,5 +22,6 @@ __all__ = [
     "dequantize_weight_fp8",
     "rms_norm_fp8",
     "matmul_fp8",
+    "moe_few_tokens",
     "check",
 ]

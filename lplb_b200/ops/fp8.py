@@ -24,7 +24,7 @@ import torch
 
 from . import reference
 
-__all__ = ["quantize_fp8", "quantize_weight_fp8", "rms_norm_fp8", "matmul_fp8", "check"]
+__all__ = ["quantize_fp8", "quantize_weight_fp8", "rms_norm_fp8", "matmul_fp8", "moe_few_tokens", "check"]
 
 
 def _native():
@@ -84,6 +84,34 @@ def matmul_fp8(
         return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32)
     result = reference.matmul_fp8_reference(a, a_scale, b, b_scale, rows).to(out_dtype)
     return result if out is None else out.copy_(result)
+
+
+def moe_few_tokens(
+    x: torch.Tensor,
+    idx: torch.Tensor,
+    weights: torch.Tensor,
+    w13: torch.Tensor,
+    w2: torch.Tensor,
+    x_scale: torch.Tensor | None = None,
+    w13_scale: torch.Tensor | None = None,
+    w2_scale: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """A whole SwiGLU mixture-of-experts layer for up to 64 tokens: two kernels that read the weights of the
+    chosen experts once.
+
+    ``out[t] = sum_k weights[t, k] * (silu(x[t] @ gate.T) * (x[t] @ up.T)) @ down.T`` of expert ``idx[t, k]``, bfloat16
+    ``[tokens, hidden]``.  ``idx`` ``[tokens, topk]`` (int64 or int32) holds physical ids; -1 and ids that no expert has
+    choose nothing, an expert chosen twice counts twice.  ``w13`` ``[experts, 2 * inter, hidden]`` is laid out in
+    blocks of 128 gate rows and their 128 up rows (``lplb_b200.models.interleave_gate_up``), ``w2`` is ``[experts,
+    hidden, inter]``; ``hidden`` is a multiple of 256, ``inter`` of 128.
+
+    bfloat16 weights take bfloat16 ``x`` and hold the activations in bfloat16.  Weights in 8 bits (``w13_scale``,
+    ``w2_scale`` as :func:`quantize_weight_fp8` gives them) take ``x`` in 8 bits with its ``x_scale``, or in bfloat16,
+    which the first kernel converts, and hold the activations in 8 bits with a scale per 128.  Sums are in 32 bits
+    throughout, over experts too; the same inputs give the same bits."""
+    if x.is_cuda:
+        return _native().moe_few_tokens(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale)
+    return reference.moe_few_tokens_reference(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale).bfloat16()
 
 
 def check(device: torch.device | int | None = None, clear: bool = False) -> int:

@@ -13,7 +13,8 @@ are what ``Planner`` executes when it is built on a CPU device.
   multisets per expert, not position by position.
 
 The 8-bit serving operators (``lplb_b200.ops.fp8``) are restated below in 32 bits, or in 64 where their
-inputs are: ``quantize_fp8_reference``, ``rms_norm_fp8_reference``, ``matmul_fp8_reference``.
+inputs are: ``quantize_fp8_reference``, ``rms_norm_fp8_reference``, ``matmul_fp8_reference``,
+``moe_few_tokens_reference``.
 """
 
 from __future__ import annotations
@@ -31,6 +32,7 @@ __all__ = [
     "quantize_weight_fp8_reference",
     "rms_norm_fp8_reference",
     "matmul_fp8_reference",
+    "moe_few_tokens_reference",
 ]
 
 _BLOCK = 256
@@ -185,4 +187,34 @@ def matmul_fp8_reference(
     for e, n in enumerate(rows.tolist()):
         out[at : at + n] = af[at : at + n] @ bf[e].T
         at += n
+    return out
+
+
+def moe_few_tokens_reference(
+    x: torch.Tensor,
+    idx: torch.Tensor,
+    weights: torch.Tensor,
+    w13: torch.Tensor,
+    w2: torch.Tensor,
+    x_scale: torch.Tensor | None = None,
+    w13_scale: torch.Tensor | None = None,
+    w2_scale: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.float32,
+) -> torch.Tensor:
+    """The layer of ``moe_few_tokens`` expert by expert, computed and returned in ``dtype``; activations are rounded as
+    the kernels round them (bfloat16, or 8 bits where the weights are)."""
+    fp8 = w13_scale is not None
+    if fp8 and x_scale is None:
+        x, x_scale = quantize_fp8_reference(x)
+    xf = dequantize_fp8(x, x_scale, dtype) if fp8 else x.to(dtype)
+    out = torch.zeros(x.shape[0], w2.shape[1], dtype=dtype, device=x.device)
+    for e in idx[(idx >= 0) & (idx < w13.shape[0])].unique().tolist():
+        tok, k = (idx == e).nonzero(as_tuple=True)
+        up_gate = dequantize_weight_fp8(w13[e], w13_scale[e], dtype) if fp8 else w13[e].to(dtype)
+        down = dequantize_weight_fp8(w2[e], w2_scale[e], dtype) if fp8 else w2[e].to(dtype)
+        both = (xf[tok] @ up_gate.T).unflatten(-1, (-1, 2, _SCALE_BLOCK))
+        gate, up = both[:, :, 0].flatten(1), both[:, :, 1].flatten(1)
+        act = torch.nn.functional.silu(gate) * up
+        act = dequantize_fp8(*quantize_fp8_reference(act), dtype) if fp8 else act.bfloat16().to(dtype)
+        out.index_add_(0, tok, act @ down.T * weights[tok, k].to(dtype).unsqueeze(1))
     return out
