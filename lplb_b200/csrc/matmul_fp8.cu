@@ -4,6 +4,7 @@
 #include <atomic>
 
 #include "matmul_fp8.cuh"
+#include "moe_gemm.cuh"
 #include "tensor_map.h"
 
 namespace lplb {
@@ -94,18 +95,61 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   const int most = (a.k_blocks + split - 1) / split;
   if (a.stages > most) a.stages = most;
   CUtensorMap map_b, map_a;
-  if ((err = rows_map(&map_b, p.b, p.n, p.k, p.b_ld, kTileRows)) != cudaSuccess) return err;
+  if ((err = rows_map(&map_b, p.b, p.n, p.k, p.k, kTileRows)) != cudaSuccess) return err;
   if ((err = rows_map(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
   cudaLaunchAttribute attrs[2]{};
   const cudaLaunchConfig_t config = cluster_config(attrs, tiles * split, split, FewLayout(a.cols, a.stages).total + 1024, stream, kernel);
   return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
 }
 
+// Many rows, or the rows of many matrices: the grouped GEMM of CTA pairs.
+template <int EPI>
+cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
+  auto kernel = moe::grouped_gemm_kernel<EPI, false, true>;
+  static std::atomic<int> sms[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  int n_sm = sms[device].load(std::memory_order_relaxed);
+  cudaError_t err = cudaSuccess;
+  if (n_sm == 0) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)moe::kGemmSmemFp8);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device);
+    if (err != cudaSuccess) return err;
+    sms[device].store(n_sm, std::memory_order_relaxed);
+  }
+  moe::GemmArgs a{};
+  if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
+  a.rows = p.rows;
+  a.n_experts = p.rows ? p.groups : 1;
+  a.w_rows = (int)p.n;
+  a.w_blocks = (int)((p.n + 127) / 128);
+  a.n_tiles_w = (int)((p.n + moe::kBM - 1) / moe::kBM);
+  a.k_blocks = (int)((p.k + kKBytes - 1) / kKBytes);
+  a.n_ranks = 1;
+  a.timeout_ns = kWaitBudgetNs;
+  a.w_scale = p.b_scale;
+  a.row_scale = p.a_scale;
+  a.row_scale_ld = p.a_scale_ld;
+  a.scale_words = a.k_blocks % 4 == 0 && p.a_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p.a_scale) & 3) == 0 &&
+                  (reinterpret_cast<uintptr_t>(p.b_scale) & 3) == 0;
+  a.out = p.out;
+  a.out_stride = p.out_ld;
+  a.n_rows = (int)p.m;
+  CUtensorMap map_w;
+  moe::RowMaps rows;
+  if ((err = rows_map(&map_w, p.b, (uint64_t)a.n_experts * p.n, p.k, p.k, moe::kCtaM)) != cudaSuccess) return err;
+  for (int b = 0; b < moe::kRowBoxes; ++b)
+    if ((err = rows_map(&rows.box[b], p.a, p.m, p.k, p.a_ld, moe::kBN / 2 >> b)) != cudaSuccess) return err;
+  return launch_after(kernel, dim3(n_sm & ~1), dim3(moe::kGemmThreadsFp8), moe::kGemmSmemFp8, stream, map_w, rows, a);
+}
+
 }  // namespace
 
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream) {
-  if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.m > kFewMaxRows) return cudaErrorInvalidValue;
+  if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.groups < 1 || p.groups > kMaxGroups || p.m > INT32_MAX || p.groups * p.n > INT32_MAX)
+    return cudaErrorInvalidValue;
   if (p.m == 0) return cudaSuccess;
+  if (p.rows != nullptr || p.m > kFewMaxRows)
+    return p.out_f32 ? launch_many<moe::kStoreF32>(p, device, stream) : launch_many<moe::kStore>(p, device, stream);
   return p.out_f32 ? launch_few<float>(p, device, stream) : launch_few<__nv_bfloat16>(p, device, stream);
 }
 

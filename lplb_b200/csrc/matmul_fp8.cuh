@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "scale_words.cuh"
 #include "tcgen05.cuh"
 
 namespace lplb {
@@ -27,7 +28,6 @@ constexpr int kKBytes = 128;                    // bytes of a row per k block
 constexpr uint32_t kWeightStage = kTileRows * kKBytes;
 constexpr int kMaxRingStages = 12;
 constexpr int kScaleSlots = 4;
-constexpr uint32_t kScaleAtom = 512;            // 128 rows x 4 blocks
 constexpr int kFewThreads = 256;
 constexpr int kFewMaxRows = 256;
 constexpr int kMaxSplit = 8;                    // portable cluster size
@@ -56,16 +56,6 @@ struct FewLayout {  // shared memory from a 1024-byte boundary on
     total = bars + (2 * kMaxRingStages + 2 * kScaleSlots + 1) * 8;
   }
 };
-
-// Four scale bytes of blocks 4 * group ... of a row, 1 beyond the last block.
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int group, int k_blocks, bool words) {
-  if (words) return __ldcg(reinterpret_cast<const uint32_t*>(row) + group);
-  uint32_t w = 0x7F7F7F7Fu;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (4 * group + i < k_blocks) w = (w & ~(0xFFu << (8 * i))) | ((uint32_t)__ldcg(row + 4 * group + i) << (8 * i));
-  return w;
-}
 
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
@@ -161,7 +151,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = lane + 32 * j;
-        t[j] = r < a.m ? scale_word(a.a_scale + (int64_t)r * a.a_scale_ld, g, a.k_blocks, a.scale_words) : 0x7F7F7F7Fu;
+        t[j] = r < a.m ? scale_word(a.a_scale + (int64_t)r * a.a_scale_ld, g, a.k_blocks, a.scale_words) : kScaleOnes;
       }
       const uint32_t w = scale_word(b_row, g, a.k_blocks, a.scale_words);
       if (!mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs)) break;

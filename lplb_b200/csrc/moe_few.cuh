@@ -351,7 +351,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int r = lane + 32 * j;
-              tk[j] = r < a.tokens && r < N && go ? scale_word(tok + r * ld, g, kbs, tok_words) : 0x7F7F7F7Fu;
+              tk[j] = r < a.tokens && r < N && go ? scale_word(tok + r * ld, g, kbs, tok_words) : kScaleOnes;
             }
             const uint32_t w0 = scale_word(w, g, kbs, words), w1 = scale_word(w + kbs, g, kbs, words);
             go = go && mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs);
@@ -359,7 +359,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
             uint8_t* dst = smem + L::kScales + ss * kFewScaleSlot + lane * 16;
             *reinterpret_cast<uint4*>(dst) = make_uint4(w0, w0, w0, w0);
             *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(w1, w1, w1, w1);
-            *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(tk[0], tk[1], 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+            *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(tk[0], tk[1], kScaleOnes, kScaleOnes);
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);

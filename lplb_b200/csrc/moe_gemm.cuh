@@ -45,6 +45,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "scale_words.cuh"
 #include "tcgen05.cuh"
 
 namespace lplb {
@@ -76,7 +77,19 @@ constexpr size_t kGemmSmem = 1024 + kRingBytes + kBarBytes + 2 * kTurnBytes;
 constexpr int kMaxLocalExperts = 128;
 constexpr int kMaxRanks = 8;
 
-enum Epilogue : int { kSwiGLU = 0, kScatter = 1 };
+// Operands in 8 bits (FP8): a k block is 128 values = 128 bytes again, and the scales take 12 columns of
+// tensor memory, so an accumulator has 224 columns; a seventh warp stages the scales of four k blocks
+// at a time, and shared memory for them comes out of the ring.
+constexpr int kBNFp8 = 224;
+constexpr int kGemmThreadsFp8 = kGemmThreads + 32;
+constexpr uint32_t kRingBytesFp8 = 192 * 1024;
+constexpr int kScaleSlots = 4;
+constexpr uint32_t kScaleSlotBytes = 3 * ops::kScaleAtom;  // 128 weight rows, 2 x 128 received rows
+constexpr size_t kGemmSmemFp8 = 1024 + kRingBytesFp8 + kBarBytes + 2 * kTurnBytes + kScaleSlots * kScaleSlotBytes;
+constexpr uint32_t kScaleColumns = 2 * kBNFp8;  // first column of the scales in tensor memory
+
+// kStore writes rows as they are (bf16, or float with OUT_F32)
+enum Epilogue : int { kSwiGLU = 0, kScatter = 1, kStore = 2, kStoreF32 = 3 };
 
 enum MoeErr : int { kMoeOk = 0, kMoeGemmTimeout = 11, kMoeFlagTimeout = 12, kMoeOverflow = 13 };
 
@@ -124,6 +137,16 @@ struct GemmArgs {
   uint32_t* arrived[kMaxRanks];  // per rank: [n_experts] cumulative rows landed
   int topk, hidden;
   int send_ctas;
+  // operands in 8 bits
+  const uint8_t* w_scale;        // [experts * w_blocks, k_blocks]
+  const uint8_t* row_scale;      // [n_rows, row_scale_ld]
+  int64_t row_scale_ld;
+  int w_rows, w_blocks;          // weight rows of an expert, blocks of 128 of them
+  int scale_words;               // scale rows start on 4-byte boundaries
+  // kStore: rows == nullptr means one group of n_rows; row_start == nullptr that the groups lie one after the other
+  void* out;                     // [n_rows, out_stride]
+  int64_t out_stride;
+  int n_rows;                    // rows of the A buffer
   unsigned long long* debug;     // optional [gridDim.x * 4] ns: kernel start, senders done, producer wait, end
 };
 
@@ -183,11 +206,12 @@ __device__ __forceinline__ void send_rows(const GemmArgs& a, int gw, int n_gw, i
 // tiles: tiles of one size keep the pairs that share operands in step.  (Tiles of 512 rows, two
 // accumulators side by side, load a quarter less but lose more to the shallower ring and the
 // uncovered epilogue: first GEMM at 8192 tokens 3170 us against 2906 us.)
+template <int TILE_N>
 struct TileCursor {
   int expert = 0, first_tile = 0;  // first tile id of `expert`
   int w = 0, row0 = 0, n = 0;      // the tile: weight tile, first row within the expert, rows rounded up to kStepN
   static __device__ __forceinline__ int steps_of(int rows) { return (rows + kStepN - 1) / kStepN; }
-  static __device__ __forceinline__ int tiles_of(int steps) { return (steps + kBN / kStepN - 1) / (kBN / kStepN); }
+  static __device__ __forceinline__ int tiles_of(int steps) { return (steps + TILE_N / kStepN - 1) / (TILE_N / kStepN); }
   // Advance to tile `t`; returns false when t is past the last tile.
   __device__ __forceinline__ bool seek(int t, const int* rows, const GemmArgs& a) {
     for (; expert < a.n_experts; ++expert) {
@@ -219,23 +243,28 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // tmap_w: weights (kSwiGLU: five dimensions, see gate_up_map; kScatter: boxes of 128 rows);
 // rows: received rows in boxes of 128, 64, 32 and 16.  Issuing a box takes the producer some 55
 // cycles whatever its size: in boxes of 16 rows, eight per K block, it held up the tensor cores.
-template <int EPI, bool FUSED = false>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FUSED ? kFusedThreads : kGemmThreads, 1)
+template <int EPI, bool FUSED = false, bool FP8 = false>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FUSED ? kFusedThreads : FP8 ? kGemmThreadsFp8 : kGemmThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ RowMaps rows,
                     const GemmArgs args) {
   using namespace sm100;
+  constexpr int kTileN = FP8 ? kBNFp8 : kBN;               // received rows of a tile
+  constexpr int kPer = FP8 ? 2 * kBK : kBK;                // values of a k block
+  constexpr uint32_t kRing = FP8 ? kRingBytesFp8 : kRingBytes;
   extern __shared__ uint8_t smem_raw[];
   // 1024-byte alignment is required by the 128-byte swizzle atoms; the offset is the same in both
   // CTAs of a pair, which the pair's matrix instructions rely on
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRingBytes);
-  uint8_t* smem_turn = smem + kRingBytes + kBarBytes;  // 2 x kTurnBytes, 256-byte aligned
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRing);
+  uint8_t* smem_turn = smem + kRing + kBarBytes;  // 2 x kTurnBytes, 256-byte aligned
   // bars: full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2], tile[kTileSlots]; full
   // and tmem_empty are used in the pair's first CTA only, the others in both
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kMaxStages);
   const uint32_t bar_tfull = smem_u32(bars + 2 * kMaxStages), bar_tempty = smem_u32(bars + 2 * kMaxStages + 2);
   const uint32_t bar_tile = smem_u32(bars + 2 * kMaxStages + 4);
-  static_assert((2 * kMaxStages + 4 + kTileSlots) * 8 <= kBarBytes, "barriers");
+  const uint32_t bar_sfull = bar_tile + 8 * kTileSlots, bar_sempty = bar_sfull + 8 * kScaleSlots;  // FP8; sfull in the first CTA only
+  uint8_t* smem_scales = smem_turn + 2 * kTurnBytes;  // FP8
+  static_assert((2 * kMaxStages + 4 + kTileSlots + 2 * kScaleSlots) * 8 <= kBarBytes, "barriers");
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int s_flags_ok;
@@ -265,6 +294,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       mbar_init(bar_tempty + 8 * b, 8);  // four epilogue warps of either CTA
     }
     for (int s = 0; s < kTileSlots; ++s) mbar_init(bar_tile + 8 * s, 1);
+    if (FP8) {
+      for (int s = 0; s < kScaleSlots; ++s) {
+        mbar_init(bar_sfull + 8 * s, 2);  // the scale warps of both CTAs
+        mbar_init(bar_sempty + 8 * s, 1);
+      }
+    }
     fence_barrier_init();
     tma_prefetch_desc(&tmap_w);
     for (int b = 0; b < kRowBoxes; ++b) tma_prefetch_desc(&rows.box[b]);
@@ -291,9 +326,19 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       }
     }
   }
-  for (int e = threadIdx.x; e < args.n_experts; e += blockDim.x) {
-    s_rows[e] = args.rows[e];
-    s_start[e] = args.row_start[e];
+  if (EPI < kStore || args.row_start != nullptr) {
+    for (int e = threadIdx.x; e < args.n_experts; e += blockDim.x) {
+      s_rows[e] = args.rows[e];
+      s_start[e] = args.row_start[e];
+    }
+  } else if (threadIdx.x == 0) {  // groups one after the other, none beyond the last row
+    int at = 0;
+    for (int e = 0; e < args.n_experts; ++e) {
+      const int n = args.rows != nullptr ? min(max(args.rows[e], 0), args.n_rows - at) : args.n_rows;
+      s_rows[e] = n;
+      s_start[e] = at;
+      at += n;
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -303,19 +348,21 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   volatile int* abort = &abort_flag;
   const uint64_t budget = args.timeout_ns;
   const bool go = s_flags_ok != 0;
-  TileCursor cur;
+  using Cursor = TileCursor<kTileN>;
+  Cursor cur;
   int largest = 1;  // steps of the launch's largest tile
   for (int e = lane; e < args.n_experts; e += 32) {
-    const int steps = TileCursor::steps_of(s_rows[e]), tiles = TileCursor::tiles_of(steps);
+    const int steps = Cursor::steps_of(s_rows[e]), tiles = Cursor::tiles_of(steps);
     if (tiles > 0) largest = max(largest, (steps + tiles - 1) / tiles);
   }
   largest = __reduce_max_sync(0xffffffffu, largest);
   const uint32_t stage_bytes = kStageBytesW + largest * (kStepN / 2) * kBK * 2;
-  const uint32_t stages = min((uint32_t)kMaxStages, kRingBytes / stage_bytes);
+  const uint32_t stages = min((uint32_t)kMaxStages, kRing / stage_bytes);
   // Number of this pair's i-th tile, for every role but the one that hands them out; past the end
   // of the list (which ends the role) when the wait was given up.
   auto tile_number = [&](uint32_t i) -> int {
     if (i == 0) return pair;
+    if (EPI >= kStore) return pair + (int)i * n_pairs;  // dealt out in turn: no counter to clear
     const uint32_t slot = i % kTileSlots;
     if (!mbar_wait_cluster(bar_tile + 8 * slot, ((i / kTileSlots) & 1) ^ (slot == 0), abort, budget)) return 0x7fffffff;
     return *(volatile int*)&s_tile[slot];
@@ -337,7 +384,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       int ready_expert = -1, t = pair;
       for (uint32_t i = 0; find(t) && !*abort;) {
         ++i;
-        if (half == 0) {  // the pair's next tile, fetched while this one is loaded
+        if (EPI >= kStore) t = tile_number(i);
+        if (EPI < kStore && half == 0) {  // the pair's next tile, fetched while this one is loaded
           t = n_pairs + (int)atomicAdd(args.next_tile, 1u);
           const uint32_t slot = i % kTileSlots;
           for (uint32_t r = 0; r < 2; ++r) {
@@ -369,6 +417,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const int mine = cur.n / 2;  // received rows that this CTA stages
         const int row_t = s_start[cur.expert] + cur.row0 + half * mine;
         const int w_tile = cur.expert * args.n_tiles_w + cur.w;
+        const int w_row = (FP8 ? cur.expert * args.w_rows + cur.w * kBM : w_tile * kBM) + half * kCtaM;
         const uint32_t pair_bytes = 2 * (kStageBytesW + (uint32_t)mine * kBK * 2);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, budget)) break;
@@ -376,37 +425,49 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           if (half == 0) mbar_expect_tx(bar_full + 8 * s, pair_bytes);
           uint32_t dst = smem_u32(smem) + s * stage_bytes;
           if constexpr (EPI == kSwiGLU)
-            tma_pair_load_5d(dst, &tmap_w, full, kb * kBK, half * (kCtaM / (2 * kGateRows)), w_tile);
+            tma_pair_load_5d(dst, &tmap_w, full, kb * kPer, half * (kCtaM / (2 * kGateRows)), w_tile);
           else
-            tma_pair_load_2d(dst, &tmap_w, full, kb * kBK, w_tile * kBM + half * kCtaM);
+            tma_pair_load_2d(dst, &tmap_w, full, kb * kPer, w_row);
           dst += kStageBytesW;
           int row = row_t;
 #pragma unroll
           for (int b = 0; b < kRowBoxes; ++b) {
             const int n = kBN / 2 >> b;
             if (mine & n) {
-              tma_pair_load_2d(dst, &rows.box[b], full, kb * kBK, row);
+              tma_pair_load_2d(dst, &rows.box[b], full, kb * kPer, row);
               dst += n * kBK * 2;
               row += n;
             }
           }
           if (++s == stages) s = 0, ph ^= 1;
         }
-        if (half != 0) t = tile_number(i);
+        if (EPI < kStore && half != 0) t = tile_number(i);
       }
     }
   } else if (go && warp == 1) {
     // ---------------- MMA issuer, for both CTAs ----------------
     if (half == 0 && elect_one()) {
-      uint32_t s = 0, ph = 0;
+      uint32_t s = 0, ph = 0, ss = 0, sph = 0;
       for (uint32_t tile_n = 0; find(tile_number(tile_n)) && !*abort; ++tile_n) {
         const uint32_t acc = tile_n & 1, acc_ph = (tile_n >> 1) & 1;
         if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, budget)) break;
         tc_fence_after_sync();
-        const uint32_t idesc = umma_idesc_bf16(kBM, cur.n);
-        const uint32_t tmem_d = tmem_base + acc * kBN;
+        const uint32_t idesc = FP8 ? umma_idesc_mxf8(kBM, cur.n) : umma_idesc_bf16(kBM, cur.n);
+        const uint32_t tmem_d = tmem_base + acc * kTileN;
         bool ok = true;
         for (int kb = 0; kb < args.k_blocks; ++kb) {
+          if (FP8 && (kb & 3) == 0) {
+            if (!mbar_wait_cluster(bar_sfull + 8 * ss, sph, abort, budget)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t src = smem_u32(smem_scales) + ss * kScaleSlotBytes;
+            for (int j = 0; j * 128 < 128 + cur.n; ++j)
+              tmem_pair_cp_scales(tmem_base + kScaleColumns + 4 * j, src + j * ops::kScaleAtom);
+            umma_pair_commit(bar_sempty + 8 * ss);
+            if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+          }
           if (!mbar_wait(bar_full + 8 * s, ph, abort, budget)) {
             ok = false;
             break;
@@ -417,8 +478,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 #pragma unroll
           for (int k = 0; k < kBK / kUmmaK; ++k) {
             // advance 16 elements = 32 bytes along K inside the swizzled 128-byte row
-            umma_pair_bf16(tmem_d, dw + (uint64_t)(k * kUmmaK * 2 >> 4), dt + (uint64_t)(k * kUmmaK * 2 >> 4), idesc,
-                           (kb | k) != 0);
+            // (8 bits: 32 elements)
+            const uint64_t ow = dw + (uint64_t)(k * kUmmaK * 2 >> 4), ot = dt + (uint64_t)(k * kUmmaK * 2 >> 4);
+            if constexpr (FP8)
+              umma_pair_mxf8(tmem_d, ow, ot, umma_idesc_scale_byte(idesc, kb & 3), tmem_base + kScaleColumns,
+                             tmem_base + kScaleColumns + 4, (kb | k) != 0);
+            else
+              umma_pair_bf16(tmem_d, ow, ot, idesc, (kb | k) != 0);
           }
           umma_pair_commit(bar_empty + 8 * s);  // stage reusable, in both CTAs, once these MMAs have read it
           if (++s == stages) s = 0, ph ^= 1;
@@ -432,6 +498,38 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (args.send_ctas == 0 && warp < 6 + kSendWarps) {
       send_rows<4>(args, blockIdx.x * kSendWarps + (warp - 6), gridDim.x * kSendWarps, lane);
       if (dbg && lane == 0) atomicMax(&dbg[1], (unsigned long long)timer_ns());
+    }
+  } else if (FP8 && warp == 6) {
+    // ---------------- scales: 128 weight rows of this CTA, all received rows of the tile ----------------
+    if (go) {
+      const uint32_t lead_sfull = map_to_rank(bar_sfull, 0);
+      uint32_t ss = 0, sph = 0;
+      for (uint32_t tile_n = 0; __all_sync(0xffffffffu, find(tile_number(tile_n)) && !*abort); ++tile_n) {
+        const int block = 2 * cur.w + (EPI == kSwiGLU ? (lane >= kGateRows) : half);  // a warp's lanes: 16 gate rows, 16 up rows
+        const uint8_t* w = args.w_scale + ((int64_t)cur.expert * args.w_blocks + min(block, args.w_blocks - 1)) * args.k_blocks;
+        const int row0 = s_start[cur.expert] + cur.row0 + lane;
+        bool ok = true;
+        for (int g = 0; 4 * g < args.k_blocks; ++g) {
+          uint32_t t[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            t[j] = 32 * j < cur.n && row0 + 32 * j < args.n_rows
+                       ? ops::scale_word(args.row_scale + (int64_t)(row0 + 32 * j) * args.row_scale_ld, g, args.k_blocks, args.scale_words)
+                       : ops::kScaleOnes;
+          const uint32_t v = ops::scale_word(w, g, args.k_blocks, args.scale_words);
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_sempty + 8 * ss, sph ^ 1, abort, budget));
+          if (!ok) break;
+          uint8_t* dst = smem_scales + ss * kScaleSlotBytes + lane * 16;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(v, v, v, v);
+          *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(t[0], t[1], t[2], t[3]);
+          *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(t[4], t[5], t[6], t[7]);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(lead_sfull + 8 * ss);
+          if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+        }
+        if (!ok) break;
+      }
     }
   } else if (go && warp >= 2) {
     // ---------------- epilogue ----------------
@@ -459,7 +557,29 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       }
       if (!epilogue_all(mbar_wait(bar_tfull + 8 * acc, acc_ph, abort, budget))) break;
       tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kBN;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileN;
+      if constexpr (EPI >= kStore) {
+        // a thread has a weight row's column of the result, its warp 32 neighbouring columns
+        const int col = cur.w * kBM + half * kCtaM + quarter * 32 + lane;
+        const int n = min(cur.n, left);
+        for (int c0 = 0; c0 < n; c0 += 16) {
+          float v[16];
+          __syncwarp();
+          tmem_ld_32x16(taddr + c0, v);
+          tmem_ld_wait();
+          if (col < args.w_rows) {
+            const int64_t at = (int64_t)(row0 + c0) * args.out_stride + col;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (c0 + i >= n) continue;
+              if constexpr (EPI == kStoreF32)
+                static_cast<float*>(args.out)[at + i * args.out_stride] = v[i];
+              else
+                static_cast<__nv_bfloat16*>(args.out)[at + i * args.out_stride] = __float2bfloat16_rn(v[i]);
+            }
+          }
+        }
+      } else
       for (int c0 = 0; c0 < cur.n; c0 += kStepN, turn ^= 1) {
         uint8_t* stage = smem_turn + turn * kTurnBytes;
         const uint32_t mine = smem_u32(stage);

@@ -36,14 +36,18 @@ cudaError_t launch_weight_fp8(const void* w, Type type, int64_t matrices, int64_
 
 // ---- block-scaled product -------------------------------------------------------------------
 // out[m, n] = sum over k of a[m, k] * b[n, k], both e4m3, a with a scale per row and 128, b with one per 128 x 128.
+// With `rows`, matrix e belongs to rows[e] rows of a, which follow those of matrix e - 1; rows behind the last group are
+// neither read nor written.
+constexpr int kMaxGroups = 128;
 struct Product {
   const void* a;           // [m, k], row stride a_ld
-  const void* b;           // [n, k], row stride b_ld
+  const void* b;           // [groups, n, k]
   const uint8_t* a_scale;  // [m, ceil(k / 128)], row stride a_scale_ld
-  const uint8_t* b_scale;  // [ceil(n / 128), ceil(k / 128)]
+  const uint8_t* b_scale;  // [groups, ceil(n / 128), ceil(k / 128)]
+  const int* rows;         // [groups] on the device, or null: one matrix, all rows
   void* out;               // [m, n], row stride out_ld, bf16 or float32
-  int64_t m, n, k, a_ld, b_ld, a_scale_ld, out_ld;
-  int out_f32;
+  int64_t m, n, k, a_ld, a_scale_ld, out_ld;
+  int groups, out_f32;
 };
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream);
 

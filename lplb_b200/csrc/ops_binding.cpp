@@ -169,10 +169,14 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
                   bool out_f32) {
   const auto device = a.device();
   OPS_CHECK(a.is_cuda() && a.dim() == 2 && a.scalar_type() == torch::kFloat8_e4m3fn, "matmul_fp8: a must be a CUDA tensor [rows, k] of float8_e4m3fn");
-  OPS_CHECK(b.device() == device && b.dim() == 2 && b.scalar_type() == torch::kFloat8_e4m3fn,
-            "matmul_fp8: b must be [n, k] of float8_e4m3fn on a's device");
-  OPS_CHECK(!rows, "matmul_fp8: rows");
-  const int64_t m = a.size(0), k = a.size(1), n = b.size(0), kb = blocks_of(k);
+  const int64_t lead = rows ? 1 : 0;  // dimensions in front of a matrix
+  OPS_CHECK(b.device() == device && b.dim() == 2 + lead && b.scalar_type() == torch::kFloat8_e4m3fn,
+            "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn on a's device");
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(-2), kb = blocks_of(k), groups = rows ? b.size(0) : 1;
+  OPS_CHECK(groups >= 1 && groups <= lplb::ops::kMaxGroups, "matmul_fp8: 1 to " << lplb::ops::kMaxGroups << " groups");
+  OPS_CHECK(!rows || (rows->device() == device && rows->scalar_type() == torch::kInt32 && rows->dim() == 1 && rows->size(0) == groups && rows->is_contiguous()),
+            "matmul_fp8: rows must be contiguous int32, one number for each matrix of b, on a's device");
+  OPS_CHECK(m <= INT32_MAX && groups * n <= INT32_MAX, "matmul_fp8: more than 2^31 rows");
   OPS_CHECK(k >= 16 && k % 16 == 0 && b.size(-1) == k, "matmul_fp8: a and b must have the same k, a multiple of 16");
   OPS_CHECK(n >= 1 && n < (1 << 28), "matmul_fp8: b has no rows, or too many");
   OPS_CHECK(a.stride(1) == 1 && (m < 2 || (a.stride(0) % 16 == 0 && a.stride(0) >= k)) && reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0,
@@ -181,9 +185,11 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   OPS_CHECK(a_scale.device() == device && a_scale.scalar_type() == torch::kFloat8_e8m0fnu && a_scale.dim() == 2 && a_scale.size(0) == m &&
                 a_scale.size(1) == kb && (a_scale.stride(1) == 1 || kb == 1),
             "matmul_fp8: a_scale must be [rows, ceil(k / 128)] of float8_e8m0fnu on a's device, rows contiguous");
-  OPS_CHECK(b_scale.device() == device && b_scale.scalar_type() == torch::kFloat8_e8m0fnu && b_scale.is_contiguous() && b_scale.dim() == 2 &&
-                b_scale.size(0) == blocks_of(n) && b_scale.size(1) == kb,
-            "matmul_fp8: b_scale must be contiguous [ceil(n / 128), ceil(k / 128)] of float8_e8m0fnu on a's device");
+  OPS_CHECK(b_scale.device() == device && b_scale.scalar_type() == torch::kFloat8_e8m0fnu && b_scale.is_contiguous() &&
+                b_scale.dim() == 2 + lead && (!rows || b_scale.size(0) == groups) && b_scale.size(-2) == blocks_of(n) && b_scale.size(-1) == kb,
+            "matmul_fp8: b_scale must be contiguous [ceil(n / 128), ceil(k / 128)] (with rows: for every group) of float8_e8m0fnu on a's device");
+  check_no_grad(a, "matmul_fp8: a");
+  check_no_grad(b, "matmul_fp8: b");
   c10::cuda::CUDAGuard guard(device);
   const auto type = out_f32 ? torch::kFloat32 : torch::kBFloat16;
   Tensor result;
@@ -205,7 +211,8 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   p.n = n;
   p.k = k;
   p.a_ld = m < 2 ? k : a.stride(0);
-  p.b_ld = k;
+  p.rows = rows ? rows->data_ptr<int>() : nullptr;
+  p.groups = (int)groups;
   p.a_scale_ld = m < 2 ? kb : a_scale.stride(0);
   p.out_ld = result.stride(0);
   p.out_f32 = out_f32;

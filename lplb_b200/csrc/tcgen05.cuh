@@ -254,6 +254,21 @@ __device__ __forceinline__ void tmem_cp_scales(uint32_t tmem, uint32_t smem_addr
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_desc(smem_addr)) : "memory");
 }
 
+// The same for a CTA pair (M = 256): every CTA holds the scales of its 128 rows of A and of all rows of B, in its own
+// shared memory at the same offset and in its own tensor memory.
+__device__ __forceinline__ void umma_pair_mxf8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_scale_a,
+                                               uint32_t tmem_scale_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_scale_a), "r"(tmem_scale_b), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_pair_cp_scales(uint32_t tmem, uint32_t smem_addr) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_desc(smem_addr)) : "memory");
+}
+
 // 32 TMEM lanes (the warp's quarter) x 16 fp32 columns: thread l receives lane l.
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
   asm volatile(

@@ -77,6 +77,10 @@ def matmul_fp8(
     """``a @ b.T`` of the values that ``a`` ``[M, K]`` (scales ``[M, ceil(K / 128)]``) and ``b`` ``[N, K]``
     (scales ``[ceil(N / 128), ceil(K / 128)]``) stand for, summed in 32 bits, in bfloat16 or float32.
 
+    With ``rows`` (int32 ``[E]``, on ``a``'s device, E up to 128) ``b`` is ``[E, N, K]`` and its matrix ``e`` takes
+    ``rows[e]`` rows of ``a``, which follow those of matrix ``e - 1``; no more rows are taken than ``a`` has.  Rows behind
+    the last group are left in ``out`` as they were (in a new ``out``: not set).
+
     ``K`` is a multiple of 16; rows of ``a`` and of ``out`` may be apart from one another."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
