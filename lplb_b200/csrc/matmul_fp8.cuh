@@ -146,23 +146,38 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   } else if (warp == 2) {
     const uint8_t* b_row = a.b_scale + (int64_t)tile * a.k_blocks;
     uint32_t ss = 0, sph = 0;
-    for (int g = kb0 / 4; 4 * g < kb1; ++g) {
-      uint32_t t[8];
+    ScaleChunk next[9], now[9];
+    auto fetch = [&](int chunk) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = lane + 32 * j;
-        t[j] = r < a.m ? scale_word(a.a_scale + (int64_t)r * a.a_scale_ld, g, a.k_blocks, a.scale_words) : kScaleOnes;
+        if (32 * j < a.cols) next[j].fetch(a.a_scale + (int64_t)r * a.a_scale_ld, chunk, a.k_blocks, a.scale_words, r < a.m);
       }
-      const uint32_t w = scale_word(b_row, g, a.k_blocks, a.scale_words);
-      if (!mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs)) break;
-      uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
-      *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(t[0], t[1], t[2], t[3]);
-      *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(t[4], t[5], t[6], t[7]);
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);
-      if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+      next[8].fetch(b_row, chunk, a.k_blocks, a.scale_words, true);
+    };
+    fetch(kb0 / kScaleChunk);
+    bool ok = true;
+    for (int chunk = kb0 / kScaleChunk; ok && chunk * kScaleChunk < kb1; ++chunk) {
+#pragma unroll
+      for (int j = 0; j < 9; ++j) now[j] = next[j];
+      if ((chunk + 1) * kScaleChunk < kb1) fetch(chunk + 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int kb = chunk * kScaleChunk + 4 * i;
+        if (!ok || kb + 4 <= kb0 || kb >= kb1) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs));
+        if (!ok) continue;
+        const uint32_t w = now[8].word[i];
+        uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
+        *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(now[0].word[i], now[1].word[i], now[2].word[i], now[3].word[i]);
+        if (a.cols > 128)
+          *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(now[4].word[i], now[5].word[i], now[6].word[i], now[7].word[i]);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);
+        if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+      }
     }
   } else if (warp >= 4) {
     const bool done = mbar_wait(bar_done, 0, abort, kWaitBudgetNs);

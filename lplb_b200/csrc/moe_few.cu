@@ -20,17 +20,16 @@ int sm_count(int device) {
   return n;
 }
 
-int cols_of(int tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : 64; }
-
 // The workspace's parts, one after the other on 256-byte boundaries.
 struct Parts {
-  size_t plan_words, expert, tokens, weight, ready, act, act_scale, q, q_scale, partial, total;
-  int slots, shares, counters;
+  size_t plan_words, slot, token, pair, ready, act, act_scale, q, q_scale, partial, product, total;
+  int slots, rows, cols, ctas, counters;
   Parts(const MoeFew& m, int device) {
-    const int cols = cols_of(m.tokens), tiles = m.hidden / kFewTileRows;
-    slots = m.experts < m.tokens * m.topk ? m.experts : m.tokens * m.topk;
-    shares = sm_count(device) > tiles ? sm_count(device) : tiles;
-    counters = slots + slots * (m.inter / 128) + tiles;
+    cols = (m.tokens + 15) / 16 * 16;
+    rows = m.tokens * m.topk;
+    slots = m.experts < rows ? m.experts : rows;
+    ctas = sm_count(device);
+    counters = slots + slots * (m.inter / 128) + m.hidden / kFewTileRows;
     const size_t value = m.w13_scale ? 1 : 2;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -39,31 +38,32 @@ struct Parts {
       return here;
     };
     plan_words = take(8);
-    expert = take((size_t)slots * 4);
-    tokens = take((size_t)slots * 8);
-    weight = take((size_t)slots * 64 * 4);
+    slot = take((size_t)slots * sizeof(int2));
+    token = take((size_t)rows + 4);
+    pair = take((size_t)rows * sizeof(int2));
     ready = take((size_t)counters * 4);
-    act = take((size_t)slots * cols * m.inter * value);
-    act_scale = take((size_t)slots * cols * (m.inter / 128));
+    act = take((size_t)rows * m.inter * value);
+    act_scale = take((size_t)rows * (m.inter / 128));
     const bool convert = m.w13_scale && !m.x_scale;
     q = take(convert ? (size_t)m.tokens * m.hidden : 0);
     q_scale = take(convert ? (size_t)m.tokens * (m.hidden / 128) : 0);
-    partial = take((size_t)shares * 2 * 2 * (2 * cols * 128) * 4);
+    // tiles in parts: fewer than two per CTA, in no more parts than give one too many
+    partial = take((size_t)4 * ctas * (2 * cols * 128) * 4);
+    product = take((size_t)kFewPieces * rows * m.hidden * 4);
     total = at;
   }
 };
 
-template <bool FP8, int N>
+template <bool FP8>
 cudaError_t launch(const FewMoeArgs& a, const CUtensorMap (&maps)[4], int n_sms, int device, cudaStream_t stream) {
-  auto kernel = moe_few_kernel<FP8, N>;
-  constexpr int smem = FewMoeLayout<N>::kTotal + 1024;
+  auto kernel = moe_few_kernel<FP8>;
   static std::atomic<bool> prepared[kMaxDevices];
   if (!prepared[device].load(std::memory_order_relaxed)) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewMoeSmem);
     if (err != cudaSuccess) return err;
     prepared[device].store(true, std::memory_order_relaxed);
   }
-  return launch_after(kernel, dim3(n_sms), dim3(kFewMoeThreads), smem, stream, maps[0], maps[1], maps[2], maps[3], a);
+  return launch_after(kernel, dim3(n_sms), dim3(kFewMoeThreads), kFewMoeSmem, stream, maps[0], maps[1], maps[2], maps[3], a);
 }
 
 bool map_of(CUtensorMap* map, bool fp8, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
@@ -86,16 +86,15 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   if (m.tokens == 0) return cudaSuccess;
   const Parts at(m, device);
   char* ws = static_cast<char*>(m.workspace);
-  const int cols = cols_of(m.tokens);
   MoeFewPlan plan;
   plan.slots = reinterpret_cast<int*>(ws + at.plan_words);
   plan.ticket = plan.slots + 1;
-  plan.expert = reinterpret_cast<int*>(ws + at.expert);
-  plan.tokens = reinterpret_cast<uint64_t*>(ws + at.tokens);
-  plan.weight = reinterpret_cast<float*>(ws + at.weight);
+  plan.slot = reinterpret_cast<int2*>(ws + at.slot);
+  plan.token = reinterpret_cast<uint8_t*>(ws + at.token);
+  plan.pair = reinterpret_cast<int2*>(ws + at.pair);
   plan.ready = reinterpret_cast<int*>(ws + at.ready);
-  plan.tile_blocks = plan.ready + at.slots;
-  plan.out_blocks = plan.tile_blocks + (size_t)at.slots * (m.inter / 128);
+  plan.tile_parts = plan.ready + at.slots;
+  plan.out_blocks = plan.tile_parts + (size_t)at.slots * (m.inter / 128);
 
   FewPlanArgs p{};
   p.plan = plan;
@@ -130,13 +129,16 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   a.act_scale = reinterpret_cast<uint8_t*>(ws + at.act_scale);
   a.partial = reinterpret_cast<float*>(ws + at.partial);
   a.out = static_cast<__nv_bfloat16*>(m.out);
+  a.product = reinterpret_cast<float*>(ws + at.product);
   a.tokens = m.tokens;
+  a.topk = m.topk;
+  a.cols = at.cols;
   a.hidden = m.hidden;
   a.inter = m.inter;
   const int per = fp8 ? 128 : 64;
   a.kb1 = m.hidden / per;
   a.kb2 = m.inter / per;
-  a.shares = at.shares;
+  a.ctas = at.ctas;
   a.x_words = a.x_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x_scale) & 3) == 0;
   a.w_words = ((reinterpret_cast<uintptr_t>(a.w13_scale) | reinterpret_cast<uintptr_t>(a.w2_scale)) & 3) == 0;
   cudaError_t err = ops_error_word(device, &a.error);
@@ -144,13 +146,12 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   CUtensorMap maps[4];
   if (!map_of(&maps[0], fp8, m.w13, (uint64_t)m.experts * 2 * m.inter, m.hidden, m.hidden, kFewTileRows) ||
       !map_of(&maps[1], fp8, m.w2, (uint64_t)m.experts * m.hidden, m.inter, m.inter, kFewTileRows) ||
-      !map_of(&maps[2], fp8, x, m.tokens, m.hidden, x_ld, cols) || !map_of(&maps[3], fp8, a.act, (uint64_t)at.slots * cols, m.inter, m.inter, cols))
+      !map_of(&maps[2], fp8, x, m.tokens, m.hidden, x_ld, 1) || !map_of(&maps[3], fp8, a.act, at.rows, m.inter, m.inter, 16))
     return cudaErrorInvalidValue;
   err = launch_after(moe_few_plan_kernel, dim3(1 + (convert ? m.tokens : 0)), dim3(kFewPlanThreads), 0, stream, p);
   if (err != cudaSuccess) return err;
   const int n = sm_count(device);
-  if (fp8) return cols == 16 ? launch<true, 16>(a, maps, n, device, stream) : cols == 32 ? launch<true, 32>(a, maps, n, device, stream) : launch<true, 64>(a, maps, n, device, stream);
-  return cols == 16 ? launch<false, 16>(a, maps, n, device, stream) : cols == 32 ? launch<false, 32>(a, maps, n, device, stream) : launch<false, 64>(a, maps, n, device, stream);
+  return fp8 ? launch<true>(a, maps, n, device, stream) : launch<false>(a, maps, n, device, stream);
 }
 
 }  // namespace ops

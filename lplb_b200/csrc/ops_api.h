@@ -52,18 +52,19 @@ struct Product {
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream);
 
 // ---- MoE layer for a few tokens ---------------------------------------------------------------
-constexpr int kMoeFewMaxTokens = 64, kMoeFewMaxTopk = 32, kMoeFewMaxExperts = 1024;
+constexpr int kMoeFewMaxTokens = 64, kMoeFewMaxTopk = 32, kMoeFewMaxExperts = 512;
 
-// What the first kernel tells the second, in a workspace of the call.
+// What the first kernel tells the second, in a workspace of the call.  A row is a token's choice of an expert; the
+// rows of a slot (an expert that was chosen) follow those of the slot before, in the tokens' order.
 struct MoeFewPlan {
-  int* slots;        // number of experts that were chosen
-  int* ticket;       // shares taken
-  int* expert;       // [slots] their ids
-  uint64_t* tokens;  // [slots] bit t: token t chose it
-  float* weight;     // [slots, 64]
-  int* ready;        // [slots] finished tiles of `act`
-  int* tile_blocks;  // [slots * inter / 128] k blocks summed so far
-  int* out_blocks;   // [hidden / 256]
+  int* slots;         // number of slots
+  int* ticket;        // shares taken
+  int2* slot;         // [slots] expert, first row << 8 | rows
+  uint8_t* token;     // [tokens * topk + 4] the rows' tokens; 0 behind the last row
+  int2* pair;         // [tokens * topk] row << 10 | slot, or -1; bits of the weight
+  int* ready;         // [slots] finished tiles of `act`
+  int* tile_parts;    // [slots * inter / 128] parts summed so far
+  int* out_blocks;    // [hidden / 256] k blocks of their products made so far
 };
 struct MoeFew {
   const void* x;             // [tokens, hidden] bf16 (row stride x_ld) or e4m3 (with x_scale)

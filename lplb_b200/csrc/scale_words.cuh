@@ -19,5 +19,18 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int group, in
   return w;
 }
 
+// Scales are fetched 16 blocks at a time and one such chunk ahead: an ordinary load waits behind
+// the operands that TMA has under way to the same SM, several microseconds where those are 200 KB.
+constexpr int kScaleChunk = 16;
+struct ScaleChunk {
+  uint32_t word[4];
+  // blocks 16 * chunk ... of a row; `on`: else ones
+  __device__ __forceinline__ void fetch(const uint8_t* row, int chunk, int k_blocks, bool words, bool on) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      word[i] = on && kScaleChunk * chunk + 4 * i < k_blocks ? scale_word(row, 4 * chunk + i, k_blocks, words) : kScaleOnes;
+  }
+};
+
 }  // namespace ops
 }  // namespace lplb
