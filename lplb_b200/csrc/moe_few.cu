@@ -29,7 +29,7 @@ struct Parts {
     rows = m.tokens * m.topk;
     slots = m.experts < rows ? m.experts : rows;
     ctas = sm_count(device);
-    counters = slots + slots * (m.inter / 128) + m.hidden / kFewTileRows;
+    counters = slots + slots * (m.inter / 128) + 1;
     const size_t value = m.w13_scale ? 1 : 2;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -47,8 +47,8 @@ struct Parts {
     const bool convert = m.w13_scale && !m.x_scale;
     q = take(convert ? (size_t)m.tokens * m.hidden : 0);
     q_scale = take(convert ? (size_t)m.tokens * (m.hidden / 128) : 0);
-    // tiles in parts: fewer than two per CTA, in no more parts than give one too many
-    partial = take((size_t)4 * ctas * (2 * cols * 128) * 4);
+    // tiles in parts: no more parts than CTAs
+    partial = take((size_t)ctas * (2 * cols * 128) * 4);
     product = take((size_t)kFewPieces * rows * m.hidden * 4);
     total = at;
   }
@@ -94,7 +94,7 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   plan.pair = reinterpret_cast<int2*>(ws + at.pair);
   plan.ready = reinterpret_cast<int*>(ws + at.ready);
   plan.tile_parts = plan.ready + at.slots;
-  plan.out_blocks = plan.tile_parts + (size_t)at.slots * (m.inter / 128);
+  plan.products = plan.tile_parts + (size_t)at.slots * (m.inter / 128);
 
   FewPlanArgs p{};
   p.plan = plan;
@@ -139,6 +139,7 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   a.kb1 = m.hidden / per;
   a.kb2 = m.inter / per;
   a.ctas = at.ctas;
+  a.slots = at.slots;
   a.x_words = a.x_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x_scale) & 3) == 0;
   a.w_words = ((reinterpret_cast<uintptr_t>(a.w13_scale) | reinterpret_cast<uintptr_t>(a.w2_scale)) & 3) == 0;
   cudaError_t err = ops_error_word(device, &a.error);

@@ -78,45 +78,64 @@ struct FewMoeArgs {
   int cols;                  // tokens rounded up to 16
   int kb1, kb2;              // k blocks of 128 bytes: hidden, inter
   int ctas;                  // of the second kernel
+  int slots;                 // at most
   int x_words, w_words;      // rows of x_scale, of the weights' scales start on 4-byte boundaries
 };
 
 // The tasks: `parts` of every tile of `act`, then the units (slot by slot, tiles of down) whole up to `split`, in two
 // pieces from there on, so that the CTAs end together.
+// Division by a number that stays the same, for n * d < 2^32 (a task is looked up by five roles; five divisions of
+// 20 instructions each were 1.5 us of a small layer's 22).
+struct FewDivisor {
+  uint32_t d, m;
+  __device__ __forceinline__ explicit FewDivisor(int d_) : d((uint32_t)d_), m(d_ > 1 ? 0xFFFFFFFFu / (uint32_t)d_ + 1 : 0) {}
+  __device__ __forceinline__ int of(int n) const { return d > 1 ? (int)__umulhi((uint32_t)n, m) : n; }
+};
 struct FewTask {
   bool first;
-  int unit, part, k0, k1;
+  int unit, slot, part, k0, k1;
 };
+__device__ __forceinline__ int few_parts(int tiles, int kb1, int ctas) {
+  // parts (of at least eight blocks) only where the tiles leave half of the CTAs without one: adding them up costs
+  // 8 us between the last block and the first product (128 tiles on 148 CTAs: 78 us, in three parts 82)
+  return max(1, min(min(kFewMaxParts, kb1 / 8), tiles > 0 ? ctas / tiles : 1));
+}
 struct FewTasks {
-  int kb1, kb2, parts, tiles, units, split, pieces, n1, n;
-  __device__ __forceinline__ FewTasks(int tiles_, int kb1_, int units_, int kb2_, int ctas) : kb1(kb1_), kb2(kb2_), tiles(tiles_), units(units_) {
-    // two tasks per CTA at least, of at least eight blocks
-    parts = max(1, min(min(kFewMaxParts, kb1 / 8), tiles > 0 ? (2 * ctas + tiles - 1) / tiles : 1));
+  int kb1, kb2, parts, pieces, split, n1, n;
+  FewDivisor by_parts, by_fb, by_ht;
+  // tiles of `act` per slot, tiles of down
+  __device__ __forceinline__ FewTasks(int slots, int fb, int kb1_, int ht, int kb2_, int ctas)
+      : kb1(kb1_), kb2(kb2_), parts(few_parts(slots * fb, kb1_, ctas)), by_parts(parts), by_fb(fb), by_ht(ht) {
+    const int units = slots * ht;
     pieces = kb2 >= 8 ? kFewPieces : 1;
     split = max(0, units - ctas);
-    n1 = tiles * parts;
+    n1 = slots * fb * parts;
     n = n1 + split + (units - split) * pieces;
   }
   __device__ __forceinline__ FewTask at(int t) const {
     FewTask k;
     k.first = t < n1;
     if (k.first) {
-      k.unit = t / parts;
+      k.unit = by_parts.of(t);
       k.part = t - k.unit * parts;
-      k.k0 = kb1 * k.part / parts;
-      k.k1 = kb1 * (k.part + 1) / parts;
-    } else if (t - n1 < split) {
-      k.unit = t - n1;
-      k.part = 0;
-      k.k0 = 0;
-      k.k1 = kb2;
-    } else {
-      t -= n1 + split;
-      k.unit = split + t / pieces;
-      k.part = t % pieces;
-      k.k0 = kb2 * k.part / pieces;
-      k.k1 = kb2 * (k.part + 1) / pieces;
+      k.slot = by_fb.of(k.unit);
+      k.k0 = by_parts.of(kb1 * k.part);
+      k.k1 = by_parts.of(kb1 * (k.part + 1));
+      return k;
     }
+    t -= n1;
+    k.part = 0;
+    k.unit = t;
+    k.k0 = 0;
+    k.k1 = kb2;
+    if (t >= split && pieces == 2) {
+      t -= split;
+      k.unit = split + (t >> 1);
+      k.part = t & 1;
+      if (k.part) k.k0 = kb2 / 2;
+      else k.k1 = kb2 / 2;
+    }
+    k.slot = by_ht.of(k.unit);
     return k;
   }
 };
@@ -216,9 +235,13 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
   if (warp == 1) tmem_alloc_single(smem_u32(&tmem_slot), 512);
   __syncthreads();
   wait_predecessors();
+  // all that the plan holds in one round trip, the first ticket too
+  int first_ticket = 0;
+  if (threadIdx.x == 0) first_ticket = atomicAdd(a.plan.ticket, 1);
   const int slots = *a.plan.slots;
-  for (int i = threadIdx.x; i < slots; i += kFewMoeThreads) {
+  for (int i = threadIdx.x; i < a.slots; i += kFewMoeThreads) {
     const int2 s = a.plan.slot[i];
+    if (i >= slots) break;
     s_slot[i] = s;
     atomicMax(&s_most, s.y & 255);
   }
@@ -230,7 +253,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
   const uint32_t stage_bytes = kFewWeightStage + (uint32_t)(s_most + 15) / 16 * 16 * kKBytes;
   const uint32_t stages = min((uint32_t)kFewMaxStages, kFewRing / stage_bytes);
   const int fb = a.inter / 128, ht = a.hidden / kFewTileRows;  // tiles per expert in the first phase, tiles in the second
-  const FewTasks tasks(slots * fb, a.kb1, ht * slots, a.kb2, a.ctas);
+  const FewTasks tasks(slots, fb, a.kb1, ht, a.kb2, a.ctas);
   const int last_ticket = tasks.n;
   // The i-th ticket of this CTA, for the roles that follow the producer.
   auto ticket = [&](uint32_t i) -> int {
@@ -239,22 +262,21 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
     return *(volatile int*)&s_ticket[s];
   };
   auto ticket_read = [&](uint32_t i) { mbar_arrive(bar_ticket_read + 8 * (i % kFewTickets)); };
-  auto slot_of = [&](const FewTask& k) { return k.unit / (k.first ? fb : ht); };
   // first row of a task's tile in w13 or w2
   auto weight_row = [&](const FewTask& k) -> int {
-    const int slot = slot_of(k), tile = k.unit - slot * (k.first ? fb : ht);
-    return s_slot[slot].x * (k.first ? 2 * a.inter : a.hidden) + tile * kFewTileRows;
+    const int tile = k.unit - k.slot * (k.first ? fb : ht);
+    return s_slot[k.slot].x * (k.first ? 2 * a.inter : a.hidden) + tile * kFewTileRows;
   };
 
   if (warp == 0) {
     // ---------------- weights ----------------
-    if (elect_one()) {
+    if (lane == 0) {
       uint32_t s = 0, ph = 0;
-      // The next share is taken, and announced, a few blocks before the end of this one: early enough for its scales,
+      // The next task is taken, and announced, a few blocks before the end of this one: early enough for its scales,
       // late enough to go to the CTA that is ahead.
       auto announce = [&](uint32_t i) -> int {
         const uint32_t ts = i % kFewTickets;
-        const int t = min(atomicAdd(a.plan.ticket, 1), last_ticket);
+        const int t = min(i == 0 ? first_ticket : atomicAdd(a.plan.ticket, 1), last_ticket);
         if (!mbar_wait(bar_ticket_read + 8 * ts, ((i / kFewTickets) & 1) ^ 1, abort, kWaitBudgetNs)) return last_ticket;
         s_ticket[ts] = t;
         mbar_arrive(bar_ticket + 8 * ts);
@@ -264,7 +286,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
       for (uint32_t i = 0; next < last_ticket; ++i) {
         const FewTask k = tasks.at(next);
         bool announced = false, ok = true;
-        const int row = weight_row(k), rows = s_slot[slot_of(k)].y & 255;
+        const int row = weight_row(k), rows = s_slot[k.slot].y & 255;
         const uint32_t bytes = kFewWeightStage + (k.first ? (rows + 3) / 4 * 4 : (rows + 15) / 16 * 16) * kKBytes;
         for (int kb = k.k0; kb < k.k1; ++kb) {
           if (!announced && k.k1 - kb <= kFewAhead) {
@@ -293,7 +315,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         const FewTask task = tasks.at(t);
         const uint32_t acc = seg & 1, acc_ph = (seg >> 1) & 1;
         ++seg;
-        const int cols = ((s_slot[slot_of(task)].y & 255) + 15) / 16 * 16;
+        const int cols = ((s_slot[task.slot].y & 255) + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? umma_idesc_mxf8(128, cols) : umma_idesc_bf16(128, cols);
         if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, kWaitBudgetNs)) break;
         tc_fence_after_sync();
@@ -341,7 +363,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         ticket_read(i);
         if (t >= last_ticket) break;
         const FewTask task = tasks.at(t);
-        const int slot = slot_of(task), row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
+        const int slot = task.slot, row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
         if (!task.first && slot != ready) {
           if (!few_wait(a.plan.ready + slot, fb, abort)) break;
           fence_proxy_async_global();  // `act` was written by ordinary stores, seen through the counter
@@ -387,7 +409,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
           task = tasks.at(t);
           kb = task.k0;
         }
-        const int slot = slot_of(task);
+        const int slot = task.slot;
         if (!task.first && slot != ready) {
           bool there;
           if (wait)
@@ -402,7 +424,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
       auto fetch = [&]() {
         const bool first = task.first;
         const int kbs = first ? a.kb1 : a.kb2, k0 = kb, chunk = k0 / kScaleChunk, k1 = min(task.k1, (chunk + 1) * kScaleChunk);
-        const int slot = slot_of(task), row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
+        const int slot = task.slot, row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
         const bool w_words = (kbs & 3) == 0 && a.w_words, row_words = (kbs & 3) == 0 && (!first || a.x_words);
         const uint8_t* w = (first ? a.w13_scale : a.w2_scale) + (int64_t)(weight_row(task) / 128) * kbs;
         uint8_t* dst = smem + kFewChunksAt + put % kFewChunks * kFewChunkBytes;
@@ -496,7 +518,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
       if (!few_all(!*abort)) break;
       if (t < last_ticket) {
         const FewTask task = tasks.at(t);
-        const int unit = task.unit, slot = slot_of(task), row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
+        const int unit = task.unit, slot = task.slot, row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
         if (!arrived()) break;
         if (task.first) {
           // `act`: whole tiles at once, the others when the sums of all their parts are there
@@ -514,12 +536,14 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
               }
             }
             release();
-            __threadfence();
             few_sync();
-            if (et == 0) s_last = atomicAdd(a.plan.tile_parts + unit, 1) == tasks.parts - 1;
+            if (et == 0) {  // one thread's fences, for all that the barriers put in front of and behind it
+              __threadfence();
+              s_last = atomicAdd(a.plan.tile_parts + unit, 1) == tasks.parts - 1;
+              __threadfence();
+            }
             few_sync();
             if (s_last == 0) continue;
-            __threadfence();
           }
           for (int c0 = half * 8; c0 < rows; c0 += 16) {
             if (whole) {
@@ -575,7 +599,6 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
             }
           }
           if (whole) release();
-          __threadfence();
           few_sync();
           if (et == 0) red_release_gpu(reinterpret_cast<uint32_t*>(a.plan.ready + slot), 1);
         } else {
@@ -592,22 +615,26 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
             }
           }
           release();
-          __threadfence();
           few_sync();
-          if (et == 0) red_release_gpu(reinterpret_cast<uint32_t*>(a.plan.out_blocks + tile), (uint32_t)(task.k1 - task.k0));
+          if (et == 0) red_release_gpu(reinterpret_cast<uint32_t*>(a.plan.products), 1);
         }
       } else {
         // Nothing is left to take.  A token's sum over its experts, 128 outputs to a warp at a time; every CTA of the
         // grid comes by here, and all products are made or being made.
-        const int parts = a.hidden / 128, gw = (int)blockIdx.x * 8 + warp - 4;
-        for (int u = gw; u < parts * a.tokens; u += (int)gridDim.x * 8) {
+        const int parts = a.hidden / 128, step = (int)gridDim.x * 8, n_out = parts * a.tokens;
+        int u = (int)blockIdx.x * 8 + warp - 4;
+        auto choice = [&](int u) {  // lane k looks up choice k
+          return u < n_out && lane < a.topk ? a.plan.pair[u / parts * a.topk + lane] : make_int2(-1, 0);
+        };
+        int2 next = choice(u);
+        bool there = true;
+        if (lane == 0) there = few_wait(a.plan.products, tasks.n - tasks.n1, abort);
+        if (!__all_sync(0xffffffffu, there)) break;
+        __threadfence();
+        for (; u < n_out; u += step) {
           const int tok = u / parts, part = u - tok * parts, tile = part >> 1;
-          int2 mine = make_int2(-1, 0);  // lane k looks up choice k
-          if (lane < a.topk) mine = a.plan.pair[tok * a.topk + lane];
-          bool there = true;
-          if (lane == 0) there = few_wait(a.plan.out_blocks + tile, slots * a.kb2, abort);
-          if (!__all_sync(0xffffffffu, there)) break;
-          __threadfence();
+          const int2 mine = next;
+          next = choice(u + step);
           const int pieces = mine.x >= 0 && (mine.x & 1023) * ht + tile >= tasks.split ? tasks.pieces : 1;
           const float4* p = reinterpret_cast<const float4*>(a.product + (size_t)part * 128) + lane;
           const size_t piece = (size_t)a.tokens * a.topk * a.hidden / 4;

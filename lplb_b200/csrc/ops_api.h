@@ -64,7 +64,7 @@ struct MoeFewPlan {
   int2* pair;         // [tokens * topk] row << 10 | slot, or -1; bits of the weight
   int* ready;         // [slots] finished tiles of `act`
   int* tile_parts;    // [slots * inter / 128] parts summed so far
-  int* out_blocks;    // [hidden / 256] k blocks of their products made so far
+  int* products;      // products with down made so far, or pieces of them
 };
 struct MoeFew {
   const void* x;             // [tokens, hidden] bf16 (row stride x_ld) or e4m3 (with x_scale)
