@@ -703,15 +703,11 @@ __global__ void __launch_bounds__(kFewPlanThreads) moe_few_plan_kernel(const Few
   if (blockIdx.x > 0) {
     const int64_t row = blockIdx.x - 1;
     const __nv_bfloat16* x = a.x + row * a.x_ld;
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
     for (int c = threadIdx.x * 8; c < a.hidden; c += kFewPlanThreads * 8) {  // whole warps: hidden is a multiple of 256
-      float v[8];
-      fp8::load8(x + c, vec, 8, v);
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, fp8::magnitude(v[i]));
-      const uint32_t e = fp8::scale_exponent(fp8::block_max(top));
-      fp8::store8_e4m3(a.q + row * a.hidden + c, true, 8, fp8::pack8(v, fp8::reciprocal_of(e)));
+      float2 v[4];
+      fp8::unpack(fp8::load_raw<true>(x + c, 8), v);
+      const uint32_t e = fp8::scale_exponent(fp8::block_max(fp8::magnitude8(v)));
+      fp8::store8_e4m3<true>(a.q + row * a.hidden + c, 8, fp8::pack8(v, fp8::reciprocal_of(e), fp8::all_finite(v)));
       if ((threadIdx.x & 15) == 0) a.scale[row * (a.hidden / 128) + c / 128] = (uint8_t)e;
     }
     return;

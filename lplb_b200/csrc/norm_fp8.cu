@@ -19,97 +19,199 @@ using namespace fp8;
 
 // A row belongs to blockDim.x threads (whole warps), every thread to V vectors of eight values that are
 // blockDim.x vectors apart; 16 neighbouring lanes hold a block of 128.  Rows of one warp share a CTA.
-template <typename T, int V, bool NORM>
+//
+// The norm's factor is the same for a row, so the scale is found from h * w, times that factor, and the conversion multiplies
+// by the factor over the scale: scaling by powers of two rounds nothing.
+
+// h * w and the sum's place in the chain: values, e4m3 and scale of one vector
+template <typename T, bool NORM, bool VEC>
+__device__ __forceinline__ void finish(const RowFp8& a, float2 (&v)[4], const float2 (&w)[4], float inv, int64_t row, int c, int n, int blocks) {
+  if (NORM) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], w[i]);
+    if (a.normed != nullptr) {
+      float2 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = mul2(v[i], make_float2(inv, inv));
+      store_raw<VEC>(static_cast<T*>(a.normed) + row * a.cols + c, n, pack<T>(f));
+    }
+  }
+  const uint32_t mine = magnitude8(v);
+  const bool finite = all_finite(v);
+  uint32_t top = block_max(mine);
+  if (NORM) top = __float_as_uint(__uint_as_float(top) * inv);
+  const uint32_t e = scale_exponent(min(top, 0x7F7FFFFFu));
+  store8_e4m3<VEC>(a.q + row * a.cols + c, n, pack8(v, NORM ? inv * reciprocal_of(e) : reciprocal_of(e), finite));
+  if (n > 0 && (threadIdx.x & 15) == 0) a.scale[row * blocks + c / kBlock] = (uint8_t)e;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weight(const RowFp8& a, int c, float2 (&w)[4]) {
+  if (a.weight_type == Type::kF32)
+    unpack(load_raw<VEC>(static_cast<const float*>(a.weight) + c, a.cols - c), w);
+  else
+    unpack(load_raw<VEC>(static_cast<const T*>(a.weight) + c, a.cols - c), w);
+}
+__device__ __forceinline__ float warp_sum(float sum) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// A CTA per row (or a warp, four to a CTA); everything that a row needs is on its way before the first sum.  VEC: all rows and
+// the weight start on 16-byte boundaries and hold whole vectors.  (Where that is asked per vector, the two
+// ways meet behind every load, and the loads go one by one.)
+template <typename T, int V, bool NORM, bool VEC>
 __global__ void __launch_bounds__(1024) row_fp8_kernel(const RowFp8 a) {
   allow_successor();
   wait_predecessors();
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const bool here = row < a.rows;
+  const bool here = row < a.rows, has_residual = NORM && a.residual != nullptr;
   const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
   const T* r = static_cast<const T*>(a.residual) + row * a.residual_ld;
-  const bool x_vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a.residual ? r : x)) & 15) == 0;
-  const bool out_vec = (a.cols & 7) == 0;
-  float v[V][8];
-  float sum = 0.f;
+  auto column = [&](int j) { return (int)(j * blockDim.x + threadIdx.x) * 8; };
+  auto count = [&](int j) { return here ? a.cols - column(j) : 0; };
+  Eight<T> rx[V], rr[V];
+  float2 w[V][4], v[V][4];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * 8, n = here ? min(8, a.cols - c) : 0;
-    load8(x + c, n >= 8 && x_vec, n, v[j]);
+    rx[j] = load_raw<VEC>(x + column(j), count(j));
+    if (has_residual) rr[j] = load_raw<VEC>(r + column(j), count(j));
+    if (NORM) load_weight<T, VEC>(a, column(j), w[j]);
   }
-  if (NORM && a.residual != nullptr) {
+  float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (j * blockDim.x + threadIdx.x) * 8, n = here ? min(8, a.cols - c) : 0;
-      float f[8];
-      load8(r + c, n >= 8 && x_vec, n, f);
+  for (int j = 0; j < V; ++j) {
+    if (has_residual) {
+      rx[j] = add(rx[j], rr[j]);
+      store_raw<VEC>(static_cast<T*>(a.sum) + row * a.cols + column(j), count(j), rx[j]);
+    }
+    unpack(rx[j], v[j]);
+    if (NORM) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = to_float(from_float<T>(v[j][i] + f[i]));
-      if (n > 0) store8(static_cast<T*>(a.sum) + row * a.cols + c, n == 8 && out_vec, n, v[j]);
+      for (int i = 0; i < 4; ++i) squares = fma2(v[j][i], v[j][i], squares);
     }
   }
+  float inv = 1.f;
   if (NORM) {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(v[j][i], v[j][i], sum);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float sum = warp_sum(squares.x + squares.y);
     if (warps > 1) {  // one row per CTA
       __shared__ float part[32];
       if (lane == 0) part[warp] = sum;
       __syncthreads();
-      sum = lane < warps ? part[lane] : 0.f;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      sum = warp_sum(lane < warps ? part[lane] : 0.f);
     }
+    inv = __frsqrt_rn(fmaf(sum, 1.f / (float)a.cols, a.eps));
   }
-  const float inv = NORM ? __frsqrt_rn(sum / (float)a.cols + a.eps) : 1.f;
   const int blocks = (a.cols + kBlock - 1) / kBlock;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = (j * blockDim.x + threadIdx.x) * 8, n = here ? min(8, a.cols - c) : 0;
-    if (NORM) {
-      float w[8];
-      const bool vec = n >= 8 && (reinterpret_cast<uintptr_t>(a.weight) & 15) == 0;
-      if (a.weight_type == Type::kF32)
-        load8(static_cast<const float*>(a.weight) + c, vec, n, w);
-      else
-        load8(static_cast<const T*>(a.weight) + c, vec, n, w);
+  for (int j = 0; j < V; ++j) finish<T, NORM, VEC>(a, v[j], w[j], inv, row, column(j), count(j), blocks);
+}
+
+// Many rows: a CTA goes through them, its threads holding V vectors of a row each, and loads the next row while it
+// works on this one; the weight stays in registers.  With one row per CTA the instructions around the arithmetic (addresses,
+// the sum over the CTA) were most of all, and issuing them the bound: 104 us for 8192 rows of 7168.
+constexpr int kStreamVectors = 2;
+constexpr int kStreamThreads = 448;  // per CTA, at most; two of them per SM leave a thread 72 registers
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(kStreamThreads, 2) row_stream_fp8_kernel(const RowFp8 a) {
+  constexpr int V = kStreamVectors;
+  allow_successor();
+  wait_predecessors();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const bool has_residual = NORM && a.residual != nullptr;
+  const int blocks = (a.cols + kBlock - 1) / kBlock;
+  const float share = 1.f / (float)a.cols;
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  auto column = [&](int j) { return (int)(j * blockDim.x + threadIdx.x) * 8; };
+  Eight<T> rx[V], rr[V], rw[V];
+  auto fetch = [&]() {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+    const T* r = static_cast<const T*>(a.residual) + row * a.residual_ld;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * inv * w[i];
-      if (a.normed != nullptr && n > 0) store8(static_cast<T*>(a.normed) + row * a.cols + c, n == 8 && out_vec, n, v[j]);
+    for (int j = 0; j < V; ++j) {
+      const int n = row < a.rows ? a.cols - column(j) : 0;
+      rx[j] = load_raw<true>(x + column(j), n);
+      if (has_residual) rr[j] = load_raw<true>(r + column(j), n);
     }
-    uint32_t top = 0;
+  };
+  fetch();
+  if (NORM) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[j][i]));
-    const uint32_t e = scale_exponent(block_max(top));
-    if (n > 0) {
-      store8_e4m3(a.q + row * a.cols + c, n == 8 && out_vec, n, pack8(v[j], reciprocal_of(e)));
-      if ((lane & 15) == 0) a.scale[row * blocks + c / kBlock] = (uint8_t)e;
+    for (int j = 0; j < V; ++j)
+      if (a.weight_type != Type::kF32) rw[j] = load_raw<true>(static_cast<const T*>(a.weight) + column(j), a.cols - column(j));
+  }
+  for (int turn = 0; row - threadIdx.y < a.rows; turn ^= 1) {  // the CTA's rows stay together
+    const int64_t here = row;
+    auto count = [&](int j) { return here < a.rows ? a.cols - column(j) : 0; };
+    float2 v[V][4], squares = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (has_residual) {
+        rx[j] = add(rx[j], rr[j]);
+        store_raw<true>(static_cast<T*>(a.sum) + here * a.cols + column(j), count(j), rx[j]);
+      }
+      unpack(rx[j], v[j]);
+      if (NORM) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) squares = fma2(v[j][i], v[j][i], squares);
+      }
+    }
+    row += step;
+    fetch();
+    float inv = 1.f;
+    if (NORM) {
+      float sum = warp_sum(squares.x + squares.y);
+      if (warps > 1) {  // one row per CTA
+        __shared__ float part[2][kStreamThreads / 32];
+        if (lane == 0) part[turn][warp] = sum;
+        __syncthreads();
+        sum = warp_sum(lane < warps ? part[turn][lane] : 0.f);
+      }
+      inv = __frsqrt_rn(fmaf(sum, share, a.eps));
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float2 w[4];
+      if (NORM && a.weight_type == Type::kF32)
+        load_weight<T, true>(a, column(j), w);
+      else if (NORM)
+        unpack(rw[j], w);
+      finish<T, NORM, true>(a, v[j], w, inv, here, column(j), count(j), blocks);
     }
   }
 }
 
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(const RowFp8& a, int n_sms, cudaStream_t stream) {
   const int vectors = (a.cols + 7) / 8;
-  // Vectors per thread: one where a row's threads are few or the rows leave SMs idle anyway (the chain
-  // of one row's loads, sums and stores is all there is), four where many rows wait.
-  const int v = vectors > 2048 || (vectors > 128 && a.rows > 4 * n_sms) ? 4 : vectors > 1024 ? 2 : 1;
+  if constexpr (VEC) {
+    constexpr int V = kStreamVectors;
+    const int threads = (vectors + 32 * V - 1) / (32 * V) * 32;
+    if (a.rows > 16 * n_sms && threads <= kStreamThreads) {
+      const int per_cta = threads == 32 ? 4 : 1;
+      int64_t grid = (a.rows + per_cta - 1) / per_cta;
+      const int64_t most = (int64_t)n_sms * (2 * kStreamThreads / (threads * per_cta));
+      if (grid > most) grid = most;
+      return launch_after(row_stream_fp8_kernel<T, NORM>, dim3((unsigned)grid), dim3(threads, per_cta), 0, stream, a);
+    }
+  }
+  // Else a CTA per row, as many threads as it has vectors: the chain of loads, sums and stores of a row
+  // is all there is.
+  const int v = vectors > 1024 ? 2 : 1;
   const int threads = (vectors + 32 * v - 1) / (32 * v) * 32;
   const int per_cta = threads == 32 ? 4 : 1;
   const dim3 block(threads, per_cta);
   const int64_t grid = (a.rows + per_cta - 1) / per_cta;
   if (threads > 1024 || grid > 0x7fffffff) return cudaErrorInvalidValue;
-  if (v == 4) return launch_after(row_fp8_kernel<T, 4, NORM>, dim3((unsigned)grid), block, 0, stream, a);
-  if (v == 2) return launch_after(row_fp8_kernel<T, 2, NORM>, dim3((unsigned)grid), block, 0, stream, a);
-  return launch_after(row_fp8_kernel<T, 1, NORM>, dim3((unsigned)grid), block, 0, stream, a);
+  if (v == 2) return launch_after(row_fp8_kernel<T, 2, NORM, VEC>, dim3((unsigned)grid), block, 0, stream, a);
+  return launch_after(row_fp8_kernel<T, 1, NORM, VEC>, dim3((unsigned)grid), block, 0, stream, a);
 }
 
 // One CTA per 128 x 128 block, a row of it to 16 threads; weights are laid out once, so this is not
 // tuned beyond reading and writing whole sectors.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) weight_fp8_kernel(const T* __restrict__ w, int64_t rows, int64_t cols, int64_t row_blocks,
                                                          int64_t col_blocks, uint8_t* q, uint8_t* scale) {
   allow_successor();
@@ -118,15 +220,13 @@ __global__ void __launch_bounds__(256) weight_fp8_kernel(const T* __restrict__ w
   const int64_t cb = block % col_blocks, rb = block / col_blocks % row_blocks, m = block / col_blocks / row_blocks;
   const int64_t c = cb * kBlock + (threadIdx.x & 15) * 8;
   const int n = (int)max((int64_t)0, min((int64_t)8, cols - c));
-  const bool vec = n == 8 && (cols & 7) == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
-  float v[8][8];
+  float2 v[8][4];
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = rb * kBlock + j * 16 + (threadIdx.x >> 4);
-    load8(w + (m * rows + r) * cols + c, vec && r < rows, r < rows ? n : 0, v[j]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[j][i]));
+    unpack(load_raw<VEC>(w + (m * rows + r) * cols + c, r < rows ? n : 0), v[j]);
+    top = max(top, magnitude8(v[j]));
   }
   __shared__ uint32_t part[8];
   top = __reduce_max_sync(0xffffffffu, top);
@@ -140,37 +240,47 @@ __global__ void __launch_bounds__(256) weight_fp8_kernel(const T* __restrict__ w
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = rb * kBlock + j * 16 + (threadIdx.x >> 4);
-    if (r < rows && n > 0) store8_e4m3(q + (m * rows + r) * cols + c, n == 8 && (cols & 7) == 0, n, pack8(v[j], reciprocal));
+    if (r < rows && n > 0) store8_e4m3<VEC>(q + (m * rows + r) * cols + c, n, pack8(v[j], reciprocal, all_finite(v[j])));
   }
 }
 
+}  // namespace
+
+namespace {
+template <typename T>
+cudaError_t launch_rows(const RowFp8& a, int n_sms, cudaStream_t stream) {
+  auto whole = [&](const void* p, int64_t ld, size_t size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (a.rows < 2 || ld * size % 16 == 0); };
+  const bool vec = a.cols % 8 == 0 && whole(a.x, a.x_ld, sizeof(T)) && whole(a.residual, a.residual_ld, sizeof(T)) && whole(a.weight, 0, 1);
+  if (a.weight) return vec ? launch_rows<T, true, true>(a, n_sms, stream) : launch_rows<T, true, false>(a, n_sms, stream);
+  return vec ? launch_rows<T, false, true>(a, n_sms, stream) : launch_rows<T, false, false>(a, n_sms, stream);
+}
+template <typename T>
+cudaError_t launch_weight(const void* w, int64_t blocks, int64_t rows, int64_t cols, uint8_t* q, uint8_t* scale, cudaStream_t stream) {
+  const int64_t rb = (rows + kBlock - 1) / kBlock, cb = (cols + kBlock - 1) / kBlock;
+  auto kernel = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0 ? weight_fp8_kernel<T, true> : weight_fp8_kernel<T, false>;
+  return launch_after(kernel, dim3((unsigned)blocks), 256, 0, stream, static_cast<const T*>(w), rows, cols, rb, cb, q, scale);
+}
 }  // namespace
 
 cudaError_t launch_row_fp8(const RowFp8& a, int n_sms, cudaStream_t stream) {
   if (a.rows < 0 || a.cols < 1 || a.cols > kMaxRowLength) return cudaErrorInvalidValue;
   if (a.rows == 0) return cudaSuccess;
   switch (a.type) {
-    case Type::kF32: return a.weight ? launch_rows<float, true>(a, n_sms, stream) : launch_rows<float, false>(a, n_sms, stream);
-    case Type::kBf16:
-      return a.weight ? launch_rows<__nv_bfloat16, true>(a, n_sms, stream) : launch_rows<__nv_bfloat16, false>(a, n_sms, stream);
-    default: return a.weight ? launch_rows<__half, true>(a, n_sms, stream) : launch_rows<__half, false>(a, n_sms, stream);
+    case Type::kF32: return launch_rows<float>(a, n_sms, stream);
+    case Type::kBf16: return launch_rows<__nv_bfloat16>(a, n_sms, stream);
+    default: return launch_rows<__half>(a, n_sms, stream);
   }
 }
 
 cudaError_t launch_weight_fp8(const void* w, Type type, int64_t matrices, int64_t rows, int64_t cols, uint8_t* q, uint8_t* scale,
                               cudaStream_t stream) {
-  const int64_t rb = (rows + kBlock - 1) / kBlock, cb = (cols + kBlock - 1) / kBlock, blocks = matrices * rb * cb;
+  const int64_t blocks = matrices * ((rows + kBlock - 1) / kBlock) * ((cols + kBlock - 1) / kBlock);
   if (matrices < 0 || rows < 0 || cols < 0 || blocks > 0x7fffffff) return cudaErrorInvalidValue;
   if (blocks == 0) return cudaSuccess;
   switch (type) {
-    case Type::kF32:
-      return launch_after(weight_fp8_kernel<float>, dim3((unsigned)blocks), 256, 0, stream, static_cast<const float*>(w), rows, cols, rb, cb, q, scale);
-    case Type::kBf16:
-      return launch_after(weight_fp8_kernel<__nv_bfloat16>, dim3((unsigned)blocks), 256, 0, stream, static_cast<const __nv_bfloat16*>(w),
-                          rows, cols, rb, cb, q, scale);
-    default:
-      return launch_after(weight_fp8_kernel<__half>, dim3((unsigned)blocks), 256, 0, stream, static_cast<const __half*>(w), rows, cols, rb, cb, q,
-                          scale);
+    case Type::kF32: return launch_weight<float>(w, blocks, rows, cols, q, scale, stream);
+    case Type::kBf16: return launch_weight<__nv_bfloat16>(w, blocks, rows, cols, q, scale, stream);
+    default: return launch_weight<__half>(w, blocks, rows, cols, q, scale, stream);
   }
 }
 

@@ -11,7 +11,7 @@ namespace ops {
 enum class Type : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
 // ---- rows in 8 bits -------------------------------------------------------------------------
-constexpr int kMaxRowLength = 32768;
+constexpr int kMaxRowLength = 16384;
 
 struct RowFp8 {
   const void* x;         // [rows, cols], row stride x_ld elements
