@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "scale_words.cuh"
 #include "tcgen05.cuh"
@@ -147,13 +149,16 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     const uint8_t* b_row = a.b_scale + (int64_t)tile * a.k_blocks;
     uint32_t ss = 0, sph = 0;
     ScaleChunk next[9], now[9];
-    auto fetch = [&](int chunk) {
+    auto fetch_as = [&](auto words, int chunk) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = lane + 32 * j;
-        if (32 * j < a.cols) next[j].fetch(a.a_scale + (int64_t)r * a.a_scale_ld, chunk, a.k_blocks, a.scale_words, r < a.m);
-      }
-      next[8].fetch(b_row, chunk, a.k_blocks, a.scale_words, true);
+      for (int j = 0; j < 8; ++j)  // a row that is not there has a column that nobody reads
+        if (j == 0 || 32 * j < a.cols)
+          next[j].fetch<decltype(words)::value>(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
+      next[8].fetch<decltype(words)::value>(b_row, chunk, a.k_blocks);
+    };
+    auto fetch = [&](int chunk) {
+      if (a.scale_words) fetch_as(std::true_type{}, chunk);
+      else fetch_as(std::false_type{}, chunk);
     };
     fetch(kb0 / kScaleChunk);
     bool ok = true;

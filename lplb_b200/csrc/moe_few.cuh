@@ -428,19 +428,27 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         const bool w_words = (kbs & 3) == 0 && a.w_words, row_words = (kbs & 3) == 0 && (!first || a.x_words);
         const uint8_t* w = (first ? a.w13_scale : a.w2_scale) + (int64_t)(weight_row(task) / 128) * kbs;
         uint8_t* dst = smem + kFewChunksAt + put % kFewChunks * kFewChunkBytes;
-        auto copy = [&](uint8_t* to, const uint8_t* row, int i, bool words) {  // word i of the chunk
+        auto row_of = [&](int r) { return first ? a.x_scale + s_token[row0 + r] * a.x_scale_ld : a.act_scale + (int64_t)(row0 + r) * kbs; };
+        auto copy = [&](uint8_t* to, const uint8_t* row, int i) {  // word i of the chunk
           const int kb = chunk * kScaleChunk + 4 * i;
-          if (kb >= kbs) return;
-          if (words)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to) + 4 * i), "l"(row + kb) : "memory");
-          else
-            reinterpret_cast<uint32_t*>(to)[i] = scale_word(row, kb / 4, kbs, false);
+          if (kb < kbs) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to) + 4 * i), "l"(row + kb) : "memory");
         };
-        if (lane < 8) copy(dst + (kMoeFewMaxTokens + (lane >> 2)) * kScaleChunk, w + (lane >> 2) * kbs, lane & 3, w_words);
-        for (int r = lane; r < rows; r += 32) {
-          const uint8_t* src = first ? a.x_scale + s_token[row0 + r] * a.x_scale_ld : a.act_scale + (int64_t)(row0 + r) * kbs;
+        if (w_words && row_words) {
+          if (lane < 8) copy(dst + (kMoeFewMaxTokens + (lane >> 2)) * kScaleChunk, w + (lane >> 2) * kbs, lane & 3);
+          for (int r = lane; r < rows; r += 32) {
+            const uint8_t* src = row_of(r);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) copy(dst + r * kScaleChunk, src, i, row_words);
+            for (int i = 0; i < 4; ++i) copy(dst + r * kScaleChunk, src, i);
+          }
+        } else {  // copies of words want words: by way of registers
+          ScaleChunk c[3];
+          c[0].fetch<false>(row_of(min(lane, rows - 1)), chunk, kbs);
+          c[1].fetch<false>(row_of(min(lane + 32, rows - 1)), chunk, kbs);
+          c[2].fetch<false>(w + (lane & 1) * kbs, chunk, kbs);
+          uint4* to = reinterpret_cast<uint4*>(dst);
+          to[lane] = make_uint4(c[0].word[0], c[0].word[1], c[0].word[2], c[0].word[3]);
+          to[lane + 32] = make_uint4(c[1].word[0], c[1].word[1], c[1].word[2], c[1].word[3]);
+          if (lane < 2) to[kMoeFewMaxTokens + lane] = make_uint4(c[2].word[0], c[2].word[1], c[2].word[2], c[2].word[3]);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         queue |= (uint32_t)((k0 & (kScaleChunk - 1)) | (k1 - k0 - 1) << 4) << (8 * flight);

@@ -44,6 +44,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "scale_words.cuh"
 #include "tcgen05.cuh"
@@ -505,20 +507,23 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       const uint32_t lead_sfull = map_to_rank(bar_sfull, 0);
       uint32_t ss = 0, sph = 0;
       ops::ScaleChunk next[8], now[8];  // the weights' rows, 7 x 32 received rows
-      const uint8_t *w = nullptr, *src = nullptr;
+      const uint8_t* w = nullptr;
       int row0 = 0;
       auto locate = [&]() {
         const int block = 2 * cur.w + (EPI == kSwiGLU ? (lane >= kGateRows) : half);  // a warp's lanes: 16 gate rows, 16 up rows
         w = args.w_scale + ((int64_t)cur.expert * args.w_blocks + min(block, args.w_blocks - 1)) * args.k_blocks;
         row0 = s_start[cur.expert] + cur.row0 + lane;
-        src = args.row_scale + (int64_t)row0 * args.row_scale_ld;
+      };
+      auto fetch_as = [&](auto words, int chunk) {
+        next[0].fetch<decltype(words)::value>(w, chunk, args.k_blocks);
+#pragma unroll
+        for (int j = 0; j < 7; ++j)  // (behind the last row: a column that nobody reads)
+          next[1 + j].fetch<decltype(words)::value>(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
+                                                    chunk, args.k_blocks);
       };
       auto fetch = [&](int chunk) {
-        next[0].fetch(w, chunk, args.k_blocks, args.scale_words, true);
-#pragma unroll
-        for (int j = 0; j < 7; ++j)
-          if (32 * j < cur.n)
-            next[1 + j].fetch(src + (int64_t)(32 * j) * args.row_scale_ld, chunk, args.k_blocks, args.scale_words, row0 + 32 * j < args.n_rows);
+        if (args.scale_words) fetch_as(std::true_type{}, chunk);
+        else fetch_as(std::false_type{}, chunk);
       };
       const int chunks = (args.k_blocks + ops::kScaleChunk - 1) / ops::kScaleChunk;
       bool ok = __all_sync(0xffffffffu, find(tile_number(0)) && !*abort);
