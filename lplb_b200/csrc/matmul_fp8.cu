@@ -134,6 +134,20 @@ cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
   a.out = p.out;
   a.out_stride = p.out_ld;
   a.n_rows = (int)p.m;
+  a.wide_rows = p.n % 8 == 0 && p.out_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  // One group: tiles of equal height, so high that the fewest rounds over the CTA pairs come out (a tile costs its
+  // steps and about one more).  Several groups: their rows are only known on the device.
+  constexpr int kMostSteps = moe::kBNFp8 / moe::kStepN;
+  a.tile_steps = kMostSteps;
+  if (!p.rows) {
+    const int64_t steps = (p.m + moe::kStepN - 1) / moe::kStepN;
+    int64_t least = INT64_MAX;
+    for (int s = kMostSteps; s >= 2; --s) {
+      const int64_t tiles = (steps + s - 1) / s, high = (steps + tiles - 1) / tiles;
+      const int64_t cost = (tiles * a.n_tiles_w + n_sm / 2 - 1) / (n_sm / 2) * (high + 1);
+      if (cost < least) least = cost, a.tile_steps = (int)high;
+    }
+  }
   CUtensorMap map_w;
   moe::RowMaps rows;
   if ((err = rows_map(&map_w, p.b, (uint64_t)a.n_experts * p.n, p.k, p.k, moe::kCtaM)) != cudaSuccess) return err;

@@ -88,7 +88,8 @@ constexpr uint32_t kRingBytesFp8 = 192 * 1024;
 constexpr int kScaleSlots = 4;
 constexpr uint32_t kScaleSlotBytes = 3 * ops::kScaleAtom;  // 128 weight rows, 2 x 128 received rows
 constexpr size_t kGemmSmemFp8 = 1024 + kRingBytesFp8 + kBarBytes + 2 * kTurnBytes + kScaleSlots * kScaleSlotBytes;
-constexpr uint32_t kScaleColumns = 2 * kBNFp8;  // first column of the scales in tensor memory
+constexpr uint32_t kScaleColumns = 2 * kBNFp8;  // first column of the scales in tensor memory: 16 for every slot
+static_assert(kScaleColumns + 16 * kScaleSlots <= kTmemCols, "tensor memory");
 
 // kStore writes rows as they are (bf16, or float with OUT_F32)
 enum Epilogue : int { kSwiGLU = 0, kScatter = 1, kStore = 2, kStoreF32 = 3 };
@@ -149,6 +150,8 @@ struct GemmArgs {
   void* out;                     // [n_rows, out_stride]
   int64_t out_stride;
   int n_rows;                    // rows of the A buffer
+  int wide_rows;                 // rows of the result start on 16-byte boundaries and hold whole ones: 256 bytes of a row at a time
+  int tile_steps;                // received rows of a tile at most, in steps of kStepN
   unsigned long long* debug;     // optional [gridDim.x * 4] ns: kernel start, senders done, producer wait, end
 };
 
@@ -208,16 +211,16 @@ __device__ __forceinline__ void send_rows(const GemmArgs& a, int gw, int n_gw, i
 // tiles: tiles of one size keep the pairs that share operands in step.  (Tiles of 512 rows, two
 // accumulators side by side, load a quarter less but lose more to the shallower ring and the
 // uncovered epilogue: first GEMM at 8192 tokens 3170 us against 2906 us.)
-template <int TILE_N>
 struct TileCursor {
   int expert = 0, first_tile = 0;  // first tile id of `expert`
   int w = 0, row0 = 0, n = 0;      // the tile: weight tile, first row within the expert, rows rounded up to kStepN
   static __device__ __forceinline__ int steps_of(int rows) { return (rows + kStepN - 1) / kStepN; }
-  static __device__ __forceinline__ int tiles_of(int steps) { return (steps + TILE_N / kStepN - 1) / (TILE_N / kStepN); }
+  // tiles of `most` steps at most
+  static __device__ __forceinline__ int tiles_of(int steps, int most) { return (steps + most - 1) / most; }
   // Advance to tile `t`; returns false when t is past the last tile.
-  __device__ __forceinline__ bool seek(int t, const int* rows, const GemmArgs& a) {
+  __device__ __forceinline__ bool seek(int t, const int* rows, const GemmArgs& a, int most) {
     for (; expert < a.n_experts; ++expert) {
-      const int steps = steps_of(rows[expert]), tiles = tiles_of(steps);
+      const int steps = steps_of(rows[expert]), tiles = tiles_of(steps, most);
       if (t < first_tile + tiles * a.n_tiles_w) {
         const int local = t - first_tile;
         w = local / tiles;
@@ -350,11 +353,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   volatile int* abort = &abort_flag;
   const uint64_t budget = args.timeout_ns;
   const bool go = s_flags_ok != 0;
-  using Cursor = TileCursor<kTileN>;
-  Cursor cur;
+  const int most = EPI >= kStore ? args.tile_steps : kTileN / kStepN;  // steps of a tile
+  TileCursor cur;
   int largest = 1;  // steps of the launch's largest tile
   for (int e = lane; e < args.n_experts; e += 32) {
-    const int steps = Cursor::steps_of(s_rows[e]), tiles = Cursor::tiles_of(steps);
+    const int steps = TileCursor::steps_of(s_rows[e]), tiles = TileCursor::tiles_of(steps, most);
     if (tiles > 0) largest = max(largest, (steps + tiles - 1) / tiles);
   }
   largest = __reduce_max_sync(0xffffffffu, largest);
@@ -369,7 +372,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (!mbar_wait_cluster(bar_tile + 8 * slot, ((i / kTileSlots) & 1) ^ (slot == 0), abort, budget)) return 0x7fffffff;
     return *(volatile int*)&s_tile[slot];
   };
-  auto find = [&](int t) { return cur.seek(t, s_rows, args); };
+  auto find = [&](int t) { return cur.seek(t, s_rows, args, most); };
 
   if (sender_cta) {
     // ---------------- dedicated sender CTA (never waits on anything) ----------------
@@ -449,7 +452,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   } else if (go && warp == 1) {
     // ---------------- MMA issuer, for both CTAs ----------------
     if (half == 0 && elect_one()) {
-      uint32_t s = 0, ph = 0, ss = 0, sph = 0;
+      uint32_t s = 0, ph = 0, ss = 0, sph = 0, tmem_scale = 0;
       for (uint32_t tile_n = 0; find(tile_number(tile_n)) && !*abort; ++tile_n) {
         const uint32_t acc = tile_n & 1, acc_ph = (tile_n >> 1) & 1;
         if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, budget)) break;
@@ -465,8 +468,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_fence_after_sync();
             const uint32_t src = smem_u32(smem_scales) + ss * kScaleSlotBytes;
-            for (int j = 0; j * 128 < 128 + cur.n; ++j)
-              tmem_pair_cp_scales(tmem_base + kScaleColumns + 4 * j, src + j * ops::kScaleAtom);
+            tmem_scale = tmem_base + kScaleColumns + 16 * ss;
+            for (int j = 0; j * 128 < 128 + cur.n; ++j) tmem_pair_cp_scales(tmem_scale + 4 * j, src + j * ops::kScaleAtom);
             umma_pair_commit(bar_sempty + 8 * ss);
             if (++ss == kScaleSlots) ss = 0, sph ^= 1;
           }
@@ -483,8 +486,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             // (8 bits: 32 elements)
             const uint64_t ow = dw + (uint64_t)(k * kUmmaK * 2 >> 4), ot = dt + (uint64_t)(k * kUmmaK * 2 >> 4);
             if constexpr (FP8)
-              umma_pair_mxf8(tmem_d, ow, ot, umma_idesc_scale_byte(idesc, kb & 3), tmem_base + kScaleColumns,
-                             tmem_base + kScaleColumns + 4, (kb | k) != 0);
+              umma_pair_mxf8(tmem_d, ow, ot, umma_idesc_scale_byte(idesc, kb & 3), tmem_scale, tmem_scale + 4, (kb | k) != 0);
             else
               umma_pair_bf16(tmem_d, ow, ot, idesc, (kb | k) != 0);
           }
@@ -600,7 +602,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       if (!epilogue_all(mbar_wait(bar_tfull + 8 * acc, acc_ph, abort, budget))) break;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kTileN;
-      if constexpr (EPI >= kStore) {
+      if (EPI == kStoreF32 || (EPI == kStore && !args.wide_rows)) {
         // a thread has a weight row's column of the result, its warp 32 neighbouring columns
         const int col = cur.w * kBM + half * kCtaM + quarter * 32 + lane;
         const int n = min(cur.n, left);
@@ -672,7 +674,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           for (int i = 0; i < 4; ++i) {
             const int r = (et >> 4) + 8 * i, chunk = et & 15;
             const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 256 + ((chunk ^ (r & 7)) << 4));
-            const unsigned long long to = s_dst[acc * kBN + c0 + r];
+            unsigned long long to = 0;
+            if constexpr (EPI == kScatter)
+              to = s_dst[acc * kBN + c0 + r];
+            else if (c0 + r < left && cur.w * kBM + half * kCtaM + chunk * 8 < args.w_rows)
+              to = reinterpret_cast<unsigned long long>(static_cast<__nv_bfloat16*>(args.out) + (row0 + c0 + r) * args.out_stride);
             if (to != 0) st_global_v4(reinterpret_cast<void*>(to + col + (size_t)chunk * 16), v.x, v.y, v.z, v.w);
           }
         }
