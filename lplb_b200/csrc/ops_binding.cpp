@@ -1,5 +1,6 @@
 // Python binding of the 8-bit serving operators: checks of the arguments, outputs, launches on the
 // current stream of the arguments' device.  The reference has no operators of this kind.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
@@ -70,6 +71,9 @@ cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(devi
 // Rows of the last dimension as one matrix, without a copy wherever the strides allow it.
 Tensor as_rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
 
+// An output on x's device, without the dispatcher's microsecond.
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& x) { return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt); }
+
 uint8_t* bytes(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
@@ -83,8 +87,7 @@ struct RowsOut {
 };
 RowsOut make_rows(const Tensor& x) {
   const int64_t cols = x.size(-1);
-  return {torch::empty(x.sizes(), x.options().dtype(torch::kFloat8_e4m3fn)),
-          torch::empty(with_last(x, blocks_of(cols)), x.options().dtype(torch::kFloat8_e8m0fnu))};
+  return {make(x.sizes(), torch::kFloat8_e4m3fn, x), make(with_last(x, blocks_of(cols)), torch::kFloat8_e8m0fnu, x)};
 }
 
 void check_rows(const Tensor& x, const char* who) {
@@ -136,13 +139,13 @@ py::tuple rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& r
     OPS_CHECK(residual->device() == x.device() && residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
               "rms_norm_fp8: residual must have x's shape, type and device");
     other = as_rows(*residual);
-    sum = torch::empty(x.sizes(), x.options());
+    sum = make(x.sizes(), x.scalar_type(), x);
     a.residual = other.data_ptr();
     a.residual_ld = other.stride(0);
     a.sum = sum.data_ptr();
   }
   if (return_normed) {
-    normed = torch::empty(x.sizes(), x.options());
+    normed = make(x.sizes(), x.scalar_type(), x);
     a.normed = normed.data_ptr();
   }
   OPS_CUDA(lplb::ops::launch_row_fp8(a, sm_count(x.get_device()), stream_of(x.get_device())));
@@ -159,8 +162,8 @@ py::tuple quantize_weight_fp8(const Tensor& w) {
   auto shape = w.sizes().vec();
   shape[shape.size() - 2] = blocks_of(rows);
   shape.back() = blocks_of(cols);
-  auto q = torch::empty(w.sizes(), w.options().dtype(torch::kFloat8_e4m3fn));
-  auto scale = torch::empty(shape, w.options().dtype(torch::kFloat8_e8m0fnu));
+  auto q = make(w.sizes(), torch::kFloat8_e4m3fn, w);
+  auto scale = make(shape, torch::kFloat8_e8m0fnu, w);
   OPS_CUDA(lplb::ops::launch_weight_fp8(w.data_ptr(), type, matrices, rows, cols, bytes(q), bytes(scale), stream_of(w.get_device())));
   return py::make_tuple(q, scale);
 }
@@ -199,7 +202,7 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
               "matmul_fp8: out must be [rows, n] of the output type on a's device, rows contiguous and apart from one another");
     result = *out;
   } else {
-    result = torch::empty({m, n}, a.options().dtype(type));
+    result = make({m, n}, type, a);
   }
   lplb::ops::Product p{};
   p.a = a.data_ptr();
@@ -269,9 +272,10 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   check_no_grad(w2, "moe_few_tokens: w2");
   c10::cuda::CUDAGuard guard(device);
   const int index = x.get_device();
-  auto out = torch::empty({tokens, hidden}, x.options().dtype(torch::kBFloat16));
+  auto out = make({tokens, hidden}, torch::kBFloat16, x);
   if (tokens == 0) return out;
-  const Tensor ids = idx.contiguous(), gate = weights.to(torch::kFloat32).contiguous();
+  const Tensor ids = idx.is_contiguous() ? idx : idx.contiguous();
+  const Tensor gate = weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() ? weights : weights.to(torch::kFloat32).contiguous();
   lplb::ops::MoeFew m{};
   m.x = x.data_ptr();
   m.x_scale = x_scale ? bytes(*x_scale) : nullptr;
@@ -291,7 +295,7 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   m.hidden = (int)hidden;
   m.inter = (int)inter;
   // a workspace of this call alone: calls on two streams, or two captured graphs, share nothing
-  auto workspace = torch::empty({(int64_t)lplb::ops::moe_few_workspace(m, index)}, x.options().dtype(torch::kUInt8));
+  auto workspace = make({(int64_t)lplb::ops::moe_few_workspace(m, index)}, torch::kUInt8, x);
   m.workspace = workspace.data_ptr();
   OPS_CUDA(lplb::ops::launch_moe_few(m, index, stream_of(index)));
   return out;

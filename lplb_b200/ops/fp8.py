@@ -27,10 +27,16 @@ from . import reference
 __all__ = ["quantize_fp8", "quantize_weight_fp8", "rms_norm_fp8", "matmul_fp8", "moe_few_tokens", "check"]
 
 
-def _native():
-    from .. import _native
+_module = None
 
-    return _native.load()
+
+def _native():
+    global _module
+    if _module is None:
+        from .. import _native
+
+        _module = _native.load()
+    return _module
 
 
 def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
