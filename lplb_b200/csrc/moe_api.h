@@ -21,19 +21,24 @@ struct LayerShape {
   int topk;
   int max_tokens;    // tokens per rank (upper bound)
   int capacity;      // rows of the receive buffer
+  bool fp8;          // weights, received rows and activations in 8 bits (e4m3 with scales, see fp8.cuh)
 };
 
 // Pointers into this rank's own and its peers' buffers (peer entries alias the local ones
 // when n_ranks == 1).
 struct LayerBuffers {
   // peer-visible
-  void* recv_x[kApiMaxRanks];          // bf16 [capacity, H]
+  void* recv_x[kApiMaxRanks];          // bf16 or e4m3 [capacity, H]
+  uint8_t* recv_scale[kApiMaxRanks];   // fp8: e8m0 [capacity, H / 128]
   int* recv_meta[kApiMaxRanks];        // int32 [capacity]
   void* comb[kApiMaxRanks];            // bf16 [max_tokens * topk, H]
   unsigned long long* cnt_words[kApiMaxRanks];  // uint64 [2][n_ranks][n_ranks * n_local]
   uint32_t* flags[kApiMaxRanks];       // uint32 [2][n_ranks]: dispatch done, combine done
   // local
-  void* act;                           // bf16 [capacity, I]
+  void* act;                           // bf16 or e4m3 [capacity, I]
+  uint8_t* act_scale;                  // fp8: e8m0 [capacity, I / 128]
+  const uint8_t* w13_scale;            // fp8: e8m0 [n_local, 2 * I / 128, H / 128]
+  const uint8_t* w2_scale;             // fp8: e8m0 [n_local, H / 128, I / 128]
   int* plan;                           // int32 plan block, see plan_words()
   int* ordinal;                        // int32 [max_tokens * topk] position of every pair among its expert's
   int* totals;                         // int32 [n_ranks * n_local], zero between launches
@@ -65,17 +70,18 @@ size_t gemm_smem_bytes();
 struct GemmMaps {
   CUtensorMap w, rows[4];
 };
-// tokens: bf16 [rows, cols]; weights: bf16 [weight_rows, cols], with `gate_up` in blocks of 128
+// tokens: bf16 (fp8: e4m3) [rows, cols]; weights: the same [weight_rows, cols], with `gate_up` in blocks of 128
 // gate rows and their 128 up rows.  Returns 0 on success.
 int make_gemm_maps(GemmMaps* out, const void* tokens, uint64_t rows, const void* weights, uint64_t weight_rows,
-                   uint64_t cols, bool gate_up);
+                   uint64_t cols, bool gate_up, bool fp8);
 
 // Step 1: rank the pairs of every physical expert, all-gather the per-expert counts of this
 // launch and derive row offsets.
 cudaError_t launch_route(const LayerShape& sh, const LayerBuffers& b, const void* phys_idx, int idx_is64, int n_tokens,
                          int n_sms, uint32_t epoch, unsigned long long timeout_ns, int fused, cudaStream_t stream);
-// Step 2: copy every (token, k) pair's hidden state into its expert's rows on the target rank.
-cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const void* x, const void* phys_idx,
+// Step 2: copy every (token, k) pair's hidden state into its expert's rows on the target rank.  fp8: x is bf16 and sent in
+// 8 bits, or already so with its scales x_scale [tokens, H / 128].
+cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const void* x, const uint8_t* x_scale, const void* phys_idx,
                             int idx_is64, int n_tokens, int n_cta, uint32_t epoch, cudaStream_t stream);
 // Step 2a (fused path only): decide the send order and every pair's target row and return slot.
 cudaError_t launch_schedule(const LayerShape& sh, const LayerBuffers& b, const void* phys_idx, int idx_is64,

@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <cstring>
+#include <optional>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -45,7 +46,7 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 class MoeEngine {
  public:
   MoeEngine(int hidden, int inter, int n_local, int n_ranks, int my_rank, int topk, int max_tokens, int capacity,
-            int device)
+            int device, bool fp8)
       : device_(device) {
     sh_.hidden = hidden;
     sh_.inter = inter;
@@ -55,13 +56,15 @@ class MoeEngine {
     sh_.topk = topk;
     sh_.max_tokens = max_tokens;
     sh_.capacity = capacity;
+    sh_.fp8 = fp8;
     MOE_CHECK(n_ranks >= 1 && n_ranks <= lplb::moe::kApiMaxRanks, "1..8 ranks supported");
     MOE_CHECK(hidden % 256 == 0 && inter % 128 == 0, "hidden must be a multiple of 256, inter of 128");
     MOE_CHECK((long long)max_tokens * topk < (1 << 20), "tokens * topk must stay below 2^20");
     MOE_CHECK(capacity % 128 == 0 && capacity < (1 << 24), "capacity must be a multiple of 128 below 2^24");
     p_ = n_ranks * n_local;
     off_recv_x_ = 0;
-    off_meta_ = align_up(off_recv_x_ + (size_t)capacity * hidden * 2, 256);
+    off_scale_ = align_up(off_recv_x_ + (size_t)capacity * hidden * (fp8 ? 1 : 2), 256);
+    off_meta_ = align_up(off_scale_ + (fp8 ? (size_t)capacity * (hidden / 128) : 0), 256);
     off_comb_ = align_up(off_meta_ + (size_t)capacity * 4, 256);
     off_cnt_ = align_up(off_comb_ + (size_t)max_tokens * topk * hidden * 2, 256);
     off_flags_ = align_up(off_cnt_ + sizeof(unsigned long long) * 2 * (size_t)n_ranks * p_, 256);
@@ -85,7 +88,8 @@ class MoeEngine {
     MOE_CUDA(cudaMalloc(&block_, block_bytes_));
     MOE_CUDA(cudaMemset(block_, 0, block_bytes_));
     auto i32 = torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, device_);
-    act_ = torch::empty({sh_.capacity, sh_.inter}, i32.dtype(torch::kBFloat16));
+    act_ = torch::empty({sh_.capacity, sh_.inter}, i32.dtype(sh_.fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16));
+    if (sh_.fp8) act_scale_ = torch::empty({sh_.capacity, sh_.inter / 128}, i32.dtype(torch::kFloat8_e8m0fnu));
     plan_ = torch::zeros({lplb::moe::plan_words(sh_.n_ranks, sh_.n_local)}, i32);
     totals_ = torch::zeros({p_}, i32);
     ordinal_ = torch::zeros({(int64_t)sh_.max_tokens * sh_.topk}, i32);
@@ -134,40 +138,61 @@ class MoeEngine {
   }
 
   // w13: [n_local, 2*inter, hidden] bf16, rows of every 256-row tile ordered 128 gate rows
-  // then the 128 matching up rows.  w2: [n_local, hidden, inter] bf16.
-  void set_weights(const torch::Tensor& w13, const torch::Tensor& w2) {
+  // then the 128 matching up rows.  w2: [n_local, hidden, inter] bf16.  An engine in 8 bits takes both in e4m3,
+  // with a scale for every 128 x 128 of them.
+  void set_weights(const torch::Tensor& w13, const torch::Tensor& w2, const std::optional<torch::Tensor>& w13_scale,
+                   const std::optional<torch::Tensor>& w2_scale) {
     MOE_CHECK(ready_, "open the peer blocks first");
-    auto ok = [&](const torch::Tensor& t) {
-      return t.is_cuda() && t.get_device() == device_ && t.scalar_type() == torch::kBFloat16 && t.is_contiguous();
+    const auto type = sh_.fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+    auto ok = [&](const torch::Tensor& t, at::ScalarType type) {
+      return t.is_cuda() && t.get_device() == device_ && t.scalar_type() == type && t.is_contiguous();
     };
-    MOE_CHECK(ok(w13) && w13.dim() == 3 && w13.size(0) == sh_.n_local && w13.size(1) == 2 * sh_.inter &&
+    MOE_CHECK(ok(w13, type) && w13.dim() == 3 && w13.size(0) == sh_.n_local && w13.size(1) == 2 * sh_.inter &&
                   w13.size(2) == sh_.hidden,
-              "w13 must be contiguous bf16 [n_local, 2*inter, hidden] on this device");
-    MOE_CHECK(ok(w2) && w2.dim() == 3 && w2.size(0) == sh_.n_local && w2.size(1) == sh_.hidden &&
+              "w13 must be contiguous " << type << " [n_local, 2*inter, hidden] on this device");
+    MOE_CHECK(ok(w2, type) && w2.dim() == 3 && w2.size(0) == sh_.n_local && w2.size(1) == sh_.hidden &&
                   w2.size(2) == sh_.inter,
-              "w2 must be contiguous bf16 [n_local, hidden, inter] on this device");
+              "w2 must be contiguous " << type << " [n_local, hidden, inter] on this device");
+    auto scale_ok = [&](const std::optional<torch::Tensor>& s, const torch::Tensor& w) {
+      return s && ok(*s, torch::kFloat8_e8m0fnu) && s->dim() == 3 && s->size(0) == w.size(0) && s->size(1) == w.size(1) / 128 &&
+             s->size(2) == w.size(2) / 128;
+    };
+    MOE_CHECK(sh_.fp8 ? scale_ok(w13_scale, w13) && scale_ok(w2_scale, w2) : !w13_scale && !w2_scale,
+              "weights in 8 bits, and only they, come with contiguous scales [n_local, rows / 128, cols / 128] on this device");
+    if (sh_.fp8) {
+      w13_scale_ = *w13_scale;
+      w2_scale_ = *w2_scale;
+      buf_.w13_scale = static_cast<const uint8_t*>(w13_scale_.data_ptr());
+      buf_.w2_scale = static_cast<const uint8_t*>(w2_scale_.data_ptr());
+    }
     w13_ = w13;
     w2_ = w2;
     c10::cuda::CUDAGuard guard(device_);
     int rc = lplb::moe::make_gemm_maps(&maps1_, buf_.recv_x[sh_.my_rank], sh_.capacity, w13.data_ptr(),
-                                       (uint64_t)sh_.n_local * 2 * sh_.inter, sh_.hidden, true);
+                                       (uint64_t)sh_.n_local * 2 * sh_.inter, sh_.hidden, true, sh_.fp8);
     MOE_CHECK(rc == 0, "tensor maps for the receive buffer and w13 failed with code " << rc);
     rc = lplb::moe::make_gemm_maps(&maps2_, act_.data_ptr(), sh_.capacity, w2.data_ptr(),
-                                   (uint64_t)sh_.n_local * sh_.hidden, sh_.inter, false);
+                                   (uint64_t)sh_.n_local * sh_.hidden, sh_.inter, false, sh_.fp8);
     MOE_CHECK(rc == 0, "tensor maps for the activation buffer and w2 failed with code " << rc);
     have_weights_ = true;
   }
 
-  // One forward pass.  x: [T, hidden] bf16, phys_idx: [T, topk] int64/int32 physical expert
-  // ids (-1 = dropped), weights: [T, topk] float32.  `upto` stops after a stage for tests:
+  // One forward pass.  x: [T, hidden] bf16 (an engine in 8 bits also takes e4m3 with x_scale), phys_idx: [T, topk]
+  // int64/int32 physical expert ids (-1 = dropped), weights: [T, topk] float32.  `upto` stops after a stage for tests:
   // 1 route (counts and plan), 2 dispatch, 3 first GEMM, 4 second GEMM, 5 (default) everything.
   torch::Tensor forward(const torch::Tensor& x, const torch::Tensor& phys_idx, const torch::Tensor& weights,
-                        int n_cta, int upto, bool fuse_dispatch) {
+                        int n_cta, int upto, bool fuse_dispatch, const std::optional<torch::Tensor>& x_scale) {
     MOE_CHECK(ready_ && have_weights_, "engine is not ready: open peers and set weights first");
-    MOE_CHECK(x.is_cuda() && x.scalar_type() == torch::kBFloat16 && x.is_contiguous() && x.dim() == 2 &&
+    MOE_CHECK(!x_scale || sh_.fp8, "x_scale needs weights in 8 bits");
+    const auto x_type = x_scale ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+    MOE_CHECK(x.is_cuda() && x.scalar_type() == x_type && x.is_contiguous() && x.dim() == 2 &&
                   x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
-              "x must be contiguous bf16 [tokens <= max_tokens, hidden]");
+              "x must be contiguous " << x_type << " [tokens <= max_tokens, hidden]");
     const int n_tokens = (int)x.size(0);
+    MOE_CHECK(!x_scale || (x_scale->is_cuda() && x_scale->is_contiguous() && x_scale->scalar_type() == torch::kFloat8_e8m0fnu &&
+                           x_scale->dim() == 2 && x_scale->size(0) == n_tokens && x_scale->size(1) == sh_.hidden / 128),
+              "x_scale must be contiguous float8_e8m0fnu [tokens, hidden / 128]");
+    MOE_CHECK(!(fuse_dispatch && sh_.fp8), "the fused dispatch sends bf16 rows only");
     MOE_CHECK(phys_idx.is_cuda() && phys_idx.is_contiguous() && phys_idx.numel() == (int64_t)n_tokens * sh_.topk &&
                   (phys_idx.scalar_type() == torch::kInt64 || phys_idx.scalar_type() == torch::kInt32),
               "phys_idx must be contiguous int64/int32 [tokens, topk]");
@@ -178,7 +203,7 @@ class MoeEngine {
     c10::cuda::CUDAGuard guard(device_);
     cudaStream_t s = c10::cuda::getCurrentCUDAStream(device_).stream();
     const int is64 = phys_idx.scalar_type() == torch::kInt64;
-    auto out = torch::empty({n_tokens, sh_.hidden}, x.options());
+    auto out = torch::empty({n_tokens, sh_.hidden}, x.options().dtype(torch::kBFloat16));
     // The fused path cannot stop between dispatch and the first GEMM: stage 2 then means both.
     const bool fused = fuse_dispatch && upto >= 3;
     lplb::moe::FusedGrid grid{};
@@ -195,7 +220,8 @@ class MoeEngine {
       MOE_CUDA(lplb::moe::launch_schedule(sh_, buf_, phys_idx.data_ptr(), is64, n_tokens, s));
       MOE_CUDA(lplb::moe::launch_dispatch_gemm(sh_, buf_, maps1_, x.data_ptr(), epoch_, timeout_ns_, grid, s));
     } else {
-      MOE_CUDA(lplb::moe::launch_dispatch(sh_, buf_, x.data_ptr(), phys_idx.data_ptr(), is64, n_tokens,
+      MOE_CUDA(lplb::moe::launch_dispatch(sh_, buf_, x.data_ptr(), x_scale ? static_cast<const uint8_t*>(x_scale->data_ptr()) : nullptr,
+                                          phys_idx.data_ptr(), is64, n_tokens,
                                           4 * n_cta, epoch_, s));
       if (upto <= 2) return out;
       MOE_CUDA(lplb::moe::launch_gemm(sh_, buf_, maps1_, 0, epoch_, timeout_ns_, gemm_ctas(), s));
@@ -262,7 +288,7 @@ class MoeEngine {
 
   // Views of this rank's peer-visible buffers (for tests).
   torch::Tensor recv_x() const {
-    auto opts = torch::TensorOptions().dtype(torch::kBFloat16).device(torch::kCUDA, device_);
+    auto opts = torch::TensorOptions().dtype(sh_.fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16).device(torch::kCUDA, device_);
     return torch::from_blob(buf_.recv_x[sh_.my_rank], {sh_.capacity, sh_.hidden}, opts);
   }
   torch::Tensor recv_meta() const {
@@ -285,6 +311,7 @@ class MoeEngine {
     for (int r = 0; r < sh_.n_ranks; ++r) {
       char* base = bases_[r];
       buf_.recv_x[r] = base + off_recv_x_;
+      buf_.recv_scale[r] = reinterpret_cast<uint8_t*>(base + off_scale_);
       buf_.recv_meta[r] = reinterpret_cast<int*>(base + off_meta_);
       buf_.comb[r] = base + off_comb_;
       buf_.cnt_words[r] = reinterpret_cast<unsigned long long*>(base + off_cnt_);
@@ -292,6 +319,7 @@ class MoeEngine {
       buf_.arrived[r] = reinterpret_cast<uint32_t*>(base + off_arrived_);
     }
     buf_.act = act_.data_ptr();
+    buf_.act_scale = sh_.fp8 ? static_cast<uint8_t*>(act_scale_.data_ptr()) : nullptr;
     buf_.plan = plan_.data_ptr<int>();
     buf_.ordinal = ordinal_.data_ptr<int>();
     buf_.totals = totals_.data_ptr<int>();
@@ -307,11 +335,12 @@ class MoeEngine {
   lplb::moe::LayerShape sh_{};
   lplb::moe::LayerBuffers buf_{};
   int device_, p_ = 0, sms_ = 0, resident_pairs_ = 0;
-  size_t off_recv_x_ = 0, off_meta_ = 0, off_comb_ = 0, off_cnt_ = 0, off_flags_ = 0, off_arrived_ = 0, block_bytes_ = 0;
+  size_t off_recv_x_ = 0, off_scale_ = 0, off_meta_ = 0, off_comb_ = 0, off_cnt_ = 0, off_flags_ = 0, off_arrived_ = 0, block_bytes_ = 0;
   void* block_ = nullptr;
   std::vector<char*> bases_;
   std::vector<void*> opened_;
-  torch::Tensor act_, plan_, totals_, ordinal_, tickets_, status_, pair_slot_, send_pair_, send_target_, debug_, w13_, w2_;
+  torch::Tensor act_, plan_, totals_, ordinal_, tickets_, status_, pair_slot_, send_pair_, send_target_, debug_, w13_, w2_,
+      act_scale_, w13_scale_, w2_scale_;
   lplb::moe::GemmMaps maps1_{}, maps2_{};
   bool ready_ = false, have_weights_ = false;
   uint32_t epoch_ = 0;
@@ -327,16 +356,17 @@ void bind_moe(py::module_& m) {
     return py::make_tuple(grid.tile, grid.send);
   });
   py::class_<MoeEngine>(m, "MoeEngine")
-      .def(py::init<int, int, int, int, int, int, int, int, int>(), py::arg("hidden"), py::arg("inter"),
+      .def(py::init<int, int, int, int, int, int, int, int, int, bool>(), py::arg("hidden"), py::arg("inter"),
            py::arg("n_local"), py::arg("n_ranks"), py::arg("my_rank"), py::arg("topk"), py::arg("max_tokens"),
-           py::arg("capacity"), py::arg("device"))
+           py::arg("capacity"), py::arg("device"), py::arg("fp8") = false)
       .def("peer_block_bytes", &MoeEngine::peer_block_bytes)
       .def("alloc", &MoeEngine::alloc)
       .def("open", &MoeEngine::open)
       .def("close", &MoeEngine::close)
-      .def("set_weights", &MoeEngine::set_weights)
+      .def("set_weights", &MoeEngine::set_weights, py::arg("w13"), py::arg("w2"), py::arg("w13_scale") = py::none(),
+           py::arg("w2_scale") = py::none())
       .def("forward", &MoeEngine::forward, py::arg("x"), py::arg("phys_idx"), py::arg("weights"), py::arg("n_cta"),
-           py::arg("upto") = 5, py::arg("fuse_dispatch") = false)
+           py::arg("upto") = 5, py::arg("fuse_dispatch") = false, py::arg("x_scale") = py::none())
       .def("capturing", &MoeEngine::capturing)
       .def("set_timeout_us", &MoeEngine::set_timeout_us)
       .def("set_send_ctas", &MoeEngine::set_send_ctas)

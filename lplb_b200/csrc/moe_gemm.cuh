@@ -47,6 +47,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "fp8.cuh"
 #include "scale_words.cuh"
 #include "tcgen05.cuh"
 
@@ -141,6 +142,7 @@ struct GemmArgs {
   int topk, hidden;
   int send_ctas;
   // operands in 8 bits
+  uint8_t* act_scale;            // kSwiGLU: [capacity, act_ld / 128]
   const uint8_t* w_scale;        // [experts * w_blocks, k_blocks]
   const uint8_t* row_scale;      // [n_rows, row_scale_ld]
   int64_t row_scale_ld;
@@ -268,14 +270,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   const uint32_t bar_tfull = smem_u32(bars + 2 * kMaxStages), bar_tempty = smem_u32(bars + 2 * kMaxStages + 2);
   const uint32_t bar_tile = smem_u32(bars + 2 * kMaxStages + 4);
   const uint32_t bar_sfull = bar_tile + 8 * kTileSlots, bar_sempty = bar_sfull + 8 * kScaleSlots;  // FP8; sfull in the first CTA only
+  const uint32_t bar_top = bar_sempty + 8 * kScaleSlots;  // FP8, kSwiGLU: both turns' largest magnitudes are there
   uint8_t* smem_scales = smem_turn + 2 * kTurnBytes;  // FP8
-  static_assert((2 * kMaxStages + 4 + kTileSlots + 2 * kScaleSlots) * 8 <= kBarBytes, "barriers");
+  static_assert((2 * kMaxStages + 4 + kTileSlots + 2 * kScaleSlots + 2) * 8 <= kBarBytes, "barriers");
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int s_flags_ok;
   __shared__ int s_tile[kTileSlots];
   __shared__ int s_rows[kMaxLocalExperts], s_start[kMaxLocalExperts];
   __shared__ unsigned long long s_dst[EPI == kScatter ? 2 * kBN : 1];
+  __shared__ uint32_t s_top[EPI == kSwiGLU && FP8 ? 2 : 1][8][32];  // largest magnitudes of 32 rows, by the pair's epilogue warps
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = (int)cluster_cta_rank();  // which CTA of the pair
@@ -304,6 +308,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         mbar_init(bar_sfull + 8 * s, 2);  // the scale warps of both CTAs
         mbar_init(bar_sempty + 8 * s, 1);
       }
+      for (int b = 0; b < 2; ++b) mbar_init(bar_top + 8 * b, 8);  // four epilogue warps of either CTA
     }
     fence_barrier_init();
     tma_prefetch_desc(&tmap_w);
@@ -579,7 +584,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;  // TMEM lanes 32*quarter .. +31 are the ones this warp may read
     const int et = threadIdx.x - 64;
-    uint32_t turn = 0;
+    uint32_t turn = 0, top_ph[2] = {0, 0};
+    bool lost = false;
     for (uint32_t tile_n = 0;; ++tile_n) {
       // All four warps leave the loop together: they meet at barriers below, and tcgen05.ld is a
       // whole-warp instruction.  A thread that gave up a wait finds no tile.
@@ -634,6 +640,59 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         tmem_ld_16x32(taddr + (16u << 16) + c0, b);  // lanes 16-31
         tmem_ld_wait();
         if constexpr (EPI == kSwiGLU) {
+         if constexpr (FP8) {
+          // 128 features of a row share a scale, 64 of them in either CTA: every warp tells all eight the largest magnitudes of
+          // its 16 features, a column per lane.
+          float v[16];
+          uint32_t top[8];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = silu(__uint_as_float(a[j])) * __uint_as_float(b[j]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // columns 8 * (j / 2) + 2 * (lane % 4) + j % 2; features lane / 4 and that + 8
+            const int i = 4 * (j / 2) + j % 2;
+            top[j] = max(fp8::magnitude(v[i]), fp8::magnitude(v[i + 2]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+          }
+          // lane c: the value of column c, which lanes c % 8 / 2 + 4 * n hold in top[2 * (c / 8) + c % 2]
+          uint32_t mine_max = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t from = __shfl_sync(0xffffffffu, top[j], (lane & 7) >> 1);
+            if (j == 2 * (lane >> 3) + (lane & 1)) mine_max = from;
+          }
+          const uint32_t slot = smem_u32(&s_top[turn][half * 4 + quarter][lane]);
+          st_cluster(map_to_rank(slot, 0), (int)mine_max);
+          st_cluster(map_to_rank(slot, 1), (int)mine_max);
+          __syncwarp();
+          if (lane < 2) mbar_arrive_remote(map_to_rank(bar_top + 8 * turn, lane));
+          if (!epilogue_all(mbar_wait_cluster(bar_top + 8 * turn, top_ph[turn], abort, budget))) {
+            lost = true;
+            break;
+          }
+          top_ph[turn] ^= 1;
+          uint32_t largest_of = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) largest_of = max(largest_of, s_top[turn][j][lane]);
+          const uint32_t e = fp8::scale_exponent(largest_of);
+          if (half == 0 && quarter == 0 && c0 + lane < left)
+            args.act_scale[(row0 + c0 + lane) * (size_t)(args.act_ld / 128) + cur.w] = (uint8_t)e;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int c = 8 * (j / 2) + 2 * (lane & 3) + (j & 1), i = 4 * (j / 2) + j % 2;
+            const float r = fp8::reciprocal_of(__shfl_sync(0xffffffffu, e, c));
+            const uint32_t two = fp8::pack2(fp8::scaled(v[i], r), fp8::scaled(v[i + 2], r));
+            uint8_t* to = stage + c * 64 + 16 * quarter + (lane >> 2);
+            to[0] = (uint8_t)two;
+            to[8] = (uint8_t)(two >> 8);
+          }
+          epilogue_sync();
+          const int r = et >> 2, chunk = et & 3;
+          const uint4 out = *reinterpret_cast<const uint4*>(stage + r * 64 + chunk * 16);
+          if (c0 + r < left)
+            st_global_v4(reinterpret_cast<uint8_t*>(args.act) + (row0 + c0 + r) * args.act_ld + (size_t)cur.w * (kBM / 2) + half * (kCtaM / 2) + chunk * 16,
+                         out.x, out.y, out.z, out.w);
+         } else {
           uint32_t o[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -652,6 +711,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4));
             if (c0 + r < left) st_global_v4(dst + (size_t)r * args.act_ld + chunk * 8, v.x, v.y, v.z, v.w);
           }
+         }
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -683,6 +743,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           }
         }
       }
+      if (lost) break;
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(map_to_rank(bar_tempty + 8 * acc, 0));

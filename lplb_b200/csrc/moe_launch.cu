@@ -22,14 +22,15 @@ bool shape_ok(const LayerShape& sh) {
 
 namespace {
 int encode_map(CUtensorMap* out, const void* base, uint32_t rank, const cuuint64_t* dims, const cuuint64_t* strides,
-               const cuuint32_t* box) {
-  return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides, box);
+               const cuuint32_t* box, bool fp8) {
+  return encode_tensor_map(out, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides, box);
 }
-int row_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+int row_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, bool fp8) {
+  const uint64_t size = fp8 ? 1 : 2;  // a k block is 128 bytes of a row
   const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {cols * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows};
-  return encode_map(out, base, 2, dims, strides, box);
+  const cuuint64_t strides[1] = {cols * size};
+  const cuuint32_t box[2] = {(cuuint32_t)(2 * kBK / size), box_rows};
+  return encode_map(out, base, 2, dims, strides, box, fp8);
 }
 // The gate/up weight tensor as [256-row block][group of 16][gate, up][16 rows][cols]: a box of four
 // groups arrives in shared memory as 16 gate rows, their 16 up rows, the next 16 gate rows, ...
@@ -37,20 +38,22 @@ int row_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, ui
 // every stride a multiple of the one before.  The encoder takes the map as it is, and set_weights
 // reports the code where one should refuse it.  With ascending strides either the layout that callers
 // lay their weights out in would change, or a stage would take four boxes instead of one.
-int gate_up_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols) {
-  const cuuint64_t row = cols * 2;
+int gate_up_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, bool fp8) {
+  const uint64_t size = fp8 ? 1 : 2;
+  const cuuint64_t row = cols * size;
   const cuuint64_t dims[5] = {cols, kGateRows, 2, kGateBlock / kGateRows, rows / (2 * kGateBlock)};
   const cuuint64_t strides[4] = {row, kGateBlock * row, kGateRows * row, 2 * kGateBlock * row};
-  const cuuint32_t box[5] = {(cuuint32_t)kBK, kGateRows, 2, kCtaM / (2 * kGateRows), 1};
-  return encode_map(out, base, 5, dims, strides, box);
+  const cuuint32_t box[5] = {(cuuint32_t)(2 * kBK / size), kGateRows, 2, kCtaM / (2 * kGateRows), 1};
+  return encode_map(out, base, 5, dims, strides, box, fp8);
 }
 }  // namespace
 
 int make_gemm_maps(GemmMaps* out, const void* tokens, uint64_t rows, const void* weights, uint64_t weight_rows,
-                   uint64_t cols, bool gate_up) {
+                   uint64_t cols, bool gate_up, bool fp8) {
   int rc = 0;
-  for (int b = 0; b < kRowBoxes && rc == 0; ++b) rc = row_map(&out->rows[b], tokens, rows, cols, kBN / 2 >> b);
-  if (rc == 0) rc = gate_up ? gate_up_map(&out->w, weights, weight_rows, cols) : row_map(&out->w, weights, weight_rows, cols, kCtaM);
+  for (int b = 0; b < kRowBoxes && rc == 0; ++b) rc = row_map(&out->rows[b], tokens, rows, cols, kBN / 2 >> b, fp8);
+  if (rc == 0)
+    rc = gate_up ? gate_up_map(&out->w, weights, weight_rows, cols, fp8) : row_map(&out->w, weights, weight_rows, cols, kCtaM, fp8);
   return rc;
 }
 
@@ -103,17 +106,20 @@ cudaError_t launch_route(const LayerShape& sh, const LayerBuffers& b, const void
   return launch_after(route_kernel, (unsigned)grid, kSupportThreads, sizeof(int) * 4 * P, stream, a);
 }
 
-cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const void* x, const void* phys_idx,
+cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const void* x, const uint8_t* x_scale, const void* phys_idx,
                             int idx_is64, int n_tokens, int n_cta, uint32_t epoch, cudaStream_t stream) {
   if (!shape_ok(sh) || n_cta < 1 || n_tokens < 0 || n_tokens > sh.max_tokens) return cudaErrorInvalidValue;
   const PlanView plan = plan_view(sh, b);
   DispatchArgs a{};
+  if (x_scale != nullptr && !sh.fp8) return cudaErrorInvalidValue;
   for (int r = 0; r < sh.n_ranks; ++r) {
-    a.recv_x[r] = static_cast<__nv_bfloat16*>(b.recv_x[r]);
+    a.recv_x[r] = static_cast<uint8_t*>(b.recv_x[r]);
+    a.recv_scale[r] = b.recv_scale[r];
     a.recv_meta[r] = b.recv_meta[r];
     a.flags[r] = b.flags[r];
   }
-  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.x = x;
+  a.x_scale = x_scale;
   a.idx = phys_idx;
   a.ordinal = b.ordinal;
   a.dst_row_start = plan.dst_row_start;
@@ -130,7 +136,7 @@ cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const v
   a.my_rank = sh.my_rank;
   a.capacity = sh.capacity;
   a.epoch = epoch;
-  return launch_after(dispatch_kernel, n_cta, kSupportThreads, 0, stream, a);
+  return launch_after(sh.fp8 ? dispatch_kernel<true> : dispatch_kernel<false>, n_cta, kSupportThreads, 0, stream, a);
 }
 
 cudaError_t launch_schedule(const LayerShape& sh, const LayerBuffers& b, const void* phys_idx, int idx_is64,
@@ -183,7 +189,7 @@ cudaError_t fused_resident_pairs(int* pairs) {
 
 cudaError_t launch_dispatch_gemm(const LayerShape& sh, const LayerBuffers& b, const GemmMaps& maps, const void* x, uint32_t epoch,
                                  unsigned long long timeout_ns, FusedGrid grid, cudaStream_t stream) {
-  if (!shape_ok(sh) || grid.tile < 2 || grid.tile % 2 || grid.send < 0 || grid.send % 2) return cudaErrorInvalidValue;
+  if (!shape_ok(sh) || sh.fp8 || grid.tile < 2 || grid.tile % 2 || grid.send < 0 || grid.send % 2) return cudaErrorInvalidValue;
   const PlanView plan = plan_view(sh, b);
   GemmArgs a{};
   a.send_ctas = grid.send;
@@ -236,21 +242,28 @@ cudaError_t launch_gemm(const LayerShape& sh, const LayerBuffers& b, const GemmM
   a.epoch = epoch;
   a.status = b.status;
   a.timeout_ns = timeout_ns;
-  cudaError_t err;
+  const int per = sh.fp8 ? 2 * kBK : kBK;  // values of a k block
+  a.n_rows = sh.capacity;
+  auto go = [&](auto kernel, int threads, size_t smem) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return err;
+    return launch_after(kernel, n_cta, threads, smem, stream, maps.w, row_maps(maps), a);
+  };
   if (which == 0) {
     a.n_tiles_w = 2 * sh.inter / kBM;
-    a.k_blocks = sh.hidden / kBK;
+    a.k_blocks = sh.hidden / per;
     a.act = static_cast<__nv_bfloat16*>(b.act);
     a.act_ld = sh.inter;
     a.wait_flags = sh.n_ranks > 1 ? b.flags[sh.my_rank] : nullptr;  // dispatch done, one word per source rank
     a.ticket = b.tickets + 1;
-    auto kernel = grouped_gemm_kernel<kSwiGLU, false>;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmSmem);
-    if (err != cudaSuccess) return err;
-    return launch_after(kernel, n_cta, kGemmThreads, kGemmSmem, stream, maps.w, row_maps(maps), a);
+    if (!sh.fp8) return go(grouped_gemm_kernel<kSwiGLU, false>, kGemmThreads, kGemmSmem);
+    a.act_scale = b.act_scale;
+    a.w_scale = b.w13_scale;
+    a.w_rows = 2 * sh.inter;
+    a.row_scale = b.recv_scale[sh.my_rank];
   } else {
     a.n_tiles_w = sh.hidden / kBM;
-    a.k_blocks = sh.inter / kBK;
+    a.k_blocks = sh.inter / per;
     a.meta = b.recv_meta[sh.my_rank];
     for (int r = 0; r < sh.n_ranks; ++r) {
       a.comb[r] = static_cast<__nv_bfloat16*>(b.comb[r]);
@@ -259,11 +272,16 @@ cudaError_t launch_gemm(const LayerShape& sh, const LayerBuffers& b, const GemmM
     a.out_ld = sh.hidden;
     a.wait_flags = nullptr;
     a.ticket = b.tickets + 2;
-    auto kernel = grouped_gemm_kernel<kScatter, false>;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemmSmem);
-    if (err != cudaSuccess) return err;
-    return launch_after(kernel, n_cta, kGemmThreads, kGemmSmem, stream, maps.w, row_maps(maps), a);
+    if (!sh.fp8) return go(grouped_gemm_kernel<kScatter, false>, kGemmThreads, kGemmSmem);
+    a.w_scale = b.w2_scale;
+    a.w_rows = sh.hidden;
+    a.row_scale = b.act_scale;
   }
+  a.w_blocks = a.w_rows / 128;
+  a.row_scale_ld = a.k_blocks;
+  a.scale_words = a.k_blocks % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w_scale) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.row_scale) & 3) == 0;
+  if (which == 0) return go(grouped_gemm_kernel<kSwiGLU, false, true>, kGemmThreadsFp8, kGemmSmemFp8);
+  return go(grouped_gemm_kernel<kScatter, false, true>, kGemmThreadsFp8, kGemmSmemFp8);
 }
 
 cudaError_t launch_combine(const LayerShape& sh, const LayerBuffers& b, const float* weights, void* out, int n_tokens,

@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "fp8.cuh"
 #include "moe_gemm.cuh"
 
 namespace lplb {
@@ -271,10 +272,12 @@ __global__ void __launch_bounds__(kSupportThreads) schedule_kernel(const Schedul
 }
 
 struct DispatchArgs {
-  __nv_bfloat16* recv_x[kMaxRanks];  // per rank: [capacity, hidden]
+  uint8_t* recv_x[kMaxRanks];        // per rank: [capacity, hidden] bf16 or e4m3
+  uint8_t* recv_scale[kMaxRanks];    // FP8, per rank: [capacity, hidden / 128]
   int* recv_meta[kMaxRanks];         // per rank: [capacity]
   uint32_t* flags[kMaxRanks];        // per rank: uint32 [2][n_ranks]
-  const __nv_bfloat16* x;            // [tokens, hidden] local hidden states
+  const void* x;                     // [tokens, hidden] local hidden states: bf16, or e4m3 with x_scale
+  const uint8_t* x_scale;            // FP8: [tokens, hidden / 128], or null
   const void* idx;                   // [tokens * topk] physical expert ids, -1 = skip
   const int* ordinal;                // [tokens * topk] from route_kernel
   const int* dst_row_start;          // [P]
@@ -303,7 +306,12 @@ constexpr int kDispatchVec = 4;  // 16-byte vectors per lane and work item: an i
 // of this rank's return buffer.  Consecutive rows of an expert therefore come back to
 // consecutive slots: the stores that cross NVLink walk through memory sequentially instead of
 // hitting a random page per row.
+//
+// FP8: rows travel in 8 bits with a scale per 128 values, half the bytes over NVLink; a bf16 row is converted
+// where its piece is loaded, once for all its pairs (16 lanes hold 128 values).
+template <bool FP8>
 __global__ void __launch_bounds__(kSupportThreads) dispatch_kernel(const DispatchArgs a) {
+  using Vec = std::conditional_t<FP8, uint2, uint4>;  // eight values
   allow_successor();
   wait_predecessors();
   const int P = a.n_ranks * a.n_local;
@@ -313,11 +321,30 @@ __global__ void __launch_bounds__(kSupportThreads) dispatch_kernel(const Dispatc
   const int n_items = a.n_tokens * pieces, n_warps = gridDim.x * (kSupportThreads / 32);
   for (int item = blockIdx.x * (kSupportThreads / 32) + warp; item < n_items; item += n_warps) {
     const int tok = item / pieces, v0 = (item - tok * pieces) * 32 * kDispatchVec + lane;
-    const uint4* src = reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.hidden);
-    uint4 q[kDispatchVec];
+    Vec q[kDispatchVec];
+    uint8_t scale[kDispatchVec];
+    if (!FP8 || a.x_scale != nullptr) {
+      const Vec* src = static_cast<const Vec*>(a.x) + (size_t)tok * vec_per_row;
 #pragma unroll
-    for (int u = 0; u < kDispatchVec; ++u)
-      if (v0 + 32 * u < vec_per_row) q[u] = __ldg(&src[v0 + 32 * u]);
+      for (int u = 0; u < kDispatchVec; ++u)
+        if (v0 + 32 * u < vec_per_row) {
+          q[u] = __ldg(&src[v0 + 32 * u]);
+          if (FP8) scale[u] = a.x_scale[(size_t)tok * (vec_per_row / 16) + (v0 + 32 * u) / 16];
+        }
+    } else if constexpr (FP8) {
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.x) + (size_t)tok * a.hidden;
+      fp8::Eight<__nv_bfloat16> raw[kDispatchVec];
+#pragma unroll
+      for (int u = 0; u < kDispatchVec; ++u) raw[u] = fp8::load_raw<true>(src + (v0 + 32 * u) * 8, vec_per_row - (v0 + 32 * u));
+#pragma unroll
+      for (int u = 0; u < kDispatchVec; ++u) {
+        float2 f[4];
+        fp8::unpack(raw[u], f);
+        const uint32_t e = fp8::scale_exponent(fp8::block_max(fp8::magnitude8(f)));
+        q[u] = fp8::pack8(f, fp8::reciprocal_of(e), fp8::all_finite(f));
+        scale[u] = (uint8_t)e;
+      }
+    }
     for (int k0 = 0; k0 < a.topk; k0 += 32) {
       const int nk = min(32, a.topk - k0);
       int t = -1;
@@ -345,10 +372,14 @@ __global__ void __launch_bounds__(kSupportThreads) dispatch_kernel(const Dispatc
       for (int k = 0; k < nk; ++k) {
         const int tg = __shfl_sync(0xffffffffu, t, k);
         if (tg < 0) continue;
-        uint4* dst = reinterpret_cast<uint4*>(a.recv_x[tg >> 24] + (size_t)(tg & 0xFFFFFF) * a.hidden);
+        Vec* dst = reinterpret_cast<Vec*>(a.recv_x[tg >> 24]) + (size_t)(tg & 0xFFFFFF) * vec_per_row;
 #pragma unroll
         for (int u = 0; u < kDispatchVec; ++u)
-          if (v0 + 32 * u < vec_per_row) dst[v0 + 32 * u] = q[u];
+          if (v0 + 32 * u < vec_per_row) {
+            dst[v0 + 32 * u] = q[u];
+            if (FP8 && (lane & 15) == 0)
+              a.recv_scale[tg >> 24][(size_t)(tg & 0xFFFFFF) * (vec_per_row / 16) + (v0 + 32 * u) / 16] = scale[u];
+          }
       }
     }
   }

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import torch
 
+from .. import ops
 from ..planner import Planner
 
 __all__ = ["MoELayer", "interleave_gate_up"]
@@ -40,6 +41,11 @@ class MoELayer:
     A forward pass cannot be captured in a CUDA graph (``RuntimeError``).
     Weights are random-init and derived from a per-logical-expert seed, so a replica holds
     the same values as its original without any weight traffic.
+
+    ``weight_dtype=torch.float8_e4m3fn`` holds the weights in 8 bits with a power-of-two scale for every 128 x 128
+    of them; hidden states then travel, and activations are held, in 8 bits with a scale per 128 values
+    (see ``lplb_b200.ops.fp8``).  ``few_tokens = True`` has passes of up to 64 tokens on one GPU take
+    ``ops.moe_few_tokens``: two kernels instead of five.
     """
 
     def __init__(
@@ -54,6 +60,7 @@ class MoELayer:
         seed: int = 0,
         weight_scale: float | None = None,
         capacity_rows: int | None = None,
+        weight_dtype: torch.dtype = torch.bfloat16,
     ) -> None:
         """``capacity_rows`` sets the receive buffer's size in rows directly (rounded up to a
         multiple of 128) instead of deriving it from ``max_tokens * topk * capacity_factor``.
@@ -62,6 +69,8 @@ class MoELayer:
         pairs they are is not fixed."""
         from .. import _native
 
+        if weight_dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"weight_dtype must be bfloat16 or float8_e4m3fn, not {weight_dtype}")
         if planner.device.type != "cuda":
             raise RuntimeError("MoELayer needs a CUDA device")
         native = _native.load()
@@ -70,6 +79,7 @@ class MoELayer:
         self.device = planner.device
         self.group = group
         self.seed = seed
+        self.weight_dtype = weight_dtype
         self.weight_scale = weight_scale if weight_scale is not None else hidden**-0.5
         if group is None:
             self.n_ranks, self.rank = 1, 0
@@ -88,7 +98,8 @@ class MoELayer:
         capacity = int(-(-max(1, int(wanted)) // 128) * 128)
         self.capacity = capacity
         self.engine = native.MoeEngine(
-            hidden, inter, self.n_local, self.n_ranks, self.rank, topk, max_tokens, capacity, self.device.index
+            hidden, inter, self.n_local, self.n_ranks, self.rank, topk, max_tokens, capacity, self.device.index,
+            weight_dtype == torch.float8_e4m3fn,
         )
         handle = bytes(self.engine.alloc())
         if group is None:
@@ -102,6 +113,7 @@ class MoELayer:
         if group is not None:
             dist.barrier(group=group)
         self.fuse_dispatch = False
+        self.few_tokens = False
         self.send_ctas = 0  # fused dispatch only: this many CTAs send rows and run no tiles (0: sender warps in every CTA)
         self._n_sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._placed_for: torch.Tensor | None = None
@@ -123,14 +135,26 @@ class MoELayer:
         phy2log = self.planner.phy2log
         first = self.rank * self.n_local
         mine = phy2log[first : first + self.n_local].tolist()
-        w13 = torch.empty(self.n_local, 2 * self.inter, self.hidden, dtype=torch.bfloat16, device=self.device)
-        w2 = torch.empty(self.n_local, self.hidden, self.inter, dtype=torch.bfloat16, device=self.device)
+        w13 = torch.empty(self.n_local, 2 * self.inter, self.hidden, dtype=self.weight_dtype, device=self.device)
+        w2 = torch.empty(self.n_local, self.hidden, self.inter, dtype=self.weight_dtype, device=self.device)
+        w13_scale = w2_scale = None
+        if self.weight_dtype == torch.float8_e4m3fn:
+            w13_scale, w2_scale = (
+                torch.empty(n, rows // 128, cols // 128, dtype=torch.float8_e8m0fnu, device=self.device)
+                for n, rows, cols in (w13.shape, w2.shape)
+            )
         for slot, expert in enumerate(mine):
             gate, up, down = self.logical_weights(expert)
-            w13[slot] = interleave_gate_up(gate, up)
-            w2[slot] = down
-        self.w13, self.w2 = w13, w2
-        self.engine.set_weights(w13, w2)
+            if w13_scale is None:
+                w13[slot] = interleave_gate_up(gate, up)
+                w2[slot] = down
+            else:
+                for made, values, scales in ((interleave_gate_up(gate, up), w13, w13_scale), (down, w2, w2_scale)):
+                    q, scale = ops.quantize_weight_fp8(made)
+                    values[slot].copy_(q)
+                    scales[slot].copy_(scale)
+        self.w13, self.w2, self.w13_scale, self.w2_scale = w13, w2, w13_scale, w2_scale
+        self.engine.set_weights(w13, w2, w13_scale, w2_scale)
         self._placed_for = phy2log.clone()
         self._placed_version = self.planner.placement_version()
 
@@ -149,11 +173,19 @@ class MoELayer:
 
     # ------------------------------------------------------------------ forward
     def forward_physical(
-        self, x: torch.Tensor, phys_idx: torch.Tensor, weights: torch.Tensor, upto: int = 5, fuse_dispatch: bool | None = None
+        self,
+        x: torch.Tensor,
+        phys_idx: torch.Tensor,
+        weights: torch.Tensor,
+        upto: int = 5,
+        fuse_dispatch: bool | None = None,
+        x_scale: torch.Tensor | None = None,
     ):
         """Run the layer on physical expert ids.  ``fuse_dispatch`` (default: the layer's
         setting) sends the rows from inside the first GEMM kernel, so the tensor cores start on
-        an expert as soon as its rows have landed instead of after the whole dispatch."""
+        an expert as soon as its rows have landed instead of after the whole dispatch (bf16 weights only).
+        A layer with weights in 8 bits also takes ``x`` in 8 bits with its ``x_scale``, as
+        ``ops.rms_norm_fp8`` and ``ops.quantize_fp8`` give them; bf16 ``x`` is converted on its way."""
         # A replay would skip the comparison below, run on weights that place_weights() has replaced
         # since, and repeat a launch number that the ranks must not see twice.
         if self.engine.capturing():
@@ -165,21 +197,30 @@ class MoELayer:
             if self._placed_for is None or not torch.equal(self._placed_for, self.planner.phy2log):
                 raise RuntimeError("expert placement changed: call place_weights() first")
             self._placed_version = version
+        if self.few_tokens and self.n_ranks == 1 and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS and self.topk <= 32:
+            return ops.moe_few_tokens(
+                x, phys_idx.view(x.shape[0], self.topk), weights.view(x.shape[0], self.topk), self.w13, self.w2,
+                x_scale, self.w13_scale, self.w2_scale,
+            )
         n_cta = self._n_sms
         fuse = self.fuse_dispatch if fuse_dispatch is None else fuse_dispatch
         if fuse:
             self.engine.set_send_ctas(int(self.send_ctas))
-        return self.engine.forward(x.contiguous(), phys_idx.contiguous(), weights.float().contiguous(), n_cta, upto, fuse)
+        if x_scale is not None:
+            x_scale = x_scale.contiguous()
+        return self.engine.forward(
+            x.contiguous(), phys_idx.contiguous(), weights.float().contiguous(), n_cta, upto, fuse, x_scale
+        )
 
-    def forward(self, x, logical_idx, weights, avail_counter, policy: str = "lplb"):
-        return self.forward_physical(x, self.route(logical_idx, avail_counter, policy), weights)
+    def forward(self, x, logical_idx, weights, avail_counter, policy: str = "lplb", x_scale=None):
+        return self.forward_physical(x, self.route(logical_idx, avail_counter, policy), weights, x_scale=x_scale)
 
     def check(self) -> int:
         """First error code raised by the layer's kernels (0 = none); synchronises.  In the
         bounds-checking build an index that left its array is reported as code 6 (the access
         was skipped; ``engine.status()[16:28]`` holds the record)."""
         status = self.engine.status().tolist()
-        return int(status[0] or status[16])
+        return int(status[0] or status[16] or ops.check(self.device))
 
     def reset(self) -> None:
         """Re-align the ranks after a timeout: clear every flag, counter and the status block
@@ -198,14 +239,23 @@ class MoELayer:
     # ------------------------------------------------------------------ reference
     def reference_forward(self, x: torch.Tensor, logical_idx: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """Plain PyTorch fp32 evaluation of the same layer on logical experts (single process):
-        bf16 inputs and weights, fp32 accumulation, bf16 rounding where the kernels round."""
+        bf16 inputs and weights, fp32 accumulation, bf16 rounding where the kernels round (8 bits: rounding of
+        weights, hidden states and activations as the kernels round them)."""
         out = torch.zeros(x.shape[0], self.hidden, dtype=torch.float32, device=x.device)
-        xf = x.float()
+        fp8 = self.weight_dtype == torch.float8_e4m3fn
+
+        def held(rows):  # rows as the layer holds them
+            return ops.dequantize_fp8(*ops.reference.quantize_fp8_reference(rows)) if fp8 else rows.bfloat16().float()
+
+        def weight(w):
+            return ops.dequantize_weight_fp8(*ops.reference.quantize_weight_fp8_reference(w)) if fp8 else w.float()
+
+        xf = held(x.float())
         for expert in logical_idx[logical_idx >= 0].unique().tolist():
-            gate, up, down = self.logical_weights(expert)
+            gate, up, down = (weight(w) for w in self.logical_weights(expert))
             tok, k = (logical_idx == expert).nonzero(as_tuple=True)
             h = xf[tok]
-            act = torch.nn.functional.silu(h @ gate.float().T) * (h @ up.float().T)
-            y = (act.bfloat16().float() @ down.float().T).bfloat16().float()
+            act = torch.nn.functional.silu(h @ gate.T) * (h @ up.T)
+            y = (held(act) @ down.T).bfloat16().float()
             out.index_add_(0, tok, y * weights[tok, k].float().unsqueeze(1))
         return out.bfloat16()

@@ -1,7 +1,8 @@
 """Operators: plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path), and
 the 8-bit serving operators that stand around a mixture-of-experts layer."""
 
-from .fp8 import check, matmul_fp8, moe_few_tokens, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
+from . import reference
+from .fp8 import MOE_FEW_MAX_TOKENS, check, matmul_fp8, moe_few_tokens, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
 from .reference import (
     count_reference,
     dequantize_fp8,
@@ -12,6 +13,8 @@ from .reference import (
 )
 
 __all__ = [
+    "MOE_FEW_MAX_TOKENS",
+    "reference",
     "count_reference",
     "quotas_reference",
     "redirect_reference",

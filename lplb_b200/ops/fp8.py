@@ -24,8 +24,18 @@ import torch
 
 from . import reference
 
-__all__ = ["quantize_fp8", "quantize_weight_fp8", "rms_norm_fp8", "matmul_fp8", "moe_few_tokens", "check"]
+__all__ = [
+    "MOE_FEW_MAX_TOKENS",
+    "quantize_fp8",
+    "quantize_weight_fp8",
+    "rms_norm_fp8",
+    "matmul_fp8",
+    "moe_few_tokens",
+    "check",
+]
 
+
+MOE_FEW_MAX_TOKENS = 64  #: tokens that moe_few_tokens takes
 
 _module = None
 
