@@ -149,10 +149,10 @@ class MoeEngine {
     };
     MOE_CHECK(ok(w13, type) && w13.dim() == 3 && w13.size(0) == sh_.n_local && w13.size(1) == 2 * sh_.inter &&
                   w13.size(2) == sh_.hidden,
-              "w13 must be contiguous " << type << " [n_local, 2*inter, hidden] on this device");
+              "w13 must be contiguous " << c10::toString(type) << " [n_local, 2*inter, hidden] on this device");
     MOE_CHECK(ok(w2, type) && w2.dim() == 3 && w2.size(0) == sh_.n_local && w2.size(1) == sh_.hidden &&
                   w2.size(2) == sh_.inter,
-              "w2 must be contiguous " << type << " [n_local, hidden, inter] on this device");
+              "w2 must be contiguous " << c10::toString(type) << " [n_local, hidden, inter] on this device");
     auto scale_ok = [&](const std::optional<torch::Tensor>& s, const torch::Tensor& w) {
       return s && ok(*s, torch::kFloat8_e8m0fnu) && s->dim() == 3 && s->size(0) == w.size(0) && s->size(1) == w.size(1) / 128 &&
              s->size(2) == w.size(2) / 128;
@@ -187,7 +187,7 @@ class MoeEngine {
     const auto x_type = x_scale ? torch::kFloat8_e4m3fn : torch::kBFloat16;
     MOE_CHECK(x.is_cuda() && x.scalar_type() == x_type && x.is_contiguous() && x.dim() == 2 &&
                   x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
-              "x must be contiguous " << x_type << " [tokens <= max_tokens, hidden]");
+              "x must be contiguous " << c10::toString(x_type) << " [tokens <= max_tokens, hidden]");
     const int n_tokens = (int)x.size(0);
     MOE_CHECK(!x_scale || (x_scale->is_cuda() && x_scale->is_contiguous() && x_scale->scalar_type() == torch::kFloat8_e8m0fnu &&
                            x_scale->dim() == 2 && x_scale->size(0) == n_tokens && x_scale->size(1) == sh_.hidden / 128),

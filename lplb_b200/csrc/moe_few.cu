@@ -149,7 +149,8 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
       !map_of(&maps[1], fp8, m.w2, (uint64_t)m.experts * m.hidden, m.inter, m.inter, kFewTileRows) ||
       !map_of(&maps[2], fp8, x, m.tokens, m.hidden, x_ld, 1) || !map_of(&maps[3], fp8, a.act, at.rows, m.inter, m.inter, 16))
     return cudaErrorInvalidValue;
-  err = launch_after(moe_few_plan_kernel, dim3(1 + (convert ? m.tokens : 0)), dim3(kFewPlanThreads), 0, stream, p);
+  auto kernel = moe_few_plan_kernel;
+  err = launch_after(kernel, dim3(1 + (convert ? m.tokens : 0)), dim3(kFewPlanThreads), 0, stream, p);
   if (err != cudaSuccess) return err;
   const int n = sm_count(device);
   return fp8 ? launch<true>(a, maps, n, device, stream) : launch<false>(a, maps, n, device, stream);

@@ -136,7 +136,8 @@ cudaError_t launch_dispatch(const LayerShape& sh, const LayerBuffers& b, const v
   a.my_rank = sh.my_rank;
   a.capacity = sh.capacity;
   a.epoch = epoch;
-  return launch_after(sh.fp8 ? dispatch_kernel<true> : dispatch_kernel<false>, n_cta, kSupportThreads, 0, stream, a);
+  if (sh.fp8) return launch_after(dispatch_kernel<true>, n_cta, kSupportThreads, 0, stream, a);
+  return launch_after(dispatch_kernel<false>, n_cta, kSupportThreads, 0, stream, a);
 }
 
 cudaError_t launch_schedule(const LayerShape& sh, const LayerBuffers& b, const void* phys_idx, int idx_is64,

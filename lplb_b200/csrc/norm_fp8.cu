@@ -41,7 +41,16 @@ __device__ __forceinline__ void finish(const RowFp8& a, float2 (&v)[4], const fl
   uint32_t top = block_max(mine);
   if (NORM) top = __float_as_uint(__uint_as_float(top) * inv);
   const uint32_t e = scale_exponent(min(top, 0x7F7FFFFFu));
-  store8_e4m3<VEC>(a.q + row * a.cols + c, n, pack8(v, NORM ? inv * reciprocal_of(e) : reciprocal_of(e), finite));
+  float factor = reciprocal_of(e);
+  if (NORM) {
+    if (inv * factor < __uint_as_float(0x7F800000u)) {
+      factor *= inv;
+    } else {  // a block of zeros or nearly so: the scale's reciprocal is 2^126, and 0 times infinity is no 0
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], make_float2(inv, inv));
+    }
+  }
+  store8_e4m3<VEC>(a.q + row * a.cols + c, n, pack8(v, factor, finite));
   if (n > 0 && (threadIdx.x & 15) == 0) a.scale[row * blocks + c / kBlock] = (uint8_t)e;
 }
 template <typename T, bool VEC>
@@ -194,7 +203,8 @@ cudaError_t launch_rows(const RowFp8& a, int n_sms, cudaStream_t stream) {
       int64_t grid = (a.rows + per_cta - 1) / per_cta;
       const int64_t most = (int64_t)n_sms * (2 * kStreamThreads / (threads * per_cta));
       if (grid > most) grid = most;
-      return launch_after(row_stream_fp8_kernel<T, NORM>, dim3((unsigned)grid), dim3(threads, per_cta), 0, stream, a);
+      auto kernel = row_stream_fp8_kernel<T, NORM>;
+      return launch_after(kernel, dim3((unsigned)grid), dim3(threads, per_cta), 0, stream, a);
     }
   }
   // Else a CTA per row, as many threads as it has vectors: the chain of loads, sums and stores of a row
@@ -205,8 +215,8 @@ cudaError_t launch_rows(const RowFp8& a, int n_sms, cudaStream_t stream) {
   const dim3 block(threads, per_cta);
   const int64_t grid = (a.rows + per_cta - 1) / per_cta;
   if (threads > 1024 || grid > 0x7fffffff) return cudaErrorInvalidValue;
-  if (v == 2) return launch_after(row_fp8_kernel<T, 2, NORM, VEC>, dim3((unsigned)grid), block, 0, stream, a);
-  return launch_after(row_fp8_kernel<T, 1, NORM, VEC>, dim3((unsigned)grid), block, 0, stream, a);
+  auto kernel = v == 2 ? row_fp8_kernel<T, 2, NORM, VEC> : row_fp8_kernel<T, 1, NORM, VEC>;
+  return launch_after(kernel, dim3((unsigned)grid), block, 0, stream, a);
 }
 
 // One CTA per 128 x 128 block, a row of it to 16 threads; weights are laid out once, so this is not

@@ -8,7 +8,6 @@
 #include <torch/extension.h>
 
 #include <optional>
-#include <sstream>
 #include <stdexcept>
 #include <string>
 
@@ -21,26 +20,24 @@ namespace {
 using torch::Tensor;
 using OptTensor = std::optional<Tensor>;
 
-// A refused argument is a ValueError, a failed launch a RuntimeError.
-#define OPS_CHECK(cond, msg)                            \
-  do {                                                  \
-    if (!(cond)) {                                      \
-      std::ostringstream oss_;                          \
-      oss_ << "lplb_b200.ops." << msg;                  \
-      throw std::invalid_argument(oss_.str());          \
-    }                                                   \
+// A refused argument is a ValueError, a failed launch a RuntimeError.  Messages are put together from strings: a
+// number written to an ostringstream ends the process where the compiler's C++ library is newer than the one that
+// is loaded.
+#define OPS_CHECK(cond, msg)                                                       \
+  do {                                                                             \
+    if (!(cond)) throw std::invalid_argument(std::string("lplb_b200.ops.") + msg); \
   } while (0)
 
-#define OPS_CUDA(expr)                                                                   \
-  do {                                                                                   \
-    cudaError_t err_ = (expr);                                                           \
-    if (err_ != cudaSuccess) {                                                           \
-      std::ostringstream oss_;                                                           \
-      oss_ << "lplb_b200.ops: " #expr " failed: " << cudaGetErrorName(err_) << ": "      \
-           << cudaGetErrorString(err_);                                                  \
-      throw std::runtime_error(oss_.str());                                              \
-    }                                                                                    \
+#define OPS_CUDA(expr)                                                                                            \
+  do {                                                                                                            \
+    cudaError_t err_ = (expr);                                                                                    \
+    if (err_ != cudaSuccess)                                                                                      \
+      throw std::runtime_error(std::string("lplb_b200.ops: " #expr " failed: ") + cudaGetErrorName(err_) + ": " + \
+                               cudaGetErrorString(err_));                                                         \
   } while (0)
+
+std::string text(int64_t n) { return std::to_string(n); }
+std::string text(at::ScalarType type) { return c10::toString(type); }
 
 constexpr int64_t kBlock = 128;
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
@@ -50,13 +47,13 @@ lplb::ops::Type type_of(const Tensor& t, const char* who) {
     case torch::kFloat32: return lplb::ops::Type::kF32;
     case torch::kBFloat16: return lplb::ops::Type::kBf16;
     case torch::kFloat16: return lplb::ops::Type::kF16;
-    default: OPS_CHECK(false, who << " must be float32, bfloat16 or float16, not " << t.scalar_type());
+    default: OPS_CHECK(false, who + std::string(" must be float32, bfloat16 or float16, not ") + text(t.scalar_type()));
   }
   return lplb::ops::Type::kF32;
 }
 
 void check_no_grad(const Tensor& t, const char* who) {
-  OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who << " requires a gradient: these operators have no backward pass (use torch.no_grad())");
+  OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who + std::string(" requires a gradient: these operators have no backward pass (use torch.no_grad())"));
 }
 
 int sm_count(int device) {
@@ -91,10 +88,10 @@ RowsOut make_rows(const Tensor& x) {
 }
 
 void check_rows(const Tensor& x, const char* who) {
-  OPS_CHECK(x.is_cuda(), who << " must be a CUDA tensor");
+  OPS_CHECK(x.is_cuda(), who + std::string(" must be a CUDA tensor"));
   OPS_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= lplb::ops::kMaxRowLength,
-            who << " must have rows of 1 to " << lplb::ops::kMaxRowLength << " values");
-  OPS_CHECK(x.stride(-1) == 1 || x.size(-1) == 1 || x.numel() == 0, who << " must have the values of a row next to one another");
+            who + std::string(" must have rows of 1 to ") + text(lplb::ops::kMaxRowLength) + " values");
+  OPS_CHECK(x.stride(-1) == 1 || x.size(-1) == 1 || x.numel() == 0, who + std::string(" must have the values of a row next to one another"));
   check_no_grad(x, who);
 }
 
@@ -176,7 +173,7 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   OPS_CHECK(b.device() == device && b.dim() == 2 + lead && b.scalar_type() == torch::kFloat8_e4m3fn,
             "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn on a's device");
   const int64_t m = a.size(0), k = a.size(1), n = b.size(-2), kb = blocks_of(k), groups = rows ? b.size(0) : 1;
-  OPS_CHECK(groups >= 1 && groups <= lplb::ops::kMaxGroups, "matmul_fp8: 1 to " << lplb::ops::kMaxGroups << " groups");
+  OPS_CHECK(groups >= 1 && groups <= lplb::ops::kMaxGroups, "matmul_fp8: 1 to " + text(lplb::ops::kMaxGroups) + " groups");
   OPS_CHECK(!rows || (rows->device() == device && rows->scalar_type() == torch::kInt32 && rows->dim() == 1 && rows->size(0) == groups && rows->is_contiguous()),
             "matmul_fp8: rows must be contiguous int32, one number for each matrix of b, on a's device");
   OPS_CHECK(m <= INT32_MAX && groups * n <= INT32_MAX, "matmul_fp8: more than 2^31 rows");
@@ -229,15 +226,15 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   const bool fp8 = w13_scale.has_value();
   OPS_CHECK(x.is_cuda() && x.dim() == 2, "moe_few_tokens: x must be a CUDA tensor [tokens, hidden]");
   const int64_t tokens = x.size(0), hidden = x.size(1);
-  OPS_CHECK(tokens <= lplb::ops::kMoeFewMaxTokens, "moe_few_tokens: at most " << lplb::ops::kMoeFewMaxTokens << " tokens, not " << tokens);
+  OPS_CHECK(tokens <= lplb::ops::kMoeFewMaxTokens, "moe_few_tokens: at most " + text(lplb::ops::kMoeFewMaxTokens) + " tokens, not " + text(tokens));
   OPS_CHECK(fp8 == w2_scale.has_value(), "moe_few_tokens: w13_scale and w2_scale come together");
   OPS_CHECK(fp8 || !x_scale, "moe_few_tokens: x_scale needs weights in 8 bits");
   const auto wtype = fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16;
   OPS_CHECK(w13.device() == device && w13.dim() == 3 && w13.scalar_type() == wtype && w13.is_contiguous() && w2.device() == device && w2.dim() == 3 &&
                 w2.scalar_type() == wtype && w2.is_contiguous(),
-            "moe_few_tokens: w13 and w2 must be contiguous, on x's device, " << wtype);
+            "moe_few_tokens: w13 and w2 must be contiguous, on x's device, " + text(wtype));
   const int64_t experts = w13.size(0), inter = w13.size(1) / 2;
-  OPS_CHECK(experts >= 1 && experts <= lplb::ops::kMoeFewMaxExperts, "moe_few_tokens: 1 to " << lplb::ops::kMoeFewMaxExperts << " experts");
+  OPS_CHECK(experts >= 1 && experts <= lplb::ops::kMoeFewMaxExperts, "moe_few_tokens: 1 to " + text(lplb::ops::kMoeFewMaxExperts) + " experts");
   OPS_CHECK(hidden >= 256 && hidden % 256 == 0 && inter >= 128 && inter % 128 == 0 && hidden <= 16384 && inter <= 65536,
             "moe_few_tokens: hidden must be a multiple of 256 (up to 16384), inter of 128 (up to 65536)");
   OPS_CHECK(w13.size(1) == 2 * inter && w13.size(2) == hidden && w2.size(0) == experts && w2.size(1) == hidden && w2.size(2) == inter,
@@ -254,7 +251,7 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   OPS_CHECK(idx.device() == device && idx.dim() == 2 && idx.size(0) == tokens && (idx.scalar_type() == torch::kInt64 || idx.scalar_type() == torch::kInt32),
             "moe_few_tokens: idx must be [tokens, topk] of int64 or int32 on x's device");
   const int64_t topk = idx.size(1);
-  OPS_CHECK(topk >= 1 && topk <= lplb::ops::kMoeFewMaxTopk, "moe_few_tokens: 1 to " << lplb::ops::kMoeFewMaxTopk << " choices per token");
+  OPS_CHECK(topk >= 1 && topk <= lplb::ops::kMoeFewMaxTopk, "moe_few_tokens: 1 to " + text(lplb::ops::kMoeFewMaxTopk) + " choices per token");
   OPS_CHECK(weights.device() == device && weights.sizes() == idx.sizes() && weights.is_floating_point(),
             "moe_few_tokens: weights must be floating point, of idx's shape, on x's device");
   auto scales_ok = [&](const Tensor& s, const Tensor& w) {

@@ -49,11 +49,28 @@ def _native():
     return _module
 
 
+def _need(ok: bool, message: str) -> None:
+    """Refusals of CPU arguments, in the words of the native binding."""
+    if not ok:
+        raise ValueError(f"lplb_b200.ops.{message}")
+
+
+def _check_rows(x: torch.Tensor, who: str) -> None:
+    _need(x.dtype in (torch.float32, torch.bfloat16, torch.float16), f"{who} must be float32, bfloat16 or float16")
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 16384, f"{who} must have rows of 1 to 16384 values")
+    _check_no_grad(x, who)
+
+
+def _check_no_grad(x: torch.Tensor, who: str) -> None:
+    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{who} requires a gradient: these operators have no backward pass")
+
+
 def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of rows ``x`` ``[..., K]`` (float32, bfloat16 or float16; rows may be apart from one
     another): ``q`` ``[..., K]`` and one scale per 128, ``[..., ceil(K / 128)]``, both contiguous."""
     if x.is_cuda:
         return _native().quantize_fp8(x)
+    _check_rows(x, "quantize_fp8: x")
     return reference.quantize_fp8_reference(x)
 
 
@@ -62,6 +79,8 @@ def quantize_weight_fp8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``[..., ceil(N / 128), ceil(K / 128)]``."""
     if w.is_cuda:
         return _native().quantize_weight_fp8(w)
+    _need(w.dim() in (2, 3) and w.is_contiguous(), "quantize_weight_fp8: w must be contiguous [rows, cols] or [matrices, rows, cols]")
+    _check_no_grad(w, "quantize_weight_fp8: w")
     return reference.quantize_weight_fp8_reference(w)
 
 
@@ -78,6 +97,14 @@ def rms_norm_fp8(
     normed rows in ``x``'s type, which a router reads."""
     if x.is_cuda:
         return _native().rms_norm_fp8(x, weight, residual, eps, return_normed)
+    _check_rows(x, "rms_norm_fp8: x")
+    _check_no_grad(weight, "rms_norm_fp8: weight")
+    _need(weight.shape == x.shape[-1:], "rms_norm_fp8: weight must have one value for each of a row")
+    _need(weight.dtype in (x.dtype, torch.float32), "rms_norm_fp8: weight must be float32 or of x's type")
+    _need(eps >= 0, "rms_norm_fp8: eps must not be negative")
+    if residual is not None:
+        _check_rows(residual, "rms_norm_fp8: residual")
+        _need(residual.shape == x.shape and residual.dtype == x.dtype, "rms_norm_fp8: residual must have x's shape and type")
     return reference.rms_norm_fp8_reference(x, weight, residual, eps, return_normed)
 
 
@@ -102,8 +129,25 @@ def matmul_fp8(
         raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
     if a.is_cuda:
         return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32)
+    e4m3, e8m0, lead = torch.float8_e4m3fn, torch.float8_e8m0fnu, 0 if rows is None else 1
+    _need(a.dim() == 2 and a.dtype == e4m3, "matmul_fp8: a must be [rows, k] of float8_e4m3fn")
+    _need(b.dim() == 2 + lead and b.dtype == e4m3, "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn")
+    m, k, n, blocks = *a.shape, b.shape[-2], -(-a.shape[1] // 128)
+    _need(k >= 16 and k % 16 == 0 and b.shape[-1] == k, "matmul_fp8: a and b must have the same k, a multiple of 16")
+    _need(a_scale.dtype == e8m0 and a_scale.shape == (m, blocks), "matmul_fp8: a_scale must be [rows, ceil(k / 128)]")
+    _need(
+        b_scale.dtype == e8m0 and b_scale.shape == (*b.shape[:lead], -(-n // 128), blocks),
+        "matmul_fp8: b_scale must be [ceil(n / 128), ceil(k / 128)] (with rows: for every group)",
+    )
+    _need(rows is None or (rows.dtype == torch.int32 and rows.shape == b.shape[:1]), "matmul_fp8: rows must be int32, one for each matrix")
+    _need(rows is None or b.shape[0] <= 128, "matmul_fp8: 1 to 128 groups")
+    _need(out is None or (out.shape == (m, n) and out.dtype == out_dtype), "matmul_fp8: out must be [rows, n] of the output type")
     result = reference.matmul_fp8_reference(a, a_scale, b, b_scale, rows).to(out_dtype)
-    return result if out is None else out.copy_(result)
+    if out is None:
+        return result
+    taken = m if rows is None else min(m, int(rows.clamp_min(0).sum()))
+    out[:taken] = result[:taken]
+    return out
 
 
 def moe_few_tokens(
@@ -131,6 +175,28 @@ def moe_few_tokens(
     throughout, over experts too; the same inputs give the same bits."""
     if x.is_cuda:
         return _native().moe_few_tokens(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale)
+    fp8, who = w13_scale is not None, "moe_few_tokens:"
+    _need(x.dim() == 2 and x.shape[0] <= MOE_FEW_MAX_TOKENS, f"{who} at most {MOE_FEW_MAX_TOKENS} tokens")
+    _need(fp8 == (w2_scale is not None), f"{who} w13_scale and w2_scale come together")
+    _need(fp8 or x_scale is None, f"{who} x_scale needs weights in 8 bits")
+    wtype = torch.float8_e4m3fn if fp8 else torch.bfloat16
+    _need(w13.dim() == 3 and w2.dim() == 3 and w13.dtype == wtype and w2.dtype == wtype, f"{who} w13 and w2 must be {wtype}")
+    experts, inter, hidden = w13.shape[0], w13.shape[1] // 2, x.shape[1]
+    _need(hidden % 256 == 0 and hidden > 0 and inter % 128 == 0 and inter > 0, f"{who} hidden must be a multiple of 256, inter of 128")
+    _need(
+        w13.shape == (experts, 2 * inter, hidden) and w2.shape == (experts, hidden, inter),
+        f"{who} w13 must be [experts, 2 * inter, hidden], w2 [experts, hidden, inter]",
+    )
+    _need(1 <= experts <= 512, f"{who} 1 to 512 experts")
+    _need(x.dtype == (torch.bfloat16 if x_scale is None else torch.float8_e4m3fn), f"{who} x must be bfloat16, or float8_e4m3fn with x_scale")
+    _need(idx.dim() == 2 and idx.shape[0] == x.shape[0] and idx.dtype in (torch.int64, torch.int32), f"{who} idx must be [tokens, topk]")
+    _need(1 <= idx.shape[1] <= 32, f"{who} 1 to 32 choices per token")
+    _need(weights.shape == idx.shape and weights.is_floating_point(), f"{who} weights must be floating point, of idx's shape")
+    for scale, of in ((w13_scale, w13), (w2_scale, w2)):
+        _need(scale is None or scale.shape == (experts, of.shape[1] // 128, of.shape[2] // 128), f"{who} scales must be [experts, rows / 128, cols / 128]")
+    _need(x_scale is None or x_scale.shape == (x.shape[0], hidden // 128), f"{who} x_scale must be [tokens, hidden / 128]")
+    for t in (x, weights, w13, w2):
+        _check_no_grad(t, f"{who} an argument")
     return reference.moe_few_tokens_reference(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale).bfloat16()
 
 

@@ -184,7 +184,7 @@ def matmul_fp8_reference(
         return af @ bf.T
     out = torch.zeros(a.shape[0], b.shape[1], dtype=dtype, device=a.device)
     at = 0
-    for e, n in enumerate(rows.tolist()):
+    for e, n in enumerate(rows.clamp_min(0).tolist()):
         out[at : at + n] = af[at : at + n] @ bf[e].T
         at += n
     return out

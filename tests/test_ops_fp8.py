@@ -124,3 +124,139 @@ def test_wrong_output_type_is_refused():
     b, sb = ops.quantize_weight_fp8(torch.randn(4, 128))
     with pytest.raises(ValueError, match="out_dtype"):
         ops.matmul_fp8(a, sa, b, sb, out_dtype=torch.float16)
+
+
+def _weights(n, k, groups=None):
+    shape = (n, k) if groups is None else (groups, n, k)
+    return ops.quantize_weight_fp8(torch.randn(shape, generator=torch.Generator().manual_seed(3)))
+
+
+def test_groups_take_their_own_matrix_and_leave_the_rest():
+    a, sa = ops.quantize_fp8(torch.randn(9, 144, generator=torch.Generator().manual_seed(2)))
+    b, sb = _weights(20, 144, 3)
+    out = torch.full((9, 20), 7.0)
+    ops.matmul_fp8(a, sa, b, sb, rows=torch.tensor([2, 0, 4], dtype=torch.int32), out=out, out_dtype=torch.float32)
+    for e, part in ((0, slice(0, 2)), (2, slice(2, 6))):
+        want = ops.matmul_fp8(a[part], sa[part], b[e], sb[e], out_dtype=torch.float32)
+        assert torch.equal(out[part], want)
+    assert (out[6:] == 7).all()
+
+
+@pytest.mark.parametrize(
+    "change,words",
+    [
+        (dict(k=17), "multiple of 16"), (dict(b_k=272), "same k"), (dict(a_scale=(3, 1)), "a_scale"), (dict(b_scale=(2, 2)), "b_scale"),
+        (dict(out=(3, 30)), "out must"), (dict(rows=4), "rows must|b must"), (dict(a_type=torch.float32), "a must"),
+    ],
+)
+def test_products_that_are_refused(change, words):
+    k = change.get("k", 256)
+    a = torch.zeros(3, k).to(change.get("a_type", torch.float8_e4m3fn))
+    b = torch.zeros(40, change.get("b_k", k)).to(torch.float8_e4m3fn)
+    e8m0 = torch.float8_e8m0fnu
+    a_scale = torch.ones(change.get("a_scale", (3, -(-k // 128)))).to(e8m0)
+    b_scale = torch.ones(change.get("b_scale", (1, -(-k // 128)))).to(e8m0)
+    rows = torch.zeros(change["rows"], dtype=torch.int32) if "rows" in change else None
+    out = torch.zeros(change["out"]) if "out" in change else None
+    with pytest.raises(ValueError, match=words):
+        ops.matmul_fp8(a, a_scale, b, b_scale, rows=rows, out=out, out_dtype=torch.float32)
+
+
+def test_rows_that_are_refused():
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        ops.quantize_fp8(torch.zeros(2, 4, dtype=torch.float64))
+    with pytest.raises(ValueError, match="1 to 16384"):
+        ops.quantize_fp8(torch.zeros(2, 16385))
+    with pytest.raises(ValueError, match="gradient"):
+        ops.quantize_fp8(torch.zeros(2, 4, requires_grad=True))
+    with pytest.raises(ValueError, match="weight must have"):
+        ops.rms_norm_fp8(torch.zeros(2, 4), torch.ones(5))
+    with pytest.raises(ValueError, match="residual must have"):
+        ops.rms_norm_fp8(torch.zeros(2, 4), torch.ones(4), torch.zeros(2, 4).half())
+
+
+def _layer(tokens=3, topk=2, experts=4, hidden=256, inter=128, fp8=True):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(tokens, hidden, generator=g).bfloat16()
+    idx = torch.stack([torch.randperm(experts, generator=g)[:topk] for _ in range(tokens)])
+    w = torch.rand(tokens, topk, generator=g)
+    w13 = torch.randn(experts, 2 * inter, hidden, generator=g).mul(hidden**-0.5).bfloat16()
+    w2 = torch.randn(experts, hidden, inter, generator=g).mul(inter**-0.5).bfloat16()
+    scales = {}
+    if fp8:
+        (w13, scales["w13_scale"]), (w2, scales["w2_scale"]) = ops.quantize_weight_fp8(w13), ops.quantize_weight_fp8(w2)
+    return x, idx, w, w13, w2, scales
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_layer_pair_by_pair(fp8):
+    x, idx, w, w13, w2, scales = _layer(fp8=fp8)
+    y = ops.moe_few_tokens(x, idx, w, w13, w2, **scales).double()
+    d = torch.float64
+    if fp8:
+        xv = reference.dequantize_fp8(*ops.quantize_fp8(x), d)
+        w13, w2 = (reference.dequantize_weight_fp8(q, s, d) for q, s in ((w13, scales["w13_scale"]), (w2, scales["w2_scale"])))
+    else:
+        xv, w13, w2 = x.double(), w13.double(), w2.double()
+    want = torch.zeros_like(y)
+    for t in range(3):
+        for k in range(2):
+            e = int(idx[t, k])
+            gate, up = w13[e, :128] @ xv[t], w13[e, 128:] @ xv[t]
+            act = gate / (1 + torch.exp(-gate)) * up
+            act = reference.dequantize_fp8(*reference.quantize_fp8_reference(act), d) if fp8 else act.bfloat16().double()
+            want[t] += w[t, k].double() * (w2[e] @ act)
+    # both round the activations; a value on a border may go either way: one step of one in 128
+    step = 2.0**-3 if fp8 else 2.0**-7
+    assert ((y - want).abs() <= want.abs() * 2.0**-8 + 2.0**-12 + step / 128 * want.abs().max()).all()
+
+
+def test_choices_that_choose_nothing_and_choices_made_twice():
+    x, idx, w, w13, w2, scales = _layer()
+    idx = torch.tensor([[-1, -1], [1, 1], [9, 2]])
+    y = ops.moe_few_tokens(x, idx, w, w13, w2, **scales)
+    assert (y[0] == 0).all()
+    once = ops.moe_few_tokens(x[1:2], idx[1:2, :1], w[1:2].sum(1, keepdim=True), w13, w2, **scales)
+    assert (y[1:2].float() - once.float()).abs().max() <= 2.0**-7 * once.float().abs().max()
+    assert torch.equal(y[2:], ops.moe_few_tokens(x[2:], idx[2:, 1:], w[2:, 1:], w13, w2, **scales))
+
+
+@pytest.mark.parametrize(
+    "change,words",
+    [
+        (dict(tokens=65), "at most 64"), (dict(hidden=384), "multiple of 256"), (dict(inter=64), "of 128"), (dict(idx=(3, 33)), "1 to 32"),
+        (dict(weights=(3, 3)), "idx's shape"), (dict(drop="w2_scale"), "come together"), (dict(x=torch.float16), "x must be"),
+        (dict(x_scale=True), "float8_e4m3fn with"),
+    ],
+)
+def test_layers_that_are_refused(change, words):
+    hidden, inter, tokens = change.get("hidden", 256), change.get("inter", 128), change.get("tokens", 3)
+    x = torch.zeros(tokens, hidden, dtype=change.get("x", torch.bfloat16))
+    idx = torch.zeros(change.get("idx", (tokens, 2)), dtype=torch.int64)
+    w = torch.zeros(change.get("weights", tuple(idx.shape)))
+    w13, w2 = torch.zeros(4, 2 * inter, hidden).to(torch.float8_e4m3fn), torch.zeros(4, hidden, inter).to(torch.float8_e4m3fn)
+    kw = {n: torch.ones(4, -(-v.shape[1] // 128), -(-v.shape[2] // 128)).to(torch.float8_e8m0fnu) for n, v in (("w13_scale", w13), ("w2_scale", w2))}
+    kw.pop(change.get("drop"), None)
+    if "x_scale" in change:
+        kw["x_scale"] = torch.ones(tokens, hidden // 128).to(torch.float8_e8m0fnu)
+    with pytest.raises(ValueError, match=words):
+        ops.moe_few_tokens(x, idx, w, w13, w2, **kw)
+
+
+def test_kernels_of_these_operators_wait_before_they_touch_memory():
+    """They start while their predecessor runs out (the launches' text, as for the layer's kernels)."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parents[1] / "lplb_b200" / "csrc"
+    access = re.compile(r"\batomic\w+\(|\b(tma_load|tma_gather)\w*\(|__ldc?g\(|load_raw<|ld_acquire\w*\(")
+    for file, kernels in (
+        ("norm_fp8.cu", ("row_fp8_kernel", "row_stream_fp8_kernel", "weight_fp8_kernel")),
+        ("matmul_fp8.cuh", ("few_rows_kernel",)), ("moe_few.cuh", ("moe_few_kernel", "moe_few_plan_kernel")),
+    ):
+        text = re.sub(r"//[^\n]*", "", (csrc / file).read_text())
+        for kernel in kernels:
+            start = re.search(r"__global__[^;{]*?\b%s\([^;{]*\{" % kernel, text, re.S)
+            assert start, kernel
+            before = text[start.end() : text.index("wait_predecessors();", start.end())]
+            assert "__global__" not in before and access.search(before) is None, kernel
