@@ -103,6 +103,9 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   volatile int* abort = &abort_flag;
+  // The first weights come into L2 while the predecessor runs out; nothing is read before it has ended.
+  if (threadIdx.x == 0)
+    for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb) tma_prefetch_2d(&map_b, kb * kKBytes, tile * kTileRows);
   wait_predecessors();
 
   if (warp == 0) {
@@ -148,42 +151,40 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   } else if (warp == 2) {
     const uint8_t* b_row = a.b_scale + (int64_t)tile * a.k_blocks;
     uint32_t ss = 0, sph = 0;
-    ScaleChunk next[9], now[9];
-    auto fetch_as = [&](auto words, int chunk) {
+    auto stage = [&](auto words) {
+      ScaleChunk next[9], now[9];
+      auto fetch = [&](int chunk) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)  // a row that is not there has a column that nobody reads
-        if (j == 0 || 32 * j < a.cols)
-          next[j].fetch<decltype(words)::value>(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
-      next[8].fetch<decltype(words)::value>(b_row, chunk, a.k_blocks);
-    };
-    auto fetch = [&](int chunk) {
-      if (a.scale_words) fetch_as(std::true_type{}, chunk);
-      else fetch_as(std::false_type{}, chunk);
-    };
-    fetch(kb0 / kScaleChunk);
-    bool ok = true;
-    for (int chunk = kb0 / kScaleChunk; ok && chunk * kScaleChunk < kb1; ++chunk) {
+        for (int j = 0; j < 8; ++j)  // a row that is not there has a column that nobody reads
+          if (j == 0 || 32 * j < a.cols) next[j].fetch<decltype(words)::value>(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
+        next[8].fetch<decltype(words)::value>(b_row, chunk, a.k_blocks);
+      };
+      const int last = (kb1 - 1) / kScaleChunk;
+      fetch(kb0 / kScaleChunk);
+      for (int chunk = kb0 / kScaleChunk; chunk <= last; ++chunk) {
 #pragma unroll
-      for (int j = 0; j < 9; ++j) now[j] = next[j];
-      if ((chunk + 1) * kScaleChunk < kb1) fetch(chunk + 1);
+        for (int j = 0; j < 9; ++j) now[j] = next[j];
+        if (chunk < last) fetch(chunk + 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kb = chunk * kScaleChunk + 4 * i;
-        if (!ok || kb + 4 <= kb0 || kb >= kb1) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs));
-        if (!ok) continue;
-        const uint32_t w = now[8].word[i];
-        uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
-        *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(now[0].word[i], now[1].word[i], now[2].word[i], now[3].word[i]);
-        if (a.cols > 128)
-          *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(now[4].word[i], now[5].word[i], now[6].word[i], now[7].word[i]);
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);
-        if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+        for (int i = 0; i < 4; ++i) {
+          const int kb = chunk * kScaleChunk + 4 * i;
+          if (kb + 4 <= kb0 || kb >= kb1) continue;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs))) return;
+          const uint32_t w = now[8].word[i];
+          uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
+          *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(now[0].word[i], now[1].word[i], now[2].word[i], now[3].word[i]);
+          if (a.cols > 128)
+            *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(now[4].word[i], now[5].word[i], now[6].word[i], now[7].word[i]);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);
+          if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+        }
       }
-    }
+    };
+    if (a.scale_words) stage(std::true_type{});
+    else stage(std::false_type{});
   } else if (warp >= 4) {
     const bool done = mbar_wait(bar_done, 0, abort, kWaitBudgetNs);
     __syncwarp();

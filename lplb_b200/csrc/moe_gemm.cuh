@@ -513,72 +513,68 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (go) {
       const uint32_t lead_sfull = map_to_rank(bar_sfull, 0);
       uint32_t ss = 0, sph = 0;
-      ops::ScaleChunk next[8], now[8];  // the weights' rows, 7 x 32 received rows
-      const uint8_t* w = nullptr;
-      int row0 = 0;
-      auto locate = [&]() {
-        const int block = 2 * cur.w + (EPI == kSwiGLU ? (lane >= kGateRows) : half);  // a warp's lanes: 16 gate rows, 16 up rows
-        w = args.w_scale + ((int64_t)cur.expert * args.w_blocks + min(block, args.w_blocks - 1)) * args.k_blocks;
-        row0 = s_start[cur.expert] + cur.row0 + lane;
-      };
-      auto fetch_as = [&](auto words, int chunk) {
-        next[0].fetch<decltype(words)::value>(w, chunk, args.k_blocks);
+      // Loads behind a branch are waited for where it ends: the next chunk, whichever it is, is fetched at one place.
+      auto stage = [&](auto words) {
+        ops::ScaleChunk next[8], now[8];  // the weights' rows, 7 x 32 received rows
+        const uint8_t* w = nullptr;
+        int row0 = 0;
+        auto locate = [&]() {
+          const int block = 2 * cur.w + (EPI == kSwiGLU ? (lane >= kGateRows) : half);  // a warp's lanes: 16 gate rows, 16 up rows
+          w = args.w_scale + ((int64_t)cur.expert * args.w_blocks + min(block, args.w_blocks - 1)) * args.k_blocks;
+          row0 = s_start[cur.expert] + cur.row0 + lane;
+        };
+        auto fetch = [&](int chunk) {
+          next[0].fetch<decltype(words)::value>(w, chunk, args.k_blocks);
 #pragma unroll
-        for (int j = 0; j < 7; ++j)  // (behind the last row: a column that nobody reads)
-          next[1 + j].fetch<decltype(words)::value>(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
-                                                    chunk, args.k_blocks);
-      };
-      auto fetch = [&](int chunk) {
-        if (args.scale_words) fetch_as(std::true_type{}, chunk);
-        else fetch_as(std::false_type{}, chunk);
-      };
-      const int chunks = (args.k_blocks + ops::kScaleChunk - 1) / ops::kScaleChunk;
-      bool ok = __all_sync(0xffffffffu, find(tile_number(0)) && !*abort);
-      if (ok) {
+          for (int j = 0; j < 7; ++j)  // (behind the last row: a column that nobody reads)
+            next[1 + j].fetch<decltype(words)::value>(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
+                                                      chunk, args.k_blocks);
+        };
+        const int chunks = (args.k_blocks + ops::kScaleChunk - 1) / ops::kScaleChunk;
+        auto find_all = [&](uint32_t i) { return __all_sync(0xffffffffu, find(tile_number(i)) && !*abort); };
+        bool more = find_all(0);
+        if (!more) return;
         locate();
         fetch(0);
-      }
-      for (uint32_t tile_n = 0; ok; ++tile_n) {
-        bool known = false, more = false;  // the next tile: looked up without waiting for its number while this one's scales are held
-        for (int chunk = 0; ok && chunk < chunks; ++chunk) {
+        for (uint32_t tile_n = 0; more; ++tile_n) {
+          bool known = false;  // the next tile: looked up without waiting for its number while this one's scales are held
+          for (int chunk = 0; chunk < chunks; ++chunk) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) now[j] = next[j];
-          if (chunk + 1 < chunks) {
-            fetch(chunk + 1);
-          } else if (EPI >= kStore || __all_sync(0xffffffffu, mbar_test(bar_tile + 8 * ((tile_n + 1) % kTileSlots),
-                                                                          (((tile_n + 1) / kTileSlots) & 1) ^ ((tile_n + 1) % kTileSlots == 0)))) {
-            known = true;
-            more = __all_sync(0xffffffffu, find(tile_number(tile_n + 1)) && !*abort);
+            for (int j = 0; j < 8; ++j) now[j] = next[j];
+            int following = chunk + 1 < chunks ? chunk + 1 : 0;
+            if (following == 0) {
+              known = EPI >= kStore || __all_sync(0xffffffffu, mbar_test(bar_tile + 8 * ((tile_n + 1) % kTileSlots),
+                                                                             (((tile_n + 1) / kTileSlots) & 1) ^ ((tile_n + 1) % kTileSlots == 0)));
+              if (known) more = find_all(tile_n + 1);
+              if (known && more) locate();
+            }
+            fetch(following);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (chunk * ops::kScaleChunk + 4 * i >= args.k_blocks) continue;
+              if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar_sempty + 8 * ss, sph ^ 1, abort, budget))) return;
+              const uint32_t v = now[0].word[i];
+              uint8_t* dst = smem_scales + ss * kScaleSlotBytes + lane * 16;
+              *reinterpret_cast<uint4*>(dst) = make_uint4(v, v, v, v);
+              *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(now[1].word[i], now[2].word[i], now[3].word[i], now[4].word[i]);
+              *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(now[5].word[i], now[6].word[i], now[7].word[i], ops::kScaleOnes);
+              fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_remote_own_data(lead_sfull + 8 * ss);
+              if (++ss == kScaleSlots) ss = 0, sph ^= 1;
+            }
+          }
+          if (!known) {
+            more = find_all(tile_n + 1);
             if (more) {
               locate();
               fetch(0);
             }
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!ok || chunk * ops::kScaleChunk + 4 * i >= args.k_blocks) continue;
-            ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_sempty + 8 * ss, sph ^ 1, abort, budget));
-            if (!ok) continue;
-            const uint32_t v = now[0].word[i];
-            uint8_t* dst = smem_scales + ss * kScaleSlotBytes + lane * 16;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(v, v, v, v);
-            *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(now[1].word[i], now[2].word[i], now[3].word[i], now[4].word[i]);
-            *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(now[5].word[i], now[6].word[i], now[7].word[i], ops::kScaleOnes);
-            fence_proxy_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(lead_sfull + 8 * ss);
-            if (++ss == kScaleSlots) ss = 0, sph ^= 1;
-          }
         }
-        if (ok && !known) {
-          more = __all_sync(0xffffffffu, find(tile_number(tile_n + 1)) && !*abort);
-          if (more) {
-            locate();
-            fetch(0);
-          }
-        }
-        ok = ok && more;
-      }
+      };
+      if (args.scale_words) stage(std::true_type{});
+      else stage(std::false_type{});
     }
   } else if (go && warp >= 2) {
     // ---------------- epilogue ----------------

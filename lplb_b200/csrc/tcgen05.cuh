@@ -128,6 +128,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
       ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+// Starts bringing a tile into L2.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(tmap), "r"(x), "r"(y) : "memory");
+}
 // Four rows y[0..3] of 128 bytes each, one below the other in shared memory; the map's box is one row high.
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, uint32_t bar, int x, const int (&y)[4]) {
   asm volatile(
@@ -171,6 +175,13 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
 }
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The same where nothing that crosses to the other CTA hangs on it: what this thread wrote to its own shared memory, and
+// fenced for the async proxy, is read by its own CTA's tensor core.  (Releasing at cluster scope waits for all memory
+// operations of the thread, some 1400 cycles beside a busy TMA.)
+__device__ __forceinline__ void mbar_arrive_remote_own_data(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- tensor memory -----------------------------------------------------------------------------
