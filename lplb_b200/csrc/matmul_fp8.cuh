@@ -103,9 +103,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   volatile int* abort = &abort_flag;
-  // The first weights come into L2 while the predecessor runs out; nothing is read before it has ended.
-  if (threadIdx.x == 0)
-    for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb) tma_prefetch_2d(&map_b, kb * kKBytes, tile * kTileRows);
   wait_predecessors();
 
   if (warp == 0) {
