@@ -15,7 +15,7 @@ namespace {
 // Half of an SM's shared memory: the next kernel's CTAs can set themselves up beside these
 // (64 rows x 4096 x 7168 10.3 -> 9.8 us; a third of it is too little, 10.8 us).
 constexpr uint32_t kRingBytes = 96 * 1024;
-constexpr int kFewSmem = 204 * 1024;  // at most: 256 rows' sums, scales, barriers and the way to a 1024-byte boundary
+constexpr int kFewSmem = 512 * kSmemPerColumn;  // at most
 
 cudaError_t rows_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld};
@@ -100,7 +100,7 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   if ((err = rows_map(&map_b, p.b, p.n, p.k, p.k, kTileRows)) != cudaSuccess) return err;
   if ((err = rows_map(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
   cudaLaunchAttribute attrs[2]{};
-  const cudaLaunchConfig_t config = cluster_config(attrs, tiles * split, split, FewLayout(a.cols, a.stages).total + 1024, stream, kernel);
+  const cudaLaunchConfig_t config = cluster_config(attrs, tiles * split, split, FewLayout(a.cols, a.stages).request, stream, kernel);
   return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
 }
 

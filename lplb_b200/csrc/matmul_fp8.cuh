@@ -33,6 +33,7 @@ constexpr int kScaleSlots = 4;
 constexpr int kFewThreads = 256;
 constexpr int kFewMaxRows = 256;
 constexpr int kMaxSplit = 8;                    // portable cluster size
+constexpr uint32_t kSmemPerColumn = 448;        // of 228 KB, 1 KB of them per CTA: columns, multiples of 64, add up to 512 at most
 
 struct FewArgs {
   const uint8_t* a_scale;  // [m, a_scale_ld]
@@ -46,8 +47,12 @@ struct FewArgs {
   int scale_words;         // scale rows start on 4-byte boundaries
 };
 
-struct FewLayout {  // shared memory from a 1024-byte boundary on
-  uint32_t stage, ring, scales, bars, total;
+// Shared memory from a 1024-byte boundary on.  A launch asks for `request` bytes: at least as large a part of an SM's shared
+// memory as its columns are of the tensor memory, so that CTAs that are on an SM together (of this kernel, any size,
+// any stream) always find their columns free.  Where one waited for columns with its cluster's other CTAs waiting for
+// it, two launches could hold each other up.
+struct FewLayout {
+  uint32_t stage, ring, scales, bars, total, columns, request;
   __host__ __device__ FewLayout(int cols, int stages) {
     stage = kWeightStage + cols * kKBytes;
     ring = 0;
@@ -56,7 +61,11 @@ struct FewLayout {  // shared memory from a 1024-byte boundary on
     if (scales < partial) scales = partial;
     bars = scales + kScaleSlots * 3 * kScaleAtom;
     total = bars + (2 * kMaxRingStages + 2 * kScaleSlots + 1) * 8;
+    const uint32_t used = scale_columns(cols) + 16;
+    columns = used <= 64 ? 64 : used <= 128 ? 128 : used <= 256 ? 256 : 512;
+    request = total + 1024 > columns * kSmemPerColumn ? total + 1024 : columns * kSmemPerColumn;
   }
+  static __host__ __device__ uint32_t scale_columns(int cols) { return (uint32_t)(cols + 31) / 32 * 32; }  // where the scales begin
 };
 
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
@@ -79,8 +88,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   const int rank = (int)cluster_cta_rank(), split = (int)(cluster_size());
   const int tile = (int)blockIdx.x / split;
   const int kb0 = (int)((int64_t)a.k_blocks * rank / split), kb1 = (int)((int64_t)a.k_blocks * (rank + 1) / split);
-  const uint32_t scale_cols = (uint32_t)(a.cols + 31) / 32 * 32;  // first column of the scales
-  const uint32_t tmem_cols = scale_cols + 16 <= 32 ? 32 : scale_cols + 16 <= 64 ? 64 : scale_cols + 16 <= 128 ? 128 : scale_cols + 16 <= 256 ? 256 : 512;
+  const uint32_t scale_cols = FewLayout::scale_columns(a.cols), tmem_cols = at.columns;
   allow_successor();
   if (threadIdx.x == 0) {
     abort_flag = 0;

@@ -108,7 +108,10 @@ class MoELayer:
             import torch.distributed as dist
 
             handles = [None] * self.n_ranks
-            dist.all_gather_object(handles, handle, group=group)
+            dist.all_gather_object(handles, (handle, str(weight_dtype)), group=group)
+            if any(dtype != str(weight_dtype) for _, dtype in handles):
+                raise ValueError("all ranks of the process group must hold their weights in the same type")
+            handles = [h for h, _ in handles]
         self.engine.open([bytes(h) for h in handles])
         if group is not None:
             dist.barrier(group=group)
@@ -199,7 +202,7 @@ class MoELayer:
             self._placed_version = version
         if self.few_tokens and self.n_ranks == 1 and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS and self.topk <= 32:
             return ops.moe_few_tokens(
-                x, phys_idx.view(x.shape[0], self.topk), weights.view(x.shape[0], self.topk), self.w13, self.w2,
+                x, phys_idx.reshape(x.shape[0], self.topk), weights.reshape(x.shape[0], self.topk), self.w13, self.w2,
                 x_scale, self.w13_scale, self.w2_scale,
             )
         n_cta = self._n_sms
