@@ -7,11 +7,12 @@
 // matrices through a ring in shared memory and never stops loading.  Its tasks are tiles of gate and up, expert by
 // expert, then tiles of down in the same order, taken from one counter: when the last tiles of `act` are
 // being made, free CTAs already work on down for the first experts, and the join of the two halves costs no time.
-// (With equal contiguous shares and all of `act` awaited, 1.8 GB of 8-bit weights took 332 us, 42 us of them waiting.)
+// (With equal contiguous shares and all of `act` awaited, 39 experts of 7168 x 2048 in 8 bits, 1.72 GB, took 332 us; now
+// 275 us, the weights at 6.4 TB/s inside the kernel.)
 //
 // 128 weight rows are the tensor core's M side, the rows of an expert (tokens that chose it, gathered by TMA) its
 // N side, rounded up to 16.  Loading all tokens for every expert instead costs no DRAM traffic, but 64 tokens
-// are 8 KB more per 32 KB of weights to bring from L2: 2.1 GB of 8-bit weights took 600 us that way.
+// are 8 KB more per 32 KB of weights to bring from L2, and four times the columns to multiply.
 //
 // Where the tiles are few, tasks are parts of a tile along k.  Their sums in 32 bits are added up by the CTA that
 // finishes the tile.  Products with down stay in 32 bits per row, and all CTAs share the sums over a token's
