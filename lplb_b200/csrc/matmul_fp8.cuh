@@ -158,12 +158,12 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     const uint8_t* b_row = a.b_scale + (int64_t)tile * a.k_blocks;
     uint32_t ss = 0, sph = 0;
     auto stage = [&](auto words) {
-      ScaleChunk next[9], now[9];
+      ScaleChunk<decltype(words)::value> next[9], now[9];
       auto fetch = [&](int chunk) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)  // a row that is not there has a column that nobody reads
-          if (j == 0 || 32 * j < a.cols) next[j].fetch<decltype(words)::value>(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
-        next[8].fetch<decltype(words)::value>(b_row, chunk, a.k_blocks);
+          if (j == 0 || 32 * j < a.cols) next[j].fetch(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
+        next[8].fetch(b_row, chunk, a.k_blocks);
       };
       const int last = (kb1 - 1) / kScaleChunk;
       fetch(kb0 / kScaleChunk);
@@ -176,12 +176,12 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
           const int kb = chunk * kScaleChunk + 4 * i;
           if (kb + 4 <= kb0 || kb >= kb1) continue;
           if (!__all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs))) return;
-          const uint32_t w = now[8].word[i];
+          const uint32_t w = now[8].word(i);
           uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
           *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
-          *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(now[0].word[i], now[1].word[i], now[2].word[i], now[3].word[i]);
+          *reinterpret_cast<uint4*>(dst + kScaleAtom) = make_uint4(now[0].word(i), now[1].word(i), now[2].word(i), now[3].word(i));
           if (a.cols > 128)
-            *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(now[4].word[i], now[5].word[i], now[6].word[i], now[7].word[i]);
+            *reinterpret_cast<uint4*>(dst + 2 * kScaleAtom) = make_uint4(now[4].word(i), now[5].word(i), now[6].word(i), now[7].word(i));
           fence_proxy_async_shared();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_sfull + 8 * ss);

@@ -442,14 +442,14 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
             for (int i = 0; i < 4; ++i) copy(dst + r * kScaleChunk, src, i);
           }
         } else {  // copies of words want words: by way of registers
-          ScaleChunk c[3];
-          c[0].fetch<false>(row_of(min(lane, rows - 1)), chunk, kbs);
-          c[1].fetch<false>(row_of(min(lane + 32, rows - 1)), chunk, kbs);
-          c[2].fetch<false>(w + (lane & 1) * kbs, chunk, kbs);
+          ScaleChunk<false> c[3];
+          c[0].fetch(row_of(min(lane, rows - 1)), chunk, kbs);
+          c[1].fetch(row_of(min(lane + 32, rows - 1)), chunk, kbs);
+          c[2].fetch(w + (lane & 1) * kbs, chunk, kbs);
           uint4* to = reinterpret_cast<uint4*>(dst);
-          to[lane] = make_uint4(c[0].word[0], c[0].word[1], c[0].word[2], c[0].word[3]);
-          to[lane + 32] = make_uint4(c[1].word[0], c[1].word[1], c[1].word[2], c[1].word[3]);
-          if (lane < 2) to[kMoeFewMaxTokens + lane] = make_uint4(c[2].word[0], c[2].word[1], c[2].word[2], c[2].word[3]);
+          to[lane] = make_uint4(c[0].word(0), c[0].word(1), c[0].word(2), c[0].word(3));
+          to[lane + 32] = make_uint4(c[1].word(0), c[1].word(1), c[1].word(2), c[1].word(3));
+          if (lane < 2) to[kMoeFewMaxTokens + lane] = make_uint4(c[2].word(0), c[2].word(1), c[2].word(2), c[2].word(3));
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         queue |= (uint32_t)((k0 & (kScaleChunk - 1)) | (k1 - k0 - 1) << 4) << (8 * flight);

@@ -516,7 +516,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       uint32_t ss = 0, sph = 0;
       // Loads behind a branch are waited for where it ends: the next chunk, whichever it is, is fetched at one place.
       auto stage = [&](auto words) {
-        ops::ScaleChunk next[8], now[8];  // the weights' rows, 7 x 32 received rows
+        ops::ScaleChunk<decltype(words)::value> next[8], now[8];  // the weights' rows, 7 x 32 received rows
         const uint8_t* w = nullptr;
         int row0 = 0;
         auto locate = [&]() {
@@ -525,10 +525,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           row0 = s_start[cur.expert] + cur.row0 + lane;
         };
         auto fetch = [&](int chunk) {
-          next[0].fetch<decltype(words)::value>(w, chunk, args.k_blocks);
+          next[0].fetch(w, chunk, args.k_blocks);
 #pragma unroll
           for (int j = 0; j < 7; ++j)  // (behind the last row: a column that nobody reads)
-            next[1 + j].fetch<decltype(words)::value>(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
+            next[1 + j].fetch(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
                                                       chunk, args.k_blocks);
         };
         const int chunks = (args.k_blocks + ops::kScaleChunk - 1) / ops::kScaleChunk;
@@ -554,11 +554,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             for (int i = 0; i < 4; ++i) {
               if (chunk * ops::kScaleChunk + 4 * i >= args.k_blocks) continue;
               if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar_sempty + 8 * ss, sph ^ 1, abort, budget))) return;
-              const uint32_t v = now[0].word[i];
+              const uint32_t v = now[0].word(i);
               uint8_t* dst = smem_scales + ss * kScaleSlotBytes + lane * 16;
               *reinterpret_cast<uint4*>(dst) = make_uint4(v, v, v, v);
-              *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(now[1].word[i], now[2].word[i], now[3].word[i], now[4].word[i]);
-              *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(now[5].word[i], now[6].word[i], now[7].word[i], ops::kScaleOnes);
+              *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(now[1].word(i), now[2].word(i), now[3].word(i), now[4].word(i));
+              *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(now[5].word(i), now[6].word(i), now[7].word(i), ops::kScaleOnes);
               fence_proxy_async_shared();
               __syncwarp();
               if (lane == 0) mbar_arrive_remote_own_data(lead_sfull + 8 * ss);

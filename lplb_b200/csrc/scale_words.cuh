@@ -14,23 +14,22 @@ constexpr uint32_t kScaleOnes = 0x7F7F7F7F;  // four scales of 1
 // go out together, so nothing is asked in between: what lies behind a row's last block is never used, and loads that
 // would start there read the last block's word again.
 constexpr int kScaleChunk = 16;
+template <bool WORDS>  // rows start on 4-byte boundaries and k_blocks is a multiple of 4
 struct ScaleChunk {
-  uint32_t word[4];
-  // blocks 16 * chunk ... of a row of k_blocks scales.  WORDS: rows start on 4-byte boundaries and k_blocks is a multiple of 4.
-  template <bool WORDS>
+  uint32_t raw[WORDS ? 4 : 5];
+  uint32_t shift;
+  // blocks 16 * chunk ... of a row of k_blocks scales
   __device__ __forceinline__ void fetch(const uint8_t* row, int chunk, int k_blocks) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(row) + kScaleChunk * chunk;
     const uintptr_t last = (reinterpret_cast<uintptr_t>(row) + k_blocks - 1) & ~(uintptr_t)3;  // word that holds the last block
-    if constexpr (WORDS) {
+    shift = 8 * (uint32_t)(p & 3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) word[i] = __ldcg(reinterpret_cast<const uint32_t*>(min(p + 4 * i, last)));
-    } else {
-      uint32_t w[5];
-#pragma unroll
-      for (int i = 0; i < 5; ++i) w[i] = __ldcg(reinterpret_cast<const uint32_t*>(min((p & ~(uintptr_t)3) + 4 * i, last)));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) word[i] = __funnelshift_r(w[i], w[i + 1], 8 * (uint32_t)(p & 3));
-    }
+    for (int i = 0; i < (WORDS ? 4 : 5); ++i) raw[i] = __ldcg(reinterpret_cast<const uint32_t*>(min((p & ~(uintptr_t)3) + 4 * i, last)));
+  }
+  // blocks 4 * i ... of the chunk: put together here, where the loads have to be there anyway
+  __device__ __forceinline__ uint32_t word(int i) const {
+    if constexpr (WORDS) return raw[i];
+    else return __funnelshift_r(raw[i], raw[i + 1], shift);
   }
 };
 
