@@ -468,3 +468,55 @@ def test_arguments_that_are_refused():
     with torch.no_grad():
         ops.quantize_fp8(torch.zeros(4, 8, device="cuda", requires_grad=True))
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------- far offsets, many launches at once
+def test_rows_behind_two_to_the_31_values():
+    rows, cols = 270_000, 8192
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    last = torch.randn(3, cols, device="cuda", generator=_gen(4)).bfloat16()
+    x[-3:] = last
+    w = torch.ones(cols, device="cuda", dtype=torch.bfloat16)
+    got = ops.rms_norm_fp8(x, w, x)
+    want = ops.rms_norm_fp8(last, w, last)
+    for a, b in zip(got, want):
+        assert torch.equal(a[-3:].view(torch.uint8), b.view(torch.uint8))
+    assert not got[0][0].float().any() and (_bits(got[1])[0] == 1).all()  # a block of zeros has the smallest scale
+
+
+def test_results_behind_two_to_the_31_values():
+    m, n, k = 70_000, 32_768, 32
+    a, sa, b, sb = _operands(64, n, k)
+    many, many_s = torch.zeros(m, k, device="cuda").to(torch.float8_e4m3fn), torch.full((m, 1), 127, dtype=torch.uint8, device="cuda")
+    many[-64:].copy_(a)
+    many_s[-64:] = _bits(sa)
+    y = ops.matmul_fp8(many, many_s.view(torch.float8_e8m0fnu), b, sb)
+    _check_product(y[-64:], a, sa, b, sb, torch.bfloat16)
+    assert not y[:64].any()
+
+
+def test_weights_behind_two_to_the_31_bytes():
+    x, idx, gate, w13, w2, scales = _layer(5, 2, 2, 2048, 2048, True)
+    experts = 300
+    far = {n: torch.zeros(experts, *t.shape[1:], dtype=torch.uint8, device="cuda") for n, t in (("w13", w13), ("w2", w2), *scales.items())}
+    for n, t in (("w13", w13), ("w2", w2), *scales.items()):
+        far[n][-2:] = _bits(t)
+    typed = {n: t.view(torch.float8_e8m0fnu if "scale" in n else torch.float8_e4m3fn) for n, t in far.items()}
+    y = ops.moe_few_tokens(x, idx, gate, w13, w2, **scales)
+    assert torch.equal(y, ops.moe_few_tokens(x, idx + experts - 2, gate, **typed))
+
+
+def test_products_of_many_sizes_at_once_on_several_streams():
+    """Clusters of several launches share SMs; none may wait for another's tensor memory."""
+    cases = [_operands(m, n, k, seed=m) for m, n, k in ((1, 7168, 2048), (33, 300, 256), (48, 4096, 128), (100, 512, 2064), (200, 1000, 512), (250, 256, 7168))]
+    want = [ops.matmul_fp8(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for i in range(20):
+        for j in range(len(cases)):
+            c = (i + j) % len(cases)
+            with torch.cuda.stream(streams[j]):
+                got[c].append(ops.matmul_fp8(*cases[c]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, ys in enumerate(got) for y in ys) and ops.check() == 0
