@@ -218,6 +218,36 @@ class MoELayer:
     def forward(self, x, logical_idx, weights, avail_counter, policy: str = "lplb", x_scale=None):
         return self.forward_physical(x, self.route(logical_idx, avail_counter, policy), weights, x_scale=x_scale)
 
+    def forward_block(
+        self,
+        x: torch.Tensor,
+        norm_weight: torch.Tensor,
+        router: torch.Tensor,
+        avail_counter: torch.Tensor,
+        residual: torch.Tensor | None = None,
+        shared: "tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor] | None" = None,
+        eps: float = 1e-6,
+        policy: str = "lplb",
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The layer as it stands in a model: ``(y, h)`` with the residual stream ``h = x + residual`` (``x`` without
+        a residual) and ``y = MoE(norm(h)) [+ shared expert(norm(h))]``, which the next block adds to ``h``.
+
+        ``x`` is bf16 ``[tokens, hidden]``.  ``router`` ``[n_logical, hidden]`` gives the gate's logits; the ``topk`` largest
+        probabilities of their softmax are the weights.  ``shared`` is an expert that every token passes: ``(w13, w13_scale, w2,
+        w2_scale)`` as ``ops.quantize_weight_fp8`` gives them, ``w13`` in the order of ``interleave_gate_up``."""
+        q, scale, h, normed = ops.rms_norm_fp8(x, norm_weight, residual, eps, return_normed=True)
+        weights, idx = torch.softmax(normed.float() @ router.float().T, dim=-1).topk(self.topk, dim=-1)
+        if self.weight_dtype == torch.float8_e4m3fn:
+            y = self.forward(q, idx, weights, avail_counter, policy, x_scale=scale)
+        else:
+            y = self.forward(normed, idx, weights, avail_counter, policy)
+        if shared is not None:
+            w13, w13_scale, w2, w2_scale = shared
+            both = ops.matmul_fp8(q, scale, w13, w13_scale, out_dtype=torch.float32).unflatten(-1, (-1, 2, 128))
+            act = (torch.nn.functional.silu(both[:, :, 0]) * both[:, :, 1]).flatten(1)
+            y = y + ops.matmul_fp8(*ops.quantize_fp8(act), w2, w2_scale)
+        return y, h
+
     def check(self) -> int:
         """First error code raised by the layer's kernels (0 = none); synchronises.  In the
         bounds-checking build an index that left its array is reported as code 6 (the access

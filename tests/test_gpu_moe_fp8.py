@@ -136,3 +136,52 @@ def test_overflowing_pairs_are_dropped_and_reported():
     x, idx, w = _inputs(64, 512, 16, 4)
     y = tight.forward(x, idx, w, _avail())
     assert tight.check() == 13 and y.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, FP8])
+@pytest.mark.parametrize("tokens,few", [(20, True), (20, False), (300, False)])
+def test_the_block_is_its_operators_one_after_the_other(tokens, few, dtype):
+    hidden, inter = 512, 256
+    layer = _layer(hidden, inter, 16, 2, 300, dtype)
+    layer.few_tokens = few
+    g = torch.Generator("cuda").manual_seed(tokens)
+    x, r = (torch.randn(tokens, hidden, device="cuda", generator=g).bfloat16() for _ in range(2))
+    norm = 1 + 0.2 * torch.randn(hidden, device="cuda", generator=g).bfloat16()
+    router = torch.randn(16, hidden, device="cuda", generator=g) * 0.1
+    w13, w2 = torch.randn(2 * 384, hidden, device="cuda", generator=g) * hidden**-0.5, torch.randn(hidden, 384, device="cuda", generator=g) * 384**-0.5
+    shared = (*ops.quantize_weight_fp8(w13), *ops.quantize_weight_fp8(w2))
+    y, h = layer.forward_block(x, norm, router, _avail(), residual=r, shared=shared)
+    assert layer.check() == 0
+    assert torch.equal(h, x + r)
+    # in plain operations, rounded where the block rounds
+    f = h.float()
+    n = f * torch.rsqrt((f * f).mean(-1, keepdim=True) + 1e-6) * norm.float()
+    q, s = ops.reference.quantize_fp8_reference(n)
+    weights, idx = torch.softmax(n.bfloat16().float() @ router.T, -1).topk(2, -1)
+    routed = layer.reference_forward(n.bfloat16(), idx, weights).float() if dtype != FP8 else None
+    if routed is None:  # the rows in 8 bits come from the norm in 32 bits, not from its bf16 form
+        held = ops.dequantize_fp8(q, s)
+        routed = torch.zeros_like(f)
+        for e in idx.unique().tolist():
+            gate, up, down = (ops.dequantize_weight_fp8(*ops.reference.quantize_weight_fp8_reference(w)) for w in layer.logical_weights(e))
+            tok, k = (idx == e).nonzero(as_tuple=True)
+            act = torch.nn.functional.silu(held[tok] @ gate.T) * (held[tok] @ up.T)
+            act = ops.dequantize_fp8(*ops.reference.quantize_fp8_reference(act))
+            routed.index_add_(0, tok, act @ down.T * weights[tok, k].unsqueeze(1))
+    both = ops.reference.matmul_fp8_reference(q, s, *shared[:2]).unflatten(-1, (-1, 2, 128))
+    act = (torch.nn.functional.silu(both[:, :, 0]) * both[:, :, 1]).flatten(1)
+    want = routed + ops.reference.matmul_fp8_reference(*ops.reference.quantize_fp8_reference(act), *shared[2:])
+    # four roundings to bf16 (pairs, their sum, the shared product, the sum of both), half a step of 2**-8 each at most, and
+    # single values on a border of 8 bits that go the other way
+    assert (y.float() - want).norm() <= 5 * 2.0**-8 * want.norm()
+
+
+def test_the_block_without_a_residual_or_a_shared_expert():
+    layer = _layer(512, 256, 16, 2, 64)
+    x = torch.randn(9, 512, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).bfloat16()
+    router, norm = torch.randn(16, 512, device="cuda") * 0.1, torch.ones(512, device="cuda")
+    y, h = layer.forward_block(x, norm, router, _avail())
+    assert h is x
+    q, s, _, normed = ops.rms_norm_fp8(x, norm, return_normed=True)
+    w, idx = torch.softmax(normed.float() @ router.T, -1).topk(2, -1)
+    assert torch.equal(y, layer.forward(q, idx, w, _avail(), x_scale=s))
