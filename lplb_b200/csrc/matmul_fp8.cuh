@@ -208,8 +208,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
         } else if (n < a.n) {
           Out* out = static_cast<Out*>(a.out) + (int64_t)c0 * a.out_ld + n;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c0 + i < a.m) store_out(out + i * a.out_ld, v[i]);
+          for (int i = 0; i < 16; ++i, out += a.out_ld)
+            if (c0 + i < a.m) store_out(out, v[i]);
         }
       }
       tc_fence_before_sync();

@@ -608,22 +608,28 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
       if (EPI == kStoreF32 || (EPI == kStore && !args.wide_rows)) {
         // a thread has a weight row's column of the result, its warp 32 neighbouring columns
         const int col = cur.w * kBM + half * kCtaM + quarter * 32 + lane;
+        // What takes time are the instructions around the stores: with a pointer that moves on, and nothing asked where all 16
+        // rows are there, 57 MB in float32 cost 8 us instead of 18 (4346 x 3304 x 1024: 36 -> 26 us).
+        using Out = std::conditional_t<EPI == kStoreF32, float, __nv_bfloat16>;
         const int n = min(cur.n, left);
+        Out* to = static_cast<Out*>(args.out) + (int64_t)row0 * args.out_stride + col;
+        auto put = [](Out* p, float v) {
+          if constexpr (EPI == kStoreF32) *p = v;
+          else *p = __float2bfloat16_rn(v);
+        };
         for (int c0 = 0; c0 < n; c0 += 16) {
           float v[16];
           __syncwarp();
           tmem_ld_32x16(taddr + c0, v);
           tmem_ld_wait();
-          if (col < args.w_rows) {
-            const int64_t at = (int64_t)(row0 + c0) * args.out_stride + col;
+          if (col >= args.w_rows) continue;
+          if (c0 + 16 <= n) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (c0 + i >= n) continue;
-              if constexpr (EPI == kStoreF32)
-                static_cast<float*>(args.out)[at + i * args.out_stride] = v[i];
-              else
-                static_cast<__nv_bfloat16*>(args.out)[at + i * args.out_stride] = __float2bfloat16_rn(v[i]);
-            }
+            for (int i = 0; i < 16; ++i, to += args.out_stride) put(to, v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i, to += args.out_stride)
+              if (c0 + i < n) put(to, v[i]);
           }
         }
       } else
