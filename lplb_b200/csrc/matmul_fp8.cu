@@ -55,6 +55,16 @@ cudaError_t resident_clusters(int device, int split, Kernel kernel, int* cluster
   return err;
 }
 
+cudaError_t multiprocessors(int device, int* count) {
+  static std::atomic<int> known[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  *count = known[device].load(std::memory_order_relaxed);
+  if (*count) return cudaSuccess;
+  cudaError_t err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
+  if (err == cudaSuccess) known[device].store(*count, std::memory_order_relaxed);
+  return err;
+}
+
 template <typename Out>
 cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   auto kernel = few_rows_kernel<Out>;
@@ -76,21 +86,27 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   a.m = (int)p.m;
   a.n = (int)p.n;
   a.k_blocks = (int)((p.k + kKBytes - 1) / kKBytes);
-  a.cols = (a.m + 15) / 16 * 16;
   a.scale_words = a.k_blocks % 4 == 0 && a.a_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.a_scale) & 3) == 0 &&
                   (reinterpret_cast<uintptr_t>(a.b_scale) & 3) == 0;
-  const int tiles = (a.n + kTileRows - 1) / kTileRows;
-  // How many CTAs share a tile: the fewest rounds of k blocks over the SMs.
-  int split = 1;
-  int64_t least = INT64_MAX;
+  a.tiles = (a.n + kTileRows - 1) / kTileRows;
+  // How many CTAs share a tile's k blocks, and in how many parts the rows of A go: the least time by this measure, in units
+  // of a k block of 128 weight rows (0.3 us): 6 for a round's beginning, the blocks with their rows, the rows' way out, 4
+  // for a join.  176 x 105 x 528 took 10 us on one CTA.
+  const int least_groups = (a.m + kFewMaxRows - 1) / kFewMaxRows;
+  int split = 1, groups = 1;
+  float least = 1e30f;
   for (int s = 1; s <= kMaxSplit && s <= a.k_blocks; ++s) {
     int fit = 0;
     if ((err = resident_clusters(device, s, kernel, &fit)) != cudaSuccess) return err;
     if (fit < 1) continue;
-    const int64_t rounds = (tiles + fit - 1) / fit, blocks = (a.k_blocks + s - 1) / s;
-    const int64_t cost = rounds * (blocks + 6) + (s > 1 ? 4 + a.cols / 32 : 0);
-    if (cost < least) least = cost, split = s;
+    for (int g = least_groups; g <= (a.m + 15) / 16 && g < least_groups + 16; ++g) {
+      const int cols = ((a.m + g - 1) / g + 15) / 16 * 16;
+      const int rounds = (a.tiles * ((a.m + cols - 1) / cols) + fit - 1) / fit, blocks = (a.k_blocks + s - 1) / s;
+      const float cost = rounds * (blocks * (1.f + cols / 256.f) + 6 + cols / 16.f) + (s > 1 ? 4 : 0);
+      if (cost < least) least = cost, split = s, groups = (a.m + cols - 1) / cols, a.cols = cols;
+    }
   }
+  if (a.cols == 0) return cudaErrorInvalidConfiguration;
   const uint32_t stage = kWeightStage + a.cols * kKBytes;
   a.stages = (int)(kRingBytes / stage);
   if (a.stages > kMaxRingStages) a.stages = kMaxRingStages;
@@ -100,7 +116,7 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   if ((err = rows_map(&map_b, p.b, p.n, p.k, p.k, kTileRows)) != cudaSuccess) return err;
   if ((err = rows_map(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
   cudaLaunchAttribute attrs[2]{};
-  const cudaLaunchConfig_t config = cluster_config(attrs, tiles * split, split, FewLayout(a.cols, a.stages).request, stream, kernel);
+  const cudaLaunchConfig_t config = cluster_config(attrs, a.tiles * groups * split, split, FewLayout(a.cols, a.stages).request, stream, kernel);
   return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
 }
 
@@ -108,15 +124,14 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
 template <int EPI>
 cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
   auto kernel = moe::grouped_gemm_kernel<EPI, false, true>;
-  static std::atomic<int> sms[kMaxDevices];
-  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
-  int n_sm = sms[device].load(std::memory_order_relaxed);
-  cudaError_t err = cudaSuccess;
-  if (n_sm == 0) {
+  static std::atomic<bool> prepared[kMaxDevices];
+  int n_sm = 0;
+  cudaError_t err = multiprocessors(device, &n_sm);
+  if (err != cudaSuccess) return err;
+  if (!prepared[device].load(std::memory_order_relaxed)) {
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)moe::kGemmSmemFp8);
-    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device);
     if (err != cudaSuccess) return err;
-    sms[device].store(n_sm, std::memory_order_relaxed);
+    prepared[device].store(true, std::memory_order_relaxed);
   }
   moe::GemmArgs a{};
   if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
@@ -158,14 +173,28 @@ cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
   return launch_after(kernel, dim3(n_sm & ~1), dim3(moe::kGemmThreadsFp8), moe::kGemmSmemFp8, stream, map_w, rows, a);
 }
 
+cudaError_t launch_rows_many(const Product& p, int device, cudaStream_t stream) {
+  return p.out_f32 ? launch_many<moe::kStoreF32>(p, device, stream) : launch_many<moe::kStore>(p, device, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream) {
   if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.groups < 1 || p.groups > kMaxGroups || p.m > INT32_MAX || p.groups * p.n > INT32_MAX)
     return cudaErrorInvalidValue;
   if (p.m == 0) return cudaSuccess;
-  if (p.rows != nullptr || p.m > kFewMaxRows)
-    return p.out_f32 ? launch_many<moe::kStoreF32>(p, device, stream) : launch_many<moe::kStore>(p, device, stream);
+  if (p.rows != nullptr) return launch_rows_many(p, device, stream);
+  // More than 256 rows go to the CTA pairs, but for small products, whose tiles of 128 x 256 find an SM each and whose k is
+  // short, up to 12 k blocks of a tile per SM.  One CTA per tile starts sooner and splits k; the pairs read less from the
+  // L2.  In us, this kernel and the pairs: 400 x 1000 x 4096 (3.5 blocks per SM) 9.1, 10.9; 600 x 4096 x 1024 (5.2) 7.9,
+  // 9.5; 2000 x 1000 x 2048 (6.9) 8.8, 10.3; 3916 x 353 x 5568 (14) 18.6, 16.2; 1024 x 2048 x 7168 (24) 24.3, 18.3; 1500 x
+  // 4096 x 512 (192 tiles) 13.0, 11.8.
+  if (p.m > kFewMaxRows) {
+    int n_sm = 0;
+    if (cudaError_t err = multiprocessors(device, &n_sm)) return err;
+    const int64_t tiles = (p.n + kTileRows - 1) / kTileRows * ((p.m + kFewMaxRows - 1) / kFewMaxRows);
+    if (tiles > n_sm || tiles * ((p.k + kKBytes - 1) / kKBytes) > 12 * n_sm) return launch_rows_many(p, device, stream);
+  }
   return p.out_f32 ? launch_few<float>(p, device, stream) : launch_few<__nv_bfloat16>(p, device, stream);
 }
 

@@ -1,9 +1,9 @@
 // C[m, n] = sum over blocks of 128 along k of sa[m, kb] * sb[n / 128, kb] * sum_k A[m, k] * B[n, k]
-// for few rows m: e4m3 operands, power-of-two scales that the tensor cores multiply in by themselves.
+// for few rows m, or small products: e4m3 operands, power-of-two scales that the tensor cores multiply in by themselves.
 //
-// Bound by reading B once.  A CTA computes 128 rows of B against all rows of A: the weights on the tensor core's M side, so that
-// few rows cost few cycles, and the k blocks of a tile are dealt out to the CTAs of a cluster, so
-// that a matrix with few tiles still occupies every SM.  The partial sums meet in distributed shared
+// Bound by reading B once.  A CTA computes 128 rows of B against all rows of A (or a part of them, where B is small): the weights
+// on the tensor core's M side, so that few rows cost few cycles, and the k blocks of a tile are dealt out to the CTAs of a
+// cluster, so that a matrix with few tiles still occupies every SM.  The partial sums meet in distributed shared
 // memory, in rank order: no workspace, nothing to clear, the same bits every time.  64 x 4096 x 7168 (29.8 MB) take
 // 9.4 us among others, 3.2 TB/s; 1 x 7168 x 2048 5.4 us: launch, the first load and the join are half of it.
 //
@@ -32,7 +32,7 @@ constexpr uint32_t kWeightStage = kTileRows * kKBytes;
 constexpr int kMaxRingStages = 12;
 constexpr int kScaleSlots = 4;
 constexpr int kFewThreads = 256;
-constexpr int kFewMaxRows = 256;
+constexpr int kFewMaxRows = 256;                // of A per CTA
 constexpr int kMaxSplit = 8;                    // portable cluster size
 constexpr uint32_t kSmemPerColumn = 448;        // of 228 KB, 1 KB of them per CTA: columns, multiples of 64, add up to 512 at most
 
@@ -43,7 +43,8 @@ struct FewArgs {
   int* error;              // the device's error word
   int64_t a_scale_ld, out_ld;
   int m, n, k_blocks;
-  int cols;                // m rounded up to 16
+  int tiles;               // of 128 rows of B
+  int cols;                // rows of A per CTA, a multiple of 16
   int stages;
   int scale_words;         // scale rows start on 4-byte boundaries
 };
@@ -87,7 +88,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_cta_rank(), split = (int)(cluster_size());
-  const int tile = (int)blockIdx.x / split;
+  const int tile = (int)blockIdx.x / split % a.tiles, m0 = (int)blockIdx.x / split / a.tiles * a.cols, m_here = min(a.cols, a.m - m0);
   const int kb0 = (int)((int64_t)a.k_blocks * rank / split), kb1 = (int)((int64_t)a.k_blocks * (rank + 1) / split);
   const uint32_t scale_cols = FewLayout::scale_columns(a.cols), tmem_cols = at.columns;
   allow_successor();
@@ -122,7 +123,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
         const uint32_t dst = base + s * at.stage;
         mbar_expect_tx(bar_full + 8 * s, at.stage);
         tma_load_2d(dst, &map_b, bar_full + 8 * s, kb * kKBytes, tile * kTileRows);
-        tma_load_2d(dst + kWeightStage, &map_a, bar_full + 8 * s, kb * kKBytes, 0);
+        tma_load_2d(dst + kWeightStage, &map_a, bar_full + 8 * s, kb * kKBytes, m0);
         if (++s == (uint32_t)a.stages) s = 0, ph ^= 1;
       }
     }
@@ -162,7 +163,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
       auto fetch = [&](int chunk) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)  // a row that is not there has a column that nobody reads
-          if (j == 0 || 32 * j < a.cols) next[j].fetch(a.a_scale + (int64_t)min(lane + 32 * j, a.m - 1) * a.a_scale_ld, chunk, a.k_blocks);
+          if (j == 0 || 32 * j < a.cols) next[j].fetch(a.a_scale + (int64_t)(m0 + min(lane + 32 * j, m_here - 1)) * a.a_scale_ld, chunk, a.k_blocks);
         next[8].fetch(b_row, chunk, a.k_blocks);
       };
       const int last = (kb1 - 1) / kScaleChunk;
@@ -206,10 +207,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 16; ++i) partial[(c0 + i) * kTileRows + row] = v[i];
         } else if (n < a.n) {
-          Out* out = static_cast<Out*>(a.out) + (int64_t)c0 * a.out_ld + n;
+          Out* out = static_cast<Out*>(a.out) + (int64_t)(m0 + c0) * a.out_ld + n;
 #pragma unroll
           for (int i = 0; i < 16; ++i, out += a.out_ld)
-            if (c0 + i < a.m) store_out(out, v[i]);
+            if (c0 + i < m_here) store_out(out, v[i]);
         }
       }
       tc_fence_before_sync();
@@ -224,7 +225,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
   if (split > 1) {
     cluster_sync();
     // 128 sums of a row of A are 32 x 4; the CTAs share the rows out among their threads
-    for (int i = rank * kFewThreads + threadIdx.x; i < a.m * 32; i += split * kFewThreads) {
+    for (int i = rank * kFewThreads + threadIdx.x; i < m_here * 32; i += split * kFewThreads) {
       const int m = i >> 5, c = (i & 31) * 4, n = tile * kTileRows + c;
       const uint32_t mine = base + (uint32_t)i * 16;
       float4 sum = ld_cluster_v4(map_to_rank(mine, 0));
@@ -232,7 +233,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
         const float4 f = ld_cluster_v4(map_to_rank(mine, r));
         sum.x += f.x, sum.y += f.y, sum.z += f.z, sum.w += f.w;
       }
-      Out* out = static_cast<Out*>(a.out) + (int64_t)m * a.out_ld + n;
+      Out* out = static_cast<Out*>(a.out) + (int64_t)(m0 + m) * a.out_ld + n;
       if (n < a.n) store_out(out, sum.x);
       if (n + 1 < a.n) store_out(out + 1, sum.y);
       if (n + 2 < a.n) store_out(out + 2, sum.z);

@@ -158,6 +158,25 @@ def test_product(m, n, k, out_dtype):
     assert ops.check() == 0
 
 
+# rows in parts for the CTAs: parts that end inside a tile, one column, both sides of the step to CTA pairs
+PRODUCTS_IN_PARTS = [
+    (17, 9, 272), (176, 105, 528), (200, 1000, 1024), (257, 1, 16), (294, 117, 1232), (349, 863, 272), (772, 2164, 816), (1000, 2048, 1024),
+    (1001, 1, 4096), (3916, 353, 1040), (3916, 353, 5568), (20011, 128, 144), (40001, 64, 272), (2304, 2048, 1536), (2305, 2049, 1536),
+]
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", PRODUCTS_IN_PARTS)
+def test_product_of_rows_in_parts(m, n, k, out_dtype):
+    a, sa, b, sb = _operands(m, n, k, seed=m + n)
+    whole = torch.full((m + 3, n + 5), 3.0, device="cuda", dtype=out_dtype)
+    y = ops.matmul_fp8(a, sa, b, sb, out=whole[:m, :n], out_dtype=out_dtype)
+    _check_product(y, a, sa, b, sb, out_dtype)
+    assert (whole[m:] == 3).all() and (whole[:, n:] == 3).all()
+    assert torch.equal(y, ops.matmul_fp8(a, sa, b, sb, out_dtype=out_dtype))
+    assert ops.check() == 0
+
+
 @pytest.mark.parametrize("m", [5, 300])
 def test_product_of_rows_apart_into_rows_apart(m):
     a, sa, b, sb = _operands(m, 200, 272)
