@@ -19,12 +19,12 @@
 #include <chrono>
 #include <map>
 #include <mutex>
-#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <utility>
 #include <vector>
 
+#include "message.h"
 #include "place_api.h"
 #include "planner_api.h"
 
@@ -33,7 +33,7 @@ namespace py = pybind11;
 #define LPLB_CHECK(cond, msg)                                   \
   do {                                                          \
     if (!(cond)) {                                              \
-      std::ostringstream oss_;                                  \
+      lplb::Message oss_;                                       \
       oss_ << "lplb_b200: " << msg << " (" #cond ")";           \
       throw std::runtime_error(oss_.str());                     \
     }                                                           \
@@ -43,7 +43,7 @@ namespace py = pybind11;
   do {                                                                                  \
     cudaError_t err_ = (expr);                                                          \
     if (err_ != cudaSuccess) {                                                          \
-      std::ostringstream oss_;                                                          \
+      lplb::Message oss_;                                                               \
       oss_ << "lplb_b200: " #expr " failed: " << cudaGetErrorName(err_) << ": "        \
            << cudaGetErrorString(err_);                                                 \
       throw std::runtime_error(oss_.str());                                             \

@@ -10,11 +10,11 @@
 
 #include <cstring>
 #include <optional>
-#include <sstream>
 #include <stdexcept>
 #include <string>
 #include <vector>
 
+#include "message.h"
 #include "moe_api.h"
 
 namespace py = pybind11;
@@ -22,7 +22,7 @@ namespace py = pybind11;
 #define MOE_CHECK(cond, msg)                                  \
   do {                                                        \
     if (!(cond)) {                                            \
-      std::ostringstream oss_;                                \
+      lplb::Message oss_;                                     \
       oss_ << "lplb_b200.moe: " << msg << " (" #cond ")";     \
       throw std::runtime_error(oss_.str());                   \
     }                                                         \
@@ -32,7 +32,7 @@ namespace py = pybind11;
   do {                                                                                          \
     cudaError_t err_ = (expr);                                                                  \
     if (err_ != cudaSuccess) {                                                                  \
-      std::ostringstream oss_;                                                                  \
+      lplb::Message oss_;                                                                       \
       oss_ << "lplb_b200.moe: " #expr " failed: " << cudaGetErrorName(err_) << ": "            \
            << cudaGetErrorString(err_);                                                         \
       throw std::runtime_error(oss_.str());                                                     \
