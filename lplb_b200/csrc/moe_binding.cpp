@@ -185,20 +185,22 @@ class MoeEngine {
     MOE_CHECK(ready_ && have_weights_, "engine is not ready: open peers and set weights first");
     MOE_CHECK(!x_scale || sh_.fp8, "x_scale needs weights in 8 bits");
     const auto x_type = x_scale ? torch::kFloat8_e4m3fn : torch::kBFloat16;
-    MOE_CHECK(x.is_cuda() && x.scalar_type() == x_type && x.is_contiguous() && x.dim() == 2 &&
-                  x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
-              "x must be contiguous " << c10::toString(x_type) << " [tokens <= max_tokens, hidden]");
+    auto here = [&](const torch::Tensor& t) { return t.is_cuda() && t.get_device() == device_ && t.is_contiguous(); };
+    MOE_CHECK(here(x) && x.scalar_type() == x_type && x.dim() == 2 && x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
+              "x must be contiguous " << c10::toString(x_type) << " [tokens <= max_tokens, hidden] on this device");
+    // rows are read 16 bytes at a time
+    MOE_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must start on a 16-byte boundary");
     const int n_tokens = (int)x.size(0);
-    MOE_CHECK(!x_scale || (x_scale->is_cuda() && x_scale->is_contiguous() && x_scale->scalar_type() == torch::kFloat8_e8m0fnu &&
-                           x_scale->dim() == 2 && x_scale->size(0) == n_tokens && x_scale->size(1) == sh_.hidden / 128),
-              "x_scale must be contiguous float8_e8m0fnu [tokens, hidden / 128]");
+    MOE_CHECK(!x_scale || (here(*x_scale) && x_scale->scalar_type() == torch::kFloat8_e8m0fnu && x_scale->dim() == 2 &&
+                           x_scale->size(0) == n_tokens && x_scale->size(1) == sh_.hidden / 128),
+              "x_scale must be contiguous float8_e8m0fnu [tokens, hidden / 128] on this device");
     MOE_CHECK(!(fuse_dispatch && sh_.fp8), "the fused dispatch sends bf16 rows only");
-    MOE_CHECK(phys_idx.is_cuda() && phys_idx.is_contiguous() && phys_idx.numel() == (int64_t)n_tokens * sh_.topk &&
+    MOE_CHECK(here(phys_idx) && phys_idx.numel() == (int64_t)n_tokens * sh_.topk &&
                   (phys_idx.scalar_type() == torch::kInt64 || phys_idx.scalar_type() == torch::kInt32),
-              "phys_idx must be contiguous int64/int32 [tokens, topk]");
-    MOE_CHECK(weights.is_cuda() && weights.is_contiguous() && weights.scalar_type() == torch::kFloat32 &&
+              "phys_idx must be contiguous int64/int32 [tokens, topk] on this device");
+    MOE_CHECK(here(weights) && weights.scalar_type() == torch::kFloat32 &&
                   weights.numel() == phys_idx.numel(),
-              "weights must be contiguous float32 [tokens, topk]");
+              "weights must be contiguous float32 [tokens, topk] on this device");
     MOE_CHECK(n_cta >= 1, "n_cta must be positive");
     c10::cuda::CUDAGuard guard(device_);
     cudaStream_t s = c10::cuda::getCurrentCUDAStream(device_).stream();

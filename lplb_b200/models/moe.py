@@ -33,6 +33,12 @@ def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor, tile: int = 128) ->
     return torch.stack([gate.reshape(i // tile, tile, h), up.reshape(i // tile, tile, h)], dim=1).reshape(2 * i, h)
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """Rows as the kernels read them: contiguous, from a 16-byte boundary on."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 class MoELayer:
     """Expert-parallel SwiGLU MoE layer on the native engine.
 
@@ -212,7 +218,7 @@ class MoELayer:
         if x_scale is not None:
             x_scale = x_scale.contiguous()
         return self.engine.forward(
-            x.contiguous(), phys_idx.contiguous(), weights.float().contiguous(), n_cta, upto, fuse, x_scale
+            _rows(x), phys_idx.contiguous(), weights.float().contiguous(), n_cta, upto, fuse, x_scale
         )
 
     def forward(self, x, logical_idx, weights, avail_counter, policy: str = "lplb", x_scale=None):
