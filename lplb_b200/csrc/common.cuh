@@ -130,6 +130,19 @@ __device__ __forceinline__ bool bounded_wait_ge(const uint32_t* flag, uint32_t t
 // one process: 64 tokens x 1024 72.4 -> 65.3 us, 128 x 2048 120 -> 109, 64 x 7168 679 -> 668, 1000 x 7168 1032 -> 1018;
 // 4096 and 8192 x 7168 differ by less than 0.5 % either way, which is their noise.
 __device__ __forceinline__ void wait_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Loads of what a predecessor may have written.  The read-only path (__ldg, and what the compiler makes of a kernel's const
+// __restrict__ parameters) is for memory that nobody writes while the kernel lives, and this kernel lives before its predecessor
+// has ended; its loads may also be moved in front of the wait.  Volatile assembly keeps its order behind the wait.
+__device__ __forceinline__ uint4 ld_behind_wait(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_behind_wait(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
 __device__ __forceinline__ void allow_successor() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... Params, typename... Args>

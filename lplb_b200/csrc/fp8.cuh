@@ -10,6 +10,8 @@
 
 #include <type_traits>
 
+#include "common.cuh"
+
 namespace lplb {
 namespace fp8 {
 
@@ -143,14 +145,14 @@ __device__ __forceinline__ Eight<T> add(const Eight<T>& a, const Eight<T>& b) {
   return sum;
 }
 template <bool VEC, typename T>
-__device__ __forceinline__ Eight<T> load_raw(const T* __restrict__ p, int n) {
+__device__ __forceinline__ Eight<T> load_raw(const T* p, int n) {
   Eight<T> raw;
 #pragma unroll
   for (int i = 0; i < 8; ++i) set_zero(raw.v[i]);
   if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      if (n > 0) reinterpret_cast<uint4*>(&raw)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      if (n > 0) reinterpret_cast<uint4*>(&raw)[i] = ld_behind_wait(reinterpret_cast<const uint4*>(p) + i);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

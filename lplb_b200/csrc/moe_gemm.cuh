@@ -164,16 +164,16 @@ constexpr int kFusedWarps = kFusedThreads / 32;
 
 // One warp copies a row of `n_vec` 16-byte words with U independent loads in flight per lane.
 template <int U>
-__device__ __forceinline__ void copy_row(const uint4* __restrict__ src, uint4* __restrict__ dst, int n_vec, int lane) {
+__device__ __forceinline__ void copy_row(const uint4* src, uint4* __restrict__ dst, int n_vec, int lane) {
   int v = lane;
   for (; v + 32 * (U - 1) < n_vec; v += 32 * U) {
     uint4 q[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) q[i] = __ldg(&src[v + 32 * i]);
+    for (int i = 0; i < U; ++i) q[i] = ld_behind_wait(&src[v + 32 * i]);
 #pragma unroll
     for (int i = 0; i < U; ++i) dst[v + 32 * i] = q[i];
   }
-  for (; v < n_vec; v += 32) dst[v] = __ldg(&src[v]);
+  for (; v < n_vec; v += 32) dst[v] = ld_behind_wait(&src[v]);
 }
 
 // Sender role of the fused kernel: warp `gw` of `n_gw` streams blocks of eight consecutive

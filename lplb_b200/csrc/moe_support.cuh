@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kSupportThreads) dispatch_kernel(const Dispatc
 #pragma unroll
       for (int u = 0; u < kDispatchVec; ++u)
         if (v0 + 32 * u < vec_per_row) {
-          q[u] = __ldg(&src[v0 + 32 * u]);
+          q[u] = ld_behind_wait(&src[v0 + 32 * u]);
           if (FP8) scale[u] = a.x_scale[(size_t)tok * (vec_per_row / 16) + (v0 + 32 * u) / 16];
         }
     } else if constexpr (FP8) {

@@ -223,7 +223,7 @@ cudaError_t launch_rows(const RowFp8& a, int n_sms, cudaStream_t stream) {
 // One CTA per 128 x 128 block, a row of it to 16 threads; weights are laid out once, so this is not
 // tuned beyond reading and writing whole sectors.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) weight_fp8_kernel(const T* __restrict__ w, int64_t rows, int64_t cols, int64_t row_blocks,
+__global__ void __launch_bounds__(256) weight_fp8_kernel(const T* w, int64_t rows, int64_t cols, int64_t row_blocks,
                                                          int64_t col_blocks, uint8_t* q, uint8_t* scale) {
   allow_successor();
   wait_predecessors();
