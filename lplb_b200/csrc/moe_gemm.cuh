@@ -87,11 +87,11 @@ constexpr int kMaxRanks = 8;
 constexpr int kBNFp8 = 224;
 constexpr int kGemmThreadsFp8 = kGemmThreads + 32;
 constexpr uint32_t kRingBytesFp8 = 192 * 1024;
-constexpr int kScaleSlots = 4;
+constexpr int kScaleSlots = 8;  // of four k blocks each: two chunks of them
 constexpr uint32_t kScaleSlotBytes = 3 * ops::kScaleAtom;  // 128 weight rows, 2 x 128 received rows
 constexpr size_t kGemmSmemFp8 = 1024 + kRingBytesFp8 + kBarBytes + 2 * kTurnBytes + kScaleSlots * kScaleSlotBytes;
-constexpr uint32_t kScaleColumns = 2 * kBNFp8;  // first column of the scales in tensor memory: 16 for every slot
-static_assert(kScaleColumns + 16 * kScaleSlots <= kTmemCols, "tensor memory");
+constexpr uint32_t kScaleColumns = 2 * kBNFp8;  // first column of the scales in tensor memory: four times 16, in turn
+static_assert(kScaleColumns + 16 * 4 <= kTmemCols, "tensor memory");
 
 // kStore writes rows as they are (bf16, or float with OUT_F32)
 enum Epilogue : int { kSwiGLU = 0, kScatter = 1, kStore = 2, kStoreF32 = 3 };
@@ -474,7 +474,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_fence_after_sync();
             const uint32_t src = smem_u32(smem_scales) + ss * kScaleSlotBytes;
-            tmem_scale = tmem_base + kScaleColumns + 16 * ss;
+            tmem_scale = tmem_base + kScaleColumns + 16 * (ss & 3);
             for (int j = 0; j * 128 < 128 + cur.n; ++j) tmem_pair_cp_scales(tmem_scale + 4 * j, src + j * ops::kScaleAtom);
             umma_pair_commit(bar_sempty + 8 * ss);
             if (++ss == kScaleSlots) ss = 0, sph ^= 1;
@@ -514,9 +514,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (go) {
       const uint32_t lead_sfull = map_to_rank(bar_sfull, 0);
       uint32_t ss = 0, sph = 0;
-      // Loads behind a branch are waited for where it ends: the next chunk, whichever it is, is fetched at one place.
+      // A chunk's scales go to their slots together, then the next chunk's loads are issued: half of the slots lie between the matrix
+      // instructions and this warp, more time than a load takes beside a busy TMA.  So nothing is under way when the
+      // first CTA is told: the fence at cluster scope waits for the thread's loads, 1400 cycles where there are some.
       auto stage = [&](auto words) {
-        ops::ScaleChunk<decltype(words)::value> next[8], now[8];  // the weights' rows, 7 x 32 received rows
+        ops::ScaleChunk<decltype(words)::value> now[8];  // the weights' rows, 7 x 32 received rows
         const uint8_t* w = nullptr;
         int row0 = 0;
         auto locate = [&]() {
@@ -525,51 +527,38 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           row0 = s_start[cur.expert] + cur.row0 + lane;
         };
         auto fetch = [&](int chunk) {
-          next[0].fetch(w, chunk, args.k_blocks);
+          now[0].fetch(w, chunk, args.k_blocks);
 #pragma unroll
           for (int j = 0; j < 7; ++j)  // (behind the last row: a column that nobody reads)
-            next[1 + j].fetch(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
+            now[1 + j].fetch(args.row_scale + (int64_t)min(row0 + min(32 * j, cur.n - 32), args.n_rows - 1) * args.row_scale_ld,
                                                       chunk, args.k_blocks);
         };
-        const int chunks = (args.k_blocks + ops::kScaleChunk - 1) / ops::kScaleChunk;
-        auto find_all = [&](uint32_t i) { return __all_sync(0xffffffffu, find(tile_number(i)) && !*abort); };
-        bool more = find_all(0);
-        if (!more) return;
-        locate();
-        fetch(0);
-        for (uint32_t tile_n = 0; more; ++tile_n) {
-          bool known = false;  // the next tile: looked up without waiting for its number while this one's scales are held
-          for (int chunk = 0; chunk < chunks; ++chunk) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) now[j] = next[j];
-            int following = chunk + 1 < chunks ? chunk + 1 : 0;
-            if (following == 0) {
-              known = EPI >= kStore || __all_sync(0xffffffffu, mbar_test(bar_tile + 8 * ((tile_n + 1) % kTileSlots),
-                                                                             (((tile_n + 1) / kTileSlots) & 1) ^ ((tile_n + 1) % kTileSlots == 0)));
-              if (known) more = find_all(tile_n + 1);
-              if (known && more) locate();
-            }
-            fetch(following);
+        for (uint32_t tile_n = 0; __all_sync(0xffffffffu, find(tile_number(tile_n)) && !*abort); ++tile_n) {
+          locate();
+          for (int chunk = 0; chunk * ops::kScaleChunk < args.k_blocks; ++chunk) {
+            fetch(chunk);
+            const uint32_t first = ss;
+            const int groups = min(4, (args.k_blocks - chunk * ops::kScaleChunk + 3) / 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              if (chunk * ops::kScaleChunk + 4 * i >= args.k_blocks) continue;
+              if (i >= groups) continue;
               if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar_sempty + 8 * ss, sph ^ 1, abort, budget))) return;
               const uint32_t v = now[0].word(i);
               uint8_t* dst = smem_scales + ss * kScaleSlotBytes + lane * 16;
               *reinterpret_cast<uint4*>(dst) = make_uint4(v, v, v, v);
               *reinterpret_cast<uint4*>(dst + ops::kScaleAtom) = make_uint4(now[1].word(i), now[2].word(i), now[3].word(i), now[4].word(i));
               *reinterpret_cast<uint4*>(dst + 2 * ops::kScaleAtom) = make_uint4(now[5].word(i), now[6].word(i), now[7].word(i), ops::kScaleOnes);
-              fence_proxy_async_shared();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_remote_own_data(lead_sfull + 8 * ss);
               if (++ss == kScaleSlots) ss = 0, sph ^= 1;
             }
-          }
-          if (!known) {
-            more = find_all(tile_n + 1);
-            if (more) {
-              locate();
-              fetch(0);
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+              if (half != 0) fence_cluster();
+              for (int i = 0; i < groups; ++i) {
+                const uint32_t slot = (first + i) % kScaleSlots;
+                if (half == 0) mbar_arrive(bar_sfull + 8 * slot);
+                else mbar_arrive_remote_fenced(lead_sfull + 8 * slot);
+              }
             }
           }
         }

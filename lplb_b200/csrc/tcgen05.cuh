@@ -173,11 +173,10 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// The same where nothing that crosses to the other CTA hangs on it: what this thread wrote to its own shared memory, and
-// fenced for the async proxy, is read by its own CTA's tensor core.  (Releasing at cluster scope waits for all memory
-// operations of the thread, some 1400 cycles beside a busy TMA.)
-__device__ __forceinline__ void mbar_arrive_remote_own_data(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// The same in two steps, one fence for several arrivals.
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive_remote_fenced(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- tensor memory -----------------------------------------------------------------------------
