@@ -51,8 +51,8 @@ struct FewArgs {
 
 // Shared memory from a 1024-byte boundary on.  A launch asks for `request` bytes: at least as large a part of an SM's shared
 // memory as its columns are of the tensor memory, so that CTAs that are on an SM together (of this kernel, any size,
-// any stream) always find their columns free.  Where one waited for columns with its cluster's other CTAs waiting for
-// it, two launches could hold each other up.
+// any stream) always find their columns free.  Columns are given back before a CTA waits for its cluster: one that has to wait
+// for another kernel's columns all the same is late, and holds nothing up.
 struct FewLayout {
   uint32_t stage, ring, scales, bars, total, columns, request;
   __host__ __device__ FewLayout(int cols, int stages) {
@@ -222,6 +222,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     while (timer_ns() - t0 < 200000) __nanosleep(1000);
     if (threadIdx.x == 0) atomicCAS(a.error, 0, kOpsTimeout);
   }
+  // The accumulators have been read: no CTA holds columns while it waits for its cluster, whatever else is on its SM.
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_single(tmem, tmem_cols);
+  }
   if (split > 1) {
     cluster_sync();
     // 128 sums of a row of A are 32 x 4; the CTAs share the rows out among their threads
@@ -241,8 +246,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     }
     cluster_sync();  // no CTA leaves while another reads its sums
   }
-  __syncthreads();
-  if (warp == 1) tmem_dealloc_single(tmem, tmem_cols);
 }
 
 }  // namespace ops
