@@ -78,6 +78,7 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   }
   FewArgs a{};
   if ((err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
+  a.budget_ns = wait_budget_ns();
   a.a_scale = p.a_scale;
   a.b_scale = p.b_scale;
   a.out = p.out;
@@ -142,7 +143,7 @@ cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
   a.n_tiles_w = (int)((p.n + moe::kBM - 1) / moe::kBM);
   a.k_blocks = (int)((p.k + kKBytes - 1) / kKBytes);
   a.n_ranks = 1;
-  a.timeout_ns = kWaitBudgetNs;
+  a.timeout_ns = wait_budget_ns();
   a.w_scale = p.b_scale;
   a.row_scale = p.a_scale;
   a.row_scale_ld = p.a_scale_ld;

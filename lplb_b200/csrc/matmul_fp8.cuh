@@ -17,14 +17,12 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "ops_api.h"
 #include "scale_words.cuh"
 #include "tcgen05.cuh"
 
 namespace lplb {
 namespace ops {
-
-enum OpsErr : int { kOpsTimeout = 21 };
-constexpr unsigned long long kWaitBudgetNs = 2000000000ull;
 
 constexpr int kTileRows = 128;                  // weight rows per CTA
 constexpr int kKBytes = 128;                    // bytes of a row per k block
@@ -41,6 +39,7 @@ struct FewArgs {
   const uint8_t* b_scale;  // [ceil(n / 128), k_blocks]
   void* out;               // [m, out_ld]
   int* error;              // the device's error word
+  unsigned long long budget_ns;
   int64_t a_scale_ld, out_ld;
   int m, n, k_blocks;
   int tiles;               // of 128 rows of B
@@ -119,7 +118,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     if (elect_one()) {
       uint32_t s = 0, ph = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, kWaitBudgetNs)) break;
+        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, a.budget_ns)) break;
         const uint32_t dst = base + s * at.stage;
         mbar_expect_tx(bar_full + 8 * s, at.stage);
         tma_load_2d(dst, &map_b, bar_full + 8 * s, kb * kKBytes, tile * kTileRows);
@@ -134,7 +133,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
       uint32_t s = 0, ph = 0, ss = 0, sph = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (kb == kb0 || (kb & 3) == 0) {
-          if (!mbar_wait(bar_sfull + 8 * ss, sph, abort, kWaitBudgetNs)) break;
+          if (!mbar_wait(bar_sfull + 8 * ss, sph, abort, a.budget_ns)) break;
           tc_fence_after_sync();
           const uint32_t src = base + at.scales + ss * 3 * kScaleAtom;
           tmem_cp_scales(tmem_sa, src);
@@ -142,7 +141,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
           umma_commit(bar_sempty + 8 * ss);
           if (++ss == kScaleSlots) ss = 0, sph ^= 1;
         }
-        if (!mbar_wait(bar_full + 8 * s, ph, abort, kWaitBudgetNs)) break;
+        if (!mbar_wait(bar_full + 8 * s, ph, abort, a.budget_ns)) break;
         tc_fence_after_sync();
         const uint32_t src = base + s * at.stage;
         const uint64_t dw = umma_desc_sw128(src), dt = umma_desc_sw128(src + kWeightStage);
@@ -176,7 +175,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
         for (int i = 0; i < 4; ++i) {
           const int kb = chunk * kScaleChunk + 4 * i;
           if (kb + 4 <= kb0 || kb >= kb1) continue;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs))) return;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, a.budget_ns))) return;
           const uint32_t w = now[8].word(i);
           uint8_t* dst = smem + at.scales + ss * 3 * kScaleAtom + lane * 16;
           *reinterpret_cast<uint4*>(dst) = make_uint4(w, w, w, w);
@@ -193,7 +192,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant
     if (a.scale_words) stage(std::true_type{});
     else stage(std::false_type{});
   } else if (warp >= 4) {
-    const bool done = mbar_wait(bar_done, 0, abort, kWaitBudgetNs);
+    const bool done = mbar_wait(bar_done, 0, abort, a.budget_ns);
     __syncwarp();
     if (__all_sync(0xffffffffu, done)) {
       tc_fence_after_sync();

@@ -142,6 +142,7 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   a.slots = at.slots;
   a.x_words = a.x_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x_scale) & 3) == 0;
   a.w_words = ((reinterpret_cast<uintptr_t>(a.w13_scale) | reinterpret_cast<uintptr_t>(a.w2_scale)) & 3) == 0;
+  a.budget_ns = wait_budget_ns();
   cudaError_t err = ops_error_word(device, &a.error);
   if (err != cudaSuccess) return err;
   CUtensorMap maps[4];

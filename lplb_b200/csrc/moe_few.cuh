@@ -75,6 +75,7 @@ struct FewMoeArgs {
   float* product;            // [kFewPieces, tokens * topk, hidden]
   __nv_bfloat16* out;        // [tokens, hidden]
   int* error;
+  unsigned long long budget_ns;
   int tokens, topk, hidden, inter;
   int cols;                  // tokens rounded up to 16
   int kb1, kb2;              // k blocks of 128 bytes: hidden, inter
@@ -173,14 +174,14 @@ __device__ __forceinline__ void tmem_ld_8(uint32_t taddr, float (&v)[8]) {
 }
 
 // Waits until *counter has reached `target`; false when the budget ran out or a role gave up.
-__device__ __forceinline__ bool few_wait(const int* counter, int target, volatile int* abort) {
+__device__ __forceinline__ bool few_wait(const int* counter, int target, volatile int* abort, uint64_t budget_ns) {
   if ((int)ld_acquire_gpu(reinterpret_cast<const uint32_t*>(counter)) >= target) return true;
   const uint64_t t0 = global_timer_ns();
   for (;;) {
     for (int i = 0; i < 64; ++i)
       if ((int)ld_acquire_gpu(reinterpret_cast<const uint32_t*>(counter)) >= target) return true;
     if (*abort) return false;
-    if (global_timer_ns() - t0 > kWaitBudgetNs) {
+    if (global_timer_ns() - t0 > budget_ns) {
       *abort = 1;
       return false;
     }
@@ -259,7 +260,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
   // The i-th ticket of this CTA, for the roles that follow the producer.
   auto ticket = [&](uint32_t i) -> int {
     const uint32_t s = i % kFewTickets;
-    if (!mbar_wait(bar_ticket + 8 * s, (i / kFewTickets) & 1, abort, kWaitBudgetNs)) return last_ticket;
+    if (!mbar_wait(bar_ticket + 8 * s, (i / kFewTickets) & 1, abort, a.budget_ns)) return last_ticket;
     return *(volatile int*)&s_ticket[s];
   };
   auto ticket_read = [&](uint32_t i) { mbar_arrive(bar_ticket_read + 8 * (i % kFewTickets)); };
@@ -278,7 +279,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
       auto announce = [&](uint32_t i) -> int {
         const uint32_t ts = i % kFewTickets;
         const int t = min(i == 0 ? first_ticket : atomicAdd(a.plan.ticket, 1), last_ticket);
-        if (!mbar_wait(bar_ticket_read + 8 * ts, ((i / kFewTickets) & 1) ^ 1, abort, kWaitBudgetNs)) return last_ticket;
+        if (!mbar_wait(bar_ticket_read + 8 * ts, ((i / kFewTickets) & 1) ^ 1, abort, a.budget_ns)) return last_ticket;
         s_ticket[ts] = t;
         mbar_arrive(bar_ticket + 8 * ts);
         return t;
@@ -294,7 +295,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
             announced = true;
             next = announce(i + 1);
           }
-          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, kWaitBudgetNs);
+          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, a.budget_ns);
           if (!ok) break;
           mbar_expect_tx(bar_full + 8 * s, bytes);
           tma_load_2d(base + s * stage_bytes, k.first ? &map_w13 : &map_w2, bar_full + 8 * s, kb * kPer, row);
@@ -318,19 +319,19 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         ++seg;
         const int cols = ((s_slot[task.slot].y & 255) + 15) / 16 * 16;
         const uint32_t idesc = FP8 ? umma_idesc_mxf8(128, cols) : umma_idesc_bf16(128, cols);
-        if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, kWaitBudgetNs)) break;
+        if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, a.budget_ns)) break;
         tc_fence_after_sync();
         const uint32_t d = tmem + acc * 2 * kFewCols;
         for (int kb = task.k0; kb < task.k1; ++kb) {
           if (FP8 && (kb == task.k0 || (kb & 3) == 0)) {
-            ok = mbar_wait(bar_sfull + 8 * ss, sph, abort, kWaitBudgetNs);
+            ok = mbar_wait(bar_sfull + 8 * ss, sph, abort, a.budget_ns);
             if (!ok) break;
             tc_fence_after_sync();
             for (int j = 0; j < 3; ++j) tmem_cp_scales(tmem_s + 4 * j, base + kFewScalesAt + ss * kFewScaleSlot + j * kScaleAtom);
             umma_commit(bar_sempty + 8 * ss);
             if (++ss == kFewScaleSlots) ss = 0, sph ^= 1;
           }
-          ok = mbar_wait(bar_full + 8 * s, ph, abort, kWaitBudgetNs);
+          ok = mbar_wait(bar_full + 8 * s, ph, abort, a.budget_ns);
           if (!ok) break;
           tc_fence_after_sync();
           const uint32_t src = base + s * stage_bytes;
@@ -366,12 +367,12 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         const FewTask task = tasks.at(t);
         const int slot = task.slot, row0 = s_slot[slot].y >> 8, rows = s_slot[slot].y & 255;
         if (!task.first && slot != ready) {
-          if (!few_wait(a.plan.ready + slot, fb, abort)) break;
+          if (!few_wait(a.plan.ready + slot, fb, abort, a.budget_ns)) break;
           fence_proxy_async_global();  // `act` was written by ordinary stores, seen through the counter
           ready = slot;
         }
         for (int kb = task.k0; kb < task.k1; ++kb) {
-          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, kWaitBudgetNs);
+          ok = mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, a.budget_ns);
           if (!ok) break;
           const uint32_t dst = base + s * stage_bytes + kFewWeightStage;
           if (task.first) {
@@ -414,7 +415,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         if (!task.first && slot != ready) {
           bool there;
           if (wait)
-            there = few_wait(a.plan.ready + slot, fb, abort);
+            there = few_wait(a.plan.ready + slot, fb, abort, a.budget_ns);
           else
             there = (int)ld_acquire_gpu(reinterpret_cast<const uint32_t*>(a.plan.ready + slot)) >= fb;
           if (!__all_sync(0xffffffffu, there)) return wait ? -1 : 0;
@@ -478,7 +479,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         for (int i = k0 / 4; ok && 4 * i < k1; ++i) {
           const uint32_t* word = reinterpret_cast<const uint32_t*>(src) + i;
           const uint32_t w0 = word[kMoeFewMaxTokens * 4], w1 = word[kMoeFewMaxTokens * 4 + 4], r0 = word[lane * 4], r1 = word[(lane + 32) * 4];
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, kWaitBudgetNs));
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * ss, sph ^ 1, abort, a.budget_ns));
           if (!ok) break;
           uint8_t* dst = smem + kFewScalesAt + ss * kFewScaleSlot + lane * 16;
           *reinterpret_cast<uint4*>(dst) = make_uint4(w0, w0, w0, w0);
@@ -510,7 +511,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
       tmem_ld_wait();
     };
     auto arrived = [&]() -> bool {
-      if (!few_all(mbar_wait(bar_tfull + 8 * (seg & 1), (seg >> 1) & 1, abort, kWaitBudgetNs))) return false;
+      if (!few_all(mbar_wait(bar_tfull + 8 * (seg & 1), (seg >> 1) & 1, abort, a.budget_ns))) return false;
       tc_fence_after_sync();
       return true;
     };
@@ -637,7 +638,7 @@ moe_few_kernel(const __grid_constant__ CUtensorMap map_w13, const __grid_constan
         };
         int2 next = choice(u);
         bool there = true;
-        if (lane == 0) there = few_wait(a.plan.products, tasks.n - tasks.n1, abort);
+        if (lane == 0) there = few_wait(a.plan.products, tasks.n - tasks.n1, abort, a.budget_ns);
         if (!__all_sync(0xffffffffu, there)) break;
         __threadfence();
         for (; u < n_out; u += step) {

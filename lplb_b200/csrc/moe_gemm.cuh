@@ -48,6 +48,7 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
+#include "ops_api.h"
 #include "scale_words.cuh"
 #include "tcgen05.cuh"
 
@@ -748,7 +749,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     // shared memory and TMEM are released.
     const uint64_t t0 = timer_ns();
     while (timer_ns() - t0 < 200000) __nanosleep(1000);
-    if (threadIdx.x == 0) atomicCAS(args.status, 0, kMoeGemmTimeout);
+    if (threadIdx.x == 0) atomicCAS(args.status, 0, EPI >= kStore ? (int)ops::kOpsTimeout : (int)kMoeGemmTimeout);
   }
   if constexpr (EPI == kScatter) __threadfence_system();  // rows stored to peers are visible before the flag
   tc_fence_before_sync();

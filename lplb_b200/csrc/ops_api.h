@@ -83,9 +83,14 @@ struct MoeFew {
 size_t moe_few_workspace(const MoeFew& m, int device);
 cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream);
 
-// First error that a kernel of these operators has seen on the current device (0: none; 21: a wait inside a
-// kernel gave up, its results are not valid).  It stays until it is cleared; reading waits for the device.
+// First error that a kernel of these operators has seen on the current device (0: none).  It stays until it is cleared; reading
+// waits for the device.
+enum OpsErr : int { kOpsTimeout = 21 };  // a wait inside a kernel gave up, its results are not valid
 cudaError_t read_ops_error(int* code, bool clear);
+// How long a wait inside a kernel lasts at most, of launches from now on (all devices).
+constexpr unsigned long long kDefaultWaitBudgetNs = 2000000000ull;
+unsigned long long wait_budget_ns();
+void set_wait_budget_ns(unsigned long long ns);
 // Where the kernels put it.
 constexpr int kMaxDevices = 64;
 cudaError_t ops_error_word(int device, int** word);

@@ -314,6 +314,7 @@ void bind_ops(py::module_& m) {
   m.def("matmul_fp8", &matmul_fp8);
   m.def("moe_few_tokens", &moe_few_tokens);
   m.def("ops_error", &ops_error);
+  m.def("set_ops_timeout_us", [](double us) { lplb::ops::set_wait_budget_ns((unsigned long long)(us * 1e3)); });
   m.attr("MOE_FEW_MAX_TOKENS") = lplb::ops::kMoeFewMaxTokens;
   m.attr("MAX_ROW_LENGTH") = lplb::ops::kMaxRowLength;
 }

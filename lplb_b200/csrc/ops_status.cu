@@ -22,6 +22,10 @@ cudaError_t ops_error_word(int device, int** word) {
   return cudaSuccess;
 }
 
+static std::atomic<unsigned long long> g_wait_budget_ns{kDefaultWaitBudgetNs};
+unsigned long long wait_budget_ns() { return g_wait_budget_ns.load(std::memory_order_relaxed); }
+void set_wait_budget_ns(unsigned long long ns) { g_wait_budget_ns.store(ns, std::memory_order_relaxed); }
+
 cudaError_t read_ops_error(int* code, bool clear) {
   cudaError_t err = cudaDeviceSynchronize();
   if (err == cudaSuccess) err = cudaMemcpyFromSymbol(code, g_ops_error, sizeof(int));

@@ -36,15 +36,16 @@ __device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-constexpr uint32_t kSuspendNs = 20000;  // a waiting thread may sleep this long before it looks at the abort flag
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+constexpr uint32_t kSuspendNs = 20000;  // a waiting thread may sleep this long, and no longer than its budget, before it looks again
+__device__ __forceinline__ uint32_t suspend_of(uint64_t budget_ns) { return budget_ns < kSuspendNs ? (uint32_t)budget_ns : kSuspendNs; }
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity, uint32_t suspend_ns = kSuspendNs) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(kSuspendNs)
+      : "r"(bar), "r"(parity), "r"(suspend_ns)
       : "memory");
   return ok != 0;
 }
@@ -83,8 +84,9 @@ template <typename Try>
 __device__ __forceinline__ bool wait_bounded(Try try_wait, volatile int* abort, uint64_t budget_ns) {
   if (try_wait()) return true;
   const uint64_t t0 = timer_ns();
+  const int tries = budget_ns < 256ull * kSuspendNs ? 1 : 256;  // between looks at the clock: they may take that long
   for (;;) {
-    for (int i = 0; i < 256; ++i)
+    for (int i = 0; i < tries; ++i)
       if (try_wait()) return true;
     if (*abort) return false;
     if (timer_ns() - t0 > budget_ns) {
@@ -94,10 +96,10 @@ __device__ __forceinline__ bool wait_bounded(Try try_wait, volatile int* abort, 
   }
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t budget_ns) {
-  return wait_bounded([&] { return mbar_try_wait(bar, parity); }, abort, budget_ns);
+  return wait_bounded([&] { return mbar_try_wait(bar, parity, suspend_of(budget_ns)); }, abort, budget_ns);
 }
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t budget_ns) {
-  return wait_bounded([&] { return mbar_try_wait_cluster(bar, parity); }, abort, budget_ns);
+  return wait_bounded([&] { return mbar_try_wait_cluster(bar, parity, suspend_of(budget_ns)); }, abort, budget_ns);
 }
 
 // ---- TMA ------------------------------------------------------------------------------------
