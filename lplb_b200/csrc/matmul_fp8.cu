@@ -77,7 +77,8 @@ cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
     prepared[device].store(true, std::memory_order_relaxed);
   }
   FewArgs a{};
-  if ((err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
+  a.error = p.status;
+  if (a.error == nullptr && (err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
   a.budget_ns = wait_budget_ns();
   a.a_scale = p.a_scale;
   a.b_scale = p.b_scale;
@@ -135,7 +136,8 @@ cudaError_t launch_many(const Product& p, int device, cudaStream_t stream) {
     prepared[device].store(true, std::memory_order_relaxed);
   }
   moe::GemmArgs a{};
-  if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
+  a.status = p.status;
+  if (a.status == nullptr && (err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
   a.rows = p.rows;
   a.n_experts = p.rows ? p.groups : 1;
   a.w_rows = (int)p.n;

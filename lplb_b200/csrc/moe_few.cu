@@ -143,8 +143,9 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   a.x_words = a.x_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x_scale) & 3) == 0;
   a.w_words = ((reinterpret_cast<uintptr_t>(a.w13_scale) | reinterpret_cast<uintptr_t>(a.w2_scale)) & 3) == 0;
   a.budget_ns = wait_budget_ns();
-  cudaError_t err = ops_error_word(device, &a.error);
-  if (err != cudaSuccess) return err;
+  cudaError_t err = cudaSuccess;
+  a.error = m.status;
+  if (a.error == nullptr && (err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
   CUtensorMap maps[4];
   if (!map_of(&maps[0], fp8, m.w13, (uint64_t)m.experts * 2 * m.inter, m.hidden, m.hidden, kFewTileRows) ||
       !map_of(&maps[1], fp8, m.w2, (uint64_t)m.experts * m.hidden, m.inter, m.inter, kFewTileRows) ||

@@ -46,6 +46,7 @@ struct Product {
   const uint8_t* b_scale;  // [groups, ceil(n / 128), ceil(k / 128)]
   const int* rows;         // [groups] on the device, or null: one matrix, all rows
   void* out;               // [m, n], row stride out_ld, bf16 or float32
+  int* status;             // takes the call's first error; null: the device's word does
   int64_t m, n, k, a_ld, a_scale_ld, out_ld;
   int groups, out_f32;
 };
@@ -77,6 +78,7 @@ struct MoeFew {
   const uint8_t* w2_scale;
   void* out;                 // [tokens, hidden] bf16
   void* workspace;           // moe_few_workspace() bytes, 256-byte aligned
+  int* status;               // takes the call's first error; null: the device's word does
   int64_t x_ld, x_scale_ld;
   int idx_is64, tokens, topk, experts, hidden, inter;
 };

@@ -165,8 +165,16 @@ py::tuple quantize_weight_fp8(const Tensor& w) {
   return py::make_tuple(q, scale);
 }
 
+// Where a call's errors go, if not to the device's word.
+int* status_of(const OptTensor& status, const at::Device& device, const char* who) {
+  if (!status) return nullptr;
+  OPS_CHECK(status->device() == device && status->scalar_type() == torch::kInt32 && status->numel() >= 1,
+            who + std::string(": status must be int32 on the arguments' device"));
+  return status->data_ptr<int>();
+}
+
 Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, const OptTensor& rows, const OptTensor& out,
-                  bool out_f32) {
+                  bool out_f32, const OptTensor& status) {
   const auto device = a.device();
   OPS_CHECK(a.is_cuda() && a.dim() == 2 && a.scalar_type() == torch::kFloat8_e4m3fn, "matmul_fp8: a must be a CUDA tensor [rows, k] of float8_e4m3fn");
   const int64_t lead = rows ? 1 : 0;  // dimensions in front of a matrix
@@ -216,12 +224,13 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   p.a_scale_ld = m < 2 ? kb : a_scale.stride(0);
   p.out_ld = result.stride(0);
   p.out_f32 = out_f32;
+  p.status = status_of(status, device, "matmul_fp8");
   OPS_CUDA(lplb::ops::launch_matmul_fp8(p, a.get_device(), stream_of(a.get_device())));
   return result;
 }
 
 Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights, const Tensor& w13, const Tensor& w2, const OptTensor& x_scale,
-                      const OptTensor& w13_scale, const OptTensor& w2_scale) {
+                      const OptTensor& w13_scale, const OptTensor& w2_scale, const OptTensor& status) {
   const auto device = x.device();
   const bool fp8 = w13_scale.has_value();
   OPS_CHECK(x.is_cuda() && x.dim() == 2, "moe_few_tokens: x must be a CUDA tensor [tokens, hidden]");
@@ -291,6 +300,7 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   m.experts = (int)experts;
   m.hidden = (int)hidden;
   m.inter = (int)inter;
+  m.status = status_of(status, device, "moe_few_tokens");
   // a workspace of this call alone: calls on two streams, or two captured graphs, share nothing
   auto workspace = make({(int64_t)lplb::ops::moe_few_workspace(m, index)}, torch::kUInt8, x);
   m.workspace = workspace.data_ptr();

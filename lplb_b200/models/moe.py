@@ -209,7 +209,7 @@ class MoELayer:
         if self.few_tokens and self.n_ranks == 1 and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS and self.topk <= 32:
             return ops.moe_few_tokens(
                 x, phys_idx.reshape(x.shape[0], self.topk), weights.reshape(x.shape[0], self.topk), self.w13, self.w2,
-                x_scale, self.w13_scale, self.w2_scale,
+                x_scale, self.w13_scale, self.w2_scale, self.engine.status(),
             )
         n_cta = self._n_sms
         fuse = self.fuse_dispatch if fuse_dispatch is None else fuse_dispatch
@@ -249,17 +249,19 @@ class MoELayer:
             y = self.forward(normed, idx, weights, avail_counter, policy)
         if shared is not None:
             w13, w13_scale, w2, w2_scale = shared
-            both = ops.matmul_fp8(q, scale, w13, w13_scale, out_dtype=torch.float32).unflatten(-1, (-1, 2, 128))
+            status = self.engine.status()
+            both = ops.matmul_fp8(q, scale, w13, w13_scale, out_dtype=torch.float32, status=status).unflatten(-1, (-1, 2, 128))
             act = (torch.nn.functional.silu(both[:, :, 0]) * both[:, :, 1]).flatten(1)
-            y = y + ops.matmul_fp8(*ops.quantize_fp8(act), w2, w2_scale)
+            y = y + ops.matmul_fp8(*ops.quantize_fp8(act), w2, w2_scale, status=status)
         return y, h
 
     def check(self) -> int:
-        """First error code raised by the layer's kernels (0 = none); synchronises.  In the
-        bounds-checking build an index that left its array is reported as code 6 (the access
-        was skipped; ``engine.status()[16:28]`` holds the record)."""
+        """First error code raised by the layer's kernels (0 = none), the 8-bit operators of its own passes
+        included; waits for the device.  ``reset`` clears it.  In the bounds-checking build an index that left
+        its array is reported as code 6 (the access was skipped; ``engine.status()[16:28]`` holds the record)."""
+        torch.cuda.synchronize(self.device)
         status = self.engine.status().tolist()
-        return int(status[0] or status[16] or ops.check(self.device))
+        return int(status[0] or status[16])
 
     def reset(self) -> None:
         """Re-align the ranks after a timeout: clear every flag, counter and the status block

@@ -116,6 +116,7 @@ def matmul_fp8(
     rows: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
     out_dtype: torch.dtype = torch.bfloat16,
+    status: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """``a @ b.T`` of the values that ``a`` ``[M, K]`` (scales ``[M, ceil(K / 128)]``) and ``b`` ``[N, K]``
     (scales ``[ceil(N / 128), ceil(K / 128)]``) stand for, summed in 32 bits, in bfloat16 or float32.
@@ -124,11 +125,11 @@ def matmul_fp8(
     ``rows[e]`` rows of ``a``, which follow those of matrix ``e - 1``; no more rows are taken than ``a`` has.  Rows behind
     the last group are left in ``out`` as they were (in a new ``out``: not set).
 
-    ``K`` is a multiple of 16; rows of ``a`` and of ``out`` may be apart from one another."""
+    ``K`` is a multiple of 16; rows of ``a`` and of ``out`` may be apart from one another.  ``status``: see :func:`check`."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
     if a.is_cuda:
-        return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32)
+        return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32, status)
     e4m3, e8m0, lead = torch.float8_e4m3fn, torch.float8_e8m0fnu, 0 if rows is None else 1
     _need(a.dim() == 2 and a.dtype == e4m3, "matmul_fp8: a must be [rows, k] of float8_e4m3fn")
     _need(b.dim() == 2 + lead and b.dtype == e4m3, "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn")
@@ -159,6 +160,7 @@ def moe_few_tokens(
     x_scale: torch.Tensor | None = None,
     w13_scale: torch.Tensor | None = None,
     w2_scale: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """A whole SwiGLU mixture-of-experts layer for up to 64 tokens: two kernels that read the weights of the
     chosen experts once.
@@ -172,9 +174,9 @@ def moe_few_tokens(
     bfloat16 weights take bfloat16 ``x`` and hold the activations in bfloat16.  Weights in 8 bits (``w13_scale``,
     ``w2_scale`` as :func:`quantize_weight_fp8` gives them) take ``x`` in 8 bits with its ``x_scale``, or in bfloat16,
     which the first kernel converts, and hold the activations in 8 bits with a scale per 128.  Sums are in 32 bits
-    throughout, over experts too; the same inputs give the same bits."""
+    throughout, over experts too; the same inputs give the same bits.  ``status``: see :func:`check`."""
     if x.is_cuda:
-        return _native().moe_few_tokens(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale)
+        return _native().moe_few_tokens(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale, status)
     fp8, who = w13_scale is not None, "moe_few_tokens:"
     _need(x.dim() == 2 and x.shape[0] <= MOE_FEW_MAX_TOKENS, f"{who} at most {MOE_FEW_MAX_TOKENS} tokens")
     _need(fp8 == (w2_scale is not None), f"{who} w13_scale and w2_scale come together")
@@ -202,6 +204,9 @@ def moe_few_tokens(
 
 def check(device: torch.device | int | None = None, clear: bool = False) -> int:
     """First error code that a kernel of these operators has raised on ``device`` (0: none; 21: a wait inside
-    a kernel gave up, its results are not valid).  Waits for the device; ``clear`` forgets the error."""
+    a kernel gave up, its results are not valid).  Waits for the device; ``clear`` forgets the error.
+
+    A call that is given ``status``, an int32 tensor on its device, leaves its first error in that tensor's first word (where that is
+    0) and not here: callers that keep their errors apart, as ``MoELayer`` does."""
     index = torch.device("cuda" if device is None else device).index if not isinstance(device, int) else device
     return _native().ops_error(torch.cuda.current_device() if index is None else index, clear)

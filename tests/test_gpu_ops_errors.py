@@ -83,3 +83,76 @@ def test_a_wait_that_runs_out_ends_the_call_with_its_code(make):
     assert call()  # the next call is right, and does not clear it
     assert ops.check(clear=True) == TIMEOUT and ops.check() == 0
     assert call() and ops.check() == 0
+
+
+# ------------------------------------------------------------------------------------------- whose error it is
+def _model(dtype, hidden=512, inter=256, few=False):
+    from lplb_b200 import Planner, cube
+    from lplb_b200.models.moe import MoELayer
+
+    planner = Planner(cube(), 32, 16, 8, device="cuda", warm_start=False)
+    layer = MoELayer(planner, hidden, inter, 4, max_tokens=128, weight_dtype=dtype)
+    layer.few_tokens = few
+    return layer
+
+
+def _pass(layer, tokens=64):
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(tokens, layer.hidden, device="cuda", generator=g).bfloat16()
+    w, idx = torch.softmax(torch.randn(tokens, 16, device="cuda", generator=g), -1).topk(4, -1)
+    return layer.forward(x, idx, w, torch.zeros(1, dtype=torch.int32, device="cuda"), "static")
+
+
+def test_a_layer_does_not_report_the_errors_of_other_calls():
+    layers = [_model(torch.bfloat16), _model(torch.float8_e4m3fn, few=True)]
+    for layer in layers:
+        _pass(layer)
+    call = few_rows()
+    with short_budget():
+        call()
+    assert [layer.check() for layer in layers] == [0, 0]
+    assert ops.check(clear=True) == TIMEOUT
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_a_layers_own_error_is_its_own_and_reset_removes_it(dtype):
+    layer, other = _model(dtype, 4096, 2048, few=True), _model(dtype, few=True)
+    want = _pass(layer)
+    assert layer.check() == 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with short_budget(), torch.cuda.stream(side):
+        _pass(layer)
+    assert layer.check() == TIMEOUT and other.check() == 0 and ops.check() == 0
+    layer.reset()
+    assert layer.check() == 0
+    assert torch.equal(_pass(layer), want) and layer.check() == 0
+
+
+def test_the_shared_experts_errors_are_the_layers():
+    layer = _model(torch.float8_e4m3fn)
+    hidden, g = layer.hidden, torch.Generator("cuda").manual_seed(2)
+    x = torch.randn(5, hidden, device="cuda", generator=g).bfloat16()
+    norm, router = torch.ones(hidden, device="cuda"), torch.randn(16, hidden, device="cuda", generator=g) * 0.1
+    shared = (*ops.quantize_weight_fp8(torch.randn(512, hidden, device="cuda")), *ops.quantize_weight_fp8(torch.randn(hidden, 256, device="cuda")))
+    avail = torch.zeros(1, dtype=torch.int32, device="cuda")
+    layer.forward_block(x, norm, router, avail, shared=shared)
+    assert layer.check() == 0
+    with short_budget():
+        layer.forward_block(x, norm, router, avail, shared=shared)
+    assert layer.check() == TIMEOUT and ops.check() == 0
+    layer.reset()
+    assert layer.check() == 0
+
+
+def test_a_status_of_the_caller_takes_the_error():
+    call, k = few_rows(), 1 << 20
+    status = torch.zeros(4, dtype=torch.int32, device="cuda")
+    args = (_ones(16, k), _unit(16, k // 128), _ones(256, k), _unit(2, k // 128))
+    with short_budget():
+        ops.matmul_fp8(*args, out_dtype=torch.float32, status=status)
+    assert status.tolist() == [TIMEOUT, 0, 0, 0] and ops.check() == 0
+    assert call()
+    for bad in (status.cpu(), status.long(), status[:0]):
+        with pytest.raises(ValueError, match="status must"):
+            ops.matmul_fp8(*args, status=bad)
