@@ -177,30 +177,38 @@ class MoeEngine {
     have_weights_ = true;
   }
 
-  // One forward pass.  x: [T, hidden] bf16 (an engine in 8 bits also takes e4m3 with x_scale), phys_idx: [T, topk]
-  // int64/int32 physical expert ids (-1 = dropped), weights: [T, topk] float32.  `upto` stops after a stage for tests:
-  // 1 route (counts and plan), 2 dispatch, 3 first GEMM, 4 second GEMM, 5 (default) everything.
-  torch::Tensor forward(const torch::Tensor& x, const torch::Tensor& phys_idx, const torch::Tensor& weights,
-                        int n_cta, int upto, bool fuse_dispatch, const std::optional<torch::Tensor>& x_scale) {
+  // What a pass accepts, whichever kernels it takes (rows of x may be apart from one another here).
+  void check_inputs(const torch::Tensor& x, const torch::Tensor& phys_idx, const torch::Tensor& weights, bool fuse_dispatch,
+                    const std::optional<torch::Tensor>& x_scale) const {
     MOE_CHECK(ready_ && have_weights_, "engine is not ready: open peers and set weights first");
     MOE_CHECK(!x_scale || sh_.fp8, "x_scale needs weights in 8 bits");
     const auto x_type = x_scale ? torch::kFloat8_e4m3fn : torch::kBFloat16;
-    auto here = [&](const torch::Tensor& t) { return t.is_cuda() && t.get_device() == device_ && t.is_contiguous(); };
-    MOE_CHECK(here(x) && x.scalar_type() == x_type && x.dim() == 2 && x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
+    auto on_device = [&](const torch::Tensor& t) { return t.is_cuda() && t.get_device() == device_; };
+    auto here = [&](const torch::Tensor& t) { return on_device(t) && t.is_contiguous(); };
+    MOE_CHECK(on_device(x) && x.scalar_type() == x_type && x.dim() == 2 && x.size(1) == sh_.hidden && x.size(0) <= sh_.max_tokens,
               "x must be contiguous " << c10::toString(x_type) << " [tokens <= max_tokens, hidden] on this device");
-    // rows are read 16 bytes at a time
-    MOE_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must start on a 16-byte boundary");
-    const int n_tokens = (int)x.size(0);
-    MOE_CHECK(!x_scale || (here(*x_scale) && x_scale->scalar_type() == torch::kFloat8_e8m0fnu && x_scale->dim() == 2 &&
-                           x_scale->size(0) == n_tokens && x_scale->size(1) == sh_.hidden / 128),
+    MOE_CHECK(!x_scale || (on_device(*x_scale) && x_scale->scalar_type() == torch::kFloat8_e8m0fnu && x_scale->dim() == 2 &&
+                           x_scale->size(0) == x.size(0) && x_scale->size(1) == sh_.hidden / 128),
               "x_scale must be contiguous float8_e8m0fnu [tokens, hidden / 128] on this device");
     MOE_CHECK(!(fuse_dispatch && sh_.fp8), "the fused dispatch sends bf16 rows only");
-    MOE_CHECK(here(phys_idx) && phys_idx.numel() == (int64_t)n_tokens * sh_.topk &&
+    MOE_CHECK(here(phys_idx) && phys_idx.numel() == x.size(0) * sh_.topk &&
                   (phys_idx.scalar_type() == torch::kInt64 || phys_idx.scalar_type() == torch::kInt32),
               "phys_idx must be contiguous int64/int32 [tokens, topk] on this device");
     MOE_CHECK(here(weights) && weights.scalar_type() == torch::kFloat32 &&
                   weights.numel() == phys_idx.numel(),
               "weights must be contiguous float32 [tokens, topk] on this device");
+  }
+
+  // One forward pass.  x: [T, hidden] bf16 (an engine in 8 bits also takes e4m3 with x_scale), phys_idx: [T, topk]
+  // int64/int32 physical expert ids (-1 = dropped), weights: [T, topk] float32.  `upto` stops after a stage for tests:
+  // 1 route (counts and plan), 2 dispatch, 3 first GEMM, 4 second GEMM, 5 (default) everything.
+  torch::Tensor forward(const torch::Tensor& x, const torch::Tensor& phys_idx, const torch::Tensor& weights,
+                        int n_cta, int upto, bool fuse_dispatch, const std::optional<torch::Tensor>& x_scale) {
+    check_inputs(x, phys_idx, weights, fuse_dispatch, x_scale);
+    const int n_tokens = (int)x.size(0);
+    // rows are read one after the other, 16 bytes at a time
+    MOE_CHECK(x.is_contiguous() && (!x_scale || x_scale->is_contiguous()), "x and x_scale must be contiguous");
+    MOE_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0, "x must start on a 16-byte boundary");
     MOE_CHECK(n_cta >= 1, "n_cta must be positive");
     c10::cuda::CUDAGuard guard(device_);
     cudaStream_t s = c10::cuda::getCurrentCUDAStream(device_).stream();
@@ -367,6 +375,8 @@ void bind_moe(py::module_& m) {
       .def("close", &MoeEngine::close)
       .def("set_weights", &MoeEngine::set_weights, py::arg("w13"), py::arg("w2"), py::arg("w13_scale") = py::none(),
            py::arg("w2_scale") = py::none())
+      .def("check_inputs", &MoeEngine::check_inputs, py::arg("x"), py::arg("phys_idx"), py::arg("weights"),
+           py::arg("fuse_dispatch") = false, py::arg("x_scale") = py::none())
       .def("forward", &MoeEngine::forward, py::arg("x"), py::arg("phys_idx"), py::arg("weights"), py::arg("n_cta"),
            py::arg("upto") = 5, py::arg("fuse_dispatch") = false, py::arg("x_scale") = py::none())
       .def("capturing", &MoeEngine::capturing)

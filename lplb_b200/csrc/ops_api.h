@@ -53,7 +53,7 @@ struct Product {
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream);
 
 // ---- MoE layer for a few tokens ---------------------------------------------------------------
-constexpr int kMoeFewMaxTokens = 64, kMoeFewMaxTopk = 32, kMoeFewMaxExperts = 512;
+constexpr int kMoeFewMaxTokens = 64, kMoeFewMaxTopk = 32, kMoeFewMaxExperts = 512, kMoeFewMaxHidden = 16384, kMoeFewMaxInter = 65536;
 
 // What the first kernel tells the second, in a workspace of the call.  A row is a token's choice of an expert; the
 // rows of a slot (an expert that was chosen) follow those of the slot before, in the tokens' order.

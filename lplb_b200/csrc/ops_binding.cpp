@@ -244,8 +244,10 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
             "moe_few_tokens: w13 and w2 must be contiguous, on x's device, " + text(wtype));
   const int64_t experts = w13.size(0), inter = w13.size(1) / 2;
   OPS_CHECK(experts >= 1 && experts <= lplb::ops::kMoeFewMaxExperts, "moe_few_tokens: 1 to " + text(lplb::ops::kMoeFewMaxExperts) + " experts");
-  OPS_CHECK(hidden >= 256 && hidden % 256 == 0 && inter >= 128 && inter % 128 == 0 && hidden <= 16384 && inter <= 65536,
-            "moe_few_tokens: hidden must be a multiple of 256 (up to 16384), inter of 128 (up to 65536)");
+  OPS_CHECK(hidden >= 256 && hidden % 256 == 0 && inter >= 128 && inter % 128 == 0 && hidden <= lplb::ops::kMoeFewMaxHidden &&
+                inter <= lplb::ops::kMoeFewMaxInter,
+            "moe_few_tokens: hidden must be a multiple of 256 (up to " + text(lplb::ops::kMoeFewMaxHidden) + "), inter of 128 (up to " +
+                text(lplb::ops::kMoeFewMaxInter) + ")");
   OPS_CHECK(w13.size(1) == 2 * inter && w13.size(2) == hidden && w2.size(0) == experts && w2.size(1) == hidden && w2.size(2) == inter,
             "moe_few_tokens: w13 must be [experts, 2 * inter, hidden], w2 [experts, hidden, inter]");
   OPS_CHECK(experts * 2 * inter <= INT32_MAX && experts * hidden <= INT32_MAX, "moe_few_tokens: more than 2^31 weight rows");
@@ -326,5 +328,9 @@ void bind_ops(py::module_& m) {
   m.def("ops_error", &ops_error);
   m.def("set_ops_timeout_us", [](double us) { lplb::ops::set_wait_budget_ns((unsigned long long)(us * 1e3)); });
   m.attr("MOE_FEW_MAX_TOKENS") = lplb::ops::kMoeFewMaxTokens;
+  m.attr("MOE_FEW_MAX_TOPK") = lplb::ops::kMoeFewMaxTopk;
+  m.attr("MOE_FEW_MAX_EXPERTS") = lplb::ops::kMoeFewMaxExperts;
+  m.attr("MOE_FEW_MAX_HIDDEN") = lplb::ops::kMoeFewMaxHidden;
+  m.attr("MOE_FEW_MAX_INTER") = lplb::ops::kMoeFewMaxInter;
   m.attr("MAX_ROW_LENGTH") = lplb::ops::kMaxRowLength;
 }

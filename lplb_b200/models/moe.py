@@ -34,9 +34,17 @@ def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor, tile: int = 128) ->
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """Rows as the kernels read them: contiguous, from a 16-byte boundary on."""
+    """Rows as the whole layer reads them: one after the other, from a 16-byte boundary on."""
     x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _rows_apart(x: torch.Tensor) -> torch.Tensor:
+    """Rows as the short pass reads them: also apart from one another, each from a 16-byte boundary on."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
+    apart = x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= x.shape[1] and x.stride(0) * x.itemsize % 16 == 0
+    return x if apart and x.data_ptr() % 16 == 0 else _rows(x)
 
 
 class MoELayer:
@@ -51,7 +59,8 @@ class MoELayer:
     ``weight_dtype=torch.float8_e4m3fn`` holds the weights in 8 bits with a power-of-two scale for every 128 x 128
     of them; hidden states then travel, and activations are held, in 8 bits with a scale per 128 values
     (see ``lplb_b200.ops.fp8``).  ``few_tokens = True`` has passes of up to 64 tokens on one GPU take
-    ``ops.moe_few_tokens``: two kernels instead of five.
+    ``ops.moe_few_tokens`` where its range holds ``hidden``, ``inter`` and ``topk``: two kernels instead of five.  They accept
+    and refuse what the whole layer does; a pass that is asked to fuse its dispatch (``fuse_dispatch=True``) is the whole layer's.
     """
 
     def __init__(
@@ -119,10 +128,14 @@ class MoELayer:
                 raise ValueError("all ranks of the process group must hold their weights in the same type")
             handles = [h for h, _ in handles]
         self.engine.open([bytes(h) for h in handles])
+        self._status = self.engine.status()
         if group is not None:
             dist.barrier(group=group)
         self.fuse_dispatch = False
         self.few_tokens = False
+        self._few_fits = (
+            self.n_ranks == 1 and topk <= ops.MOE_FEW_MAX_TOPK and hidden <= ops.MOE_FEW_MAX_HIDDEN and inter <= ops.MOE_FEW_MAX_INTER
+        )
         self.send_ctas = 0  # fused dispatch only: this many CTAs send rows and run no tiles (0: sender warps in every CTA)
         self._n_sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._placed_for: torch.Tensor | None = None
@@ -206,20 +219,24 @@ class MoELayer:
             if self._placed_for is None or not torch.equal(self._placed_for, self.planner.phy2log):
                 raise RuntimeError("expert placement changed: call place_weights() first")
             self._placed_version = version
-        if self.few_tokens and self.n_ranks == 1 and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS and self.topk <= 32:
-            return ops.moe_few_tokens(
-                x, phys_idx.reshape(x.shape[0], self.topk), weights.reshape(x.shape[0], self.topk), self.w13, self.w2,
-                x_scale, self.w13_scale, self.w2_scale, self.engine.status(),
-            )
-        n_cta = self._n_sms
         fuse = self.fuse_dispatch if fuse_dispatch is None else fuse_dispatch
+        phys_idx, weights = phys_idx.contiguous(), weights.float().contiguous()
+        if self._few_fits and self.few_tokens and not fuse_dispatch and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS:
+            x = _rows_apart(x)
+            if x_scale is not None and x_scale.stride(-1) != 1:
+                x_scale = x_scale.contiguous()
+            self.engine.check_inputs(x, phys_idx, weights, fuse, x_scale)  # accepted and refused as by the whole layer
+            if x.requires_grad or weights.requires_grad:  # no pass of the layer has a backward
+                x, weights = x.detach(), weights.detach()
+            shape = (x.shape[0], self.topk)
+            return ops.moe_few_tokens(
+                x, phys_idx.view(shape), weights.view(shape), self.w13, self.w2, x_scale, self.w13_scale, self.w2_scale, self._status
+            )
         if fuse:
             self.engine.set_send_ctas(int(self.send_ctas))
         if x_scale is not None:
             x_scale = x_scale.contiguous()
-        return self.engine.forward(
-            _rows(x), phys_idx.contiguous(), weights.float().contiguous(), n_cta, upto, fuse, x_scale
-        )
+        return self.engine.forward(_rows(x), phys_idx, weights, self._n_sms, upto, fuse, x_scale)
 
     def forward(self, x, logical_idx, weights, avail_counter, policy: str = "lplb", x_scale=None):
         return self.forward_physical(x, self.route(logical_idx, avail_counter, policy), weights, x_scale=x_scale)
@@ -249,10 +266,9 @@ class MoELayer:
             y = self.forward(normed, idx, weights, avail_counter, policy)
         if shared is not None:
             w13, w13_scale, w2, w2_scale = shared
-            status = self.engine.status()
-            both = ops.matmul_fp8(q, scale, w13, w13_scale, out_dtype=torch.float32, status=status).unflatten(-1, (-1, 2, 128))
+            both = ops.matmul_fp8(q, scale, w13, w13_scale, out_dtype=torch.float32, status=self._status).unflatten(-1, (-1, 2, 128))
             act = (torch.nn.functional.silu(both[:, :, 0]) * both[:, :, 1]).flatten(1)
-            y = y + ops.matmul_fp8(*ops.quantize_fp8(act), w2, w2_scale, status=status)
+            y = y + ops.matmul_fp8(*ops.quantize_fp8(act), w2, w2_scale, status=self._status)
         return y, h
 
     def check(self) -> int:
@@ -260,7 +276,7 @@ class MoELayer:
         included; waits for the device.  ``reset`` clears it.  In the bounds-checking build an index that left
         its array is reported as code 6 (the access was skipped; ``engine.status()[16:28]`` holds the record)."""
         torch.cuda.synchronize(self.device)
-        status = self.engine.status().tolist()
+        status = self._status.tolist()
         return int(status[0] or status[16])
 
     def reset(self) -> None:

@@ -25,7 +25,11 @@ import torch
 from . import reference
 
 __all__ = [
+    "MOE_FEW_MAX_EXPERTS",
+    "MOE_FEW_MAX_HIDDEN",
+    "MOE_FEW_MAX_INTER",
     "MOE_FEW_MAX_TOKENS",
+    "MOE_FEW_MAX_TOPK",
     "quantize_fp8",
     "quantize_weight_fp8",
     "rms_norm_fp8",
@@ -36,6 +40,7 @@ __all__ = [
 
 
 MOE_FEW_MAX_TOKENS = 64  #: tokens that moe_few_tokens takes
+MOE_FEW_MAX_TOPK, MOE_FEW_MAX_EXPERTS, MOE_FEW_MAX_HIDDEN, MOE_FEW_MAX_INTER = 32, 512, 16384, 65536  # and the rest of its range
 
 _module = None
 
@@ -169,7 +174,7 @@ def moe_few_tokens(
     ``[tokens, hidden]``.  ``idx`` ``[tokens, topk]`` (int64 or int32) holds physical ids; -1 and ids that no expert has
     choose nothing, an expert chosen twice counts twice.  ``w13`` ``[experts, 2 * inter, hidden]`` is laid out in
     blocks of 128 gate rows and their 128 up rows (``lplb_b200.models.interleave_gate_up``), ``w2`` is ``[experts,
-    hidden, inter]``; ``hidden`` is a multiple of 256, ``inter`` of 128.
+    hidden, inter]``; ``hidden`` is a multiple of 256 up to 16384, ``inter`` of 128 up to 65536; up to 512 experts and 32 choices per token.
 
     bfloat16 weights take bfloat16 ``x`` and hold the activations in bfloat16.  Weights in 8 bits (``w13_scale``,
     ``w2_scale`` as :func:`quantize_weight_fp8` gives them) take ``x`` in 8 bits with its ``x_scale``, or in bfloat16,
@@ -184,15 +189,18 @@ def moe_few_tokens(
     wtype = torch.float8_e4m3fn if fp8 else torch.bfloat16
     _need(w13.dim() == 3 and w2.dim() == 3 and w13.dtype == wtype and w2.dtype == wtype, f"{who} w13 and w2 must be {wtype}")
     experts, inter, hidden = w13.shape[0], w13.shape[1] // 2, x.shape[1]
-    _need(hidden % 256 == 0 and hidden > 0 and inter % 128 == 0 and inter > 0, f"{who} hidden must be a multiple of 256, inter of 128")
+    _need(
+        hidden % 256 == 0 and 0 < hidden <= MOE_FEW_MAX_HIDDEN and inter % 128 == 0 and 0 < inter <= MOE_FEW_MAX_INTER,
+        f"{who} hidden must be a multiple of 256 (up to {MOE_FEW_MAX_HIDDEN}), inter of 128 (up to {MOE_FEW_MAX_INTER})",
+    )
     _need(
         w13.shape == (experts, 2 * inter, hidden) and w2.shape == (experts, hidden, inter),
         f"{who} w13 must be [experts, 2 * inter, hidden], w2 [experts, hidden, inter]",
     )
-    _need(1 <= experts <= 512, f"{who} 1 to 512 experts")
+    _need(1 <= experts <= MOE_FEW_MAX_EXPERTS, f"{who} 1 to {MOE_FEW_MAX_EXPERTS} experts")
     _need(x.dtype == (torch.bfloat16 if x_scale is None else torch.float8_e4m3fn), f"{who} x must be bfloat16, or float8_e4m3fn with x_scale")
     _need(idx.dim() == 2 and idx.shape[0] == x.shape[0] and idx.dtype in (torch.int64, torch.int32), f"{who} idx must be [tokens, topk]")
-    _need(1 <= idx.shape[1] <= 32, f"{who} 1 to 32 choices per token")
+    _need(1 <= idx.shape[1] <= MOE_FEW_MAX_TOPK, f"{who} 1 to {MOE_FEW_MAX_TOPK} choices per token")
     _need(weights.shape == idx.shape and weights.is_floating_point(), f"{who} weights must be floating point, of idx's shape")
     for scale, of in ((w13_scale, w13), (w2_scale, w2)):
         _need(scale is None or scale.shape == (experts, of.shape[1] // 128, of.shape[2] // 128), f"{who} scales must be [experts, rows / 128, cols / 128]")
