@@ -183,7 +183,7 @@ cudaError_t launch_rows_many(const Product& p, int device, cudaStream_t stream) 
 }  // namespace
 
 cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream) {
-  if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.groups < 1 || p.groups > kMaxGroups || p.m > INT32_MAX || p.groups * p.n > INT32_MAX)
+  if (p.m < 0 || p.n < 1 || p.k < 1 || p.k % 16 || p.groups < 1 || p.groups > kMaxGroups || p.m > kMaxRows || p.groups * p.n > kMaxRows)
     return cudaErrorInvalidValue;
   if (p.m == 0) return cudaSuccess;
   if (p.rows != nullptr) return launch_rows_many(p, device, stream);

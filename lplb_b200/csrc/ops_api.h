@@ -39,6 +39,7 @@ cudaError_t launch_weight_fp8(const void* w, Type type, int64_t matrices, int64_
 // With `rows`, matrix e belongs to rows[e] rows of a, which follow those of matrix e - 1; rows behind the last group are
 // neither read nor written.
 constexpr int kMaxGroups = 128;
+constexpr int kMaxRows = INT32_MAX - 255;  // of a, and of all matrices of b: no tile ends behind 2^31
 struct Product {
   const void* a;           // [m, k], row stride a_ld
   const void* b;           // [groups, n, k]

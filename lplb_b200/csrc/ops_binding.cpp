@@ -184,7 +184,8 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   OPS_CHECK(groups >= 1 && groups <= lplb::ops::kMaxGroups, "matmul_fp8: 1 to " + text(lplb::ops::kMaxGroups) + " groups");
   OPS_CHECK(!rows || (rows->device() == device && rows->scalar_type() == torch::kInt32 && rows->dim() == 1 && rows->size(0) == groups && rows->is_contiguous()),
             "matmul_fp8: rows must be contiguous int32, one number for each matrix of b, on a's device");
-  OPS_CHECK(m <= INT32_MAX && groups * n <= INT32_MAX, "matmul_fp8: more than 2^31 rows");
+  OPS_CHECK(m <= lplb::ops::kMaxRows && groups * n <= lplb::ops::kMaxRows,
+            "matmul_fp8: at most " + text(lplb::ops::kMaxRows) + " rows of a, and of all matrices of b together");
   OPS_CHECK(k >= 16 && k % 16 == 0 && b.size(-1) == k, "matmul_fp8: a and b must have the same k, a multiple of 16");
   OPS_CHECK(n >= 1 && n < (1 << 28), "matmul_fp8: b has no rows, or too many");
   OPS_CHECK(a.stride(1) == 1 && (m < 2 || (a.stride(0) % 16 == 0 && a.stride(0) >= k)) && reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0,

@@ -130,7 +130,7 @@ def matmul_fp8(
     ``rows[e]`` rows of ``a``, which follow those of matrix ``e - 1``; no more rows are taken than ``a`` has.  Rows behind
     the last group are left in ``out`` as they were (in a new ``out``: not set).
 
-    ``K`` is a multiple of 16; rows of ``a`` and of ``out`` may be apart from one another.  ``status``: see :func:`check`."""
+    ``K`` is a multiple of 16; ``a``, and all matrices of ``b`` together, have up to 2**31 - 256 rows; rows of ``a`` and of ``out`` may be apart from one another.  ``status``: see :func:`check`."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
     if a.is_cuda:
@@ -139,6 +139,8 @@ def matmul_fp8(
     _need(a.dim() == 2 and a.dtype == e4m3, "matmul_fp8: a must be [rows, k] of float8_e4m3fn")
     _need(b.dim() == 2 + lead and b.dtype == e4m3, "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn")
     m, k, n, blocks = *a.shape, b.shape[-2], -(-a.shape[1] // 128)
+    most = 2**31 - 256
+    _need(m <= most and n * (b.shape[0] if lead else 1) <= most, f"matmul_fp8: at most {most} rows of a, and of all matrices of b together")
     _need(k >= 16 and k % 16 == 0 and b.shape[-1] == k, "matmul_fp8: a and b must have the same k, a multiple of 16")
     _need(a_scale.dtype == e8m0 and a_scale.shape == (m, blocks), "matmul_fp8: a_scale must be [rows, ceil(k / 128)]")
     _need(
