@@ -40,8 +40,11 @@ __device__ __forceinline__ void finish(const RowFp8& a, float2 (&v)[4], const fl
   const uint32_t mine = magnitude8(v);
   const bool finite = all_finite(v);
   uint32_t top = block_max(mine);
-  if (NORM) top = __float_as_uint(__uint_as_float(top) * inv);
-  const uint32_t e = scale_exponent(min(top, 0x7F7FFFFFu));
+  if (NORM) {  // a factor that is NaN, or infinite times zero, leaves no finite value: as for a block of zeros
+    const float largest = __uint_as_float(top) * inv;
+    top = largest >= 0.f ? min(__float_as_uint(largest), 0x7F7FFFFFu) : 0u;
+  }
+  const uint32_t e = scale_exponent(top);
   float factor = reciprocal_of(e);
   if (NORM) {
     if (inv * factor < __uint_as_float(0x7F800000u)) {
