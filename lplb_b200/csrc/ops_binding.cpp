@@ -206,7 +206,10 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     OPS_CHECK(out->device() == device && out->scalar_type() == type && out->dim() == 2 && out->size(0) == m && out->size(1) == n &&
                   (out->stride(1) == 1 || n == 1) && (m < 2 || out->stride(0) >= n),
               "matmul_fp8: out must be [rows, n] of the output type on a's device, rows contiguous and apart from one another");
+    check_no_grad(*out, "matmul_fp8: out");
     result = *out;
+    // what autograd has saved of `out` is no longer what it was
+    if (!result.is_inference()) result.unsafeGetTensorImpl()->bump_version();
   } else {
     result = make({m, n}, type, a);
   }

@@ -150,6 +150,8 @@ def matmul_fp8(
     _need(rows is None or (rows.dtype == torch.int32 and rows.shape == b.shape[:1]), "matmul_fp8: rows must be int32, one for each matrix")
     _need(rows is None or b.shape[0] <= 128, "matmul_fp8: 1 to 128 groups")
     _need(out is None or (out.shape == (m, n) and out.dtype == out_dtype), "matmul_fp8: out must be [rows, n] of the output type")
+    if out is not None:
+        _check_no_grad(out, "matmul_fp8: out")
     result = reference.matmul_fp8_reference(a, a_scale, b, b_scale, rows).to(out_dtype)
     if out is None:
         return result
