@@ -113,7 +113,9 @@ def _scale_exponents(amax: torch.Tensor) -> torch.Tensor:
 
 
 def _powers(scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return torch.ldexp(torch.ones((), dtype=dtype, device=scale.device), scale.view(torch.uint8).to(dtype) - 127)
+    byte = scale.view(torch.uint8)
+    power = torch.ldexp(torch.ones((), dtype=dtype, device=scale.device), byte.to(dtype) - 127)
+    return torch.where(byte == 255, torch.full_like(power, float("nan")), power)  # the one byte of the type that is no power
 
 
 def dequantize_fp8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
