@@ -55,16 +55,6 @@ cudaError_t resident_clusters(int device, int split, Kernel kernel, int* cluster
   return err;
 }
 
-cudaError_t multiprocessors(int device, int* count) {
-  static std::atomic<int> known[kMaxDevices];
-  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
-  *count = known[device].load(std::memory_order_relaxed);
-  if (*count) return cudaSuccess;
-  cudaError_t err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
-  if (err == cudaSuccess) known[device].store(*count, std::memory_order_relaxed);
-  return err;
-}
-
 template <typename Out>
 cudaError_t launch_few(const Product& p, int device, cudaStream_t stream) {
   auto kernel = few_rows_kernel<Out>;

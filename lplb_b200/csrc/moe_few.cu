@@ -9,26 +9,14 @@ namespace lplb {
 namespace ops {
 namespace {
 
-int sm_count(int device) {
-  static std::atomic<int> known[kMaxDevices];
-  if (device < 0 || device >= kMaxDevices) return 1;
-  int n = known[device].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 1;
-    known[device].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 // The workspace's parts, one after the other on 256-byte boundaries.
 struct Parts {
   size_t plan_words, slot, token, pair, ready, act, act_scale, q, q_scale, partial, product, total;
   int slots, rows, cols, ctas, counters;
-  Parts(const MoeFew& m, int device) {
+  Parts(const MoeFew& m, int ctas_) : ctas(ctas_) {
     cols = (m.tokens + 15) / 16 * 16;
     rows = m.tokens * m.topk;
     slots = m.experts < rows ? m.experts : rows;
-    ctas = sm_count(device);
     counters = slots + slots * (m.inter / 128) + 1;
     const size_t value = m.w13_scale ? 1 : 2;
     size_t at = 0;
@@ -75,7 +63,12 @@ bool map_of(CUtensorMap* map, bool fp8, const void* base, uint64_t rows, uint64_
 
 }  // namespace
 
-size_t moe_few_workspace(const MoeFew& m, int device) { return Parts(m, device).total; }
+cudaError_t moe_few_workspace(const MoeFew& m, int device, size_t* bytes) {
+  int n = 0;
+  const cudaError_t err = multiprocessors(device, &n);
+  if (err == cudaSuccess) *bytes = Parts(m, n).total;
+  return err;
+}
 
 cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   const bool fp8 = m.w13_scale != nullptr;
@@ -84,7 +77,10 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
       (int64_t)m.experts * 2 * m.inter > INT32_MAX || (int64_t)m.experts * m.hidden > INT32_MAX)
     return cudaErrorInvalidValue;
   if (m.tokens == 0) return cudaSuccess;
-  const Parts at(m, device);
+  int n_sms = 0;
+  cudaError_t err = multiprocessors(device, &n_sms);
+  if (err != cudaSuccess) return err;
+  const Parts at(m, n_sms);
   char* ws = static_cast<char*>(m.workspace);
   MoeFewPlan plan;
   plan.slots = reinterpret_cast<int*>(ws + at.plan_words);
@@ -143,7 +139,6 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   a.x_words = a.x_scale_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x_scale) & 3) == 0;
   a.w_words = ((reinterpret_cast<uintptr_t>(a.w13_scale) | reinterpret_cast<uintptr_t>(a.w2_scale)) & 3) == 0;
   a.budget_ns = wait_budget_ns();
-  cudaError_t err = cudaSuccess;
   a.error = m.status;
   if (a.error == nullptr && (err = ops_error_word(device, &a.error)) != cudaSuccess) return err;
   CUtensorMap maps[4];
@@ -154,8 +149,7 @@ cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream) {
   auto kernel = moe_few_plan_kernel;
   err = launch_after(kernel, dim3(1 + (convert ? m.tokens : 0)), dim3(kFewPlanThreads), 0, stream, p);
   if (err != cudaSuccess) return err;
-  const int n = sm_count(device);
-  return fp8 ? launch<true>(a, maps, n, device, stream) : launch<false>(a, maps, n, device, stream);
+  return fp8 ? launch<true>(a, maps, n_sms, device, stream) : launch<false>(a, maps, n_sms, device, stream);
 }
 
 }  // namespace ops

@@ -83,7 +83,7 @@ struct MoeFew {
   int64_t x_ld, x_scale_ld;
   int idx_is64, tokens, topk, experts, hidden, inter;
 };
-size_t moe_few_workspace(const MoeFew& m, int device);
+cudaError_t moe_few_workspace(const MoeFew& m, int device, size_t* bytes);
 cudaError_t launch_moe_few(const MoeFew& m, int device, cudaStream_t stream);
 
 // First error that a kernel of these operators has seen on the current device (0: none).  It stays until it is cleared; reading
@@ -97,6 +97,8 @@ void set_wait_budget_ns(unsigned long long ns);
 // Where the kernels put it.
 constexpr int kMaxDevices = 64;
 cudaError_t ops_error_word(int device, int** word);
+// Multiprocessors of a device, asked for once.
+cudaError_t multiprocessors(int device, int* count);
 
 }  // namespace ops
 }  // namespace lplb

@@ -57,10 +57,9 @@ void check_no_grad(const Tensor& t, const char* who) {
 }
 
 int sm_count(int device) {
-  static int known[lplb::ops::kMaxDevices] = {};
-  if (device < 0 || device >= lplb::ops::kMaxDevices) return 1;
-  if (known[device] == 0) OPS_CUDA(cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device));
-  return known[device];
+  int n = 0;
+  OPS_CUDA(lplb::ops::multiprocessors(device, &n));
+  return n;
 }
 
 cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
@@ -308,7 +307,9 @@ Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights,
   m.inter = (int)inter;
   m.status = status_of(status, device, "moe_few_tokens");
   // a workspace of this call alone: calls on two streams, or two captured graphs, share nothing
-  auto workspace = make({(int64_t)lplb::ops::moe_few_workspace(m, index)}, torch::kUInt8, x);
+  size_t workspace_bytes = 0;
+  OPS_CUDA(lplb::ops::moe_few_workspace(m, index, &workspace_bytes));
+  auto workspace = make({(int64_t)workspace_bytes}, torch::kUInt8, x);
   m.workspace = workspace.data_ptr();
   OPS_CUDA(lplb::ops::launch_moe_few(m, index, stream_of(index)));
   return out;

@@ -22,6 +22,16 @@ cudaError_t ops_error_word(int device, int** word) {
   return cudaSuccess;
 }
 
+cudaError_t multiprocessors(int device, int* count) {
+  static std::atomic<int> known[kMaxDevices];
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  *count = known[device].load(std::memory_order_relaxed);
+  if (*count) return cudaSuccess;
+  cudaError_t err = cudaDeviceGetAttribute(count, cudaDevAttrMultiProcessorCount, device);
+  if (err == cudaSuccess) known[device].store(*count, std::memory_order_relaxed);
+  return err;
+}
+
 static std::atomic<unsigned long long> g_wait_budget_ns{kDefaultWaitBudgetNs};
 unsigned long long wait_budget_ns() { return g_wait_budget_ns.load(std::memory_order_relaxed); }
 void set_wait_budget_ns(unsigned long long ns) { g_wait_budget_ns.store(ns, std::memory_order_relaxed); }
