@@ -301,6 +301,11 @@ class MoeEngine {
     auto opts = torch::TensorOptions().dtype(sh_.fp8 ? torch::kFloat8_e4m3fn : torch::kBFloat16).device(torch::kCUDA, device_);
     return torch::from_blob(buf_.recv_x[sh_.my_rank], {sh_.capacity, sh_.hidden}, opts);
   }
+  torch::Tensor recv_scale() const {
+    MOE_CHECK(sh_.fp8, "rows in 16 bits have no scales");
+    auto opts = torch::TensorOptions().dtype(torch::kFloat8_e8m0fnu).device(torch::kCUDA, device_);
+    return torch::from_blob(buf_.recv_scale[sh_.my_rank], {sh_.capacity, sh_.hidden / 128}, opts);
+  }
   torch::Tensor recv_meta() const {
     auto opts = torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, device_);
     return torch::from_blob(buf_.recv_meta[sh_.my_rank], {sh_.capacity}, opts);
@@ -390,6 +395,7 @@ void bind_moe(py::module_& m) {
       .def("enable_debug", &MoeEngine::enable_debug)
       .def("epoch", &MoeEngine::epoch)
       .def("recv_x", &MoeEngine::recv_x)
+      .def("recv_scale", &MoeEngine::recv_scale)
       .def("recv_meta", &MoeEngine::recv_meta)
       .def("comb", &MoeEngine::comb);
 }
