@@ -60,8 +60,16 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(f"lplb_b200.ops.{message}")
 
 
+def _check_type(x: torch.Tensor, who: str) -> None:
+    _need(x.dtype in (torch.float32, torch.bfloat16, torch.float16), f"{who} must be float32, bfloat16 or float16, not {x.dtype}")
+
+
+def _check_device(who: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    _need(all(t is None or t.device == first.device for t in others), f"{who} all arguments must be on one device")
+
+
 def _check_rows(x: torch.Tensor, who: str) -> None:
-    _need(x.dtype in (torch.float32, torch.bfloat16, torch.float16), f"{who} must be float32, bfloat16 or float16")
+    _check_type(x, who)
     _need(x.dim() >= 1 and 1 <= x.shape[-1] <= 16384, f"{who} must have rows of 1 to 16384 values")
     _check_no_grad(x, who)
 
@@ -80,11 +88,12 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def quantize_weight_fp8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(q, scale)`` of contiguous weights ``[N, K]`` or ``[E, N, K]``: one scale per 128 x 128,
+    """``(q, scale)`` of contiguous weights ``[N, K]`` or ``[E, N, K]`` (float32, bfloat16 or float16): one scale per 128 x 128,
     ``[..., ceil(N / 128), ceil(K / 128)]``."""
     if w.is_cuda:
         return _native().quantize_weight_fp8(w)
     _need(w.dim() in (2, 3) and w.is_contiguous(), "quantize_weight_fp8: w must be contiguous [rows, cols] or [matrices, rows, cols]")
+    _check_type(w, "quantize_weight_fp8: w")
     _check_no_grad(w, "quantize_weight_fp8: w")
     return reference.quantize_weight_fp8_reference(w)
 
@@ -103,6 +112,7 @@ def rms_norm_fp8(
     if x.is_cuda:
         return _native().rms_norm_fp8(x, weight, residual, eps, return_normed)
     _check_rows(x, "rms_norm_fp8: x")
+    _check_device("rms_norm_fp8:", x, weight, residual)
     _check_no_grad(weight, "rms_norm_fp8: weight")
     _need(weight.shape == x.shape[-1:], "rms_norm_fp8: weight must have one value for each of a row")
     _need(weight.dtype in (x.dtype, torch.float32), "rms_norm_fp8: weight must be float32 or of x's type")
@@ -130,11 +140,14 @@ def matmul_fp8(
     ``rows[e]`` rows of ``a``, which follow those of matrix ``e - 1``; no more rows are taken than ``a`` has.  Rows behind
     the last group are left in ``out`` as they were (in a new ``out``: not set).
 
-    ``K`` is a multiple of 16; ``a``, and all matrices of ``b`` together, have up to 2**31 - 256 rows; rows of ``a`` and of ``out`` may be apart from one another.  ``status``: see :func:`check`."""
+    ``K`` is a multiple of 16; ``a``, and all matrices of ``b`` together, have up to 2**31 - 256 rows.  Rows of ``a``, of
+    ``a_scale`` and of ``out`` may be apart from one another; those of ``a`` start on 16-byte boundaries, as does ``b``, which is
+    contiguous with its scales.  ``status``: see :func:`check`."""
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"lplb_b200.ops.matmul_fp8: out_dtype must be bfloat16 or float32, not {out_dtype}")
     if a.is_cuda:
         return _native().matmul_fp8(a, a_scale, b, b_scale, rows, out, out_dtype == torch.float32, status)
+    _check_device("matmul_fp8:", a, a_scale, b, b_scale, rows, out)
     e4m3, e8m0, lead = torch.float8_e4m3fn, torch.float8_e8m0fnu, 0 if rows is None else 1
     _need(a.dim() == 2 and a.dtype == e4m3, "matmul_fp8: a must be [rows, k] of float8_e4m3fn")
     _need(b.dim() == 2 + lead and b.dtype == e4m3, "matmul_fp8: b must be [n, k] (with rows: [groups, n, k]) of float8_e4m3fn")
@@ -187,6 +200,7 @@ def moe_few_tokens(
     if x.is_cuda:
         return _native().moe_few_tokens(x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale, status)
     fp8, who = w13_scale is not None, "moe_few_tokens:"
+    _check_device(who, x, idx, weights, w13, w2, x_scale, w13_scale, w2_scale)
     _need(x.dim() == 2 and x.shape[0] <= MOE_FEW_MAX_TOKENS, f"{who} at most {MOE_FEW_MAX_TOKENS} tokens")
     _need(fp8 == (w2_scale is not None), f"{who} w13_scale and w2_scale come together")
     _need(fp8 or x_scale is None, f"{who} x_scale needs weights in 8 bits")
@@ -206,6 +220,8 @@ def moe_few_tokens(
     _need(idx.dim() == 2 and idx.shape[0] == x.shape[0] and idx.dtype in (torch.int64, torch.int32), f"{who} idx must be [tokens, topk]")
     _need(1 <= idx.shape[1] <= MOE_FEW_MAX_TOPK, f"{who} 1 to {MOE_FEW_MAX_TOPK} choices per token")
     _need(weights.shape == idx.shape and weights.is_floating_point(), f"{who} weights must be floating point, of idx's shape")
+    for scale in (x_scale, w13_scale, w2_scale):
+        _need(scale is None or scale.dtype == torch.float8_e8m0fnu, f"{who} scales must be float8_e8m0fnu")
     for scale, of in ((w13_scale, w13), (w2_scale, w2)):
         _need(scale is None or scale.shape == (experts, of.shape[1] // 128, of.shape[2] // 128), f"{who} scales must be [experts, rows / 128, cols / 128]")
     _need(x_scale is None or x_scale.shape == (x.shape[0], hidden // 128), f"{who} x_scale must be [tokens, hidden / 128]")
