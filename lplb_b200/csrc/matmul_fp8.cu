@@ -179,9 +179,9 @@ cudaError_t launch_matmul_fp8(const Product& p, int device, cudaStream_t stream)
   if (p.rows != nullptr) return launch_rows_many(p, device, stream);
   // More than 256 rows go to the CTA pairs, but for small products, whose tiles of 128 x 256 find an SM each and whose k is
   // short, up to 12 k blocks of a tile per SM.  One CTA per tile starts sooner and splits k; the pairs read less from the
-  // L2.  In us, this kernel and the pairs: 400 x 1000 x 4096 (3.5 blocks per SM) 9.1, 10.9; 600 x 4096 x 1024 (5.2) 7.9,
-  // 9.5; 2000 x 1000 x 2048 (6.9) 8.8, 10.3; 3916 x 353 x 5568 (14) 18.6, 16.2; 1024 x 2048 x 7168 (24) 24.3, 18.3; 1500 x
-  // 4096 x 512 (192 tiles) 13.0, 11.8.
+  // L2.  In us, this kernel and the pairs: 400 x 1000 x 4096 (3.5 blocks per SM) 9.0, 11.7; 600 x 4096 x 1024 (5.2) 7.7,
+  // 9.9; 2000 x 1000 x 2048 (6.9) 8.1, 10.6; 3916 x 353 x 5568 (14) 22.2, 17.1; 1024 x 2048 x 7168 (24) 28.7, 19.7; 1500 x
+  // 4096 x 512 (192 tiles) 12.7, 12.0.
   if (p.m > kFewMaxRows) {
     int n_sm = 0;
     if (cudaError_t err = multiprocessors(device, &n_sm)) return err;

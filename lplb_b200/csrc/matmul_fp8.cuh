@@ -5,7 +5,7 @@
 // on the tensor core's M side, so that few rows cost few cycles, and the k blocks of a tile are dealt out to the CTAs of a
 // cluster, so that a matrix with few tiles still occupies every SM.  The partial sums meet in distributed shared
 // memory, in rank order: no workspace, nothing to clear, the same bits every time.  64 x 4096 x 7168 (29.8 MB) take
-// 9.4 us among others, 3.2 TB/s; 1 x 7168 x 2048 5.4 us: launch, the first load and the join are half of it.
+// 10.4 us among others, 2.9 TB/s; 1 x 7168 x 2048 5.4 us: launch, the first load and the join are half of it.
 //
 // Roles (256 threads): warp 0 TMA producer, warp 1 matrix instructions, warp 2 scales, warps 4-7
 // epilogue; all of them add up the partial sums.
