@@ -82,8 +82,8 @@ constexpr int kMaxLocalExperts = 128;
 constexpr int kMaxRanks = 8;
 
 // Operands in 8 bits (FP8): a k block is 128 values = 128 bytes again, and the scales take 12 columns of
-// tensor memory, so an accumulator has 224 columns; a seventh warp stages the scales of four k blocks
-// at a time, and shared memory for them comes out of the ring.  The tensor pipe is 89 % active (8192 x 4096 x 7168: 165 us
+// tensor memory, so an accumulator has 224 columns; a seventh warp stages the scales of 16 k blocks
+// at a time, four to a slot, and shared memory for them comes out of the ring.  The tensor pipe is 89 % active (8192 x 4096 x 7168: 165 us
 // in one launch, 2.9 PFLOP/s, at the 1.35 GHz that the power cap leaves; 196-214 us in a loop).
 constexpr int kBNFp8 = 224;
 constexpr int kGemmThreadsFp8 = kGemmThreads + 32;

@@ -331,7 +331,10 @@ void bind_ops(py::module_& m) {
   m.def("matmul_fp8", &matmul_fp8);
   m.def("moe_few_tokens", &moe_few_tokens);
   m.def("ops_error", &ops_error);
-  m.def("set_ops_timeout_us", [](double us) { lplb::ops::set_wait_budget_ns((unsigned long long)(us * 1e3)); });
+  m.def("set_ops_timeout_us", [](double us) {
+    OPS_CHECK(us >= 0 && us <= 1e9, "set_ops_timeout_us: between 0 and 1e9");
+    lplb::ops::set_wait_budget_ns((unsigned long long)(us * 1e3));
+  });
   m.attr("MOE_FEW_MAX_TOKENS") = lplb::ops::kMoeFewMaxTokens;
   m.attr("MOE_FEW_MAX_TOPK") = lplb::ops::kMoeFewMaxTopk;
   m.attr("MOE_FEW_MAX_EXPERTS") = lplb::ops::kMoeFewMaxExperts;

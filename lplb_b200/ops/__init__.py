@@ -2,7 +2,19 @@
 the 8-bit serving operators that stand around a mixture-of-experts layer."""
 
 from . import reference
-from .fp8 import MOE_FEW_MAX_HIDDEN, MOE_FEW_MAX_INTER, MOE_FEW_MAX_TOKENS, MOE_FEW_MAX_TOPK, check, matmul_fp8, moe_few_tokens, quantize_fp8, quantize_weight_fp8, rms_norm_fp8
+from .fp8 import (
+    MOE_FEW_MAX_EXPERTS,
+    MOE_FEW_MAX_HIDDEN,
+    MOE_FEW_MAX_INTER,
+    MOE_FEW_MAX_TOKENS,
+    MOE_FEW_MAX_TOPK,
+    check,
+    matmul_fp8,
+    moe_few_tokens,
+    quantize_fp8,
+    quantize_weight_fp8,
+    rms_norm_fp8,
+)
 from .reference import (
     count_reference,
     dequantize_fp8,
@@ -13,6 +25,7 @@ from .reference import (
 )
 
 __all__ = [
+    "MOE_FEW_MAX_EXPERTS",
     "MOE_FEW_MAX_HIDDEN",
     "MOE_FEW_MAX_INTER",
     "MOE_FEW_MAX_TOKENS",

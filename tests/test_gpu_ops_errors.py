@@ -85,6 +85,12 @@ def test_a_wait_that_runs_out_ends_the_call_with_its_code(make):
     assert call() and ops.check() == 0
 
 
+@pytest.mark.parametrize("us", [-1.0, float("nan"), float("inf")])
+def test_a_limit_that_is_none_is_refused(us):
+    with pytest.raises(ValueError, match="set_ops_timeout_us"):
+        _native.load().set_ops_timeout_us(us)
+
+
 # ------------------------------------------------------------------------------------------- whose error it is
 def _model(dtype, hidden=512, inter=256, few=False):
     from lplb_b200 import Planner, cube
