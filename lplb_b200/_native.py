@@ -57,6 +57,9 @@ SOURCES = [
     "norm_fp8.cu",
     "matmul_fp8.cu",
     "moe_few.cu",
+    "experts_binding.cpp",
+    "gate.cu",
+    "expert_rows.cu",
 ]
 
 NVCC_FLAGS = [

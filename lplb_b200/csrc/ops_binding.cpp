@@ -1,76 +1,13 @@
 // Python binding of the 8-bit serving operators: checks of the arguments, outputs, launches on the
 // current stream of the arguments' device.  The reference has no operators of this kind.
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <pybind11/pybind11.h>
-#include <pybind11/stl.h>
-#include <torch/extension.h>
-
-#include <optional>
-#include <stdexcept>
-#include <string>
-
-#include "ops_api.h"
+#include "ops_check.h"
 
 namespace py = pybind11;
 
 namespace {
 
-using torch::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-// A refused argument is a ValueError, a failed launch a RuntimeError.  Messages are put together from strings: a
-// number written to an ostringstream ends the process where the compiler's C++ library is newer than the one that
-// is loaded.
-#define OPS_CHECK(cond, msg)                                                       \
-  do {                                                                             \
-    if (!(cond)) throw std::invalid_argument(std::string("lplb_b200.ops.") + msg); \
-  } while (0)
-
-#define OPS_CUDA(expr)                                                                                            \
-  do {                                                                                                            \
-    cudaError_t err_ = (expr);                                                                                    \
-    if (err_ != cudaSuccess)                                                                                      \
-      throw std::runtime_error(std::string("lplb_b200.ops: " #expr " failed: ") + cudaGetErrorName(err_) + ": " + \
-                               cudaGetErrorString(err_));                                                         \
-  } while (0)
-
-std::string text(int64_t n) { return std::to_string(n); }
-std::string text(at::ScalarType type) { return c10::toString(type); }
-
 constexpr int64_t kBlock = 128;
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
-
-lplb::ops::Type type_of(const Tensor& t, const char* who) {
-  switch (t.scalar_type()) {
-    case torch::kFloat32: return lplb::ops::Type::kF32;
-    case torch::kBFloat16: return lplb::ops::Type::kBf16;
-    case torch::kFloat16: return lplb::ops::Type::kF16;
-    default: OPS_CHECK(false, who + std::string(" must be float32, bfloat16 or float16, not ") + text(t.scalar_type()));
-  }
-  return lplb::ops::Type::kF32;
-}
-
-void check_no_grad(const Tensor& t, const char* who) {
-  OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who + std::string(" requires a gradient: these operators have no backward pass (use torch.no_grad())"));
-}
-
-int sm_count(int device) {
-  int n = 0;
-  OPS_CUDA(lplb::ops::multiprocessors(device, &n));
-  return n;
-}
-
-cudaStream_t stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
-
-// Rows of the last dimension as one matrix, without a copy wherever the strides allow it.
-Tensor as_rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
-
-// An output on x's device, without the dispatcher's microsecond.
-Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& x) { return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt); }
-
-uint8_t* bytes(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
   auto shape = t.sizes().vec();

@@ -1,7 +1,18 @@
-"""Operators: plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path), and
-the 8-bit serving operators that stand around a mixture-of-experts layer."""
+"""Operators: plain PyTorch statements of the planner's kernels (the numerics oracles and the CPU path), the
+8-bit serving operators that stand around a mixture-of-experts layer, and the operators around and inside its experts in
+16 and 32 bits, with their gradients."""
 
 from . import reference
+from .experts import (
+    GATE_MAX_EXPERTS,
+    GATE_MAX_TOPK,
+    ORDER_MAX_EXPERTS,
+    ExpertOrder,
+    combine_rows,
+    expert_order,
+    gate_topk,
+    take_rows,
+)
 from .fp8 import (
     MOE_FEW_MAX_EXPERTS,
     MOE_FEW_MAX_HIDDEN,
@@ -43,4 +54,12 @@ __all__ = [
     "matmul_fp8",
     "moe_few_tokens",
     "check",
+    "GATE_MAX_EXPERTS",
+    "GATE_MAX_TOPK",
+    "ORDER_MAX_EXPERTS",
+    "ExpertOrder",
+    "gate_topk",
+    "expert_order",
+    "take_rows",
+    "combine_rows",
 ]

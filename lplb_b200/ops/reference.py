@@ -14,7 +14,9 @@ are what ``Planner`` executes when it is built on a CPU device.
 
 The 8-bit serving operators (``lplb_b200.ops.fp8``) are restated below in 32 bits, or in 64 where their
 inputs are: ``quantize_fp8_reference``, ``rms_norm_fp8_reference``, ``matmul_fp8_reference``,
-``moe_few_tokens_reference``.
+``moe_few_tokens_reference``.  So are the operators around a layer's experts (``lplb_b200.ops.experts``):
+``gate_topk_reference``, ``expert_order_reference``, ``take_rows_reference``, ``combine_rows_reference`` and the
+gradients of the first and the last.
 """
 
 from __future__ import annotations
@@ -33,6 +35,12 @@ __all__ = [
     "rms_norm_fp8_reference",
     "matmul_fp8_reference",
     "moe_few_tokens_reference",
+    "gate_topk_reference",
+    "gate_topk_backward_reference",
+    "expert_order_reference",
+    "take_rows_reference",
+    "combine_rows_reference",
+    "combine_rows_backward_reference",
 ]
 
 _BLOCK = 256
@@ -220,3 +228,100 @@ def moe_few_tokens_reference(
         act = dequantize_fp8(*quantize_fp8_reference(act), dtype) if fp8 else act.bfloat16().to(dtype)
         out.index_add_(0, tok, act @ down.T * weights[tok, k].to(dtype).unsqueeze(1))
     return out
+
+
+def _scores(x: torch.Tensor, most: torch.Tensor, score: str, renormalize: bool) -> torch.Tensor:
+    """Scores of logits ``x`` in rows whose largest is ``most`` (finite); for a renormalised weight up to a factor of the row."""
+    if score == "softmax":
+        return torch.exp(x - most)
+    over = most.clamp_max(0) if renormalize else torch.zeros_like(most)
+    return torch.exp(x.clamp_max(0) - over) / (1 + torch.exp(-x.abs()))
+
+
+def gate_topk_reference(
+    logits: torch.Tensor, topk: int, score: str = "softmax", renormalize: bool = False, scale: float = 1.0
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(weights, idx)`` of the largest logits (kernel: ``gate_kernel`` in ``csrc/gate.cu``)."""
+    x = _wide(logits)
+    top, idx = torch.sort(x, dim=-1, descending=True, stable=True)  # NaN first; equal ones in the order of experts
+    top, idx = top[:, :topk], idx[:, :topk]
+    there = ~torch.isneginf(top)
+    most = torch.where(there[:, :1], top[:, :1], torch.zeros_like(top[:, :1]))
+    w = torch.where(there, _scores(top, most, score, renormalize), torch.zeros_like(top))
+    if renormalize:
+        w = w / torch.where(there[:, :1], w.sum(-1, keepdim=True), torch.ones_like(most))
+    elif score == "softmax":
+        w = w / torch.where(there[:, :1], _scores(x, most, score, False).sum(-1, keepdim=True), torch.ones_like(most))
+    return torch.where(there, scale * w, torch.zeros_like(w)), torch.where(there, idx, torch.full_like(idx, -1))
+
+
+def gate_topk_backward_reference(
+    logits: torch.Tensor, idx: torch.Tensor, dweights: torch.Tensor, score: str = "softmax", renormalize: bool = False, scale: float = 1.0
+) -> torch.Tensor:
+    """The logits' gradient (kernel: ``gate_backward_kernel``)."""
+    x = _wide(logits)
+    there = idx >= 0
+    at = idx.clamp_min(0)
+    mine = torch.where(there, x.gather(1, at), torch.zeros_like(x[:, :1]))
+    w = gate_topk_reference(logits, idx.shape[1], score, renormalize)[0]
+    d = torch.where(there, scale * dweights.to(x.dtype), torch.zeros_like(w))
+    along = (d * w).sum(-1, keepdim=True)
+    dx = torch.zeros_like(x)
+    if renormalize:
+        each = w * (d - along)
+    else:
+        each = w * d
+        if score == "softmax":
+            alive = there[:, :1].expand_as(x)
+            p = torch.softmax(torch.where(alive, x, torch.zeros_like(x)), -1)
+            dx = torch.where(alive, -along * p, dx)
+    if score == "sigmoid":
+        each = each / (1 + torch.exp(mine))
+    dx.scatter_add_(1, at, torch.where(there, each, torch.zeros_like(each)))
+    return dx.to(logits.dtype)
+
+
+def expert_order_reference(idx: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(counts, place, source)`` of a stable sort by expert (kernel: ``order_kernel`` in ``csrc/expert_rows.cu``)."""
+    flat = idx.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < n_experts), flat, torch.full_like(flat, n_experts))
+    key, pair = torch.sort(key, stable=True)
+    there = key < n_experts
+    at = torch.arange(flat.numel(), device=flat.device)
+    counts = torch.bincount(key, minlength=n_experts + 1)[:n_experts]
+    place = torch.empty_like(flat)
+    place[pair] = torch.where(there, at, torch.full_like(at, -1))
+    return counts.int(), place.view(idx.shape).int(), torch.where(there, pair, torch.full_like(pair, -1)).int()
+
+
+def take_rows_reference(x: torch.Tensor, place: torch.Tensor, source: torch.Tensor) -> torch.Tensor:
+    """A row for every choice, in the order of experts; zeros behind the last (kernel: ``take_rows_kernel``)."""
+    raw = x if x.element_size() > 1 else x.view(torch.uint8)
+    if raw.shape[0] == 0:
+        return x.new_empty(0, x.shape[1])
+    rows = raw[source.clamp_min(0).long() // place.shape[1]]
+    return torch.where((source >= 0).unsqueeze(1), rows, torch.zeros_like(rows)).view(x.dtype)
+
+
+def combine_rows_reference(rows: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows of a token's choices, weighted and added up, rounded once (kernel: ``combine_rows_kernel``)."""
+    out = _wide(rows.new_zeros(place.shape[0], rows.shape[1]))
+    for k in range(place.shape[1] if rows.shape[0] else 0):
+        there, at = (place[:, k] >= 0).unsqueeze(1), place[:, k].clamp_min(0).long()
+        y = _wide(rows[at])
+        out += torch.where(there, y if weights is None else y * weights[:, k : k + 1].to(y.dtype), torch.zeros_like(y))
+    return out.to(rows.dtype)
+
+
+def combine_rows_backward_reference(
+    dout: torch.Tensor, rows: torch.Tensor, place: torch.Tensor, weights: torch.Tensor
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of rows and weights (kernel: ``combine_rows_backward_kernel``)."""
+    d, y = _wide(dout), _wide(rows)
+    drows, dweights = torch.zeros_like(y), d.new_zeros(place.shape)
+    for k in range(place.shape[1] if rows.shape[0] else 0):
+        token = (place[:, k] >= 0).nonzero().squeeze(1)
+        at = place[token, k].long()
+        drows[at] = d[token] * weights[token, k : k + 1].to(d.dtype)
+        dweights[token, k] = (d[token] * y[at]).sum(-1)
+    return drows.to(rows.dtype), dweights
