@@ -31,8 +31,15 @@ inline int encode_tensor_map(CUtensorMap* out, CUtensorMapDataType type, const v
   if (!fn) return -1;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || strides[0] % 16) return -2;
   const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
-  const CUresult rc = fn(out, type, rank, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(out, type, rank, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = encode();
+  // The driver's call wants a current context, which a thread that has not called the runtime yet (a backward pass's, whose first
+  // kernel this is) does not have: the runtime makes one current when the device is set.
+  int device = 0;
+  if (rc == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) rc = encode();
   return rc == CUDA_SUCCESS ? 0 : (int)rc;
 }
 
