@@ -60,6 +60,8 @@ SOURCES = [
     "experts_binding.cpp",
     "gate.cu",
     "expert_rows.cu",
+    "matmul_binding.cpp",
+    "matmul.cu",
 ]
 
 NVCC_FLAGS = [

@@ -619,6 +619,7 @@ torch::Tensor debug_reciprocals(const torch::Tensor& x) {
 void bind_moe(py::module_& m);  // moe_binding.cpp
 void bind_ops(py::module_& m);  // ops_binding.cpp
 void bind_expert_ops(py::module_& m);  // experts_binding.cpp
+void bind_matmul(py::module_& m);  // matmul_binding.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "lplb_b200 native runtime (sm_100a)";
@@ -665,6 +666,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_moe(m);
   bind_ops(m);
   bind_expert_ops(m);
+  bind_matmul(m);
   m.attr("MAX_GROUP_SIZE") = lplb::kMaxGroupSize;
   m.attr("MAX_DUP") = lplb::kMaxDup;
   m.attr("MAX_LOGICAL_EXPERTS") = lplb::kMaxLogicalExperts;

@@ -1,0 +1,464 @@
+// Launchers of the product with an epilogue and of its gradients, and the kernel that takes a gradient through the activation.
+#include "matmul_api.h"
+
+#include <atomic>
+
+#include "matmul.cuh"
+#include "matmul_few.cuh"
+#include "tensor_map.h"
+
+namespace lplb {
+namespace ops {
+
+namespace {
+
+// ---- the activation's gradient -----------------------------------------------------------------------
+// dz = dout * act'(z), rounded to the operands' type for the products behind it, and the sum of dz (before the rounding) over
+// parts of a group's rows.  A CTA has 256 columns of z, a part of a group's rows, eight of them at a time; bound by DRAM.
+constexpr int kPreColumns = 256, kPreRows = 8;
+
+__device__ __forceinline__ float slope(float z, int activation) {
+  if (activation == kSilu) {
+    const float s = sigmoid_of(z);
+    return s * (1.f + z * (1.f - s));
+  }
+  if (activation == kGelu) return normcdff(z) + z * 0.3989422804f * __expf(-0.5f * z * z);  // 1 / sqrt(2 pi)
+  return 1.f;
+}
+__device__ __forceinline__ float through(float d, float z, int activation) {
+  return activation == kRelu ? (z > 0.f ? d : 0.f) : d * slope(z, activation);
+}
+
+struct PreArgs {
+  const void* dout;
+  const void* pre;
+  const int* rows;
+  void* dz;
+  void* dbias;   // where one part is all of a group
+  float* parts;  // [groups, splits, n]
+  int64_t dout_ld, pre_ld, dz_ld;
+  int m, n, groups, splits, activation;
+  Type type, out_type, bias_type;
+};
+
+// VEC: everything is there in whole vectors of four values
+template <bool VEC, bool GATED>
+__global__ void __launch_bounds__(256) pre_gradient_kernel(const PreArgs a) {
+  constexpr int S = VEC ? 1 : GATED ? 32 : 64;          // the thread's columns are this far apart
+  constexpr int kVectors = GATED ? 1 : 2;               // of four columns: 32 lanes x 4 (and 128 behind, or the up columns)
+  constexpr int kNext = VEC ? 128 : 32;                 // from the thread's first vector to its second
+  __shared__ float s_sum[kPreRows][kPreColumns];
+  __shared__ long long s_before[8];
+  allow_successor();
+  wait_predecessors();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int split = blockIdx.y, group = blockIdx.z;
+  int from = 0, rows = a.m;
+  if (a.rows != nullptr) {  // the group's rows, none beyond the last
+    long long before = 0;
+    for (int e = threadIdx.x; e < group; e += 256) before += max(a.rows[e], 0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (lane == 0) s_before[warp] = before;
+    __syncthreads();
+    before = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) before += s_before[w];
+    from = (int)min((long long)a.m, before);
+    rows = (int)min((long long)a.m - from, (long long)max(a.rows[group], 0));
+  }
+  const int r0 = from + (int)((int64_t)rows * split / a.splits), r1 = from + (int)((int64_t)rows * (split + 1) / a.splits);
+  // the first column of a vector in dout, and in z
+  int at_out[kVectors], at_z[kVectors], limit[kVectors];
+#pragma unroll
+  for (int v = 0; v < kVectors; ++v) {
+    const int f = (VEC ? 4 * lane : lane) + v * kNext;
+    at_out[v] = GATED ? blockIdx.x * kGateBlock + f : blockIdx.x * kPreColumns + f;
+    at_z[v] = blockIdx.x * kPreColumns + f;
+    limit[v] = GATED ? 4 * S : a.n - at_z[v];
+  }
+  float sum[2][4] = {};
+  for (int r = r0 + warp; r < r1; r += kPreRows) {
+    float d[2][4] = {}, z[2][4] = {};
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+      load4<S>(a.dout, a.out_type, r * a.dout_ld + at_out[v], limit[v], d[v]);
+      if (a.pre != nullptr) load4<S>(a.pre, a.out_type, r * a.pre_ld + at_z[v], limit[v], z[v]);
+    }
+    if (GATED) {
+      load4<S>(a.pre, a.out_type, r * a.pre_ld + at_z[0] + kGateBlock, limit[0], z[1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float s = sigmoid_of(z[0][j]), g = d[0][j];
+        d[0][j] = g * z[1][j] * s * (1.f + z[0][j] * (1.f - s));
+        d[1][j] = g * z[0][j] * s;
+      }
+    } else if (a.activation != kNoActivation) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[v][j] = through(d[v][j], z[v][j], a.activation);
+    }
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      if (a.dz != nullptr) {
+        const int i = GATED ? 0 : v;
+        store4<S>(a.dz, a.type, r * a.dz_ld + at_z[i] + (GATED && v ? kGateBlock : 0), limit[i], d[v]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[v][j] += d[v][j];
+    }
+  }
+  if (a.dbias == nullptr && a.parts == nullptr) return;
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s_sum[warp][(VEC ? 4 * lane : lane) + j * S + (GATED ? v * kGateBlock : v * kNext)] = sum[v][j];
+  __syncthreads();
+  const int column = blockIdx.x * kPreColumns + threadIdx.x;
+  if (column >= a.n) return;
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPreRows; ++w) all += s_sum[w][threadIdx.x];
+  if (a.parts != nullptr)
+    a.parts[((int64_t)group * a.splits + split) * a.n + column] = all;
+  else
+    store_float(a.dbias, a.bias_type, (int64_t)group * a.n + column, all);
+}
+
+// dbias[g, c] = sum of its parts, in their order
+__global__ void __launch_bounds__(256) bias_parts_kernel(const float* parts, void* dbias, Type type, int64_t n, int splits, int64_t total) {
+  allow_successor();
+  wait_predecessors();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t group = i / n, column = i - group * n;
+  const float* from = parts + group * splits * n + column;
+  float all = 0.f;
+  for (int s = 0; s < splits; ++s) all += from[s * n];
+  store_float(dbias, type, i, all);
+}
+
+uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+// Whether four neighbouring values of rows `ld` apart always start on a boundary of their size.
+bool fours(const void* p, int64_t ld, Type type) { return p == nullptr || (ld % 4 == 0 && address(p) % (type == Type::kF32 ? 16 : 8) == 0); }
+
+// ---- tensor maps ----------------------------------------------------------------------------------------
+constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_UINT16;  // TMA copies bits; the zeros it fills in are those of both types
+
+// [rows, cols] with rows `ld` apart, boxes of 64 columns
+cudaError_t map_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)kPairK, box_rows};
+  return encode_tensor_map(map, kMapType, base, 2, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+// [matrices, rows, cols]: zeros behind a matrix's last row, not the next one's values
+cudaError_t map_3d(CUtensorMap* map, const void* base, uint64_t matrices, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  const cuuint64_t dims[3] = {cols, rows, matrices}, strides[2] = {cols * 2, rows * cols * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)kPairK, box_rows, 1};
+  return encode_tensor_map(map, kMapType, base, 3, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+// Weights in blocks of 128 gate rows and their 128 up rows, dealt out so that 32 rows in shared memory are 16 gate rows and their
+// 16 up rows.
+cudaError_t map_gated(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
+  const cuuint64_t row = cols * 2;
+  const cuuint64_t dims[5] = {cols, 16, 2, kGateBlock / 16, rows / (2 * kGateBlock)};
+  const cuuint64_t strides[4] = {row, kGateBlock * row, 16 * row, 2 * kGateBlock * row};
+  const cuuint32_t box[5] = {(cuuint32_t)kPairK, 16, 2, kHalfM / 32, 1};
+  return encode_tensor_map(map, kMapType, base, 5, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+cudaError_t maps_of_rows(PairMaps* maps, const void* base, uint64_t rows, uint64_t cols, uint64_t ld) {
+  cudaError_t err = cudaSuccess;
+  for (int b = 0; b < 4 && err == cudaSuccess; ++b) err = map_2d(&maps->q[b], base, rows, cols, ld, kPairN / 2 >> b);
+  return err;
+}
+
+// ---- CTA pairs --------------------------------------------------------------------------------------------
+// One group: result rows in tiles of equal height, so high that the fewest rounds over the CTA pairs come out (a tile costs its
+// steps and about one more).  Several groups: their rows are only known on the device.
+int steps_per_tile(int64_t rows, int step, int64_t tiles_p, int n_sm, bool grouped) {
+  const int most = kPairN / step;
+  if (grouped) return most;
+  const int64_t steps = (rows + step - 1) / step;
+  int64_t least = INT64_MAX;
+  int best = most;
+  for (int s = most; s >= 1; --s) {
+    if (s * step < 64 && steps > 1) break;
+    const int64_t tiles = (steps + s - 1) / s, high = (steps + tiles - 1) / tiles;
+    const int64_t cost = (tiles * tiles_p + n_sm / 2 - 1) / (n_sm / 2) * (high * step + 32);
+    if (cost < least) least = cost, best = (int)high;
+  }
+  return best;
+}
+
+template <Mode MODE>
+cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStream_t stream) {
+  auto kernel = pair_matmul_kernel<MODE>;
+  static std::atomic<bool> prepared[kMaxDevices];
+  int n_sm = 0;
+  cudaError_t err = multiprocessors(device, &n_sm);
+  if (err != cudaSuccess) return err;
+  if (!prepared[device].load(std::memory_order_relaxed)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem);
+    if (err != cudaSuccess) return err;
+    prepared[device].store(true, std::memory_order_relaxed);
+  }
+  if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
+  a.budget_ns = wait_budget_ns();
+  a.tiles_p = (a.features + kPairM - 1) / kPairM;
+  a.tile_steps = steps_per_tile(MODE == kWeight ? a.result_rows : a.n_rows, PairTile<MODE>::kStep, a.tiles_p, n_sm, a.rows != nullptr && MODE != kWeight);
+  return launch_after(kernel, dim3(n_sm & ~1), dim3(kPairThreads), kPairSmem, stream, maps, a);
+}
+
+Epilogue epilogue_of(const Matmul& p) {
+  Epilogue e{};
+  e.bias = p.bias;
+  e.residual = p.residual;
+  e.out = p.out;
+  e.pre = p.pre;
+  e.residual_ld = p.residual_ld;
+  e.out_ld = p.out_ld;
+  e.pre_ld = p.pre_ld;
+  e.n = (int)p.n;
+  e.activation = p.activation;
+  e.type = p.out_type;
+  e.bias_type = p.bias_type;
+  return e;
+}
+int is_wide(const Matmul& p) {
+  return p.n % 4 == 0 && fours(p.out, p.out_ld, p.out_type) && fours(p.residual, p.residual_ld, p.out_type) && fours(p.pre, p.pre_ld, p.out_type) &&
+         fours(p.bias, p.n, p.bias_type);
+}
+
+cudaError_t launch_forward(const Matmul& p, int device, cudaStream_t stream) {
+  PairMaps maps{};
+  PairArgs a{};
+  a.rows = p.rows;
+  a.groups = p.rows ? p.groups : 1;
+  a.n_rows = (int)p.m;
+  a.features = (int)p.n;
+  a.k_blocks = (int)((p.k + kPairK - 1) / kPairK);
+  a.wide = is_wide(p);
+  a.idesc = sm100::umma_idesc_16(p.type == Type::kBf16, false, false);
+  a.e = epilogue_of(p);
+  cudaError_t err = maps_of_rows(&maps, p.a, p.m, p.k, p.a_ld);
+  if (err != cudaSuccess) return err;
+  if (p.activation == kSwiglu) {
+    if ((err = map_gated(&maps.p[0], p.b, (uint64_t)a.groups * p.n, p.k)) != cudaSuccess) return err;
+    return launch_pairs<kForwardGated>(maps, a, device, stream);
+  }
+  if ((err = map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kHalfM)) != cudaSuccess) return err;
+  return launch_pairs<kForward>(maps, a, device, stream);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------
+// Half of an SM's shared memory: the next kernel's CTAs can set themselves up beside these.
+constexpr uint32_t kFewRing = 96 * 1024;
+constexpr int kFewSmem = 256 * kFewSmemPerColumn > 1024 + kFewMostRows * kFewTileRows * 4 + 1024 ? 256 * kFewSmemPerColumn : 2048 + kFewMostRows * kFewTileRows * 4;
+
+template <typename Kernel>
+cudaLaunchConfig_t few_config(cudaLaunchAttribute (&attrs)[2], int ctas, int split, uint32_t smem, cudaStream_t stream, Kernel) {
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = split;
+  attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(kFewBlock);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attrs;
+  config.numAttrs = 2;
+  return config;
+}
+// Clusters of `split` CTAs that the device holds at once, one CTA per SM.
+template <typename Kernel>
+cudaError_t resident_clusters(int device, int split, Kernel kernel, int* clusters) {
+  static std::atomic<int> known[kMaxDevices][kFewMostSplit + 1];
+  *clusters = known[device][split].load(std::memory_order_relaxed);
+  if (*clusters > 0) return cudaSuccess;
+  cudaLaunchAttribute attrs[2]{};
+  cudaLaunchConfig_t config = few_config(attrs, split, split, kFewSmem, nullptr, kernel);
+  config.numAttrs = 1;
+  const cudaError_t err = cudaOccupancyMaxActiveClusters(clusters, kernel, &config);
+  if (err == cudaSuccess) known[device][split].store(*clusters, std::memory_order_relaxed);
+  return err;
+}
+
+template <bool GATED>
+cudaError_t launch_few(const Matmul& p, int device, cudaStream_t stream) {
+  auto kernel = few_product_kernel<GATED>;
+  static std::atomic<bool> prepared[kMaxDevices];
+  cudaError_t err = cudaSuccess;
+  if (!prepared[device].load(std::memory_order_relaxed)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    if (err != cudaSuccess) return err;
+    prepared[device].store(true, std::memory_order_relaxed);
+  }
+  FewProductArgs a{};
+  if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
+  a.budget_ns = wait_budget_ns();
+  a.m = (int)p.m;
+  a.k_blocks = (int)((p.k + kPairK - 1) / kPairK);
+  a.wide = is_wide(p);
+  a.idesc = sm100::umma_idesc_16(p.type == Type::kBf16, false, false);
+  a.e = epilogue_of(p);
+  a.tiles = (int)((p.n + kFewTileRows - 1) / kFewTileRows);
+  // How many CTAs share a tile's k blocks, and in how many parts the rows of a go: the least time by this measure, in units
+  // of a k block of 128 weight rows: 6 for a round's beginning, the blocks with their rows, the rows' way out, 4 for a join.
+  const int least_groups = (a.m + kFewMostRows - 1) / kFewMostRows;
+  int split = 1, groups = 1;
+  float least = 1e30f;
+  for (int s = 1; s <= kFewMostSplit && s <= a.k_blocks; ++s) {
+    int fit = 0;
+    if ((err = resident_clusters(device, s, kernel, &fit)) != cudaSuccess) return err;
+    if (fit < 1) continue;
+    for (int g = least_groups; g <= (a.m + 15) / 16 && g < least_groups + 16; ++g) {
+      const int cols = ((a.m + g - 1) / g + 15) / 16 * 16;
+      const int rounds = (a.tiles * ((a.m + cols - 1) / cols) + fit - 1) / fit, blocks = (a.k_blocks + s - 1) / s;
+      const float cost = rounds * (blocks * (1.f + cols / 256.f) + 6 + cols / 16.f) + (s > 1 ? 4 : 0);
+      if (cost < least) least = cost, split = s, groups = (a.m + cols - 1) / cols, a.cols = cols;
+    }
+  }
+  if (a.cols == 0) return cudaErrorInvalidConfiguration;
+  const uint32_t stage = kFewWeightStage + a.cols * kFewKBytes;
+  a.stages = (int)(kFewRing / stage);
+  if (a.stages > kFewStageMax) a.stages = kFewStageMax;
+  const int most = (a.k_blocks + split - 1) / split;
+  if (a.stages > most) a.stages = most;
+  CUtensorMap map_b, map_a;
+  if ((err = map_2d(&map_b, p.b, p.n, p.k, p.k, GATED ? kFewTileRows / 2 : kFewTileRows)) != cudaSuccess) return err;
+  if ((err = map_2d(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
+  cudaLaunchAttribute attrs[2]{};
+  const cudaLaunchConfig_t config = few_config(attrs, a.tiles * groups * split, split, FewProductLayout(a.cols, a.stages).request, stream, kernel);
+  return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
+}
+
+bool refused(int64_t m, int64_t n, int64_t k, int groups, int device) {
+  return m < 0 || n < 1 || k < 1 || groups < 1 || groups > kMatmulMaxGroups || m > kMaxRows || n > kMaxRows || k > kMaxRows || device < 0 ||
+         device >= kMaxDevices;
+}
+
+PreArgs pre_args(const MatmulPre& p) {
+  PreArgs a{};
+  a.dout = p.dout;
+  a.pre = p.pre;
+  a.rows = p.rows;
+  a.dz = p.dz;
+  a.dbias = p.dbias;
+  a.parts = p.parts;
+  a.dout_ld = p.dout_ld;
+  a.pre_ld = p.pre_ld;
+  a.dz_ld = p.dz_ld;
+  a.m = (int)p.m;
+  a.n = (int)p.n;
+  a.groups = p.rows ? p.groups : 1;
+  a.activation = p.activation;
+  a.type = p.type;
+  a.out_type = p.out_type;
+  a.bias_type = p.bias_type;
+  return a;
+}
+
+}  // namespace
+
+cudaError_t launch_matmul(const Matmul& p, int device, cudaStream_t stream) {
+  if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || (p.activation == kSwiglu && p.n % (2 * kGateBlock))) return cudaErrorInvalidValue;
+  if (p.m == 0) return cudaSuccess;
+  if (p.rows == nullptr) {
+    bool few = p.m <= kFewMostRows;
+    if (!few) {  // small products, whose tiles of 128 x 256 find an SM each and whose k is short
+      int n_sm = 0;
+      if (cudaError_t err = multiprocessors(device, &n_sm)) return err;
+      const int64_t tiles = (p.n + kFewTileRows - 1) / kFewTileRows * ((p.m + kFewMostRows - 1) / kFewMostRows);
+      few = tiles <= n_sm && tiles * ((p.k + kPairK - 1) / kPairK) <= 12 * n_sm;
+    }
+    if (few) return p.activation == kSwiglu ? launch_few<true>(p, device, stream) : launch_few<false>(p, device, stream);
+  }
+  return launch_forward(p, device, stream);
+}
+
+cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t stream) {
+  if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || p.dz_ld % 8) return cudaErrorInvalidValue;
+  if (p.m == 0) return cudaSuccess;
+  PairMaps maps{};
+  PairArgs a{};
+  a.rows = p.rows;
+  a.groups = p.rows ? p.groups : 1;
+  a.n_rows = (int)p.m;
+  a.features = (int)p.k;
+  a.k_blocks = (int)((p.n + kPairK - 1) / kPairK);
+  a.wide = fours(p.da, p.da_ld, p.type);
+  a.idesc = sm100::umma_idesc_16(p.type == Type::kBf16, true, false);
+  a.e.out = p.da;
+  a.e.out_ld = p.da_ld;
+  a.e.n = (int)p.k;
+  a.e.type = p.type;
+  cudaError_t err = maps_of_rows(&maps, p.dz, p.m, p.n, p.dz_ld);
+  if (err == cudaSuccess) err = map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kPairK);
+  return err != cudaSuccess ? err : launch_pairs<kInput>(maps, a, device, stream);
+}
+
+cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t stream) {
+  if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || p.dz_ld % 8) return cudaErrorInvalidValue;
+  PairArgs a{};
+  a.rows = p.rows;
+  a.groups = p.rows ? p.groups : 1;
+  a.n_rows = (int)p.m;
+  a.features = (int)p.k;
+  a.result_rows = (int)p.n;
+  a.wide = fours(p.db, p.k, p.type);
+  a.idesc = sm100::umma_idesc_16(p.type == Type::kBf16, true, true);
+  a.e.out = p.db;
+  a.e.out_ld = p.k;
+  a.e.n = (int)p.k;
+  a.e.type = p.type;
+  PairMaps maps{};
+  if (p.m > 0) {  // (without a row there is nothing to load: every matrix is cleared)
+    const int rows[kBoxes] = {64, 16, 8, 4, 2, 1};
+    for (int b = 0; b < kBoxes; ++b) {
+      cudaError_t err = map_2d(&maps.p[b], p.a, p.m, p.k, p.a_ld, rows[b]);
+      if (err == cudaSuccess) err = map_2d(&maps.q[b], p.dz, p.m, p.n, p.dz_ld, rows[b]);
+      if (err != cudaSuccess) return err;
+    }
+  }
+  return launch_pairs<kWeight>(maps, a, device, stream);
+}
+
+cudaError_t matmul_pre_parts(const MatmulPre& p, int device, int64_t* floats, int* splits) {
+  int n_sm = 0;
+  cudaError_t err = multiprocessors(device, &n_sm);
+  if (err != cudaSuccess) return err;
+  // about eight CTAs per SM, no part of less than 32 rows on average
+  const int64_t groups = p.rows ? p.groups : 1, columns = (p.n + kPreColumns - 1) / kPreColumns;
+  int64_t parts = (8 * (int64_t)n_sm + columns * groups - 1) / (columns * groups);
+  const int64_t most = p.m / groups / 32;
+  if (parts > most) parts = most;
+  if (parts < 1) parts = 1;
+  *splits = (int)parts;
+  *floats = p.dbias != nullptr && parts > 1 ? groups * parts * p.n : 0;
+  return cudaSuccess;
+}
+
+cudaError_t launch_matmul_pre(const MatmulPre& p, int device, cudaStream_t stream) {
+  if (refused(p.m, p.n, 1, p.groups, device) || (p.activation == kSwiglu && p.n % (2 * kGateBlock))) return cudaErrorInvalidValue;
+  int64_t floats = 0;
+  PreArgs a = pre_args(p);
+  cudaError_t err = matmul_pre_parts(p, device, &floats, &a.splits);
+  if (err != cudaSuccess) return err;
+  if (floats == 0) a.parts = nullptr;
+  else if (a.parts == nullptr) return cudaErrorInvalidValue;
+  const bool vec = p.n % 4 == 0 && fours(p.dout, p.dout_ld, p.out_type) && fours(p.pre, p.pre_ld, p.out_type) && fours(p.dz, p.dz_ld, p.type);
+  const dim3 grid((unsigned)((p.n + kPreColumns - 1) / kPreColumns), (unsigned)a.splits, (unsigned)a.groups);
+  const bool gated = p.activation == kSwiglu;
+  auto kernel = gated ? vec ? pre_gradient_kernel<true, true> : pre_gradient_kernel<false, true>
+                      : vec ? pre_gradient_kernel<true, false> : pre_gradient_kernel<false, false>;
+  if ((err = launch_after(kernel, grid, dim3(256), 0, stream, a)) != cudaSuccess || floats == 0) return err;
+  const int64_t total = (int64_t)a.groups * a.n;
+  return launch_after(bias_parts_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, a.parts, a.dbias, a.bias_type, (int64_t)a.n, a.splits,
+                      total);
+}
+
+}  // namespace ops
+}  // namespace lplb

@@ -1,0 +1,215 @@
+// Python binding of the product with an epilogue and of its gradients: checks of the arguments, outputs, launches on the current
+// stream of the arguments' device.  The reference has no operators of this kind.
+#include "matmul_api.h"
+
+#include "ops_check.h"
+
+namespace py = pybind11;
+
+namespace {
+
+using lplb::ops::Activation;
+using lplb::ops::Type;
+
+int64_t up_to(int64_t n, int64_t step) { return (n + step - 1) / step * step; }
+bool on_boundary(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// Rows that TMA can read: values of a row next to one another, every row on a 16-byte boundary; others are copied.
+Tensor rows_for_tma(const Tensor& t) {
+  const int64_t m = t.size(0), k = t.size(1);
+  if ((t.stride(1) == 1 || k == 1) && on_boundary(t) && (m < 2 || (t.stride(0) * t.element_size() % 16 == 0 && t.stride(0) >= k))) return t;
+  if (t.size(1) * t.element_size() % 16 == 0) {
+    const Tensor c = t.contiguous();
+    return on_boundary(c) ? c : c.clone();
+  }
+  auto wide = make({m, up_to(k, 16 / t.element_size())}, t.scalar_type(), t).narrow(1, 0, k);
+  wide.copy_(t);
+  return wide;
+}
+int64_t ld_of(const Tensor& t) { return t.size(0) < 2 ? up_to(t.size(1), 8) : t.stride(0); }
+Tensor rows_together(const Tensor& t) { return t.size(-1) < 2 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+struct Shape {
+  int64_t m, n, k, groups;
+};
+Shape check_operands(const Tensor& a, const Tensor& b, const OptTensor& rows) {
+  const auto device = a.device();
+  const int64_t lead = rows ? 1 : 0;  // dimensions in front of a matrix
+  OPS_CHECK(a.is_cuda() && a.dim() == 2 && (a.scalar_type() == torch::kBFloat16 || a.scalar_type() == torch::kFloat16),
+            "matmul: a must be a CUDA tensor [rows, k] of bfloat16 or float16");
+  OPS_CHECK(b.device() == device && b.dim() == 2 + lead && b.scalar_type() == a.scalar_type(),
+            "matmul: b must be [n, k] (with rows: [groups, n, k]) of a's type on a's device");
+  Shape s{a.size(0), b.size(-2), a.size(1), rows ? b.size(0) : 1};
+  OPS_CHECK(s.groups >= 1 && s.groups <= lplb::ops::kMatmulMaxGroups, "matmul: 1 to " + text(lplb::ops::kMatmulMaxGroups) + " groups");
+  OPS_CHECK(!rows || (rows->device() == device && rows->scalar_type() == torch::kInt32 && rows->dim() == 1 && rows->size(0) == s.groups && rows->is_contiguous()),
+            "matmul: rows must be contiguous int32, one number for each matrix of b, on a's device");
+  OPS_CHECK(s.m <= lplb::ops::kMaxRows && s.groups * s.n <= lplb::ops::kMaxRows,
+            "matmul: at most " + text(lplb::ops::kMaxRows) + " rows of a, and of all matrices of b together");
+  OPS_CHECK(s.k >= 8 && s.k % 8 == 0 && s.k <= (1 << 28) && b.size(-1) == s.k, "matmul: a and b must have the same k, a multiple of 8");
+  OPS_CHECK(s.n >= 1 && s.n <= (1 << 28), "matmul: b has no rows, or too many");
+  OPS_CHECK(b.is_contiguous() && on_boundary(b), "matmul: b must be contiguous and start on a 16-byte boundary");
+  return s;
+}
+Activation activation_of(int64_t code, const Shape& s) {
+  const auto act = static_cast<Activation>(code);
+  OPS_CHECK(act != lplb::ops::kSwiglu || s.n % (2 * lplb::ops::kGateBlock) == 0,
+            "matmul: 'swiglu' needs blocks of 128 gate rows and their 128 up rows: n must be a multiple of 256");
+  return act;
+}
+const int* rows_of(const OptTensor& rows) { return rows ? rows->data_ptr<int>() : nullptr; }
+
+// (out, pre): pre is the sum before the activation, in out's type, where `keep`
+py::tuple matmul(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_t activation, const OptTensor& residual, const OptTensor& rows, bool out_f32,
+                 bool keep) {
+  const Shape s = check_operands(a, b, rows);
+  lplb::ops::Matmul p{};
+  p.activation = activation_of(activation, s);
+  const int64_t cols = p.activation == lplb::ops::kSwiglu ? s.n / 2 : s.n;
+  const auto type = out_f32 ? torch::kFloat32 : a.scalar_type();
+  OPS_CHECK(!bias || (bias->device() == a.device() && (bias->scalar_type() == a.scalar_type() || bias->scalar_type() == torch::kFloat32) &&
+                      bias->dim() == b.dim() - 1 && bias->size(-1) == s.n && bias->numel() == s.groups * s.n),
+            "matmul: bias must be [n] (with rows: [groups, n]) of a's type or float32 on a's device");
+  OPS_CHECK(!residual || (residual->device() == a.device() && residual->scalar_type() == type && residual->dim() == 2 && residual->size(0) == s.m &&
+                          residual->size(1) == cols),
+            "matmul: residual must be of the output's shape, type and device");
+  c10::cuda::CUDAGuard guard(a.device());
+  const Tensor from = rows_for_tma(a);
+  const Tensor added = bias ? bias->contiguous() : Tensor(), carried = residual ? rows_together(*residual) : Tensor();
+  auto out = make({s.m, cols}, type, a);
+  Tensor pre;
+  p.a = from.data_ptr();
+  p.b = b.data_ptr();
+  p.rows = rows_of(rows);
+  p.out = out.data_ptr();
+  p.m = s.m;
+  p.n = s.n;
+  p.k = s.k;
+  p.a_ld = ld_of(from);
+  p.out_ld = cols;
+  p.groups = (int)s.groups;
+  p.type = type_of(a, "matmul: a");
+  p.out_type = out_f32 ? Type::kF32 : p.type;
+  if (bias) {
+    p.bias = added.data_ptr();
+    p.bias_type = type_of(added, "matmul: bias");
+  }
+  if (residual) {
+    p.residual = carried.data_ptr();
+    p.residual_ld = carried.stride(0);
+  }
+  if (keep) {
+    pre = make({s.m, up_to(s.n, 8)}, type, a);
+    p.pre = pre.data_ptr();
+    p.pre_ld = pre.size(1);
+  }
+  OPS_CUDA(lplb::ops::launch_matmul(p, a.get_device(), stream_of(a.get_device())));
+  return py::make_tuple(out, keep ? py::cast(pre) : py::none());
+}
+
+// (da, db, dbias), each where it is needed.  bias: its type, float32 or a's.
+py::tuple matmul_backward(const Tensor& dout, const Tensor& a, const Tensor& b, const OptTensor& pre, int64_t activation, const OptTensor& rows, bool out_f32,
+                          bool bias_f32, bool need_a, bool need_b, bool need_bias) {
+  const Shape s = check_operands(a, b, rows);
+  const auto act = activation_of(activation, s);
+  const int64_t cols = act == lplb::ops::kSwiglu ? s.n / 2 : s.n;
+  const auto out_type = out_f32 ? torch::kFloat32 : a.scalar_type();
+  OPS_CHECK(dout.device() == a.device() && dout.scalar_type() == out_type && dout.dim() == 2 && dout.size(0) == s.m && dout.size(1) == cols,
+            "matmul: the gradient must be of the output's shape, type and device");
+  OPS_CHECK((act == lplb::ops::kNoActivation) == !pre, "matmul: an activation's gradient needs what it was taken of");
+  c10::cuda::CUDAGuard guard(a.device());
+  const int device = a.get_device();
+  const auto stream = stream_of(device);
+  const auto type = type_of(a, "matmul: a");
+  Tensor da, db, dbias;
+  if (need_a) da = make({s.m, s.k}, a.scalar_type(), a);
+  if (need_b) db = make(b.sizes(), b.scalar_type(), a);
+  if (need_bias) {
+    auto shape = b.sizes().vec();
+    shape.pop_back();
+    dbias = make(shape, bias_f32 ? torch::kFloat32 : a.scalar_type(), a);
+  }
+  if (s.m == 0) {
+    if (need_b) db.zero_();
+    if (need_bias) dbias.zero_();
+  } else {
+    // without an activation dz is dout, where the products can read it
+    const bool same = act == lplb::ops::kNoActivation && !out_f32;
+    Tensor dz = same ? rows_for_tma(dout) : Tensor();
+    if (!same || need_bias) {
+      const Tensor d = rows_together(dout);
+      lplb::ops::MatmulPre p{};
+      if (!same && (need_a || need_b)) {
+        dz = make({s.m, up_to(s.n, 8)}, a.scalar_type(), a);
+        p.dz = dz.data_ptr();
+        p.dz_ld = dz.size(1);
+      }
+      p.dout = d.data_ptr();
+      p.dout_ld = d.stride(0);
+      if (pre) {
+        p.pre = pre->data_ptr();
+        p.pre_ld = pre->size(1);
+      }
+      p.rows = rows_of(rows);
+      p.m = s.m;
+      p.n = s.n;
+      p.groups = (int)s.groups;
+      p.activation = act;
+      p.type = type;
+      p.out_type = out_f32 ? Type::kF32 : type;
+      p.bias_type = bias_f32 ? Type::kF32 : type;
+      Tensor parts;
+      if (need_bias) {
+        p.dbias = dbias.data_ptr();
+        int64_t floats = 0;
+        int splits = 0;
+        OPS_CUDA(lplb::ops::matmul_pre_parts(p, device, &floats, &splits));
+        if (floats > 0) {
+          parts = make({floats}, torch::kFloat32, a);
+          p.parts = parts.data_ptr<float>();
+        }
+      }
+      OPS_CUDA(lplb::ops::launch_matmul_pre(p, device, stream));
+    }
+    if (need_a) {
+      lplb::ops::MatmulInput p{};
+      p.dz = dz.data_ptr();
+      p.b = b.data_ptr();
+      p.rows = rows_of(rows);
+      p.da = da.data_ptr();
+      p.m = s.m;
+      p.n = s.n;
+      p.k = s.k;
+      p.dz_ld = ld_of(dz);
+      p.da_ld = s.k;
+      p.groups = (int)s.groups;
+      p.type = type;
+      OPS_CUDA(lplb::ops::launch_matmul_input(p, device, stream));
+    }
+    if (need_b) {
+      const Tensor from = rows_for_tma(a);
+      lplb::ops::MatmulWeight p{};
+      p.dz = dz.data_ptr();
+      p.a = from.data_ptr();
+      p.rows = rows_of(rows);
+      p.db = db.data_ptr();
+      p.m = s.m;
+      p.n = s.n;
+      p.k = s.k;
+      p.dz_ld = ld_of(dz);
+      p.a_ld = ld_of(from);
+      p.groups = (int)s.groups;
+      p.type = type;
+      OPS_CUDA(lplb::ops::launch_matmul_weight(p, device, stream));
+    }
+  }
+  auto given = [](bool need, const Tensor& t) -> py::object { return need ? py::cast(t) : py::none(); };
+  return py::make_tuple(given(need_a, da), given(need_b, db), given(need_bias, dbias));
+}
+
+}  // namespace
+
+void bind_matmul(py::module_& m) {
+  m.def("matmul", &matmul);
+  m.def("matmul_backward", &matmul_backward);
+  m.attr("MATMUL_MAX_GROUPS") = lplb::ops::kMatmulMaxGroups;
+}

@@ -3,6 +3,7 @@
 16 and 32 bits, with their gradients."""
 
 from . import reference
+from .dense import MATMUL_ACTIVATIONS, MATMUL_MAX_GROUPS, matmul
 from .experts import (
     GATE_MAX_EXPERTS,
     GATE_MAX_TOPK,
@@ -62,4 +63,7 @@ __all__ = [
     "expert_order",
     "take_rows",
     "combine_rows",
+    "MATMUL_ACTIVATIONS",
+    "MATMUL_MAX_GROUPS",
+    "matmul",
 ]

@@ -16,7 +16,8 @@ The 8-bit serving operators (``lplb_b200.ops.fp8``) are restated below in 32 bit
 inputs are: ``quantize_fp8_reference``, ``rms_norm_fp8_reference``, ``matmul_fp8_reference``,
 ``moe_few_tokens_reference``.  So are the operators around a layer's experts (``lplb_b200.ops.experts``):
 ``gate_topk_reference``, ``expert_order_reference``, ``take_rows_reference``, ``combine_rows_reference`` and the
-gradients of the first and the last.
+gradients of the first and the last, and the product with an epilogue (``lplb_b200.ops.dense``) with its gradients,
+``matmul_reference`` and ``matmul_backward_reference``.
 """
 
 from __future__ import annotations
@@ -41,6 +42,8 @@ __all__ = [
     "take_rows_reference",
     "combine_rows_reference",
     "combine_rows_backward_reference",
+    "matmul_reference",
+    "matmul_backward_reference",
 ]
 
 _BLOCK = 256
@@ -325,3 +328,82 @@ def combine_rows_backward_reference(
         drows[at] = d[token] * weights[token, k : k + 1].to(d.dtype)
         dweights[token, k] = (d[token] * y[at]).sum(-1)
     return drows.to(rows.dtype), dweights
+
+
+def _groups(m: int, rows: torch.Tensor | None) -> list[tuple[int | None, slice]]:
+    """``(matrix, rows of a)``; one matrix has no number."""
+    if rows is None:
+        return [(None, slice(0, m))]
+    parts, at = [], 0
+    for e, n in enumerate(rows.clamp_min(0).tolist()):
+        parts.append((e, slice(at, min(m, at + n))))
+        at = min(m, at + n)
+    return parts
+
+
+def _normal_cdf(z: torch.Tensor) -> torch.Tensor:
+    return 0.5 * torch.special.erfc(-z * 0.5**0.5)
+
+
+def _activated(z: torch.Tensor, activation: str | None) -> torch.Tensor:
+    if activation == "relu":
+        return z.clamp_min(0)
+    if activation == "gelu":
+        return z * _normal_cdf(z)
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    if activation == "swiglu":
+        gate, up = z.unflatten(-1, (-1, 2, _SCALE_BLOCK)).unbind(-2)
+        return (gate * torch.sigmoid(gate) * up).flatten(-2)
+    return z
+
+
+def _through_activation(dout: torch.Tensor, z: torch.Tensor, activation: str) -> torch.Tensor:
+    if activation == "relu":
+        return torch.where(z > 0, dout, torch.zeros_like(dout))
+    if activation == "gelu":
+        return dout * (_normal_cdf(z) + z * torch.exp(-0.5 * z * z) * (2 * torch.pi) ** -0.5)
+    if activation == "silu":
+        s = torch.sigmoid(z)
+        return dout * s * (1 + z * (1 - s))
+    gate, up = z.unflatten(-1, (-1, 2, _SCALE_BLOCK)).unbind(-2)
+    d, s = dout.unflatten(-1, (-1, _SCALE_BLOCK)), torch.sigmoid(gate)
+    return torch.stack((d * up * s * (1 + gate * (1 - s)), d * gate * s), -2).flatten(-3)
+
+
+def matmul_reference(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    residual: torch.Tensor | None = None,
+    rows: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(act(z) + residual, z)`` with ``z = a @ b.T + bias`` (kernels: ``pair_matmul_kernel`` and ``few_product_kernel`` in
+    ``csrc/matmul.cuh`` and ``matmul_few.cuh``); rows behind the last group have no product."""
+    af = _wide(a)
+    z = af.new_zeros(a.shape[0], b.shape[-2])
+    out = af.new_zeros(a.shape[0], b.shape[-2] // (2 if activation == "swiglu" else 1))
+    for e, part in _groups(a.shape[0], rows):
+        here = af[part] @ _wide(b if e is None else b[e]).T
+        if bias is not None:
+            here = here + _wide(bias if e is None else bias[e]).to(here.dtype)
+        z[part], out[part] = here, _activated(here, activation)
+    return (out if residual is None else out + _wide(residual).to(out.dtype)), z
+
+
+def matmul_backward_reference(
+    dout: torch.Tensor, a: torch.Tensor, b: torch.Tensor, z: torch.Tensor | None, activation: str | None = None, rows: torch.Tensor | None = None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(da, db, dbias)``; ``z`` is what the activation was taken of."""
+    af, bf = _wide(a), _wide(b)
+    da, db, dbias = torch.zeros_like(af), torch.zeros_like(bf), bf.new_zeros(b.shape[:-1])
+    for e, part in _groups(a.shape[0], rows):
+        dz = _wide(dout[part]).to(af.dtype)
+        if activation is not None:
+            dz = _through_activation(dz, _wide(z[part]).to(af.dtype), activation)
+        at = slice(None) if e is None else e
+        dbias[at] = dz.sum(0)
+        dz = dz.to(a.dtype).to(af.dtype)  # as the products behind it take it
+        da[part], db[at] = dz @ bf[at], dz.T @ af[part]
+    return da, db, dbias
