@@ -2,9 +2,7 @@
 // stream of the arguments' device.  The reference has no operators of this kind.
 #include "experts_api.h"
 
-#include "ops_check.h"
-
-namespace py = pybind11;
+#include "ops_autograd.h"
 
 namespace {
 
@@ -33,7 +31,7 @@ Gate gate_args(const Tensor& logits, int64_t topk, bool sigmoid, bool renormaliz
 }
 Tensor rows_together(const Tensor& t) { return t.size(-1) < 2 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
-py::tuple gate_topk(const Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale) {
+variable_list gate_forward(const Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale) {
   OPS_CHECK(logits.dim() == 2, "gate_topk: logits must be a CUDA tensor [tokens, experts]");
   c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
   const Tensor x = rows_together(logits);
@@ -42,10 +40,10 @@ py::tuple gate_topk(const Tensor& logits, int64_t topk, bool sigmoid, bool renor
   g.weights = weights.data_ptr<float>();
   g.idx = idx.data_ptr<int64_t>();
   OPS_CUDA(lplb::ops::launch_gate(g, stream_of(x.get_device())));
-  return py::make_tuple(weights, idx);
+  return {weights, idx};
 }
 
-Tensor gate_topk_backward(const Tensor& logits, const Tensor& idx, const Tensor& dweights, bool sigmoid, bool renormalize, double scale) {
+Tensor gate_backward(const Tensor& logits, const Tensor& idx, const Tensor& dweights, bool sigmoid, bool renormalize, double scale) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
   const Tensor x = rows_together(logits), d = dweights.contiguous();
   auto g = gate_args(x, idx.size(1), sigmoid, renormalize, scale);
@@ -58,6 +56,31 @@ Tensor gate_topk_backward(const Tensor& logits, const Tensor& idx, const Tensor&
   g.dlogits = dlogits.data_ptr();
   OPS_CUDA(lplb::ops::launch_gate_backward(g, stream_of(x.get_device())));
   return dlogits;
+}
+
+struct GateTopk : torch::autograd::Function<GateTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale) {
+    auto out = gate_forward(logits, topk, sigmoid, renormalize, scale);
+    ctx->save_for_backward({logits, out[1]});
+    ctx->mark_non_differentiable({out[1]});
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor dlogits;
+    if (grads[0].defined())
+      dlogits = gate_backward(saved[0], saved[1], grads[0], ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renormalize"].toBool(),
+                              ctx->saved_data["scale"].toDouble());
+    return first_order({dlogits, Tensor(), Tensor(), Tensor(), Tensor()}, "gate_topk");
+  }
+};
+
+py::tuple gate_topk(const Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale) {
+  const auto out = wants_grad({&logits}, "gate_topk") ? GateTopk::apply(logits, topk, sigmoid, renormalize, scale) : gate_forward(logits, topk, sigmoid, renormalize, scale);
+  return py::make_tuple(out[0], out[1]);
 }
 
 // ---- rows sorted by expert ----------------------------------------------------------------------------
@@ -89,7 +112,7 @@ void check_order(const Tensor& rows_or_tokens, const Tensor& place, const Tensor
             who + std::string(": order must be one of expert_order's, on the same device"));
 }
 
-Tensor take_rows(const Tensor& x, const Tensor& place, const Tensor& source) {
+Tensor take_forward(const Tensor& x, const Tensor& place, const Tensor& source) {
   OPS_CHECK(x.is_cuda() && x.dim() == 2, "take_rows: x must be a CUDA tensor [tokens, values]");
   check_order(x, place, source, "take_rows");
   OPS_CHECK(place.size(0) == x.size(0), "take_rows: x must have a row for each of the order's tokens");
@@ -118,7 +141,7 @@ CombineRows combine_args(const Tensor& rows, const Tensor& place, const Tensor& 
   OPS_CHECK(rows.size(1) >= 1 && rows.size(1) <= INT32_MAX / 16, who + std::string(": rows without values, or too long"));
   OPS_CHECK(!weights || (weights->device() == rows.device() && weights->scalar_type() == torch::kFloat32 && weights->sizes() == place.sizes() &&
                          weights->is_contiguous()),
-            who + std::string(": weights must be floating point [tokens, topk] on the rows' device"));
+            who + std::string(": weights must be [tokens, topk] on the rows' device"));
   CombineRows c{};
   c.type = type_of(rows, who);
   c.rows = rows.data_ptr();
@@ -132,7 +155,7 @@ CombineRows combine_args(const Tensor& rows, const Tensor& place, const Tensor& 
   return c;
 }
 
-Tensor combine_rows(const Tensor& rows, const Tensor& place, const Tensor& source, const OptTensor& weights) {
+Tensor combine_forward(const Tensor& rows, const Tensor& place, const Tensor& source, const OptTensor& weights) {
   OPS_CHECK(rows.dim() == 2, "combine_rows: rows must be a CUDA tensor [tokens * topk, values]");
   c10::cuda::OptionalCUDAGuard guard(at::device_of(rows));
   const Tensor from = rows_together(rows);
@@ -143,7 +166,7 @@ Tensor combine_rows(const Tensor& rows, const Tensor& place, const Tensor& sourc
   return out;
 }
 
-py::tuple combine_rows_backward(const Tensor& dout, const Tensor& rows, const Tensor& place, const Tensor& source, const Tensor& weights,
+variable_list combine_backward(const Tensor& dout, const Tensor& rows, const Tensor& place, const Tensor& source, const Tensor& weights,
                                 bool need_rows, bool need_weights) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(rows));
   const Tensor from = rows_together(rows), d = rows_together(dout);
@@ -162,18 +185,63 @@ py::tuple combine_rows_backward(const Tensor& dout, const Tensor& rows, const Te
   c.dout = d.data_ptr();
   c.dout_ld = d.stride(0);
   OPS_CUDA(lplb::ops::launch_combine_rows_backward(c, stream_of(rows.get_device())));
-  return py::make_tuple(need_rows ? py::cast(drows) : py::none(), need_weights ? py::cast(dweights) : py::none());
+  return {drows, dweights};
+}
+
+struct TakeRows : torch::autograd::Function<TakeRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& place, const Tensor& source) {
+    ctx->save_for_backward({place, source});
+    return take_forward(x, place, source);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    return first_order({combine_forward(grads[0], saved[0], saved[1], std::nullopt), Tensor(), Tensor()}, "take_rows");
+  }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& place, const Tensor& source, const Tensor& weights) {
+    ctx->save_for_backward({place, source, weights, rows});
+    return combine_forward(rows, place, source, weights);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto found = combine_backward(grads[0], saved[3], saved[0], saved[1], saved[2], ctx->needs_input_grad(0), ctx->needs_input_grad(3));
+    return first_order({found[0], Tensor(), Tensor(), found[1]}, "combine_rows");
+  }
+};
+// without weights the gradient is take_rows, and no row is kept
+struct Gather : torch::autograd::Function<Gather> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& place, const Tensor& source) {
+    ctx->save_for_backward({place, source});
+    return combine_forward(rows, place, source, std::nullopt);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    return first_order({take_forward(grads[0], saved[0], saved[1]), Tensor(), Tensor()}, "combine_rows");
+  }
+};
+
+Tensor take_rows(const Tensor& x, const Tensor& place, const Tensor& source) {
+  if (!wants_grad({&x}, "take_rows")) return take_forward(x, place, source);
+  type_of(x, "take_rows: x that requires a gradient");
+  return TakeRows::apply(x, place, source);
+}
+
+Tensor combine_rows(const Tensor& rows, const Tensor& place, const Tensor& source, const OptTensor& weights) {
+  if (!weights) return wants_grad({&rows}, "combine_rows") ? Gather::apply(rows, place, source) : combine_forward(rows, place, source, std::nullopt);
+  OPS_CHECK(weights->is_floating_point(), "combine_rows: weights must be floating point [tokens, topk] on the rows' device");
+  const Tensor w = weights->to(torch::kFloat32).contiguous();
+  return wants_grad({&rows, &w}, "combine_rows") ? Combine::apply(rows, place, source, w) : combine_forward(rows, place, source, w);
 }
 
 }  // namespace
 
 void bind_expert_ops(py::module_& m) {
   m.def("gate_topk", &gate_topk);
-  m.def("gate_topk_backward", &gate_topk_backward);
   m.def("expert_order", &expert_order);
   m.def("take_rows", &take_rows);
   m.def("combine_rows", &combine_rows);
-  m.def("combine_rows_backward", &combine_rows_backward);
   m.attr("GATE_MAX_EXPERTS") = lplb::ops::kGateMaxExperts;
   m.attr("GATE_MAX_TOPK") = lplb::ops::kGateMaxTopk;
   m.attr("ORDER_MAX_EXPERTS") = lplb::ops::kOrderMaxExperts;

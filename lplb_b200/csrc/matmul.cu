@@ -83,10 +83,10 @@ __global__ void __launch_bounds__(256) pre_gradient_kernel(const PreArgs a) {
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
       load4<S>(a.dout, a.out_type, r * a.dout_ld + at_out[v], limit[v], d[v]);
-      if (a.pre != nullptr) load4<S>(a.pre, a.out_type, r * a.pre_ld + at_z[v], limit[v], z[v]);
+      if (a.pre != nullptr) load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[v], limit[v], z[v]);
     }
     if (GATED) {
-      load4<S>(a.pre, a.out_type, r * a.pre_ld + at_z[0] + kGateBlock, limit[0], z[1]);
+      load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[0] + kGateBlock, limit[0], z[1]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float s = sigmoid_of(z[0][j]), g = d[0][j];
@@ -176,8 +176,8 @@ cudaError_t maps_of_rows(PairMaps* maps, const void* base, uint64_t rows, uint64
 // ---- CTA pairs --------------------------------------------------------------------------------------------
 // One group: result rows in tiles of equal height, so high that the fewest rounds over the CTA pairs come out (a tile costs its
 // steps and about one more).  Several groups: their rows are only known on the device.
-int steps_per_tile(int64_t rows, int step, int64_t tiles_p, int n_sm, bool grouped) {
-  const int most = kPairN / step;
+int steps_per_tile(int64_t rows, int step, int most_rows, int64_t tiles_p, int n_sm, bool grouped) {
+  const int most = most_rows / step;
   if (grouped) return most;
   const int64_t steps = (rows + step - 1) / step;
   int64_t least = INT64_MAX;
@@ -191,9 +191,9 @@ int steps_per_tile(int64_t rows, int step, int64_t tiles_p, int n_sm, bool group
   return best;
 }
 
-template <Mode MODE>
+template <Mode MODE, bool IN_32 = false>
 cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStream_t stream) {
-  auto kernel = pair_matmul_kernel<MODE>;
+  auto kernel = pair_matmul_kernel<MODE, IN_32>;
   static std::atomic<bool> prepared[kMaxDevices];
   int n_sm = 0;
   cudaError_t err = multiprocessors(device, &n_sm);
@@ -206,7 +206,9 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
   a.budget_ns = wait_budget_ns();
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
-  a.tile_steps = steps_per_tile(MODE == kWeight ? a.result_rows : a.n_rows, PairTile<MODE>::kStep, a.tiles_p, n_sm, a.rows != nullptr && MODE != kWeight);
+  const int out_cols = MODE == kForwardGated ? a.features / 2 : a.features;
+  a.plain = a.e.type != Type::kF32 && a.e.residual == nullptr && a.e.pre == nullptr && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
+  a.tile_steps = steps_per_tile(MODE == kWeight ? a.result_rows : a.n_rows, PairTile<MODE>::kStep, IN_32 ? kSumRows : kPairN, a.tiles_p, n_sm, a.rows != nullptr && MODE != kWeight);
   return launch_after(kernel, dim3(n_sm & ~1), dim3(kPairThreads), kPairSmem, stream, maps, a);
 }
 
@@ -226,7 +228,7 @@ Epilogue epilogue_of(const Matmul& p) {
   return e;
 }
 int is_wide(const Matmul& p) {
-  return p.n % 4 == 0 && fours(p.out, p.out_ld, p.out_type) && fours(p.residual, p.residual_ld, p.out_type) && fours(p.pre, p.pre_ld, p.out_type) &&
+  return p.n % 4 == 0 && fours(p.out, p.out_ld, p.out_type) && fours(p.residual, p.residual_ld, p.out_type) && fours(p.pre, p.pre_ld, Type::kF32) &&
          fours(p.bias, p.n, p.bias_type);
 }
 
@@ -245,10 +247,10 @@ cudaError_t launch_forward(const Matmul& p, int device, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   if (p.activation == kSwiglu) {
     if ((err = map_gated(&maps.p[0], p.b, (uint64_t)a.groups * p.n, p.k)) != cudaSuccess) return err;
-    return launch_pairs<kForwardGated>(maps, a, device, stream);
+    return p.out_type == Type::kF32 ? launch_pairs<kForwardGated, true>(maps, a, device, stream) : launch_pairs<kForwardGated>(maps, a, device, stream);
   }
   if ((err = map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kHalfM)) != cudaSuccess) return err;
-  return launch_pairs<kForward>(maps, a, device, stream);
+  return p.out_type == Type::kF32 ? launch_pairs<kForward, true>(maps, a, device, stream) : launch_pairs<kForward>(maps, a, device, stream);
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------
@@ -307,7 +309,9 @@ cudaError_t launch_few(const Matmul& p, int device, cudaStream_t stream) {
   a.tiles = (int)((p.n + kFewTileRows - 1) / kFewTileRows);
   // How many CTAs share a tile's k blocks, and in how many parts the rows of a go: the least time by this measure, in units
   // of a k block of 128 weight rows: 6 for a round's beginning, the blocks with their rows, the rows' way out, 4 for a join.
-  const int least_groups = (a.m + kFewMostRows - 1) / kFewMostRows;
+  const bool in_32 = p.out_type == Type::kF32;
+  const int most_rows = in_32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
+  const int least_groups = (a.m + most_rows - 1) / most_rows;
   int split = 1, groups = 1;
   float least = 1e30f;
   for (int s = 1; s <= kFewMostSplit && s <= a.k_blocks; ++s) {
@@ -327,11 +331,13 @@ cudaError_t launch_few(const Matmul& p, int device, cudaStream_t stream) {
   if (a.stages > kFewStageMax) a.stages = kFewStageMax;
   const int most = (a.k_blocks + split - 1) / split;
   if (a.stages > most) a.stages = most;
+  a.chains = 1;
+  while (in_32 && a.chains * kSumBlocks < most && (a.chains + 1) * a.cols <= kFewMostRows) ++a.chains;
   CUtensorMap map_b, map_a;
   if ((err = map_2d(&map_b, p.b, p.n, p.k, p.k, GATED ? kFewTileRows / 2 : kFewTileRows)) != cudaSuccess) return err;
   if ((err = map_2d(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
   cudaLaunchAttribute attrs[2]{};
-  const cudaLaunchConfig_t config = few_config(attrs, a.tiles * groups * split, split, FewProductLayout(a.cols, a.stages).request, stream, kernel);
+  const cudaLaunchConfig_t config = few_config(attrs, a.tiles * groups * split, split, FewProductLayout(a.cols, a.chains, a.stages).request, stream, kernel);
   return cudaLaunchKernelEx(&config, kernel, map_b, map_a, a);
 }
 
@@ -449,7 +455,7 @@ cudaError_t launch_matmul_pre(const MatmulPre& p, int device, cudaStream_t strea
   if (err != cudaSuccess) return err;
   if (floats == 0) a.parts = nullptr;
   else if (a.parts == nullptr) return cudaErrorInvalidValue;
-  const bool vec = p.n % 4 == 0 && fours(p.dout, p.dout_ld, p.out_type) && fours(p.pre, p.pre_ld, p.out_type) && fours(p.dz, p.dz_ld, p.type);
+  const bool vec = p.n % 4 == 0 && fours(p.dout, p.dout_ld, p.out_type) && fours(p.pre, p.pre_ld, Type::kF32) && fours(p.dz, p.dz_ld, p.type);
   const dim3 grid((unsigned)((p.n + kPreColumns - 1) / kPreColumns), (unsigned)a.splits, (unsigned)a.groups);
   const bool gated = p.activation == kSwiglu;
   auto kernel = gated ? vec ? pre_gradient_kernel<true, true> : pre_gradient_kernel<false, true>

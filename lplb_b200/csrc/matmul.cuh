@@ -43,7 +43,7 @@ struct Epilogue {
   int64_t residual_ld, out_ld, pre_ld;
   int n;            // features: weight rows, the length of a bias row
   int activation;
-  Type type, bias_type;  // of out, residual and pre; of the bias
+  Type type, bias_type;  // of out and residual; of the bias.  pre is in 32 bits: what is rounded there comes back in every gradient
 };
 
 __device__ __forceinline__ float load_as_float(const void* p, Type type, int64_t i) {
@@ -142,8 +142,8 @@ struct Columns {
       for (int j = 0; j < 4; ++j) up[j] += up_bias[j];
     }
     if (e.pre != nullptr) {
-      store4<S>(e.pre, e.type, row * e.pre_ld + gate, limit, z);
-      if (GATED) store4<S>(e.pre, e.type, row * e.pre_ld + gate + kGateBlock, limit, up);
+      store4<S>(e.pre, Type::kF32, row * e.pre_ld + gate, limit, z);
+      if (GATED) store4<S>(e.pre, Type::kF32, row * e.pre_ld + gate + kGateBlock, limit, up);
     }
     if (GATED) {
 #pragma unroll
@@ -175,11 +175,17 @@ constexpr int kBoxes = 6;         // K-major: 128, 64, 32, 16 result rows; kWeig
 constexpr uint32_t kStageP = kHalfM * kPairK * 2;
 constexpr uint32_t kPairRing = 192 * 1024;
 constexpr int kPairStages = 11;
-constexpr int kTurnRows = 16;     // result rows that go through shared memory at a time
-constexpr uint32_t kTurn = kTurnRows * kHalfM * 4;
+constexpr int kStoreWarps = 8;      // of the epilogue: two for every quarter of tensor memory's lanes
+constexpr uint32_t kTurn = 2048;   // of one such warp: 32 features x 32 result rows in 16 bits, or x 16 in 32
 constexpr uint32_t kPairBars = 256;
-constexpr size_t kPairSmem = 1024 + kPairRing + kPairBars + 2 * kTurn;
-constexpr int kPairThreads = 192, kPairColumns = 512;
+constexpr size_t kPairSmem = 1024 + kPairRing + kPairBars + kStoreWarps * kTurn;
+constexpr int kPairThreads = 64 + 32 * kStoreWarps, kPairColumns = 512;
+// The tensor cores cut an accumulator's last bits off at every addition, which makes a long sum too small: by 1.6e-8 of it per 16
+// products, 7e-6 over 7168, where sums in 32 bits that are rounded are off by 1e-6.  A result in 32 bits shows that, so its sum is
+// taken over `kSumBlocks` blocks at a time in tensor memory, and these sums are added in registers (off by 5e-7 whatever the length).
+// Tiles of at most `kSumRows` result rows: a thread holds half of them.  8192 x 4096 x 7168 in 450-500 us (16 bits 340-370),
+// 1001 x 4100 x 2064 in 24.3 (20.7); blocks of 4 541 and 25.9; 192 rows, whose sums do not fit the registers, 612 and 37.8.
+constexpr int kSumBlocks = 8, kSumRows = 128;
 
 struct PairMaps {
   CUtensorMap p[kBoxes], q[kBoxes];  // K-major P: the first only
@@ -194,6 +200,7 @@ struct PairArgs {
   int tiles_p;      // ceil(features / 256)
   int tile_steps;   // result rows of a tile at most, in steps
   int wide;         // four neighbouring values of everything in the epilogue start on a boundary of their size
+  int plain;        // a result in 16 bits, no residual, nothing kept, rows of whole 16-byte words
   uint32_t idesc;
   int* status;
   unsigned long long budget_ns;
@@ -224,9 +231,12 @@ struct PairTile {
   }
 };
 
-// Roles: warp 0 TMA, warp 1 tensor memory and (in the pair's first CTA) matrix instructions, warps 2-5 epilogue.  Two accumulators:
-// the epilogue of a tile runs beside the sums of the next.
-template <Mode MODE>
+// Roles: warp 0 TMA, warp 1 tensor memory and (in the pair's first CTA) matrix instructions, warps 2-9 epilogue, every one by itself:
+// it turns 32 features x 32 result rows round in shared memory of its own.  Two accumulators: the epilogue of a tile runs beside the
+// sums of the next.  (With four warps that met at a barrier every 16 rows a weight's gradient of 32 experts, 512 rows each on average,
+// 4096 x 7168, took 3070 us: its tiles have 8 blocks to sum, and 1750 cycles went into every 16 rows.)
+// IN_32: a result in 32 bits, summed in parts.
+template <Mode MODE, bool IN_32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   using namespace sm100;
@@ -234,7 +244,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPairRing);
-  float* turns = reinterpret_cast<float*>(smem + kPairRing + kPairBars);
+  uint8_t* turns = smem + kPairRing + kPairBars;
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kPairStages);
   const uint32_t bar_tfull = smem_u32(bars + 2 * kPairStages), bar_tempty = smem_u32(bars + 2 * kPairStages + 2);
   static_assert((2 * kPairStages + 4) * 8 <= kPairBars, "barriers");
@@ -253,7 +263,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_tfull + 8 * b, 1);
-      mbar_init(bar_tempty + 8 * b, 8);  // four epilogue warps of either CTA
+      mbar_init(bar_tempty + 8 * b, 2 * kStoreWarps);  // of both CTAs
     }
     fence_barrier_init();
     tma_prefetch_desc(&maps.p[0]);
@@ -373,15 +383,23 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   } else if (warp == 1) {
     // ---------------- matrix instructions, for both CTAs ----------------
     if (half == 0 && elect_one()) {
-      uint32_t s = 0, ph = 0;
+      uint32_t s = 0, ph = 0, part = 0;  // part: sums handed to the epilogue, one per tile but for IN_32
       for (uint32_t i = 0; find(i) && !*abort; ++i) {
-        const uint32_t acc = i & 1, acc_ph = (i >> 1) & 1;
-        if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, abort, budget)) break;
-        tc_fence_after_sync();
-        const uint32_t idesc = a.idesc | umma_idesc_size(kPairM, cur.n), tmem_d = tmem_base + acc * kPairN;
+        const uint32_t idesc = a.idesc | umma_idesc_size(kPairM, cur.n);
         const int blocks = blocks_of();
         bool ok = true;
+        uint32_t tmem_d = 0;
         for (int kb = 0; kb < blocks; ++kb) {
+          const bool first = kb == 0 || (IN_32 && kb % kSumBlocks == 0), last = kb == blocks - 1 || (IN_32 && kb % kSumBlocks == kSumBlocks - 1);
+          const uint32_t acc = part & 1;
+          if (first) {
+            if (!mbar_wait(bar_tempty + 8 * acc, ((part >> 1) & 1) ^ 1, abort, budget)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            tmem_d = tmem_base + acc * kPairN;
+          }
           if (!mbar_wait(bar_full + 8 * s, ph, abort, budget)) {
             ok = false;
             break;
@@ -393,31 +411,36 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           const int steps = (rows_of(kb) + 15) / 16;
 #pragma unroll
           for (int k = 0; k < kPairK / 16; ++k)  // 16 of the sum: 32 bytes of a K-major row, 16 rows of an MN-major chunk
-            if (k < steps) umma_pair_bf16(tmem_d, dp + k * (kPmn ? 2048 >> 4 : 2), dq + k * (kQmn ? 2048 >> 4 : 2), idesc, (kb | k) != 0);
+            if (k < steps) umma_pair_bf16(tmem_d, dp + k * (kPmn ? 2048 >> 4 : 2), dq + k * (kQmn ? 2048 >> 4 : 2), idesc, !first || k != 0);
           umma_pair_commit(bar_empty + 8 * s);
           if (++s == stages) s = 0, ph ^= 1;
+          if (last) {
+            umma_pair_commit(bar_tfull + 8 * acc);
+            ++part;
+          }
         }
         if (!ok) break;
-        umma_pair_commit(bar_tfull + 8 * acc);
       }
     }
   } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3;  // the tensor memory lanes that this warp may read
-    const int ew = warp - 2, et = threadIdx.x - 64;
+    const int which = (warp - 2) >> 2;  // of its two warps: takes every other 32 result rows of a tile
+    const int et = threadIdx.x - 64;
     const Epilogue& e = a.e;
+    uint8_t* stage = turns + (warp - 2) * kTurn;
     // What has no product: rows behind the last group, matrices without rows.  (The first tile's sums are under way meanwhile.)
     const int64_t cta = blockIdx.x, ctas = gridDim.x;
     const int out_cols = kGated ? a.features / 2 : a.features;
     auto clear_row = [&](int64_t row) {
       if (a.wide) {
-        for (int c = 4 * et; c < out_cols; c += 512) {
+        for (int c = 4 * et; c < out_cols; c += 4 * 32 * kStoreWarps) {
           float v[4] = {0.f, 0.f, 0.f, 0.f};
           if (e.residual != nullptr) load4<1>(e.residual, e.type, row * e.residual_ld + c, 4, v);
           store4<1>(e.out, e.type, row * e.out_ld + c, 4, v);
         }
       } else {
-        for (int c = et; c < out_cols; c += 128)
+        for (int c = et; c < out_cols; c += 32 * kStoreWarps)
           store_float(e.out, e.type, row * e.out_ld + c, e.residual != nullptr ? load_as_float(e.residual, e.type, row * e.residual_ld + c) : 0.f);
       }
     };
@@ -428,72 +451,208 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     } else {
       for (int64_t r = s_start[a.groups] + cta; r < a.n_rows; r += ctas) clear_row(r);
     }
-    uint32_t turn = 0;
-    auto tiles = [&](auto wide) {
+    uint32_t part = 0;  // as the matrix instructions' side counts
+    const uint32_t lead_tempty = map_to_rank(bar_tempty, 0);
+    auto await = [&]() {  // the next accumulator's sums, all of the warp together
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * (part & 1), (part >> 1) & 1, abort, budget))) return false;
+      tc_fence_after_sync();
+      return true;
+    };
+    // The accumulator has been read: tcgen05.wait::ld has returned, and nothing else is handed over.  So the arrival does not release: at
+    // cluster scope that waits for the thread's loads and stores under way, some 1500 cycles each time.
+    auto release = [&]() {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote_fenced(lead_tempty + 8 * (part & 1));
+      ++part;
+    };
+    const uint32_t tmem_mine = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    int n = 0;           // result rows of the tile that are there
+    int64_t row0 = 0;    // the first of them
+    auto next = [&](uint32_t i) {
+      if (!__all_sync(0xffffffffu, find(i) && !*abort)) return false;
+      n = min(cur.n, (MODE == kWeight ? a.result_rows : s_rows[cur.group]) - cur.row0);
+      row0 = (MODE == kWeight ? (int64_t)cur.group * a.result_rows : (int64_t)s_start[cur.group]) + cur.row0;
+      return true;
+    };
+
+    // A result in 16 bits that nothing is added to: bias and activation on the matrix fragments, turned round by stmatrix, stored by 16 bytes.
+    auto plain = [&](auto is_bf16) {
+      constexpr bool kBf = decltype(is_bf16)::value;
+      auto pack = [](float lo, float hi) {
+        if constexpr (kBf) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+          return *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __half2 v = __floats2half2_rn(lo, hi);
+          return *reinterpret_cast<const uint32_t*>(&v);
+        }
+      };
+      const uint32_t mine = smem_u32(stage);
+      constexpr int kRowBytes = kGated ? 32 : 64, kChunks = kRowBytes / 16;  // of a result row, this warp's
+      auto chunk_at = [&](int row, int chunk) {  // swizzled: eight rows' chunks lie in different banks
+        return row * kRowBytes + ((chunk ^ (kGated ? (row >> 2) & 1 : (row >> 1) & 3)) << 4);
+      };
+      for (uint32_t i = 0; next(i); ++i) {
+        // this thread's features: lane / 4, and 8, 16 (gated: the up row of the first) and 24 behind
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        const int first = cur.p * kPairM + half * (kGated ? kHalfM / 2 : kHalfM) + quarter * (kGated ? 16 : 32) + (lane >> 2);
+        if (MODE <= kForwardGated && e.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = first + (j & 1) * 8 + (j >> 1) * (kGated ? kGateBlock : 16);
+            if (c < e.n) bias[j] = load_as_float(e.bias, e.bias_type, (int64_t)cur.group * e.n + c);
+          }
+        }
+        const int column = (kGated ? cur.p * kHalfM + half * (kHalfM / 2) + quarter * 16 : cur.p * kPairM + half * kHalfM + quarter * 32) + lane % kChunks * 8;
+        uint16_t* out = static_cast<uint16_t*>(e.out) + column;
+        const bool inside = column < out_cols;
+        if (!await()) break;
+        for (int c0 = 32 * which; c0 < n; c0 += 64) {
+          // fragments: lanes l/4 and l/4 + 8 of a 16-lane half, result rows 8j + 2(l%4) and the next
+          uint32_t raw[2][16];
+          __syncwarp();
+          tmem_ld_16x32(tmem_mine + (part & 1) * kPairN + c0, raw[0]);
+          tmem_ld_16x32(tmem_mine + (16u << 16) + (part & 1) * kPairN + c0, raw[1]);
+          tmem_ld_wait();
+          float v[2][16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[h][j] = __uint_as_float(raw[h][j]) + (MODE <= kForwardGated ? bias[2 * h + (j >> 1 & 1)] : 0.f);
+          if constexpr (kGated) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[0][j] = v[0][j] * sigmoid_of(v[0][j]) * v[1][j];
+          } else if (MODE == kForward && e.activation != kNoActivation) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[h][j] = activated(v[h][j], e.activation);
+          }
+          __syncwarp();  // the rows before have been read
+#pragma unroll
+          for (int q = 0; q < kChunks; ++q) {
+            const float(&f)[16] = v[q >> 1];
+            const int h = 2 * (q & 1);
+            stmatrix_trans(mine + chunk_at(lane, q), pack(f[h], f[h + 1]), pack(f[4 + h], f[5 + h]), pack(f[8 + h], f[9 + h]), pack(f[12 + h], f[13 + h]));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < kChunks; ++q) {
+            const int r = lane / kChunks + q * (32 / kChunks);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + chunk_at(r, lane % kChunks));
+            if (c0 + r < n && inside) *reinterpret_cast<uint4*>(out + (row0 + c0 + r) * e.out_ld) = w;
+          }
+        }
+        release();
+      }
+    };
+
+    // Everything else, in 32 bits through shared memory, 16 result rows at a time; a lane finishes four columns of a row.
+    auto full = [&](auto wide) {
       constexpr bool kWide = decltype(wide)::value;
-      constexpr int kLanes = kGated ? 16 : 32;              // that share a row of 64 or 128 columns
+      constexpr int kLanes = kGated ? 4 : 8;                // that share a row of 16 or 32 columns
       constexpr int S = kWide ? 1 : kLanes;
-      constexpr int kPer = kTurnRows * kLanes / 128;        // rows of a turn per thread
-      const int in_row = lane & (kLanes - 1);
-      const int f = kWide ? 4 * in_row : in_row;            // first of the thread's four columns, of the CTA's
-      const int row_of = ew * (32 / kLanes) + lane / kLanes;  // its first row of a turn; the next are 128 / kLanes behind
-      for (uint32_t i = 0;; ++i) {
-        // All four warps leave together: they meet at barriers, and tcgen05.ld is a whole-warp instruction.
-        if (!epilogue_all(find(i) && !*abort)) break;
-        const uint32_t acc = i & 1, acc_ph = (i >> 1) & 1;
-        const int left = (MODE == kWeight ? a.result_rows : s_rows[cur.group]) - cur.row0, n = min(cur.n, left);
-        const int64_t row0 = (MODE == kWeight ? (int64_t)cur.group * a.result_rows : (int64_t)s_start[cur.group]) + cur.row0;
+      constexpr int kPer = kLanes / 2;                      // of 16 rows, per lane
+      const int f = kWide ? 4 * (lane % kLanes) : lane % kLanes;  // first of its columns, of the warp's
+      float* turned = reinterpret_cast<float*>(stage);      // [16 rows][32 lanes of tensor memory]
+      for (uint32_t i = 0; next(i); ++i) {
         Columns<S, kGated> mine;
         if constexpr (kGated) {
-          mine.out = cur.p * kHalfM + half * (kHalfM / 2) + f;
-          mine.gate = cur.p * kPairM + half * (kHalfM / 2) + f;
+          mine.out = cur.p * kHalfM + half * (kHalfM / 2) + quarter * 16 + f;
+          mine.gate = cur.p * kPairM + half * (kHalfM / 2) + quarter * 16 + f;
           mine.limit = kHalfM;  // whole blocks
         } else {
-          mine.out = mine.gate = cur.p * kPairM + half * kHalfM + f;
+          mine.out = mine.gate = cur.p * kPairM + half * kHalfM + quarter * 32 + f;
           mine.limit = a.features - mine.out;
         }
         mine.load_bias(e, cur.group);
-        if (!epilogue_all(mbar_wait(bar_tfull + 8 * acc, acc_ph, abort, budget))) break;
-        tc_fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * kPairN;
-        for (int c0 = 0; c0 < n; c0 += kTurnRows, turn ^= 1) {
-          float* stage = turns + turn * (kTurnRows * kHalfM);
+        auto turn16 = [&](const float (&v)[16]) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) turned[j * 32 + lane] = v[j];
+        };
+        auto finish16 = [&](int c0, auto&& turn) {  // result rows c0 .. c0 + 15 of the tile
           float r[kPer][4];
 #pragma unroll
           for (int q = 0; q < kPer; ++q) {
-            const int at = c0 + row_of + q * (128 / kLanes);
+            const int at = c0 + lane / kLanes + q * (32 / kLanes);
             if (at < n) mine.load_residual(e, row0 + at, r[q]);
           }
-          float v[16];
+          __syncwarp();  // the rows before have been read
+          turn();
           __syncwarp();
-          tmem_ld_32x16(taddr + c0, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) stage[j * kHalfM + quarter * 32 + lane] = v[j];
-          epilogue_sync();
 #pragma unroll
           for (int q = 0; q < kPer; ++q) {
-            const int in_turn = row_of + q * (128 / kLanes), at = c0 + in_turn;
+            const int in_turn = lane / kLanes + q * (32 / kLanes), at = c0 + in_turn;
             if (at >= n) continue;
-            const float* from = stage + in_turn * kHalfM;
+            const float* from = turned + in_turn * 32 + f;
             float z[4], up[4];
-            // a warp's 32 lanes of tensor memory are, gated, 16 gate rows and their 16 up rows
+            // gated: 16 gate rows and their 16 up rows
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int c = f + j * S;
-              z[j] = from[kGated ? (c >> 4) * 32 + (c & 15) : c];
-              up[j] = kGated ? from[(c >> 4) * 32 + 16 + (c & 15)] : 0.f;
+              z[j] = from[j * S];
+              up[j] = kGated ? from[16 + j * S] : 0.f;
             }
             mine.finish(e, row0 + at, z, up, r[q]);
           }
+        };
+        if constexpr (IN_32) {
+          constexpr int kBlocks = kSumRows / 64;
+          float sum[kBlocks][2][16];  // this warp's 32 result rows of every 64
+          const int parts = (a.k_blocks + kSumBlocks - 1) / kSumBlocks;
+          bool ok = true;
+          for (int p = 0; p < parts; ++p) {
+            if (!(ok = await())) break;
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c) {
+              if (32 * which + 64 * c >= n) continue;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float v[16];
+                __syncwarp();
+                tmem_ld_32x16(tmem_mine + (part & 1) * kPairN + 32 * which + 64 * c + 16 * h, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[c][h][j] = p == 0 ? v[j] : sum[c][h][j] + v[j];
+              }
+            }
+            release();
+          }
+          if (!ok) break;
+#pragma unroll 1
+          for (int b = 0; b < 2 * kBlocks; ++b) {  // one copy of the code behind
+            const int c0 = 32 * which + 64 * (b >> 1) + 16 * (b & 1);
+            if (c0 >= n) break;
+            finish16(c0, [&] {
+#pragma unroll
+              for (int of = 0; of < 2 * kBlocks; ++of)
+                if (of == b) turn16(sum[of >> 1][of & 1]);
+            });
+          }
+        } else {
+          if (!await()) break;
+          for (int c0 = 32 * which; c0 < n; c0 += 64)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (c0 + 16 * h >= n) continue;
+              float v[16];
+              __syncwarp();
+              tmem_ld_32x16(tmem_mine + (part & 1) * kPairN + c0 + 16 * h, v);
+              tmem_ld_wait();
+              finish16(c0 + 16 * h, [&] { turn16(v); });
+            }
+          release();
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(map_to_rank(bar_tempty + 8 * acc, 0));
       }
     };
-    if (a.wide) tiles(std::true_type{});
-    else tiles(std::false_type{});
+    if (!IN_32 && a.plain) {
+      if (e.type == Type::kBf16) plain(std::true_type{});
+      else plain(std::false_type{});
+    } else if (a.wide) {
+      full(std::true_type{});
+    } else {
+      full(std::false_type{});
+    }
   }
 
   // ---------------- teardown ----------------

@@ -23,7 +23,7 @@ struct Matmul {
   const void* bias;      // [groups, n] of bias_type, or null
   const void* residual;  // [m, cols] of out_type, row stride residual_ld, or null
   void* out;             // [m, cols] of out_type, row stride out_ld; cols is n, with kSwiglu n / 2
-  void* pre;             // [m, n] of out_type, row stride pre_ld: z, or null
+  float* pre;            // [m, n], row stride pre_ld: z, or null
   int64_t m, n, k, a_ld, residual_ld, out_ld, pre_ld;
   int groups;
   Activation activation;
@@ -58,7 +58,7 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
 // dz = dout * act'(pre), and the bias's gradient, the sum of dz over the rows of a group
 struct MatmulPre {
   const void* dout;  // [m, cols] of out_type, row stride dout_ld
-  const void* pre;   // [m, n] of out_type, row stride pre_ld; null without an activation
+  const float* pre;  // [m, n], row stride pre_ld; null without an activation
   const int* rows;
   void* dz;          // [m, n] of `type`, row stride dz_ld, or null: not wanted
   void* dbias;       // [groups, n] of bias_type, or null

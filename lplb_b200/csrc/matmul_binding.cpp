@@ -2,9 +2,7 @@
 // stream of the arguments' device.  The reference has no operators of this kind.
 #include "matmul_api.h"
 
-#include "ops_check.h"
-
-namespace py = pybind11;
+#include "ops_autograd.h"
 
 namespace {
 
@@ -58,9 +56,9 @@ Activation activation_of(int64_t code, const Shape& s) {
 }
 const int* rows_of(const OptTensor& rows) { return rows ? rows->data_ptr<int>() : nullptr; }
 
-// (out, pre): pre is the sum before the activation, in out's type, where `keep`
-py::tuple matmul(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_t activation, const OptTensor& residual, const OptTensor& rows, bool out_f32,
-                 bool keep) {
+// (out, pre): pre is the sum before the activation, in 32 bits, where `keep`
+variable_list run_forward(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_t activation, const OptTensor& residual, const OptTensor& rows,
+                      bool out_f32, bool keep) {
   const Shape s = check_operands(a, b, rows);
   lplb::ops::Matmul p{};
   p.activation = activation_of(activation, s);
@@ -98,17 +96,17 @@ py::tuple matmul(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_
     p.residual_ld = carried.stride(0);
   }
   if (keep) {
-    pre = make({s.m, up_to(s.n, 8)}, type, a);
-    p.pre = pre.data_ptr();
+    pre = make({s.m, up_to(s.n, 4)}, torch::kFloat32, a);
+    p.pre = pre.data_ptr<float>();
     p.pre_ld = pre.size(1);
   }
   OPS_CUDA(lplb::ops::launch_matmul(p, a.get_device(), stream_of(a.get_device())));
-  return py::make_tuple(out, keep ? py::cast(pre) : py::none());
+  return {out, pre};
 }
 
 // (da, db, dbias), each where it is needed.  bias: its type, float32 or a's.
-py::tuple matmul_backward(const Tensor& dout, const Tensor& a, const Tensor& b, const OptTensor& pre, int64_t activation, const OptTensor& rows, bool out_f32,
-                          bool bias_f32, bool need_a, bool need_b, bool need_bias) {
+variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b, const OptTensor& pre, int64_t activation, const OptTensor& rows, bool out_f32,
+                       bool bias_f32, bool need_a, bool need_b, bool need_bias) {
   const Shape s = check_operands(a, b, rows);
   const auto act = activation_of(activation, s);
   const int64_t cols = act == lplb::ops::kSwiglu ? s.n / 2 : s.n;
@@ -146,7 +144,7 @@ py::tuple matmul_backward(const Tensor& dout, const Tensor& a, const Tensor& b, 
       p.dout = d.data_ptr();
       p.dout_ld = d.stride(0);
       if (pre) {
-        p.pre = pre->data_ptr();
+        p.pre = pre->data_ptr<float>();
         p.pre_ld = pre->size(1);
       }
       p.rows = rows_of(rows);
@@ -202,14 +200,45 @@ py::tuple matmul_backward(const Tensor& dout, const Tensor& a, const Tensor& b, 
       OPS_CUDA(lplb::ops::launch_matmul_weight(p, device, stream));
     }
   }
-  auto given = [](bool need, const Tensor& t) -> py::object { return need ? py::cast(t) : py::none(); };
-  return py::make_tuple(given(need_a, da), given(need_b, db), given(need_bias, dbias));
+  return {da, db, dbias};
+}
+
+struct Product : torch::autograd::Function<Product> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& a, const Tensor& b, const OptTensor& bias, const OptTensor& residual, const OptTensor& rows,
+                        int64_t activation, bool out_f32) {
+    const bool keep = activation != lplb::ops::kNoActivation && (a.requires_grad() || b.requires_grad() || (bias && bias->requires_grad()));
+    const auto out = run_forward(a, b, bias, activation, residual, rows, out_f32, keep);
+    ctx->save_for_backward({a, b, or_none(rows), out[1]});
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["out_f32"] = out_f32;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["bias_f32"] = bias && bias->scalar_type() == torch::kFloat32;
+    ctx->saved_data["residual"] = residual.has_value();
+    return out[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool has_bias = ctx->saved_data["bias"].toBool();
+    // the tensors that there are, in their order
+    const bool need_a = ctx->needs_input_grad(0), need_b = ctx->needs_input_grad(1), need_bias = has_bias && ctx->needs_input_grad(2);
+    const bool need_residual = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2);
+    variable_list found(3);
+    if (need_a || need_b || need_bias)
+      found = run_backward(grads[0], saved[0], saved[1], or_none(saved[3]), ctx->saved_data["activation"].toInt(), or_none(saved[2]),
+                         ctx->saved_data["out_f32"].toBool(), ctx->saved_data["bias_f32"].toBool(), need_a, need_b, need_bias);
+    return first_order({found[0], found[1], found[2], need_residual ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()}, "matmul");
+  }
+};
+
+Tensor matmul(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_t activation, const OptTensor& residual, const OptTensor& rows, bool out_f32) {
+  const Tensor added = or_none(bias), carried = or_none(residual);
+  if (wants_grad({&a, &b, &added, &carried}, "matmul")) return Product::apply(a, b, bias, residual, rows, activation, out_f32);
+  return run_forward(a, b, bias, activation, residual, rows, out_f32, false)[0];
 }
 
 }  // namespace
 
 void bind_matmul(py::module_& m) {
   m.def("matmul", &matmul);
-  m.def("matmul_backward", &matmul_backward);
   m.attr("MATMUL_MAX_GROUPS") = lplb::ops::kMatmulMaxGroups;
 }

@@ -24,6 +24,7 @@ struct FewProductArgs {
   int m, k_blocks;
   int tiles;   // of 128 rows of b
   int cols;    // rows of a per CTA, a multiple of 16
+  int chains;  // accumulators, of consecutive k blocks each: a result in 32 bits is summed in parts (kSumBlocks)
   int stages;
   int wide;    // as PairArgs
   uint32_t idesc;
@@ -34,13 +35,13 @@ struct FewProductArgs {
 // columns are of the tensor memory, so that CTAs that are on an SM together always find their columns free.
 struct FewProductLayout {
   uint32_t stage, bars, total, columns, request;
-  __host__ __device__ FewProductLayout(int cols, int stages) {
+  __host__ __device__ FewProductLayout(int cols, int chains, int stages) {
     stage = kFewWeightStage + cols * kFewKBytes;
     bars = stage * stages;
     const uint32_t partial = (uint32_t)cols * kFewTileRows * 4;  // over the ring, once it has been read
     if (bars < partial) bars = partial;
     total = bars + (2 * kFewStageMax + 1) * 8;
-    columns = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+    columns = cols * chains <= 64 ? 64 : cols * chains <= 128 ? 128 : 256;
     request = total + 1024 > columns * kFewSmemPerColumn ? total + 1024 : columns * kFewSmemPerColumn;
   }
 };
@@ -51,7 +52,7 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   using namespace sm100;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const FewProductLayout at(a.cols, a.stages);
+  const FewProductLayout at(a.cols, a.chains, a.stages);
   const uint32_t base = smem_u32(smem);
   const uint32_t bar_full = base + at.bars, bar_empty = bar_full + 8 * kFewStageMax, bar_done = bar_empty + 8 * kFewStageMax;
   __shared__ uint32_t tmem_slot;
@@ -60,6 +61,7 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   const int rank = (int)cluster_cta_rank(), split = (int)cluster_size();
   const int tile = (int)blockIdx.x / split % a.tiles, m0 = (int)blockIdx.x / split / a.tiles * a.cols, m_here = min(a.cols, a.m - m0);
   const int kb0 = (int)((int64_t)a.k_blocks * rank / split), kb1 = (int)((int64_t)a.k_blocks * (rank + 1) / split);
+  const int per_chain = (kb1 - kb0 + a.chains - 1) / a.chains;  // k blocks
   allow_successor();
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -102,13 +104,15 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
     if (elect_one()) {
       const uint32_t idesc = a.idesc | umma_idesc_size(kFewTileRows, a.cols);
       uint32_t s = 0, ph = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      uint32_t tmem_d = tmem - a.cols;
+      for (int kb = kb0, in_chain = 0; kb < kb1; ++kb, in_chain = in_chain + 1 < per_chain ? in_chain + 1 : 0) {
         if (!mbar_wait(bar_full + 8 * s, ph, abort, a.budget_ns)) break;
         tc_fence_after_sync();
+        if (in_chain == 0) tmem_d += a.cols;
         const uint32_t src = base + s * at.stage;
         const uint64_t dw = umma_desc_sw128(src), dt = umma_desc_sw128(src + kFewWeightStage);
 #pragma unroll
-        for (int k = 0; k < kPairK / 16; ++k) umma_bf16(tmem, dw + 2 * k, dt + 2 * k, idesc, kb != kb0 || k != 0);
+        for (int k = 0; k < kPairK / 16; ++k) umma_bf16(tmem_d, dw + 2 * k, dt + 2 * k, idesc, in_chain != 0 || k != 0);
         umma_commit(bar_empty + 8 * s);
         if (++s == (uint32_t)a.stages) s = 0, ph ^= 1;
       }
@@ -125,6 +129,13 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
         float v[16];
         tmem_ld_32x16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0, v);
         tmem_ld_wait();
+        for (int chain = 1; chain * per_chain < kb1 - kb0; ++chain) {
+          float more[16];
+          tmem_ld_32x16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + chain * a.cols + c0, more);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] += more[i];
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) partial[(c0 + i) * kFewTileRows + row] = v[i];
       }

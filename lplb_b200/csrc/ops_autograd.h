@@ -1,0 +1,58 @@
+// What the operators with gradients share: when a call is recorded, and what its gradients may be used for.
+#pragma once
+
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
+
+#include <initializer_list>
+#include <memory>
+
+#include "ops_check.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Whether the call is recorded.  Inside a capture a leaf whose gradient is collected on the default stream, because a graph
+// that was recorded there still lives, is refused: the backward pass would make that stream wait for the captured one, which
+// breaks the capture off with an error that names neither.
+inline bool wants_grad(std::initializer_list<const Tensor*> tensors, const char* who) {
+  if (!at::GradMode::is_enabled()) return false;
+  bool wanted = false;
+  for (const Tensor* t : tensors) wanted = wanted || (t->defined() && t->requires_grad());
+  if (!wanted || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return wanted;
+  for (const Tensor* t : tensors) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto collects = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = collects ? collects->stream() : std::nullopt;
+    if (stream && *stream == c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap())
+      throw std::runtime_error(std::string("lplb_b200.ops.") + who +
+                               ": a graph recorded on the default stream still holds this leaf; delete its outputs before a backward pass is captured");
+  }
+  return true;
+}
+inline Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
+inline OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+inline py::object given(const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); }
+
+// Gradients as a backward pass returns them.  A pass that is itself recorded (create_graph=True) gets ones that refuse to be
+// differentiated: these operators' gradients have none.
+inline variable_list first_order(variable_list grads, const char* who) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list leaves;
+  for (const Tensor& g : grads)
+    if (g.defined()) leaves.push_back(g.detach().requires_grad_());
+  if (leaves.empty()) return grads;
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(std::string("lplb_b200.ops.") + who + ": a gradient's gradient is not computed",
+                                                                (int64_t)leaves.size());
+  const variable_list marked = refuse->apply(std::move(leaves));
+  size_t at = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = marked[at++];
+  return grads;
+}
+
+}  // namespace

@@ -2,8 +2,6 @@
 // current stream of the arguments' device.  The reference has no operators of this kind.
 #include "ops_check.h"
 
-namespace py = pybind11;
-
 namespace {
 
 constexpr int64_t kBlock = 128;

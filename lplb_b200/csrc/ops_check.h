@@ -14,6 +14,8 @@
 
 #include "ops_api.h"
 
+namespace py = pybind11;
+
 namespace {
 
 using torch::Tensor;

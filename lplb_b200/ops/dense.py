@@ -3,10 +3,9 @@
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import reference
-from .experts import _wants_grad
+from .experts import _first_order, _wants_grad
 from .fp8 import _check_device, _native, _need
 
 __all__ = ["MATMUL_ACTIVATIONS", "MATMUL_MAX_GROUPS", "matmul"]
@@ -17,41 +16,32 @@ MATMUL_MAX_GROUPS = 1024  #: matrices that matmul takes with ``rows``
 _MOST_ROWS = 2**31 - 256
 
 
-def _forward(a, b, bias, activation, residual, rows, out_dtype, keep):
-    """``(out, z)`` with the sum ``z`` before the activation where ``keep``."""
-    if a.is_cuda:
-        return _native().matmul(a, b, bias, MATMUL_ACTIVATIONS.index(activation), residual, rows, out_dtype == torch.float32, keep)
-    out, z = reference.matmul_reference(a, b, bias, activation, residual, rows)
-    return out.to(out_dtype), z.to(out_dtype) if keep else None
-
-
 class _Matmul(torch.autograd.Function):
+    """On the CPU."""
+
     @staticmethod
     def forward(ctx, a, b, bias, residual, rows, activation, out_dtype):
-        keep = activation is not None and any(ctx.needs_input_grad[:3])
-        out, z = _forward(a, b, bias, activation, residual, rows, out_dtype, keep)
-        ctx.save_for_backward(a, b, rows, z)
-        ctx.options = activation, out_dtype, None if bias is None else bias.dtype
-        return out
+        out, z = reference.matmul_reference(a, b, bias, activation, residual, rows)
+        ctx.save_for_backward(a, b, rows, z if activation is not None else None)
+        ctx.options = activation, None if bias is None else bias.dtype
+        return out.to(out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         a, b, rows, z = ctx.saved_tensors
-        activation, out_dtype, bias_dtype = ctx.options
+        activation, bias_dtype = ctx.options
         need_a, need_b, need_bias, need_residual = ctx.needs_input_grad[:4]
-        da = db = dbias = None
-        if need_a or need_b or need_bias:
-            if a.is_cuda:
-                da, db, dbias = _native().matmul_backward(
-                    dout, a, b, z, MATMUL_ACTIVATIONS.index(activation), rows, out_dtype == torch.float32, bias_dtype == torch.float32,
-                    need_a, need_b, need_bias,
-                )
-            else:
-                da, db, dbias = reference.matmul_backward_reference(dout, a, b, z, activation, rows)
-                da, db = da.to(a.dtype) if need_a else None, db.to(b.dtype) if need_b else None
-                dbias = dbias.to(bias_dtype) if need_bias else None
-        return da, db, dbias, dout if need_residual else None, None, None, None
+        da, db, dbias = reference.matmul_backward_reference(dout, a, b, z, activation, rows)
+        return (
+            da.to(a.dtype) if need_a else None,
+            db.to(b.dtype) if need_b else None,
+            dbias.to(bias_dtype) if need_bias else None,
+            dout if need_residual else None,
+            None,
+            None,
+            None,
+        )
 
 
 def matmul(
@@ -80,19 +70,19 @@ def matmul(
     on a 16-byte boundary; rows of ``a`` that do not are copied first.
 
     Differentiable with respect to ``a``, ``b``, ``bias`` and ``residual``.  For the backward pass the sums before an activation are
-    kept in ``out_dtype``, and their gradients are rounded to ``a``'s type before they are multiplied; all sums are in 32
-    bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
+    kept, in 32 bits, and their gradients are rounded to ``a``'s type before they are multiplied; all sums are in 32 bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
     tensors on plain statements; calls and backward passes can be captured in a CUDA graph, and the same inputs give the same
     bits.  Wrong arguments raise ``ValueError``; :func:`~lplb_b200.ops.check` tells of waits that ran out."""
     who = "matmul:"
     _need(activation in MATMUL_ACTIVATIONS, f"{who} activation must be one of {MATMUL_ACTIVATIONS}, not {activation!r}")
     out_dtype = a.dtype if out_dtype is None else out_dtype
     _need(out_dtype in (a.dtype, torch.float32), f"{who} out_dtype must be a's type or float32, not {out_dtype}")
-    if not a.is_cuda:
-        _check(a, b, bias, activation, residual, rows, out_dtype, who)
+    if a.is_cuda:
+        return _native().matmul(a, b, bias, MATMUL_ACTIVATIONS.index(activation), residual, rows, out_dtype == torch.float32)
+    _check(a, b, bias, activation, residual, rows, out_dtype, who)
     if _wants_grad(a, b, bias, residual):
         return _Matmul.apply(a, b, bias, residual, rows, activation, out_dtype)
-    return _forward(a, b, bias, activation, residual, rows, out_dtype, False)[0]
+    return reference.matmul_reference(a, b, bias, activation, residual, rows)[0].to(out_dtype)
 
 
 def _check(a, b, bias, activation, residual, rows, out_dtype, who):

@@ -27,7 +27,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import reference
 from .fp8 import _check_device, _check_type, _native, _need
@@ -42,32 +41,39 @@ def _wants_grad(*tensors: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _first_order(backward):
+    """For a backward pass on the CPU: its gradients refuse to be differentiated, as the native ones do."""
+
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            found = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return found
+        leaves = [g.detach().requires_grad_() for g in found if g is not None]
+        refuse = torch._C._functions.DelayedError(b"lplb_b200.ops: a gradient's gradient is not computed", len(leaves))
+        marked = iter(refuse(*leaves) if len(leaves) > 1 else (refuse(*leaves),)) if leaves else iter(())
+        return tuple(None if g is None else next(marked) for g in found)
+
+    return wrapped
+
+
 # ---------------------------------------------------------------------------------- the router's choice
 class _GateTopk(torch.autograd.Function):
+    """On the CPU."""
+
     @staticmethod
     def forward(ctx, logits, topk, score, renormalize, scale):
-        weights, idx = _gate(logits, topk, score, renormalize, scale)
+        weights, idx = reference.gate_topk_reference(logits, topk, score, renormalize, scale)
         ctx.save_for_backward(logits, idx)
         ctx.mark_non_differentiable(idx)
         ctx.options = score, renormalize, scale
         return weights, idx
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dweights, _):
         logits, idx = ctx.saved_tensors
-        score, renormalize, scale = ctx.options
-        if logits.is_cuda:
-            dlogits = _native().gate_topk_backward(logits, idx, dweights, score == "sigmoid", renormalize, scale)
-        else:
-            dlogits = reference.gate_topk_backward_reference(logits, idx, dweights, score, renormalize, scale)
-        return dlogits, None, None, None, None
-
-
-def _gate(logits, topk, score, renormalize, scale):
-    if logits.is_cuda:
-        return _native().gate_topk(logits, topk, score == "sigmoid", renormalize, scale)
-    return reference.gate_topk_reference(logits, topk, score, renormalize, scale)
+        return reference.gate_topk_backward_reference(logits, idx, dweights, *ctx.options), None, None, None, None
 
 
 def gate_topk(
@@ -84,14 +90,15 @@ def gate_topk(
     who = "gate_topk:"
     _need(score in ("softmax", "sigmoid"), f"{who} score must be 'softmax' or 'sigmoid', not {score!r}")
     topk, renormalize, scale = int(topk), bool(renormalize), float(scale)
-    if not logits.is_cuda:
-        _check_type(logits, f"{who} logits")
-        _need(logits.dim() == 2, f"{who} logits must be [tokens, experts]")
-        _need(1 <= logits.shape[1] <= GATE_MAX_EXPERTS, f"{who} 1 to {GATE_MAX_EXPERTS} experts")
-        _need(1 <= topk <= min(GATE_MAX_TOPK, logits.shape[1]), f"{who} topk must be 1 to {GATE_MAX_TOPK}, and no more than there are experts")
+    if logits.is_cuda:
+        return _native().gate_topk(logits, topk, score == "sigmoid", renormalize, scale)
+    _check_type(logits, f"{who} logits")
+    _need(logits.dim() == 2, f"{who} logits must be [tokens, experts]")
+    _need(1 <= logits.shape[1] <= GATE_MAX_EXPERTS, f"{who} 1 to {GATE_MAX_EXPERTS} experts")
+    _need(1 <= topk <= min(GATE_MAX_TOPK, logits.shape[1]), f"{who} topk must be 1 to {GATE_MAX_TOPK}, and no more than there are experts")
     if _wants_grad(logits):
         return _GateTopk.apply(logits, topk, score, renormalize, scale)
-    return _gate(logits, topk, score, renormalize, scale)
+    return reference.gate_topk_reference(logits, topk, score, renormalize, scale)
 
 
 # ---------------------------------------------------------------------------------- rows sorted by expert
@@ -127,47 +134,36 @@ def _check_order(rows: torch.Tensor, order: ExpertOrder, who: str) -> None:
     )
 
 
-def _take(x, place, source):
-    return _native().take_rows(x, place, source) if x.is_cuda else reference.take_rows_reference(x, place, source)
-
-
-def _combine(rows, place, source, weights):
-    if rows.is_cuda:
-        return _native().combine_rows(rows, place, source, weights)
-    return reference.combine_rows_reference(rows, place, weights)
-
-
 class _TakeRows(torch.autograd.Function):
+    """On the CPU."""
+
     @staticmethod
     def forward(ctx, x, place, source):
-        ctx.save_for_backward(place, source)
-        return _take(x, place, source)
+        ctx.save_for_backward(place)
+        return reference.take_rows_reference(x, place, source)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, drows):
-        place, source = ctx.saved_tensors
-        return _combine(drows, place, source, None), None, None
+        return reference.combine_rows_reference(drows, *ctx.saved_tensors), None, None
 
 
 class _CombineRows(torch.autograd.Function):
+    """On the CPU."""
+
     @staticmethod
     def forward(ctx, rows, weights, place, source):
         ctx.save_for_backward(*((place, source) if weights is None else (place, source, rows, weights)))
-        return _combine(rows, place, source, weights)
+        return reference.combine_rows_reference(rows, place, weights)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         place, source, *kept = ctx.saved_tensors
         if not kept:
-            return _take(dout, place, source), None, None, None
-        rows, weights = kept
+            return reference.take_rows_reference(dout, place, source), None, None, None
+        drows, dweights = reference.combine_rows_backward_reference(dout, kept[0], place, kept[1])
         need_rows, need_weights = ctx.needs_input_grad[:2]
-        if rows.is_cuda:
-            drows, dweights = _native().combine_rows_backward(dout, rows, place, source, weights, need_rows, need_weights)
-        else:
-            drows, dweights = reference.combine_rows_backward_reference(dout, rows, place, weights)
         return drows if need_rows else None, dweights if need_weights else None, None, None
 
 
@@ -175,14 +171,15 @@ def take_rows(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """``rows`` ``[tokens * topk, values]``, contiguous: ``rows[order.place[t, k]] = x[t]``; rows behind the last
     expert's are zero.  ``x`` is ``[tokens, values]`` of any type, values in 8 bits and their scales among them; rows may be apart
     from one another.  Differentiable for float32, bfloat16 and float16: ``dx[t]`` is the sum of its rows' gradients, in 32 bits."""
-    if not x.is_cuda:
-        _need(x.dim() == 2 and x.shape[1] >= 1, "take_rows: x must be [tokens, values]")
-        _check_order(x, order, "take_rows:")
-        _need(order.place.shape[0] == x.shape[0], "take_rows: x must have a row for each of the order's tokens")
+    if x.is_cuda:
+        return _native().take_rows(x, order.place, order.source)
+    _need(x.dim() == 2 and x.shape[1] >= 1, "take_rows: x must be [tokens, values]")
+    _check_order(x, order, "take_rows:")
+    _need(order.place.shape[0] == x.shape[0], "take_rows: x must have a row for each of the order's tokens")
     if _wants_grad(x):
         _check_type(x, "take_rows: x that requires a gradient")
         return _TakeRows.apply(x, order.place, order.source)
-    return _take(x, order.place, order.source)
+    return reference.take_rows_reference(x, order.place, order.source)
 
 
 def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | None = None) -> torch.Tensor:
@@ -191,16 +188,16 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: torch.Tensor |
     ``[tokens * topk, values]``; choices without a row add nothing, and rows behind the last expert's are not read.  ``weights``
     ``[tokens, topk]`` is of any floating type and used in 32 bits.  Differentiable with respect to ``rows`` (zero where a row is
     nobody's) and ``weights`` (zero where a choice has no row)."""
-    if weights is not None:
-        _need(weights.is_floating_point(), "combine_rows: weights must be floating point [tokens, topk] on the rows' device")
-        weights = weights.float().contiguous()
-    if not rows.is_cuda:
-        _check_type(rows, "combine_rows: rows")
-        _need(rows.dim() == 2 and rows.shape[1] >= 1, "combine_rows: rows must be [tokens * topk, values]")
-        _check_device("combine_rows:", rows, weights)
-        _check_order(rows, order, "combine_rows:")
-        _need(rows.shape[0] == order.place.numel(), "combine_rows: rows must have one for each of the order's choices")
-        _need(weights is None or weights.shape == order.place.shape, "combine_rows: weights must be floating point [tokens, topk]")
+    if rows.is_cuda:
+        return _native().combine_rows(rows, order.place, order.source, weights)
+    who = "combine_rows:"
+    _check_type(rows, f"{who} rows")
+    _need(rows.dim() == 2 and rows.shape[1] >= 1, f"{who} rows must be [tokens * topk, values]")
+    _check_device(who, rows, weights)
+    _check_order(rows, order, who)
+    _need(rows.shape[0] == order.place.numel(), f"{who} rows must have one for each of the order's choices")
+    _need(weights is None or (weights.is_floating_point() and weights.shape == order.place.shape), f"{who} weights must be floating point [tokens, topk]")
+    weights = None if weights is None else weights.float()
     if _wants_grad(rows, weights):
         return _CombineRows.apply(rows, weights, order.place, order.source)
-    return _combine(rows, order.place, order.source, weights)
+    return reference.combine_rows_reference(rows, order.place, weights)

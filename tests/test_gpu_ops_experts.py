@@ -5,7 +5,7 @@ import math
 import experts_oracle as oracle
 import pytest
 import torch
-from test_ops_experts import SCORES, ids_of, logits_of
+from test_ops_experts import SCORES, ids_of, logits_of, no_second_gradient, second_gradients
 
 from lplb_b200 import ops
 
@@ -319,3 +319,8 @@ def test_an_order_that_points_elsewhere_is_not_followed():
     y = torch.ones(4, 64, device="cuda", requires_grad=True)
     dy, dw = torch.autograd.grad(ops.combine_rows(y, order, w), (y, w), torch.ones(2, 64, device="cuda"))
     assert dw.tolist() == [[64, 0], [0, 0]] and torch.equal(dy[0], torch.ones(64, device="cuda")) and not dy[1:].any()
+
+
+@pytest.mark.parametrize("name", list(second_gradients("cpu")))
+def test_no_second_gradient(name):
+    no_second_gradient(name, "cuda")

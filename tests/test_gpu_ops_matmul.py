@@ -238,3 +238,26 @@ def test_refuses_other_devices_and_weights_off_a_boundary():
             ops.matmul(**{"a": a, "b": b, **changed})
     with pytest.raises(ValueError, match="16-byte"):
         ops.matmul(a, torch.zeros(129, dtype=BF16, device="cuda")[1:].view(8, 16))
+
+
+@pytest.mark.parametrize("through_leaf", [False, True])
+def test_a_capture_beside_a_living_graph(through_leaf):
+    """A leaf whose gradient is collected on the default stream, by a graph that still lives, is refused inside a capture; once that
+    graph is gone, or where it hangs on no leaf of the call, the capture goes through."""
+    a = torch.randn(32, 64, device="cuda").bfloat16().requires_grad_()
+    b = torch.randn(64, 64, device="cuda").bfloat16().requires_grad_()
+    living = ops.matmul(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still holds this leaf"):
+        with torch.cuda.graph(graph):
+            ops.matmul(a, b)
+    del living
+    dout = torch.ones(32, 64, device="cuda", dtype=BF16)
+    other = ops.matmul(a.detach().clone().requires_grad_(), b.detach()) if through_leaf else None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        da, db = torch.autograd.grad(ops.matmul(a, b), (a, b), dout)
+    graph.replay()
+    want = torch.autograd.grad(ops.matmul(a, b), (a, b), dout)
+    assert torch.equal(da, want[0]) and torch.equal(db, want[1])
+    assert other is None or other.requires_grad

@@ -86,11 +86,33 @@ def test_gate_refuses():
         ops.gate_topk(torch.randn(2, 64), 33)
 
 
-def test_gate_has_no_second_gradient():
-    x = torch.randn(2, 8, requires_grad=True)
-    (dx,) = torch.autograd.grad(ops.gate_topk(x, 2)[0].sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        dx.sum().backward()
+def second_gradients(device):
+    """A function of x for every operator with a gradient."""
+    order = ops.expert_order(torch.tensor([[0, 1], [1, -1]], device=device), 2)
+    w = torch.rand(2, 2, device=device)
+    b = torch.randn(8, 8, device=device).bfloat16()
+    return {
+        "gate_topk": lambda x: ops.gate_topk(x[:2], 2)[0],
+        "take_rows": lambda x: ops.take_rows(x[:2], order),
+        "combine_rows": lambda x: ops.combine_rows(x, order, w),
+        "combine_rows without weights": lambda x: ops.combine_rows(x, order),
+        "matmul": lambda x: ops.matmul(x.bfloat16(), b, activation="silu"),
+    }
+
+
+def no_second_gradient(name, device):
+    x = torch.randn(4, 8, device=device, requires_grad=True)
+    y = second_gradients(device)[name](x)
+    (dx,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    want = torch.autograd.grad((y * y).sum(), x)[0]
+    assert torch.equal(dx.detach(), want)
+    with pytest.raises(RuntimeError, match="gradient's gradient"):
+        (dx * dx).sum().backward()
+
+
+@pytest.mark.parametrize("name", list(second_gradients("cpu")))
+def test_no_second_gradient(name):
+    no_second_gradient(name, "cpu")
 
 
 def ids_of(tokens, topk, experts, seed, dtype=torch.int64):

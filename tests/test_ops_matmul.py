@@ -92,14 +92,6 @@ def test_only_what_is_asked_for():
     assert not ops.matmul(**args).requires_grad
 
 
-def test_has_no_second_gradient():
-    args, dout = make_case(3, 8, 8, None, None, None, False, torch.bfloat16, torch.bfloat16, 1)
-    a = args["a"].requires_grad_()
-    (da,) = torch.autograd.grad(ops.matmul(**args).float().sum(), a, create_graph=True)
-    with pytest.raises(RuntimeError):
-        da.float().sum().backward()
-
-
 def refusals(device):
     """(changed arguments, words of the refusal)"""
     def t(*shape, dtype=torch.bfloat16):
