@@ -15,6 +15,7 @@
 #include <initializer_list>
 
 #include "common.cuh"
+#include "expert_bulk.cuh"
 #include "experts_api.h"
 #include "tcgen05.cuh"
 
@@ -167,12 +168,10 @@ template <> struct Bytes<4> { using type = uint32_t; };
 template <> struct Bytes<2> { using type = uint16_t; };
 template <> struct Bytes<1> { using type = uint8_t; };
 
-constexpr int kRowsAtOnce = 8;  // of a token
-
 // ---- rows to their experts ------------------------------------------------------------------------
 constexpr int kTakeVectors = 4;  // of a row, per thread and round
 template <int N>
-__global__ void __launch_bounds__(256) take_rows_kernel(const TakeRows a) {
+__global__ void __launch_bounds__(256, 4) take_rows_kernel(const TakeRows a) {
   using V = typename Bytes<N>::type;
   allow_successor();
   wait_predecessors();
@@ -181,36 +180,28 @@ __global__ void __launch_bounds__(256) take_rows_kernel(const TakeRows a) {
   const int64_t vectors = a.row_bytes / N, n_rows = a.tokens * a.topk;
   const V* x = reinterpret_cast<const V*>(static_cast<const uint8_t*>(a.x) + token * a.ld_bytes);
   V* rows = static_cast<V*>(a.rows);
+  const int* place = a.place + token * a.topk;
+  const int* source = a.source + token * a.topk;
   const int64_t step = (int64_t)gridDim.y * blockDim.x;
-  const V zero{};
   for (int64_t v0 = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; v0 < vectors; v0 += step * kTakeVectors) {
     V v[kTakeVectors];
 #pragma unroll
-    for (int i = 0; i < kTakeVectors; ++i) v[i] = v0 + i * step < vectors ? x[v0 + i * step] : zero;
-    for (int k0 = 0; k0 < a.topk; k0 += kRowsAtOnce) {
-      int place[kRowsAtOnce], source[kRowsAtOnce];
+    for (int i = 0; i < kTakeVectors; ++i) v[i] = v0 + i * step < vectors ? x[v0 + i * step] : V{};
+    auto put = [&](int64_t row, const V (&what)[kTakeVectors]) {
+      V* to = rows + row * vectors + v0;
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j) {
-        const bool in = k0 + j < a.topk;
-        place[j] = in ? a.place[token * a.topk + k0 + j] : -1;
-        source[j] = in ? a.source[token * a.topk + k0 + j] : 0;
-      }
-#pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j) {
-        if (place[j] >= 0 && place[j] < n_rows) {
-          V* to = rows + place[j] * vectors;
-#pragma unroll
-          for (int i = 0; i < kTakeVectors; ++i)
-            if (v0 + i * step < vectors) to[v0 + i * step] = v[i];
-        }
-        if (source[j] < 0) {  // a row that nobody has
-          V* to = rows + (token * a.topk + k0 + j) * vectors;
-#pragma unroll
-          for (int i = 0; i < kTakeVectors; ++i)
-            if (v0 + i * step < vectors) to[v0 + i * step] = zero;
-        }
-      }
+      for (int i = 0; i < kTakeVectors; ++i)
+        if (v0 + i * step < vectors) to[i * step] = what[i];
+    };
+    const V zero[kTakeVectors]{};
+#pragma unroll 4
+    for (int k = 0; k < a.topk; ++k) {
+      const int64_t to = place[k];
+      if (to >= 0 && to < n_rows) put(to, v);
     }
+#pragma unroll 4
+    for (int k = 0; k < a.topk; ++k)
+      if (source[k] < 0) put(token * a.topk + k, zero);  // a row that nobody has
   }
 }
 
@@ -242,8 +233,9 @@ __device__ __forceinline__ void narrow(__nv_bfloat16& p, float v) { p = __float2
 __device__ __forceinline__ void narrow(__half& p, float v) { p = __float2half_rn(v); }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(256) combine_rows_kernel(const CombineRows a) {
-  using V = Few<T, N>;
+__global__ void __launch_bounds__(256, 3) combine_rows_kernel(const CombineRows a) {
+  constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
+  constexpr int kRows = 4;                        // of a token, under way
   allow_successor();
   wait_predecessors();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -251,113 +243,141 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(const CombineRows a) 
   const int64_t n_rows = a.tokens * a.topk;
   const int vectors = a.cols / N, step = gridDim.y * blockDim.x;
   const T* rows = static_cast<const T*>(a.rows);
+  const int* place = a.place + token * a.topk;
   T* out = static_cast<T*>(a.out) + token * a.cols;
-  for (int v0 = blockIdx.y * blockDim.x + threadIdx.x; v0 < vectors; v0 += step) {
-    float sum[N];
+  for (int v0 = blockIdx.y * blockDim.x + threadIdx.x; v0 < vectors; v0 += step * kVectors) {
+    float sum[kVectors][N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) sum[n] = 0.f;
-    for (int k0 = 0; k0 < a.topk; k0 += kRowsAtOnce) {
-      int place[kRowsAtOnce];
-      float w[kRowsAtOnce];
-      V y[kRowsAtOnce];
+    for (int v = 0; v < kVectors; ++v)
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j) {
-        const bool in = k0 + j < a.topk;
-        place[j] = in ? a.place[token * a.topk + k0 + j] : -1;
-        w[j] = in && a.weights != nullptr ? a.weights[token * a.topk + k0 + j] : 1.f;
-        if (place[j] >= n_rows) place[j] = -1;
+      for (int n = 0; n < N; ++n) sum[v][n] = 0.f;
+    for (int k0 = 0; k0 < a.topk; k0 += kRows) {
+      // Nothing is asked between the loads (each would wait for the one before): what is not there is read from the first row, or the
+      // row's first vector, and left out below.
+      Few<T, N> y[kRows][kVectors];
+      float w[kRows];
+      bool there[kRows];
+      int64_t at[kRows];
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int k = min(k0 + j, a.topk - 1);
+        at[j] = place[k];
+        w[j] = a.weights != nullptr ? a.weights[token * a.topk + k] : 1.f;
       }
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j)
-        if (place[j] >= 0) y[j] = load_few<T, N>(rows + place[j] * a.ld + (int64_t)v0 * N);
+      for (int j = 0; j < kRows; ++j) {
+        there[j] = k0 + j < a.topk && at[j] >= 0 && at[j] < n_rows;
+        const T* from = rows + (there[j] ? at[j] : 0) * a.ld;
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j) {
-        if (place[j] < 0) continue;
+        for (int v = 0; v < kVectors; ++v) y[j][v] = load_few<T, N>(from + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
+      }
 #pragma unroll
-        for (int n = 0; n < N; ++n) sum[n] = fmaf(w[j], widen(y[j].v[n]), sum[n]);
+      for (int j = 0; j < kRows; ++j) {
+        if (!there[j]) continue;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v)
+#pragma unroll
+          for (int n = 0; n < N; ++n) sum[v][n] = fmaf(w[j], widen(y[j][v].v[n]), sum[v][n]);
       }
     }
-    V r;
 #pragma unroll
-    for (int n = 0; n < N; ++n) narrow(r.v[n], sum[n]);
-    store_few(out + (int64_t)v0 * N, r);
+    for (int v = 0; v < kVectors; ++v) {
+      Few<T, N> r;
+#pragma unroll
+      for (int n = 0; n < N; ++n) narrow(r.v[n], sum[v][n]);
+      if (v0 + v * step < vectors) store_few(out + (int64_t)(v0 + v * step) * N, r);
+    }
   }
 }
 
 template <typename T, int N>
-__global__ void __launch_bounds__(256) combine_rows_backward_kernel(const CombineRows a) {
-  using V = Few<T, N>;
-  __shared__ float part[kRowsAtOnce][8];
+__global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const CombineRows a) {
+  constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
+  constexpr int kRows = 4;                        // of a token, at a time
+  __shared__ float part[kRows][8];
   allow_successor();
   wait_predecessors();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   if (token >= a.tokens) return;  // a CTA of several warps per token has one token
   const int64_t n_rows = a.tokens * a.topk;
-  const int vectors = a.cols / N;
+  const int vectors = a.cols / N, step = blockDim.x;
   const T* rows = static_cast<const T*>(a.rows);
   T* drows = static_cast<T*>(a.drows);
   const T* dout = static_cast<const T*>(a.dout) + token * a.dout_ld;
-  for (int k0 = 0; k0 < a.topk; k0 += kRowsAtOnce) {
-    int place[kRowsAtOnce];
-    float w[kRowsAtOnce], dot[kRowsAtOnce];
-    bool spare[kRowsAtOnce];
+  for (int k0 = 0; k0 < a.topk; k0 += kRows) {
+    int place[kRows];
+    float w[kRows], dot[kRows];
+    bool spare[kRows];
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j) {
-      const bool in = k0 + j < a.topk;
-      place[j] = in ? a.place[token * a.topk + k0 + j] : -1;
-      w[j] = in ? a.weights[token * a.topk + k0 + j] : 0.f;
-      spare[j] = in && drows != nullptr && a.source[token * a.topk + k0 + j] < 0;
+    for (int j = 0; j < kRows; ++j) {
+      const int k = min(k0 + j, a.topk - 1);
+      place[j] = a.place[token * a.topk + k];
+      w[j] = a.weights[token * a.topk + k];
+      spare[j] = drows != nullptr && a.source[token * a.topk + k] < 0;
       dot[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      if (k0 + j >= a.topk) place[j] = -1, spare[j] = false;
       if (place[j] >= n_rows) place[j] = -1;
     }
-    for (int v0 = threadIdx.x; v0 < vectors; v0 += blockDim.x) {
-      const V d = load_few<T, N>(dout + (int64_t)v0 * N);
-      V y[kRowsAtOnce];
+    for (int v0 = threadIdx.x; v0 < vectors; v0 += step * kVectors) {
+      Few<T, N> d[kVectors], y[kRows][kVectors];  // (nothing is asked between the loads, as above)
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) d[v] = load_few<T, N>(dout + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
       if (a.dweights != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kRowsAtOnce; ++j)
-          if (place[j] >= 0) y[j] = load_few<T, N>(rows + place[j] * a.ld + (int64_t)v0 * N);
+        for (int j = 0; j < kRows; ++j) {
+          const T* from = rows + (int64_t)max(place[j], 0) * a.ld;
+#pragma unroll
+          for (int v = 0; v < kVectors; ++v) y[j][v] = load_few<T, N>(from + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j) {
-        if (place[j] >= 0) {
-          if (drows != nullptr) {
-            V r;
+      for (int v = 0; v < kVectors; ++v) {
+        if (v0 + v * step >= vectors) continue;
+        const int64_t column = (int64_t)(v0 + v * step) * N;
 #pragma unroll
-            for (int n = 0; n < N; ++n) narrow(r.v[n], w[j] * widen(d.v[n]));
-            store_few(drows + (int64_t)place[j] * a.cols + (int64_t)v0 * N, r);
+        for (int j = 0; j < kRows; ++j) {
+          if (place[j] >= 0) {
+            if (drows != nullptr) {
+              Few<T, N> r;
+#pragma unroll
+              for (int n = 0; n < N; ++n) narrow(r.v[n], w[j] * widen(d[v].v[n]));
+              store_few(drows + (int64_t)place[j] * a.cols + column, r);
+            }
+            if (a.dweights != nullptr) {
+#pragma unroll
+              for (int n = 0; n < N; ++n) dot[j] = fmaf(widen(d[v].v[n]), widen(y[j][v].v[n]), dot[j]);
+            }
           }
-          if (a.dweights != nullptr) {
+          if (spare[j]) {
+            Few<T, N> zero;
 #pragma unroll
-            for (int n = 0; n < N; ++n) dot[j] = fmaf(widen(d.v[n]), widen(y[j].v[n]), dot[j]);
+            for (int n = 0; n < N; ++n) narrow(zero.v[n], 0.f);
+            store_few(drows + (token * a.topk + k0 + j) * a.cols + column, zero);
           }
-        }
-        if (spare[j]) {
-          V zero;
-#pragma unroll
-          for (int n = 0; n < N; ++n) narrow(zero.v[n], 0.f);
-          store_few(drows + (token * a.topk + k0 + j) * a.cols + (int64_t)v0 * N, zero);
         }
       }
     }
     if (a.dweights == nullptr) continue;
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j) {
+    for (int j = 0; j < kRows; ++j) {
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1) dot[j] += __shfl_xor_sync(kAll, dot[j], s);
     }
     if (warps == 1) {
 #pragma unroll
-      for (int j = 0; j < kRowsAtOnce; ++j)
+      for (int j = 0; j < kRows; ++j)
         if (lane == j && k0 + j < a.topk) a.dweights[token * a.topk + k0 + j] = dot[j];
       continue;
     }
 #pragma unroll
-    for (int j = 0; j < kRowsAtOnce; ++j)
+    for (int j = 0; j < kRows; ++j)
       if (lane == j) part[j][warp] = dot[j];
     __syncthreads();
-    if (warp == 0 && lane < kRowsAtOnce && k0 + lane < a.topk) {
+    if (warp == 0 && lane < kRows && k0 + lane < a.topk) {
       float sum = 0.f;
       for (int i = 0; i < warps; ++i) sum += part[lane][i];
       a.dweights[token * a.topk + k0 + lane] = sum;
@@ -374,11 +394,64 @@ int widest(std::initializer_list<uint64_t> of) {
 }
 uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
+// The shape of a pass by bulk copies: pieces of at most `most` bytes, `rows` of them to a slot, and so many that the SMs have
+// about two each.
+BulkArgs bulk_args(int64_t tokens, int64_t row_bytes, uint32_t most, uint32_t rows, int spare, int n_sms) {
+  BulkArgs a{};
+  int64_t pieces = (row_bytes + most - 1) / most;
+  while (tokens * pieces < 2 * n_sms && row_bytes / pieces > 1024) ++pieces;
+  a.piece = (uint32_t)(((row_bytes + pieces - 1) / pieces + 127) / 128 * 128);
+  a.pieces = (row_bytes + a.piece - 1) / a.piece;
+  a.slot = a.piece * rows;
+  a.slots = (int)(kBulkRing / a.slot) - spare;
+  if (a.slots > kBulkSlots) a.slots = kBulkSlots;
+  a.budget_ns = wait_budget_ns();
+  return a;
+}
+template <auto KERNEL>
+cudaError_t prepare_bulk(BulkArgs& a) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (device >= kMaxDevices) return cudaErrorInvalidDevice;
+  static std::atomic<bool> prepared[kMaxDevices];
+  if (!prepared[device].load(std::memory_order_relaxed)) {
+    if ((err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBulkSmem)) != cudaSuccess) return err;
+    prepared[device].store(true, std::memory_order_relaxed);
+  }
+  return ops_error_word(device, &a.status);
+}
+
+cudaError_t launch_take_bulk(const TakeRows& t, int n_sms, cudaStream_t stream) {
+  BulkArgs a = bulk_args(t.tokens, t.row_bytes, kTakeMostPiece, 1, 1, n_sms);
+  const cudaError_t err = prepare_bulk<take_rows_bulk_kernel>(a);
+  if (err != cudaSuccess) return err;
+  const int64_t items = t.tokens * a.pieces;
+  return launch_after(take_rows_bulk_kernel, dim3((unsigned)(items < n_sms ? items : n_sms)), dim3(32), kBulkSmem, stream, t, a);
+}
+
+template <typename T, bool BACKWARD, int KEEP>
+cudaError_t launch_join(const CombineRows& c, int n_sms, cudaStream_t stream) {
+  const uint32_t rows = c.topk + (BACKWARD ? 1 : 0);
+  uint32_t most = kBulkRing / (4 * rows) / 128 * 128;  // four slots at least
+  if (most > kJoinMostPiece) most = kJoinMostPiece;
+  BulkArgs a = bulk_args(BACKWARD ? INT32_MAX : c.tokens, (int64_t)c.cols * sizeof(T), most, rows, 0, n_sms);
+  constexpr auto kernel = combine_rows_bulk_kernel<T, BACKWARD, KEEP>;
+  const cudaError_t err = prepare_bulk<kernel>(a);
+  if (err != cudaSuccess) return err;
+  a.whole = BACKWARD || c.tokens >= 4 * n_sms;
+  const int64_t units = a.whole ? c.tokens : c.tokens * a.pieces;
+  return launch_after(kernel, dim3((unsigned)(units < n_sms ? units : n_sms)), dim3(kJoinThreads), kBulkSmem, stream, c, a);
+}
+
 template <int N>
 cudaError_t launch_take(const TakeRows& t, int n_sms, cudaStream_t stream) {
   const Shape s = shape_of(t.tokens, t.row_bytes / N, kTakeVectors, n_sms, false);
   return launch_after(take_rows_kernel<N>, s.grid, s.block, 0, stream, t);
 }
+
+// Bytes of a token and its rows from which on bulk copies pay.
+constexpr uint64_t kBulkLeast = 16 * 1024;
 
 bool refused(const CombineRows& c) { return c.tokens < 0 || c.tokens > INT32_MAX || c.cols < 1 || c.topk < 1; }
 
@@ -386,10 +459,10 @@ template <typename T, int N>
 cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaStream_t stream) {
   const int vectors = c.cols / N;
   if (backward) {
-    const Shape s = shape_of(c.tokens, vectors, 2, n_sms, true);
+    const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, true);
     return launch_after(combine_rows_backward_kernel<T, N>, s.grid, s.block, 0, stream, c);
   }
-  const Shape s = shape_of(c.tokens, vectors, 1, n_sms, false);
+  const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, false);
   return launch_after(combine_rows_kernel<T, N>, s.grid, s.block, 0, stream, c);
 }
 template <typename T>
@@ -397,7 +470,14 @@ cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaS
   const uint64_t size = sizeof(T);
   int wide = backward ? widest({address(c.rows), c.ld * size, c.cols * size, address(c.dout), c.dout_ld * size, address(c.drows)})
                       : widest({address(c.rows), c.ld * size, c.cols * size, address(c.out)});
-  if (wide == 16) return launch_combine<T, 16 / sizeof(T)>(c, n_sms, backward, stream);
+  if (wide == 16) {
+    if (c.cols * size * (c.topk + 1) >= kBulkLeast) {
+      if (!backward && c.topk <= kJoinMostTopk) return launch_join<T, false, 1>(c, n_sms, stream);
+      if (backward && c.topk <= 8) return launch_join<T, true, 8>(c, n_sms, stream);
+      if (backward && c.topk <= 16) return launch_join<T, true, 16>(c, n_sms, stream);
+    }
+    return launch_combine<T, 16 / sizeof(T)>(c, n_sms, backward, stream);
+  }
   if (wide >= 4) return launch_combine<T, 4 / sizeof(T)>(c, n_sms, backward, stream);
   if constexpr (sizeof(T) == 2) return launch_combine<T, 1>(c, n_sms, backward, stream);
   return cudaErrorMisalignedAddress;
@@ -454,7 +534,9 @@ cudaError_t launch_take_rows(const TakeRows& t, int n_sms, cudaStream_t stream) 
   if (t.tokens < 0 || t.tokens > INT32_MAX || t.row_bytes < 1 || t.topk < 1) return cudaErrorInvalidValue;
   if (t.tokens == 0) return cudaSuccess;
   switch (widest({address(t.x), (uint64_t)t.ld_bytes, (uint64_t)t.row_bytes, address(t.rows)})) {
-    case 16: return launch_take<16>(t, n_sms, stream);
+    case 16:
+      if ((uint64_t)t.row_bytes * (t.topk + 1) >= kBulkLeast) return launch_take_bulk(t, n_sms, stream);
+      return launch_take<16>(t, n_sms, stream);
     case 8: return launch_take<8>(t, n_sms, stream);
     case 4: return launch_take<4>(t, n_sms, stream);
     case 2: return launch_take<2>(t, n_sms, stream);
@@ -463,7 +545,7 @@ cudaError_t launch_take_rows(const TakeRows& t, int n_sms, cudaStream_t stream) 
 }
 
 cudaError_t launch_combine_rows(const CombineRows& c, int n_sms, cudaStream_t stream) { return launch_combine(c, n_sms, false, stream); }
-cudaError_t launch_combine_rows_backward(const CombineRows& c, cudaStream_t stream) { return launch_combine(c, 1, true, stream); }
+cudaError_t launch_combine_rows_backward(const CombineRows& c, int n_sms, cudaStream_t stream) { return launch_combine(c, n_sms, true, stream); }
 
 }  // namespace ops
 }  // namespace lplb

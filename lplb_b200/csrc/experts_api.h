@@ -64,7 +64,7 @@ struct CombineRows {
   Type type;
 };
 cudaError_t launch_combine_rows(const CombineRows& c, int n_sms, cudaStream_t stream);
-cudaError_t launch_combine_rows_backward(const CombineRows& c, cudaStream_t stream);
+cudaError_t launch_combine_rows_backward(const CombineRows& c, int n_sms, cudaStream_t stream);
 
 }  // namespace ops
 }  // namespace lplb

@@ -184,7 +184,7 @@ variable_list combine_backward(const Tensor& dout, const Tensor& rows, const Ten
   }
   c.dout = d.data_ptr();
   c.dout_ld = d.stride(0);
-  OPS_CUDA(lplb::ops::launch_combine_rows_backward(c, stream_of(rows.get_device())));
+  OPS_CUDA(lplb::ops::launch_combine_rows_backward(c, sm_count(rows.get_device()), stream_of(rows.get_device())));
   return {drows, dweights};
 }
 

@@ -118,6 +118,7 @@ def off(shape, dtype, by, g, pad=0):
     [
         (1, 1, 1, 0, 0), (3, 2, 7, 0, 0), (5, 8, 8, 0, 0), (64, 8, 7168, 0, 0), (70, 9, 2064, 0, 8), (21, 6, 2065, 0, 0), (21, 3, 2066, 0, 0),
         (18, 33, 40, 0, 0), (19, 4, 256, 1, 0), (19, 4, 256, 2, 6), (300, 5, 96, 0, 32), (2, 2, 20000, 0, 0),
+        (1, 8, 4096, 0, 0), (300, 1, 8192, 0, 0), (700, 8, 1024, 0, 0), (40, 16, 2048, 0, 0), (30, 17, 1032, 0, 8), (20, 32, 1024, 0, 0), (20, 33, 1024, 0, 0),
     ],
 )
 def test_rows_there_and_back(tokens, topk, hidden, by, pad, dtype):
