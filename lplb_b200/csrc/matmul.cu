@@ -22,7 +22,7 @@ __device__ __forceinline__ float slope(float z, int activation) {
     const float s = sigmoid_of(z);
     return s * (1.f + z * (1.f - s));
   }
-  if (activation == kGelu) return normcdff(z) + z * 0.3989422804f * __expf(-0.5f * z * z);  // 1 / sqrt(2 pi)
+  if (activation == kGelu) return normal_cdf(z) + z * 0.3989422804f * __expf(-0.5f * z * z);  // 1 / sqrt(2 pi)
   return 1.f;
 }
 __device__ __forceinline__ float through(float d, float z, int activation) {
@@ -78,35 +78,45 @@ __global__ void __launch_bounds__(256) pre_gradient_kernel(const PreArgs a) {
     limit[v] = GATED ? 4 * S : a.n - at_z[v];
   }
   float sum[2][4] = {};
-  for (int r = r0 + warp; r < r1; r += kPreRows) {
-    float d[2][4] = {}, z[2][4] = {};
+  constexpr int kAtOnce = 2;  // rows whose loads are under way together
+  for (int base = r0 + warp; base < r1; base += kPreRows * kAtOnce) {
+    float d[kAtOnce][2][4] = {}, z[kAtOnce][2][4] = {};
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-      load4<S>(a.dout, a.out_type, r * a.dout_ld + at_out[v], limit[v], d[v]);
-      if (a.pre != nullptr) load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[v], limit[v], z[v]);
-    }
-    if (GATED) {
-      load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[0] + kGateBlock, limit[0], z[1]);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t r = min(base + i * kPreRows, r1 - 1);  // (the last row again, and left out below)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float s = sigmoid_of(z[0][j]), g = d[0][j];
-        d[0][j] = g * z[1][j] * s * (1.f + z[0][j] * (1.f - s));
-        d[1][j] = g * z[0][j] * s;
+      for (int v = 0; v < kVectors; ++v) {
+        load4<S>(a.dout, a.out_type, r * a.dout_ld + at_out[v], limit[v], d[i][v]);
+        if (a.pre != nullptr) load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[v], limit[v], z[i][v]);
       }
-    } else if (a.activation != kNoActivation) {
-#pragma unroll
-      for (int v = 0; v < 2; ++v)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[v][j] = through(d[v][j], z[v][j], a.activation);
+      if (GATED) load4<S>(a.pre, Type::kF32, r * a.pre_ld + at_z[0] + kGateBlock, limit[0], z[i][1]);
     }
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      if (a.dz != nullptr) {
-        const int i = GATED ? 0 : v;
-        store4<S>(a.dz, a.type, r * a.dz_ld + at_z[i] + (GATED && v ? kGateBlock : 0), limit[i], d[v]);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t r = base + i * kPreRows;
+      if (r >= r1) break;
+      if (GATED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float s = sigmoid_of(z[i][0][j]), g = d[i][0][j];
+          d[i][0][j] = g * z[i][1][j] * s * (1.f + z[i][0][j] * (1.f - s));
+          d[i][1][j] = g * z[i][0][j] * s;
+        }
+      } else if (a.activation != kNoActivation) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[i][v][j] = through(d[i][v][j], z[i][v][j], a.activation);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[v][j] += d[v][j];
+      for (int v = 0; v < 2; ++v) {
+        if (a.dz != nullptr) {
+          const int w = GATED ? 0 : v;
+          store4<S>(a.dz, a.type, r * a.dz_ld + at_z[w] + (GATED && v ? kGateBlock : 0), limit[w], d[i][v]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[v][j] += d[i][v][j];
+      }
     }
   }
   if (a.dbias == nullptr && a.parts == nullptr) return;
@@ -158,6 +168,17 @@ cudaError_t map_3d(CUtensorMap* map, const void* base, uint64_t matrices, uint64
   const cuuint32_t box[3] = {(cuuint32_t)kPairK, box_rows, 1};
   return encode_tensor_map(map, kMapType, base, 3, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
 }
+// MN-major operands whose columns come in whole chunks of 64: [rows, cols] as [chunks, rows, 64], boxes of two chunks
+cudaError_t map_chunks(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  const cuuint64_t dims[3] = {kChunk, rows, cols / kChunk}, strides[2] = {ld * 2, kChunk * 2};
+  const cuuint32_t box[3] = {kChunk, box_rows, 2};
+  return encode_tensor_map(map, kMapType, base, 3, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+cudaError_t map_chunks(CUtensorMap* map, const void* base, uint64_t matrices, uint64_t rows, uint64_t cols) {
+  const cuuint64_t dims[4] = {kChunk, rows, cols / kChunk, matrices}, strides[3] = {cols * 2, kChunk * 2, rows * cols * 2};
+  const cuuint32_t box[4] = {kChunk, kPairK, 2, 1};
+  return encode_tensor_map(map, kMapType, base, 4, dims, strides, box) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
 // Weights in blocks of 128 gate rows and their 128 up rows, dealt out so that 32 rows in shared memory are 16 gate rows and their
 // 16 up rows.
 cudaError_t map_gated(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
@@ -205,6 +226,8 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   }
   if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
   a.budget_ns = wait_budget_ns();
+  if (a.p_chunks == 0) a.p_chunks = 1;
+  if (a.q_chunks == 0) a.q_chunks = 1;
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
   const int out_cols = MODE == kForwardGated ? a.features / 2 : a.features;
   a.plain = a.e.type != Type::kF32 && a.e.residual == nullptr && a.e.pre == nullptr && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
@@ -346,6 +369,73 @@ bool refused(int64_t m, int64_t n, int64_t k, int groups, int device) {
          device >= kMaxDevices;
 }
 
+// ---- a weight's gradient over groups: their last blocks ------------------------------------------------------
+// Rows of a and dz behind a group's last whole block of 64, and zeros up to a multiple of 16 (the rest is not read).  By words of
+// 16 bytes; a row's last one may end behind its values, with zeros.
+struct LastBlocks {
+  const void* from[2];
+  void* to[2];
+  int64_t from_ld[2], to_ld[2], bytes[2];  // in bytes
+  int words[2];
+  const int* rows;
+  int groups, m;
+};
+__global__ void __launch_bounds__(256) last_blocks_kernel(const LastBlocks a) {
+  __shared__ long long s_before[8];
+  allow_successor();
+  wait_predecessors();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.y;
+  long long before = 0;
+  for (int e = threadIdx.x; e < group; e += 256) before += max(a.rows[e], 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) s_before[warp] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) before += s_before[w];
+  const int first = (int)min((long long)a.m, before), rows = (int)min((long long)a.m - first, (long long)max(a.rows[group], 0));
+  const int count = rows % kPairK, padded = (count + 15) / 16 * 16;
+  int word = blockIdx.x * 256 + threadIdx.x;
+  const int which = word >= a.words[0];
+  if (which) word -= a.words[0];
+  if (word >= a.words[which]) return;
+  const uint8_t* from = static_cast<const uint8_t*>(a.from[which]) + (int64_t)(first + rows - count) * a.from_ld[which] + (int64_t)word * 16;
+  uint8_t* to = static_cast<uint8_t*>(a.to[which]) + (int64_t)group * kPairK * a.to_ld[which] + (int64_t)word * 16;
+  const int64_t left = a.bytes[which] - (int64_t)word * 16;
+  constexpr int kAtOnce = 8;  // rows; nothing is asked between their loads
+  for (int r0 = blockIdx.z * kAtOnce; r0 < padded; r0 += gridDim.z * kAtOnce) {
+    uint4 v[kAtOnce];
+    if (left >= 16) {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) v[i] = ld_behind_wait(reinterpret_cast<const uint4*>(from + min(r0 + i, count - 1) * a.from_ld[which]));
+    } else {  // nothing behind the row's values is read
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        alignas(16) uint16_t part[8] = {};
+        for (int c = 0; c < left / 2; ++c) part[c] = reinterpret_cast<const uint16_t*>(from + min(r0 + i, count - 1) * a.from_ld[which])[c];
+        v[i] = *reinterpret_cast<const uint4*>(part);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (r0 + i >= count) v[i] = make_uint4(0, 0, 0, 0);
+      if (r0 + i < padded) *reinterpret_cast<uint4*>(to + (r0 + i) * a.to_ld[which]) = v[i];
+    }
+  }
+}
+struct WeightCopies {
+  int64_t a_ld, dz_ld, a_bytes, bytes;  // values; bytes of a's copies, and of all
+};
+WeightCopies weight_copies(const MatmulWeight& p) {
+  WeightCopies c;
+  c.a_ld = (p.k + 7) / 8 * 8;
+  c.dz_ld = (p.n + 7) / 8 * 8;
+  c.a_bytes = (int64_t)p.groups * kPairK * c.a_ld * 2;
+  c.bytes = c.a_bytes + (int64_t)p.groups * kPairK * c.dz_ld * 2;
+  return c;
+}
+
 PreArgs pre_args(const MatmulPre& p) {
   PreArgs a{};
   a.dout = p.dout;
@@ -402,9 +492,12 @@ cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t s
   a.e.n = (int)p.k;
   a.e.type = p.type;
   cudaError_t err = maps_of_rows(&maps, p.dz, p.m, p.n, p.dz_ld);
-  if (err == cudaSuccess) err = map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kPairK);
+  a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
+  if (err == cudaSuccess) err = a.p_chunks == 2 ? map_chunks(&maps.p[0], p.b, a.groups, p.n, p.k) : map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kPairK);
   return err != cudaSuccess ? err : launch_pairs<kInput>(maps, a, device, stream);
 }
+
+int64_t matmul_weight_copies(const MatmulWeight& p) { return p.rows != nullptr ? weight_copies(p).bytes : 0; }
 
 cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t stream) {
   if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || p.dz_ld % 8) return cudaErrorInvalidValue;
@@ -422,12 +515,37 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
   a.e.type = p.type;
   PairMaps maps{};
   if (p.m > 0) {  // (without a row there is nothing to load: every matrix is cleared)
-    const int rows[kBoxes] = {64, 16, 8, 4, 2, 1};
-    for (int b = 0; b < kBoxes; ++b) {
-      cudaError_t err = map_2d(&maps.p[b], p.a, p.m, p.k, p.a_ld, rows[b]);
-      if (err == cudaSuccess) err = map_2d(&maps.q[b], p.dz, p.m, p.n, p.dz_ld, rows[b]);
-      if (err != cudaSuccess) return err;
+    int n_sm = 0;
+    cudaError_t err = multiprocessors(device, &n_sm);
+    const int steps = steps_per_tile(p.n, kWeightStep, kPairN, (p.k + kPairM - 1) / kPairM, n_sm, false);
+    a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
+    a.q_chunks = p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1;  // every tile has 256 result rows
+    auto map = [](CUtensorMap* m, int chunks, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+      return chunks == 2 ? map_chunks(m, base, rows, cols, ld, kPairK) : map_2d(m, base, rows, cols, ld, kPairK);
+    };
+    if (err == cudaSuccess) err = map(&maps.p[0], a.p_chunks, p.a, p.m, p.k, p.a_ld);
+    if (err == cudaSuccess) err = map(&maps.q[0], a.q_chunks, p.dz, p.m, p.n, p.dz_ld);
+    if (p.rows != nullptr) {
+      if (p.copies == nullptr) return cudaErrorInvalidValue;
+      a.copies = 1;
+      const WeightCopies c = weight_copies(p);
+      uint8_t* of_dz = static_cast<uint8_t*>(p.copies) + c.a_bytes;
+      if (err == cudaSuccess) err = map(&maps.p[1], a.p_chunks, p.copies, (int64_t)a.groups * kPairK, p.k, c.a_ld);
+      if (err == cudaSuccess) err = map(&maps.q[1], a.q_chunks, of_dz, (int64_t)a.groups * kPairK, p.n, c.dz_ld);
+      LastBlocks l{};
+      l.from[0] = p.a, l.from[1] = p.dz;
+      l.to[0] = p.copies, l.to[1] = of_dz;
+      l.from_ld[0] = p.a_ld * 2, l.from_ld[1] = p.dz_ld * 2;
+      l.to_ld[0] = c.a_ld * 2, l.to_ld[1] = c.dz_ld * 2;
+      l.words[0] = (int)(c.a_ld / 8), l.words[1] = (int)(c.dz_ld / 8);
+      l.bytes[0] = p.k * 2, l.bytes[1] = p.n * 2;
+      l.rows = p.rows;
+      l.groups = a.groups;
+      l.m = (int)p.m;
+      const int words = l.words[0] + l.words[1];
+      if (err == cudaSuccess) err = launch_after(last_blocks_kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
     }
+    if (err != cudaSuccess) return err;
   }
   return launch_pairs<kWeight>(maps, a, device, stream);
 }

@@ -16,9 +16,11 @@
 // MN-major operands are read as they lie in memory: nothing is transposed on the way.  P is on the tensor core's M side (256 a
 // pair of CTAs), Q on its N side, where a tile takes any multiple of 32 rows: the number of rows of a group is arbitrary.
 //
-// With groups the tiles go group by group.  A weight tile sums over its group's rows alone: its last block of 64 rows is fetched in
-// boxes of 16, 8, 4, 2 and 1 rows, and what is missing of the last 16 is fetched from behind the tensor's last row, where TMA
-// fills in zeros, so that nothing of the next group (an infinity times zero) comes in.
+// With groups the tiles go group by group.  A weight tile sums over its group's rows alone, and nothing of the next group (an infinity
+// times zero) may come in: a group's last block of 64 rows, where it is not whole, is copied beforehand, with zeros behind it up to the
+// 16 rows of a matrix instruction.  (Fetched in boxes of 16, 8, 4, 2 and 1 rows, the rest from behind the tensor's last row, where TMA
+// fills in zeros, such a block cost 1.5 to 3 us of a tile's 7: issuing a box takes the producer some 100 cycles whatever its size.  So a
+// box also holds both chunks of 64 columns that a CTA has, where it can.)
 #pragma once
 
 #include <cuda.h>
@@ -110,9 +112,11 @@ __device__ __forceinline__ void store4(void* p, Type type, int64_t i, int limit,
 // (__expf is off by 2 + 1.2 |x| units in the last place, the quotient by two: 2^-20 of the value where it matters, and the
 // result, of up to 24 bits, is mostly rounded to 8 or 11)
 __device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// (of a third of normcdff's instructions; off by 2^-24, not of the value, below zero)
+__device__ __forceinline__ float normal_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678f), 0.5f); }
 __device__ __forceinline__ float activated(float z, int activation) {
   if (activation == kSilu) return z * sigmoid_of(z);
-  if (activation == kGelu) return z * normcdff(z);
+  if (activation == kGelu) return z * normal_cdf(z);
   if (activation == kRelu) return z < 0.f ? 0.f : z;  // NaN stays
   return z;
 }
@@ -171,7 +175,7 @@ constexpr int kRowStep = 32;      // result rows of a tile come in these
 constexpr int kWeightStep = 128;  // kWeight: whole chunks of 64 for either CTA
 constexpr int kChunk = 64;        // values of an MN-major operand in one swizzled row
 constexpr uint32_t kChunkBytes = kChunk * kPairK * 2;
-constexpr int kBoxes = 6;         // K-major: 128, 64, 32, 16 result rows; kWeight: 64, 16, 8, 4, 2, 1 rows of the sum
+constexpr int kBoxes = 4;         // K-major Q: 128, 64, 32, 16 result rows; kWeight: 64 rows of the sum, of a group's copy
 constexpr uint32_t kStageP = kHalfM * kPairK * 2;
 constexpr uint32_t kPairRing = 192 * 1024;
 constexpr int kPairStages = 11;
@@ -188,7 +192,7 @@ constexpr int kPairThreads = 64 + 32 * kStoreWarps, kPairColumns = 512;
 constexpr int kSumBlocks = 8, kSumRows = 128;
 
 struct PairMaps {
-  CUtensorMap p[kBoxes], q[kBoxes];  // K-major P: the first only
+  CUtensorMap p[2], q[kBoxes];  // P: the first only, but for kWeight
 };
 struct PairArgs {
   const int* rows;  // [groups] or null
@@ -199,6 +203,8 @@ struct PairArgs {
   int k_blocks;     // blocks of r; kWeight: of the group's rows
   int tiles_p;      // ceil(features / 256)
   int tile_steps;   // result rows of a tile at most, in steps
+  int p_chunks, q_chunks;  // chunks of an MN-major operand that a box holds: 2 where columns come in whole chunks (q: and a CTA has two)
+  int copies;       // kWeight: the last blocks of groups have been copied
   int wide;         // four neighbouring values of everything in the epilogue start on a boundary of their size
   int plain;        // a result in 16 bits, no residual, nothing kept, rows of whole 16-byte words
   uint32_t idesc;
@@ -328,16 +334,19 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort, budget)) break;
           const uint32_t full = lead_full + 8 * s;
-          const int there = rows_of(kb), deep = (there + 15) / 16 * 16;
-          if (half == 0) mbar_expect_tx(bar_full + 8 * s, 2 * (uint32_t)(kHalfM + mine) * (uint32_t)deep * 2);
+          const int there = rows_of(kb);
+          if (half == 0) mbar_expect_tx(bar_full + 8 * s, 2 * (uint32_t)(kHalfM + mine) * kPairK * 2);
           uint32_t dst = smem_u32(smem) + s * stage_bytes;
           if constexpr (MODE == kForward) {
             tma_pair_load_3d(dst, &maps.p[0], full, kb * kPairK, feature, cur.group);
           } else if constexpr (MODE == kForwardGated) {
             tma_pair_load_5d(dst, &maps.p[0], full, kb * kPairK, half * (kHalfM / 32), cur.group * a.tiles_p + cur.p);
           } else if constexpr (MODE == kInput) {
-            for (int c = 0; c < kHalfM / kChunk; ++c)
-              tma_pair_load_3d(dst + c * kChunkBytes, &maps.p[0], full, feature + c * kChunk, kb * kPairK, cur.group);
+            if (a.p_chunks == 2)
+              tma_pair_load_4d(dst, &maps.p[0], full, kb * kPairK, feature / kChunk, cur.group);
+            else
+              for (int c = 0; c < kHalfM / kChunk; ++c)
+                tma_pair_load_3d(dst + c * kChunkBytes, &maps.p[0], full, feature + c * kChunk, kb * kPairK, cur.group);
           }
           if constexpr (MODE != kWeight) {
             dst += kStageP;
@@ -352,29 +361,16 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
               }
             }
           } else {
-            const int from = s_start[cur.group] + kb * kPairK;
-            auto chunk = [&](uint32_t to, const CUtensorMap* map, int x) {
-              if (there == kPairK) {
-                tma_pair_load_2d(to, &map[0], full, x, from);
-                return;
-              }
-              int at = 0;
-              auto box = [&](int b, int n, int y) {
-                tma_pair_load_2d(to + at * 128, &map[b], full, x, y);
-                at += n;
-              };
-              while (at + 16 <= there) box(1, 16, from + at);
-#pragma unroll
-              for (int b = 2; b < kBoxes; ++b)
-                if ((there & 15) & (32 >> b)) box(b, 32 >> b, from + at);
-              const int missing = deep - there;
-#pragma unroll
-              for (int b = kBoxes - 1; b >= 2; --b)  // the smallest first: every box starts on a multiple of its size
-                if (missing & (32 >> b)) box(b, 32 >> b, a.n_rows);
+            // a group's last block, where it is not whole, from its copy
+            const int from_copy = a.copies && there < kPairK;
+            const int from = from_copy ? cur.group * kPairK : s_start[cur.group] + kb * kPairK;
+            auto load = [&](uint32_t to, const CUtensorMap* map, int chunks, int x) {  // x: of the first column, a multiple of 64
+              if (chunks == 2) tma_pair_load_3d(to, map, full, 0, from, x / kChunk);
+              else tma_pair_load_2d(to, map, full, x, from);
             };
-            for (int c = 0; c < kHalfM / kChunk; ++c) chunk(dst + c * kChunkBytes, maps.p, feature + c * kChunk);
+            for (int c = 0; c < kHalfM / kChunk; c += a.p_chunks) load(dst + c * kChunkBytes, &maps.p[from_copy], a.p_chunks, feature + c * kChunk);
             dst += kStageP;
-            for (int c = 0; c < mine / kChunk; ++c) chunk(dst + c * kChunkBytes, maps.q, row + c * kChunk);
+            for (int c = 0; c < mine / kChunk; c += a.q_chunks) load(dst + c * kChunkBytes, &maps.q[from_copy], a.q_chunks, row + c * kChunk);
           }
           if (++s == stages) s = 0, ph ^= 1;
         }

@@ -49,10 +49,12 @@ struct MatmulWeight {
   const void* a;   // [m, k], row stride a_ld
   const int* rows;
   void* db;
+  void* copies;    // with rows: matmul_weight_copies() bytes on a 16-byte boundary, of this call alone
   int64_t m, n, k, dz_ld, a_ld;
   int groups;
   Type type;
 };
+int64_t matmul_weight_copies(const MatmulWeight& p);
 cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t stream);
 
 // dz = dout * act'(pre), and the bias's gradient, the sum of dz over the rows of a group

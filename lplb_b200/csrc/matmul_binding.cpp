@@ -197,6 +197,11 @@ variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b,
       p.a_ld = ld_of(from);
       p.groups = (int)s.groups;
       p.type = type;
+      Tensor copies;  // of this call alone: calls on two streams, or two captured graphs, share nothing
+      if (rows) {
+        copies = make({lplb::ops::matmul_weight_copies(p)}, torch::kUInt8, a);
+        p.copies = copies.data_ptr();
+      }
       OPS_CUDA(lplb::ops::launch_matmul_weight(p, device, stream));
     }
   }

@@ -129,6 +129,13 @@ __device__ __forceinline__ void tma_pair_load_3d(uint32_t dst, const void* tmap,
       ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// the first of four coordinates is 0
+__device__ __forceinline__ void tma_pair_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(tmap), "r"(bar), "r"(0), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 
 // Tile load of one CTA: the barrier is its own.  The innermost coordinate obeys the rule above.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int x, int y) {

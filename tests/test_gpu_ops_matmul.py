@@ -63,6 +63,13 @@ def test_groups_of_odd_sizes(n, k, activation):
     check(333, n, k, [100, 0, 7, 129, 64, 21], activation, bias=BF16, residual=True, out_dtype=F32)
 
 
+@pytest.mark.parametrize("n,k", [(256, 64), (512, 128), (768, 320), (264, 192), (512, 200), (1024, 72)])
+def test_weights_in_whole_chunks_and_others(n, k):
+    """Operands that lie across the sum are loaded by chunks of 64 columns, two at a time where all are whole."""
+    check(400, n, k, [15, 129, 0, 64, 1, 191])
+    check(333, n, k)
+
+
 def test_many_groups():
     g = torch.Generator().manual_seed(0)
     groups = torch.randint(0, 4, (1024,), generator=g).tolist()
