@@ -145,7 +145,13 @@ __global__ void __launch_bounds__(256) bias_parts_kernel(const float* parts, voi
   const int64_t group = i / n, column = i - group * n;
   const float* from = parts + group * splits * n + column;
   float all = 0.f;
-  for (int s = 0; s < splits; ++s) all += from[s * n];
+  for (int s0 = 0; s0 < splits; s0 += 16) {  // 16 loads under way
+    float v[16];
+#pragma unroll
+    for (int s = 0; s < 16; ++s) v[s] = from[min(s0 + s, splits - 1) * n];
+#pragma unroll
+    for (int s = 0; s < 16; ++s) all += s0 + s < splits ? v[s] : 0.f;
+  }
   store_float(dbias, type, i, all);
 }
 
@@ -195,21 +201,29 @@ cudaError_t maps_of_rows(PairMaps* maps, const void* base, uint64_t rows, uint64
 }
 
 // ---- CTA pairs --------------------------------------------------------------------------------------------
-// One group: result rows in tiles of equal height, so high that the fewest rounds over the CTA pairs come out (a tile costs its
-// steps and about one more).  Several groups: their rows are only known on the device.
-int steps_per_tile(int64_t rows, int step, int most_rows, int64_t tiles_p, int n_sm, bool grouped) {
-  const int most = most_rows / step;
-  if (grouped) return most;
+// What a product takes, in cycles beside the launch: an SM is fed by some 64 bytes a cycle from the L2 and computes a block of 64 of 256
+// features x n rows (a pair) in 2 n cycles; then the last tile's way out.
+int64_t block_cycles(int64_t n) { return n < 256 ? 256 + n : 2 * n; }
+// One group: result rows in tiles of equal height, so high that this is least over the rounds of CTA pairs.  Several groups: their
+// rows are only known on the device.
+struct PairCost {
+  int64_t cycles;
+  int steps;  // of a tile
+};
+PairCost pair_cost(int64_t rows, int step, int most_rows, int64_t tiles_p, int64_t k_blocks, int n_sm) {
   const int64_t steps = (rows + step - 1) / step;
-  int64_t least = INT64_MAX;
-  int best = most;
-  for (int s = most; s >= 1; --s) {
-    if (s * step < 64 && steps > 1) break;
-    const int64_t tiles = (steps + s - 1) / s, high = (steps + tiles - 1) / tiles;
-    const int64_t cost = (tiles * tiles_p + n_sm / 2 - 1) / (n_sm / 2) * (high * step + 32);
-    if (cost < least) least = cost, best = (int)high;
+  PairCost best{INT64_MAX, most_rows / step};
+  for (int s = most_rows / step; s >= 1; --s) {
+    const int64_t tiles = (steps + s - 1) / s, high = (steps + tiles - 1) / tiles, n = high * step;
+    const int64_t rounds = (tiles * tiles_p + n_sm / 2 - 1) / (n_sm / 2), cycles = rounds * (k_blocks * block_cycles(n) + 100) + 8 * n;
+    if (cycles < best.cycles) best = {cycles, (int)high};
   }
   return best;
+}
+
+// Of a weight's gradient: the groups' rows are what is summed, here as if they were equal.
+int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm) {
+  return pair_cost(result_rows, kWeightStep, kPairN, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
 }
 
 template <Mode MODE, bool IN_32 = false>
@@ -231,7 +245,10 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
   const int out_cols = MODE == kForwardGated ? a.features / 2 : a.features;
   a.plain = a.e.type != Type::kF32 && a.e.residual == nullptr && a.e.pre == nullptr && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
-  a.tile_steps = steps_per_tile(MODE == kWeight ? a.result_rows : a.n_rows, PairTile<MODE>::kStep, IN_32 ? kSumRows : kPairN, a.tiles_p, n_sm, a.rows != nullptr && MODE != kWeight);
+  const int most_rows = IN_32 ? kSumRows : kPairN;
+  a.tile_steps = most_rows / PairTile<MODE>::kStep;
+  if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm);
+  else if (a.rows == nullptr) a.tile_steps = pair_cost(a.n_rows, PairTile<MODE>::kStep, most_rows, a.tiles_p, a.k_blocks, n_sm).steps;
   return launch_after(kernel, dim3(n_sm & ~1), dim3(kPairThreads), kPairSmem, stream, maps, a);
 }
 
@@ -277,9 +294,10 @@ cudaError_t launch_forward(const Matmul& p, int device, cudaStream_t stream) {
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------
-// Half of an SM's shared memory: the next kernel's CTAs can set themselves up beside these.
-constexpr uint32_t kFewRing = 96 * 1024;
-constexpr int kFewSmem = 256 * kFewSmemPerColumn > 1024 + kFewMostRows * kFewTileRows * 4 + 1024 ? 256 * kFewSmemPerColumn : 2048 + kFewMostRows * kFewTileRows * 4;
+// us, cold weights, rings of 96 KB, for which the next kernel's CTAs could be set up beside these, and of 192: 64 x 4096 x 7168 16.3,
+// 13.8; 128 x 4096 x 7168 19.8, 16.0; 16 x 4096 x 4096 9.8, 9.3.
+constexpr uint32_t kFewRing = 192 * 1024;
+constexpr int kFewSmem = 226 * 1024;  // at most
 
 template <typename Kernel>
 cudaLaunchConfig_t few_config(cudaLaunchAttribute (&attrs)[2], int ctas, int split, uint32_t smem, cudaStream_t stream, Kernel) {
@@ -310,19 +328,57 @@ cudaError_t resident_clusters(int device, int split, Kernel kernel, int* cluster
   if (err == cudaSuccess) known[device][split].store(*clusters, std::memory_order_relaxed);
   return err;
 }
+// Accumulators, and stages of the ring, of CTAs with `cols` rows of a and `blocks` k blocks.
+int few_chains(int cols, int blocks, bool in_32) {
+  int chains = 1;
+  while (in_32 && chains * kSumBlocks < blocks && (chains + 1) * cols <= kFewMostRows) ++chains;
+  return chains;
+}
+int few_stages(int cols, int blocks) {
+  const int stages = (int)(kFewRing / (kFewWeightStage + cols * kFewKBytes));
+  return stages < kFewStageMax ? stages < blocks ? stages : blocks : kFewStageMax < blocks ? kFewStageMax : blocks;
+}
+
+// How many CTAs share a tile's k blocks, and how many rows of a a CTA has: so that the cycles of block_cycles' kind are least.
+struct FewCost {
+  int64_t cycles;
+  int split, cols;
+};
+cudaError_t prepare_few(int device) {
+  static std::atomic<bool> prepared[kMaxDevices];
+  if (prepared[device].load(std::memory_order_relaxed)) return cudaSuccess;
+  cudaError_t err = cudaFuncSetAttribute(few_product_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(few_product_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  if (err == cudaSuccess) prepared[device].store(true, std::memory_order_relaxed);
+  return err;
+}
+cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
+  cudaError_t err = prepare_few(device);
+  if (err != cudaSuccess) return err;
+  const int most_rows = p.out_type == Type::kF32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
+  const int64_t tiles = (p.n + kFewTileRows - 1) / kFewTileRows, k_blocks = (p.k + kPairK - 1) / kPairK;
+  *best = {INT64_MAX, 0, 0};
+  for (int s = 1; s <= kFewMostSplit && s <= k_blocks; ++s) {
+    int fit = 0;
+    if ((err = resident_clusters(device, s, few_product_kernel<false>, &fit)) != cudaSuccess) return err;
+    if (fit < 1) continue;
+    const int64_t least_groups = (p.m + most_rows - 1) / most_rows;
+    for (int64_t g = least_groups; g <= (p.m + 15) / 16 && g < least_groups + 16; ++g) {
+      const int64_t cols = ((p.m + g - 1) / g + 15) / 16 * 16, groups = (p.m + cols - 1) / cols;
+      const int64_t rounds = (tiles * groups + fit - 1) / fit, blocks = (k_blocks + s - 1) / s;
+      const int64_t cycles = rounds * (blocks * (256 + 2 * cols) + 10 * cols + (s > 1 ? 1500 + 2 * cols : 0));
+      if (cycles < best->cycles) *best = {cycles, s, (int)cols};
+    }
+  }
+  return best->cols > 0 ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
 
 template <bool GATED>
-cudaError_t launch_few(const Matmul& p, int device, cudaStream_t stream) {
+cudaError_t launch_few(const Matmul& p, const FewCost& how, int device, cudaStream_t stream) {
   auto kernel = few_product_kernel<GATED>;
-  static std::atomic<bool> prepared[kMaxDevices];
-  cudaError_t err = cudaSuccess;
-  if (!prepared[device].load(std::memory_order_relaxed)) {
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
-    if (err != cudaSuccess) return err;
-    prepared[device].store(true, std::memory_order_relaxed);
-  }
   FewProductArgs a{};
-  if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
+  cudaError_t err = ops_error_word(device, &a.status);
+  if (err != cudaSuccess) return err;
   a.budget_ns = wait_budget_ns();
   a.m = (int)p.m;
   a.k_blocks = (int)((p.k + kPairK - 1) / kPairK);
@@ -330,32 +386,10 @@ cudaError_t launch_few(const Matmul& p, int device, cudaStream_t stream) {
   a.idesc = sm100::umma_idesc_16(p.type == Type::kBf16, false, false);
   a.e = epilogue_of(p);
   a.tiles = (int)((p.n + kFewTileRows - 1) / kFewTileRows);
-  // How many CTAs share a tile's k blocks, and in how many parts the rows of a go: the least time by this measure, in units
-  // of a k block of 128 weight rows: 6 for a round's beginning, the blocks with their rows, the rows' way out, 4 for a join.
-  const bool in_32 = p.out_type == Type::kF32;
-  const int most_rows = in_32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
-  const int least_groups = (a.m + most_rows - 1) / most_rows;
-  int split = 1, groups = 1;
-  float least = 1e30f;
-  for (int s = 1; s <= kFewMostSplit && s <= a.k_blocks; ++s) {
-    int fit = 0;
-    if ((err = resident_clusters(device, s, kernel, &fit)) != cudaSuccess) return err;
-    if (fit < 1) continue;
-    for (int g = least_groups; g <= (a.m + 15) / 16 && g < least_groups + 16; ++g) {
-      const int cols = ((a.m + g - 1) / g + 15) / 16 * 16;
-      const int rounds = (a.tiles * ((a.m + cols - 1) / cols) + fit - 1) / fit, blocks = (a.k_blocks + s - 1) / s;
-      const float cost = rounds * (blocks * (1.f + cols / 256.f) + 6 + cols / 16.f) + (s > 1 ? 4 : 0);
-      if (cost < least) least = cost, split = s, groups = (a.m + cols - 1) / cols, a.cols = cols;
-    }
-  }
-  if (a.cols == 0) return cudaErrorInvalidConfiguration;
-  const uint32_t stage = kFewWeightStage + a.cols * kFewKBytes;
-  a.stages = (int)(kFewRing / stage);
-  if (a.stages > kFewStageMax) a.stages = kFewStageMax;
-  const int most = (a.k_blocks + split - 1) / split;
-  if (a.stages > most) a.stages = most;
-  a.chains = 1;
-  while (in_32 && a.chains * kSumBlocks < most && (a.chains + 1) * a.cols <= kFewMostRows) ++a.chains;
+  a.cols = how.cols;
+  const int split = how.split, groups = (a.m + a.cols - 1) / a.cols, blocks = (a.k_blocks + split - 1) / split;
+  a.stages = few_stages(a.cols, blocks);
+  a.chains = few_chains(a.cols, blocks, p.out_type == Type::kF32);
   CUtensorMap map_b, map_a;
   if ((err = map_2d(&map_b, p.b, p.n, p.k, p.k, GATED ? kFewTileRows / 2 : kFewTileRows)) != cudaSuccess) return err;
   if ((err = map_2d(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
@@ -462,15 +496,16 @@ PreArgs pre_args(const MatmulPre& p) {
 cudaError_t launch_matmul(const Matmul& p, int device, cudaStream_t stream) {
   if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || (p.activation == kSwiglu && p.n % (2 * kGateBlock))) return cudaErrorInvalidValue;
   if (p.m == 0) return cudaSuccess;
-  if (p.rows == nullptr) {
-    bool few = p.m <= kFewMostRows;
-    if (!few) {  // small products, whose tiles of 128 x 256 find an SM each and whose k is short
-      int n_sm = 0;
-      if (cudaError_t err = multiprocessors(device, &n_sm)) return err;
-      const int64_t tiles = (p.n + kFewTileRows - 1) / kFewTileRows * ((p.m + kFewMostRows - 1) / kFewMostRows);
-      few = tiles <= n_sm && tiles * ((p.k + kPairK - 1) / kPairK) <= 12 * n_sm;
-    }
-    if (few) return p.activation == kSwiglu ? launch_few<true>(p, device, stream) : launch_few<false>(p, device, stream);
+  // One matrix and not too many rows: by the kernel that takes the fewer cycles.  us, few_product_kernel and the pairs, cold weights: 64 x
+  // 4096 x 7168 13.8, 20.5; 128 x 2048 x 2048 7.3, 8.9; 400 x 1000 x 4096 10.0, 13.0; 200 x 7168 x 2048 14.0, 11.2; 600 x 4096 x 1024 13.6, 8.9.
+  if (p.rows == nullptr && p.m <= 2048) {
+    int n_sm = 0;
+    FewCost few{};
+    cudaError_t err = multiprocessors(device, &n_sm);
+    if (err == cudaSuccess) err = few_cost(p, device, &few);
+    if (err != cudaSuccess) return err;
+    const PairCost pairs = pair_cost(p.m, kRowStep, p.out_type == Type::kF32 ? kSumRows : kPairN, (p.n + kPairM - 1) / kPairM, (p.k + kPairK - 1) / kPairK, n_sm);
+    if (few.cycles <= pairs.cycles) return p.activation == kSwiglu ? launch_few<true>(p, few, device, stream) : launch_few<false>(p, few, device, stream);
   }
   return launch_forward(p, device, stream);
 }
@@ -517,7 +552,7 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
   if (p.m > 0) {  // (without a row there is nothing to load: every matrix is cleared)
     int n_sm = 0;
     cudaError_t err = multiprocessors(device, &n_sm);
-    const int steps = steps_per_tile(p.n, kWeightStep, kPairN, (p.k + kPairM - 1) / kPairM, n_sm, false);
+    const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm);
     a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
     a.q_chunks = p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1;  // every tile has 256 result rows
     auto map = [](CUtensorMap* m, int chunks, const void* base, int64_t rows, int64_t cols, int64_t ld) {
