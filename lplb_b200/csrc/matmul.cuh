@@ -115,8 +115,9 @@ __device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.
 // (of a third of normcdff's instructions; off by 2^-24, not of the value, below zero)
 __device__ __forceinline__ float normal_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678f), 0.5f); }
 __device__ __forceinline__ float activated(float z, int activation) {
-  if (activation == kSilu) return z * sigmoid_of(z);
-  if (activation == kGelu) return z * normal_cdf(z);
+  // (rounded by itself, not fused with what is added to it: every path of a product has the same bits)
+  if (activation == kSilu) return __fmul_rn(z, sigmoid_of(z));
+  if (activation == kGelu) return __fmul_rn(z, normal_cdf(z));
   if (activation == kRelu) return z < 0.f ? 0.f : z;  // NaN stays
   return z;
 }
@@ -151,7 +152,7 @@ struct Columns {
     }
     if (GATED) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[j] = z[j] * sigmoid_of(z[j]) * up[j];
+      for (int j = 0; j < 4; ++j) z[j] = __fmul_rn(__fmul_rn(z[j], sigmoid_of(z[j])), up[j]);
     } else if (e.activation != kNoActivation) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) z[j] = activated(z[j], e.activation);
@@ -206,7 +207,7 @@ struct PairArgs {
   int p_chunks, q_chunks;  // chunks of an MN-major operand that a box holds: 2 where columns come in whole chunks (q: and a CTA has two)
   int copies;       // kWeight: the last blocks of groups have been copied
   int wide;         // four neighbouring values of everything in the epilogue start on a boundary of their size
-  int plain;        // a result in 16 bits, no residual, nothing kept, rows of whole 16-byte words
+  int plain;        // a result in 16 bits, nothing kept, rows (the residual's too) of whole 16-byte words on boundaries
   uint32_t idesc;
   int* status;
   unsigned long long budget_ns;
@@ -472,7 +473,8 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
       return true;
     };
 
-    // A result in 16 bits that nothing is added to: bias and activation on the matrix fragments, turned round by stmatrix, stored by 16 bytes.
+    // A result in 16 bits: bias, activation and residual on the matrix fragments, turned round by stmatrix, stored by 16 bytes.  The residual
+    // comes the same way back.
     auto plain = [&](auto is_bf16) {
       constexpr bool kBf = decltype(is_bf16)::value;
       auto pack = [](float lo, float hi) {
@@ -483,6 +485,10 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           const __half2 v = __floats2half2_rn(lo, hi);
           return *reinterpret_cast<const uint32_t*>(&v);
         }
+      };
+      auto unpack = [](uint32_t w) {
+        if constexpr (kBf) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&w));
       };
       const uint32_t mine = smem_u32(stage);
       constexpr int kRowBytes = kGated ? 32 : 64, kChunks = kRowBytes / 16;  // of a result row, this warp's
@@ -503,6 +509,17 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
         const int column = (kGated ? cur.p * kHalfM + half * (kHalfM / 2) + quarter * 16 : cur.p * kPairM + half * kHalfM + quarter * 32) + lane % kChunks * 8;
         uint16_t* out = static_cast<uint16_t*>(e.out) + column;
         const bool inside = column < out_cols;
+        uint4 carried[kChunks];  // the residual of the step that is next
+        auto fetch = [&](int c0) {
+          if (MODE > kForwardGated || e.residual == nullptr) return;
+          const uint16_t* from = static_cast<const uint16_t*>(e.residual) + (inside ? column : 0);
+#pragma unroll
+          for (int q = 0; q < kChunks; ++q) {
+            const int r = min(c0 + lane / kChunks + q * (32 / kChunks), n - 1);  // (what is not there is not stored)
+            carried[q] = *reinterpret_cast<const uint4*>(from + (row0 + r) * e.residual_ld);
+          }
+        };
+        fetch(32 * which);
         if (!await()) break;
         for (int c0 = 32 * which; c0 < n; c0 += 64) {
           // fragments: lanes l/4 and l/4 + 8 of a 16-lane half, result rows 8j + 2(l%4) and the next
@@ -518,7 +535,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
             for (int j = 0; j < 16; ++j) v[h][j] = __uint_as_float(raw[h][j]) + (MODE <= kForwardGated ? bias[2 * h + (j >> 1 & 1)] : 0.f);
           if constexpr (kGated) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[0][j] = v[0][j] * sigmoid_of(v[0][j]) * v[1][j];
+            for (int j = 0; j < 16; ++j) v[0][j] = __fmul_rn(__fmul_rn(v[0][j], sigmoid_of(v[0][j])), v[1][j]);
           } else if (MODE == kForward && e.activation != kNoActivation) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -526,6 +543,25 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
               for (int j = 0; j < 16; ++j) v[h][j] = activated(v[h][j], e.activation);
           }
           __syncwarp();  // the rows before have been read
+          if (MODE <= kForwardGated && e.residual != nullptr) {
+#pragma unroll
+            for (int q = 0; q < kChunks; ++q) *reinterpret_cast<uint4*>(stage + chunk_at(lane / kChunks + q * (32 / kChunks), lane % kChunks)) = carried[q];
+            fetch(c0 + 64);
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < kChunks; ++q) {
+              uint32_t two[4];
+              ldmatrix_trans(mine + chunk_at(lane, q), two);
+              float(&f)[16] = v[q >> 1];
+              const int h = 2 * (q & 1);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 more = unpack(two[j]);
+                f[4 * j + h] += more.x, f[4 * j + h + 1] += more.y;
+              }
+            }
+            __syncwarp();
+          }
 #pragma unroll
           for (int q = 0; q < kChunks; ++q) {
             const float(&f)[16] = v[q >> 1];
@@ -567,13 +603,23 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) turned[j * 32 + lane] = v[j];
         };
-        auto finish16 = [&](int c0, auto&& turn) {  // result rows c0 .. c0 + 15 of the tile
-          float r[kPer][4];
+        float next_r[kPer][4];  // the residual of the 16 rows that are finished next, under way while these are
+        auto fetch = [&](int c0) {
 #pragma unroll
           for (int q = 0; q < kPer; ++q) {
             const int at = c0 + lane / kLanes + q * (32 / kLanes);
-            if (at < n) mine.load_residual(e, row0 + at, r[q]);
+            if (at < n) mine.load_residual(e, row0 + at, next_r[q]);
           }
+        };
+        auto after = [&](int c0) { return c0 & 16 ? c0 + 48 : c0 + 16; };  // the warp's 16 rows behind these
+        fetch(32 * which);
+        auto finish16 = [&](int c0, auto&& turn) {  // result rows c0 .. c0 + 15 of the tile
+          float r[kPer][4];
+#pragma unroll
+          for (int q = 0; q < kPer; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[q][j] = next_r[q][j];
+          fetch(after(c0));
           __syncwarp();  // the rows before have been read
           turn();
           __syncwarp();

@@ -360,6 +360,13 @@ __device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32
                ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
+// The way back: lane l's address is row l%8 of matrix l/8.
+__device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared::cta.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
 // Barrier of the four epilogue warps; epilogue_all also says whether every thread passed true.
 __device__ __forceinline__ void epilogue_sync() {
   __syncwarp();

@@ -70,6 +70,17 @@ def test_weights_in_whole_chunks_and_others(n, k):
     check(333, n, k)
 
 
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("groups", [None, [600, 1, 0, 99]])
+def test_a_residual_in_16_bits(activation, groups):
+    """Through shared memory on its way to the matrix fragments, or not, where its rows are off a boundary: the same bits."""
+    args, dout, got = check(707, 512, 136, groups, activation, F32, True)
+    wide = torch.zeros(708, args["residual"].shape[1] + 4, dtype=BF16, device="cuda")
+    off = wide[1:, 4:]
+    off.copy_(args["residual"])
+    assert torch.equal(ops.matmul(**{**args, "residual": off}), got["out"])
+
+
 def test_many_groups():
     g = torch.Generator().manual_seed(0)
     groups = torch.randint(0, 4, (1024,), generator=g).tolist()
