@@ -63,7 +63,6 @@ static __global__ void __launch_bounds__(32) take_rows_bulk_kernel(const TakeRow
   const uint32_t ring = smem_u32(smem), zero = ring + a.slots * a.slot, bars = ring + kBulkRing;
   __shared__ int abort_flag;
   const int lane = threadIdx.x;
-  allow_successor();
   if (lane == 0) {
     abort_flag = 0;
     for (int s = 0; s < a.slots; ++s) mbar_init(bars + 8 * s, 1);
@@ -73,6 +72,7 @@ static __global__ void __launch_bounds__(32) take_rows_bulk_kernel(const TakeRow
   fence_proxy_async_shared();
   __syncwarp();
   wait_predecessors();
+  allow_successor();
   const int64_t items = t.tokens * a.pieces, n_rows = t.tokens * t.topk;
   const int64_t mine = (items - blockIdx.x + gridDim.x - 1) / gridDim.x;  // of this CTA: blockIdx.x, and gridDim.x apart
   const uint8_t* x = static_cast<const uint8_t*>(t.x);
@@ -159,7 +159,6 @@ __global__ void __launch_bounds__(kJoinThreads, 1) combine_rows_bulk_kernel(cons
   __shared__ uint32_t s_spare[kBulkSlots];  // BACKWARD: bit k: the row of this number is nobody's
   __shared__ float s_dot[BACKWARD ? kBulkTurns : 1][kJoinWarps][BACKWARD ? KEEP : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  allow_successor();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < a.slots; ++s) {
@@ -171,6 +170,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) combine_rows_bulk_kernel(cons
   }
   __syncthreads();
   wait_predecessors();
+  allow_successor();
   volatile int* abort = &abort_flag;
   const int64_t n_rows = c.tokens * c.topk, row_bytes = (int64_t)c.cols * sizeof(T);
   // The CTA's units are tokens, all pieces of each, or (few tokens) single pieces.

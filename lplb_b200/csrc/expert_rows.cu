@@ -26,10 +26,10 @@ namespace {
 constexpr uint32_t kAll = 0xffffffffu;
 
 // ---- the order ------------------------------------------------------------------------------------
-// One cluster of up to 8 CTAs sorts all pairs.  Every warp counts a stretch of consecutive pairs per expert, in shared memory of
+// One cluster of up to 16 CTAs sorts all pairs.  Every warp counts a stretch of consecutive pairs per expert, in shared memory of
 // its own; the counts of the warps and CTAs before it, and of the experts before, are where its pairs begin; then it goes through
 // its stretch again, 32 pairs at a time, and lanes with the same expert take consecutive places in the order of lanes.
-constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderMaxCluster = 8;
+constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderMaxCluster = 16;
 constexpr int kBatch = 8;  // loads of 32 pairs under way
 
 size_t order_smem(int warps, int experts) { return (size_t)(warps + 2) * experts * sizeof(uint32_t); }
@@ -51,10 +51,10 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const Order o, int
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int rank = (int)cluster_cta_rank(), ctas = (int)cluster_size();
   const I* idx = static_cast<const I*>(o.idx);
-  allow_successor();
   for (int i = tid; i < warps * o.experts; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
   wait_predecessors();
+  allow_successor();
   // this warp's stretch, a multiple of 32 pairs
   int64_t from = o.pairs, to = o.pairs;
   if (warp < warps) {
@@ -62,14 +62,16 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const Order o, int
     to = min(o.pairs, from + stretch);
   }
   uint32_t* mine = hist + warp * o.experts;
-  auto each = [&](auto&& use) {  // 32 pairs at a time: the pair and its expert, -1 where there is none
+  int e[kBatch];
+  auto each = [&](auto&& use, bool kept) {  // 32 pairs at a time: the pair and its expert, -1 where there is none
     for (int64_t at = from; at < to; at += 32 * kBatch) {
-      int e[kBatch];
+      if (!kept) {  // (a stretch of one batch stays in registers for the second time)
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int64_t p = at + 32 * i + lane;
-        const long long v = p < to ? (long long)idx[p] : -1;
-        e[i] = v >= 0 && v < o.experts ? (int)v : -1;
+        for (int i = 0; i < kBatch; ++i) {
+          const int64_t p = at + 32 * i + lane;
+          const long long v = p < to ? (long long)idx[p] : -1;
+          e[i] = v >= 0 && v < o.experts ? (int)v : -1;
+        }
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const Order o, int
   };
   each([&](int64_t, int e) {
     if (e >= 0) atomicAdd(&mine[e], 1u);
-  });
+  }, false);
   __syncthreads();
   for (int e = tid; e < o.experts; e += kOrderThreads) {
     uint32_t run = 0;
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const Order o, int
       o.place[p] = e >= 0 ? (int)at : -1;
       if (e >= 0) o.source[at] = (int)p;
     }
-  });
+  }, to - from <= 32 * kBatch);
   for (int64_t r = used + (int64_t)rank * kOrderThreads + tid; r < o.pairs; r += (int64_t)ctas * kOrderThreads) o.source[r] = -1;
   if (ctas > 1) cluster_sync();  // nobody leaves while another reads its totals
 }
@@ -173,8 +175,8 @@ constexpr int kTakeVectors = 4;  // of a row, per thread and round
 template <int N>
 __global__ void __launch_bounds__(256, 4) take_rows_kernel(const TakeRows a) {
   using V = typename Bytes<N>::type;
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (token >= a.tokens) return;
   const int64_t vectors = a.row_bytes / N, n_rows = a.tokens * a.topk;
@@ -236,8 +238,8 @@ template <typename T, int N>
 __global__ void __launch_bounds__(256, 3) combine_rows_kernel(const CombineRows a) {
   constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
   constexpr int kRows = 4;                        // of a token, under way
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (token >= a.tokens) return;
   const int64_t n_rows = a.tokens * a.topk;
@@ -295,8 +297,8 @@ __global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const Com
   constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
   constexpr int kRows = 4;                        // of a token, at a time
   __shared__ float part[kRows][8];
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   if (token >= a.tokens) return;  // a CTA of several warps per token has one token
@@ -427,7 +429,8 @@ cudaError_t launch_take_bulk(const TakeRows& t, int n_sms, cudaStream_t stream) 
   const cudaError_t err = prepare_bulk<take_rows_bulk_kernel>(a);
   if (err != cudaSuccess) return err;
   const int64_t items = t.tokens * a.pieces;
-  return launch_after(take_rows_bulk_kernel, dim3((unsigned)(items < n_sms ? items : n_sms)), dim3(32), kBulkSmem, stream, t, a);
+  auto kernel = take_rows_bulk_kernel;
+  return launch_after(kernel, dim3((unsigned)(items < n_sms ? items : n_sms)), dim3(32), kBulkSmem, stream, t, a);
 }
 
 template <typename T, bool BACKWARD, int KEEP>
@@ -447,7 +450,8 @@ cudaError_t launch_join(const CombineRows& c, int n_sms, cudaStream_t stream) {
 template <int N>
 cudaError_t launch_take(const TakeRows& t, int n_sms, cudaStream_t stream) {
   const Shape s = shape_of(t.tokens, t.row_bytes / N, kTakeVectors, n_sms, false);
-  return launch_after(take_rows_kernel<N>, s.grid, s.block, 0, stream, t);
+  auto kernel = take_rows_kernel<N>;
+  return launch_after(kernel, s.grid, s.block, 0, stream, t);
 }
 
 // Bytes of a token and its rows from which on bulk copies pay.
@@ -460,10 +464,12 @@ cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaS
   const int vectors = c.cols / N;
   if (backward) {
     const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, true);
-    return launch_after(combine_rows_backward_kernel<T, N>, s.grid, s.block, 0, stream, c);
+    auto kernel = combine_rows_backward_kernel<T, N>;
+    return launch_after(kernel, s.grid, s.block, 0, stream, c);
   }
   const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, false);
-  return launch_after(combine_rows_kernel<T, N>, s.grid, s.block, 0, stream, c);
+  auto kernel = combine_rows_kernel<T, N>;
+  return launch_after(kernel, s.grid, s.block, 0, stream, c);
 }
 template <typename T>
 cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaStream_t stream) {
@@ -503,6 +509,8 @@ cudaError_t launch_order(const Order& o, int device, cudaStream_t stream) {
     const int most = (int)order_smem(kOrderWarps, kOrderMaxExperts);
     cudaError_t err = cudaFuncSetAttribute(order_kernel<int64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (err == cudaSuccess) err = cudaFuncSetAttribute(order_kernel<int32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(order_kernel<int64_t>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(order_kernel<int32_t>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (err != cudaSuccess) return err;
     prepared[device].store(true, std::memory_order_relaxed);
   }

@@ -88,40 +88,39 @@ __device__ __forceinline__ float softmax_sum(const float (&x)[V], float most) {
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(const Gate g) {
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * kGateWarps + (threadIdx.x >> 5);
   if (token >= g.tokens) return;
   float x[V];
   load_logits<T, V>(g, token, lane, x);
-  uint32_t key[V], best = 0;
+  uint32_t key[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    key[j] = key_of(x[j]);
-    best = max(best, key[j]);
-  }
+  for (int j = 0; j < V; ++j) key[j] = key_of(x[j]);
+  uint32_t best = 0;
+  int best_at = 0;  // this lane's largest, the lowest of equal ones
+  auto look = [&] {
+    best = key[0], best_at = 0;
+#pragma unroll
+    for (int j = 1; j < V; ++j)
+      if (key[j] > best) best = key[j], best_at = j;
+  };
+  look();
   uint32_t largest = 0, mine = 0;
   int expert = -1;
   for (int r = 0; r < g.topk; ++r) {
     const uint32_t top = __reduce_max_sync(kAll, best);
     if (top == 0) break;
     if (r == 0) largest = top;
-    int candidate = INT32_MAX;
-    if (best == top) {
-#pragma unroll
-      for (int j = V - 1; j >= 0; --j)
-        if (key[j] == top) candidate = j * 32 + lane;
-    }
+    const int candidate = best == top ? best_at * 32 + lane : INT32_MAX;
     const int winner = __reduce_min_sync(kAll, candidate);
     if (lane == r) mine = top, expert = winner;
     if (candidate == winner) {  // one lane's: the numbers differ
-      best = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j * 32 + lane == winner) key[j] = 0;
-        best = max(best, key[j]);
-      }
+      for (int j = 0; j < V; ++j)
+        if (j == best_at) key[j] = 0;
+      look();
     }
   }
   const float most = value_of(largest);
@@ -135,8 +134,8 @@ __global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(const Gate g) {
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kGateWarps * 32) gate_backward_kernel(const Gate g) {
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * kGateWarps + (threadIdx.x >> 5);
   if (token >= g.tokens) return;

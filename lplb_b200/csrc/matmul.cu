@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(256) pre_gradient_kernel(const PreArgs a) {
   constexpr int kNext = VEC ? 128 : 32;                 // from the thread's first vector to its second
   __shared__ float s_sum[kPreRows][kPreColumns];
   __shared__ long long s_before[8];
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = blockIdx.y, group = blockIdx.z;
   int from = 0, rows = a.m;
@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(256) pre_gradient_kernel(const PreArgs a) {
 
 // dbias[g, c] = sum of its parts, in their order
 __global__ void __launch_bounds__(256) bias_parts_kernel(const float* parts, void* dbias, Type type, int64_t n, int splits, int64_t total) {
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= total) return;
   const int64_t group = i / n, column = i - group * n;
@@ -416,8 +416,8 @@ struct LastBlocks {
 };
 __global__ void __launch_bounds__(256) last_blocks_kernel(const LastBlocks a) {
   __shared__ long long s_before[8];
-  allow_successor();
   wait_predecessors();
+  allow_successor();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.y;
   long long before = 0;
   for (int e = threadIdx.x; e < group; e += 256) before += max(a.rows[e], 0);
@@ -578,7 +578,8 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
       l.groups = a.groups;
       l.m = (int)p.m;
       const int words = l.words[0] + l.words[1];
-      if (err == cudaSuccess) err = launch_after(last_blocks_kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
+      auto kernel = last_blocks_kernel;
+      if (err == cudaSuccess) err = launch_after(kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
     }
     if (err != cudaSuccess) return err;
   }
@@ -615,7 +616,8 @@ cudaError_t launch_matmul_pre(const MatmulPre& p, int device, cudaStream_t strea
                       : vec ? pre_gradient_kernel<true, false> : pre_gradient_kernel<false, false>;
   if ((err = launch_after(kernel, grid, dim3(256), 0, stream, a)) != cudaSuccess || floats == 0) return err;
   const int64_t total = (int64_t)a.groups * a.n;
-  return launch_after(bias_parts_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, a.parts, a.dbias, a.bias_type, (int64_t)a.n, a.splits,
+  auto sum = bias_parts_kernel;
+  return launch_after(sum, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, a.parts, a.dbias, a.bias_type, (int64_t)a.n, a.splits,
                       total);
 }
 

@@ -261,7 +261,6 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = (int)cluster_cta_rank();
   const int n_pairs = (int)gridDim.x / 2, pair = (int)blockIdx.x / 2;
-  allow_successor();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kPairStages; ++s) {
@@ -278,6 +277,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), kPairColumns);
   wait_predecessors();
+  allow_successor();
   if (warp == 2) {  // groups one after the other, none beyond the last row
     long long before = 0;
     for (int e0 = 0; e0 < a.groups; e0 += 32) {
@@ -460,7 +460,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     auto release = [&]() {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote_fenced(lead_tempty + 8 * (part & 1));
+      if (lane == 0) mbar_arrive_remote_read(lead_tempty + 8 * (part & 1));
       ++part;
     };
     const uint32_t tmem_mine = tmem_base + ((uint32_t)(quarter * 32) << 16);

@@ -62,7 +62,6 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   const int tile = (int)blockIdx.x / split % a.tiles, m0 = (int)blockIdx.x / split / a.tiles * a.cols, m_here = min(a.cols, a.m - m0);
   const int kb0 = (int)((int64_t)a.k_blocks * rank / split), kb1 = (int)((int64_t)a.k_blocks * (rank + 1) / split);
   const int per_chain = (kb1 - kb0 + a.chains - 1) / a.chains;  // k blocks
-  allow_successor();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kFewStageMax; ++s) {
@@ -81,6 +80,7 @@ few_product_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_const
   const uint32_t tmem = tmem_slot;
   volatile int* abort = &abort_flag;
   wait_predecessors();
+  allow_successor();
 
   if (warp == 0) {
     if (elect_one()) {
