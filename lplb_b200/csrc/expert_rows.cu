@@ -7,15 +7,16 @@
 //
 // take_rows and combine_rows without weights are each other's gradient.  All three go by token, not by sorted row: the token's side is
 // read or written once, and its rows, which lie far apart but are each of one piece, all at once.  Bound by DRAM; nothing is summed
-// by atomics, the same inputs give the same bits.
+// by atomics, the same inputs give the same bits.  What decided their speed: few enough registers for three or four CTAs per SM, and no branch
+// between a thread's loads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <atomic>
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.cuh"
-#include "expert_bulk.cuh"
 #include "experts_api.h"
 #include "tcgen05.cuh"
 
@@ -171,6 +172,7 @@ template <> struct Bytes<2> { using type = uint16_t; };
 template <> struct Bytes<1> { using type = uint8_t; };
 
 // ---- rows to their experts ------------------------------------------------------------------------
+// us, 8192 tokens x 8 rows of 7168 in bf16: 171 (6.2 TB/s).  By bulk copies through shared memory, a row loaded once and stored eight times, 186.
 constexpr int kTakeVectors = 4;  // of a row, per thread and round
 template <int N>
 __global__ void __launch_bounds__(256, 4) take_rows_kernel(const TakeRows a) {
@@ -234,10 +236,23 @@ __device__ __forceinline__ void narrow(float& p, float v) { p = v; }
 __device__ __forceinline__ void narrow(__nv_bfloat16& p, float v) { p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(__half& p, float v) { p = __float2half_rn(v); }
 
+// ROWS of a token's rows at vectors v0, v0 + step, ... of their columns.  Nothing is asked between the loads (each would wait for the one
+// before): what is not there is read from the first row, or the row's first vector, and left out by the caller.
+template <int ROWS, int VECTORS, typename T, int N>
+__device__ __forceinline__ void load_rows(const T* rows, int64_t ld, const int64_t (&at)[ROWS], int v0, int step, int vectors, Few<T, N> (&y)[ROWS][VECTORS]) {
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const T* from = rows + (at[j] < 0 ? 0 : at[j]) * ld;
+#pragma unroll
+    for (int v = 0; v < VECTORS; ++v) y[j][v] = load_few<T, N>(from + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
+  }
+}
+
+// us, 8192 tokens x 8, 2, 1 rows of 7168 in bf16: 172, 78, 51 (6.1 TB/s at 8); with four rows at a time whatever is left 178, 82, 57.  Bulk copies into
+// shared memory, 190 KB per SM under way, took 195, 104 and 84.
 template <typename T, int N>
-__global__ void __launch_bounds__(256, 3) combine_rows_kernel(const CombineRows a) {
+__global__ void __launch_bounds__(256, 4) combine_rows_kernel(const CombineRows a) {
   constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
-  constexpr int kRows = 4;                        // of a token, under way
   wait_predecessors();
   allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -253,35 +268,33 @@ __global__ void __launch_bounds__(256, 3) combine_rows_kernel(const CombineRows 
     for (int v = 0; v < kVectors; ++v)
 #pragma unroll
       for (int n = 0; n < N; ++n) sum[v][n] = 0.f;
-    for (int k0 = 0; k0 < a.topk; k0 += kRows) {
-      // Nothing is asked between the loads (each would wait for the one before): what is not there is read from the first row, or the
-      // row's first vector, and left out below.
+    auto add = [&](int k0, auto count) {
+      constexpr int kRows = decltype(count)::value;
       Few<T, N> y[kRows][kVectors];
       float w[kRows];
-      bool there[kRows];
       int64_t at[kRows];
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        const int k = min(k0 + j, a.topk - 1);
-        at[j] = place[k];
-        w[j] = a.weights != nullptr ? a.weights[token * a.topk + k] : 1.f;
+        at[j] = place[k0 + j];
+        w[j] = a.weights != nullptr ? a.weights[token * a.topk + k0 + j] : 1.f;
       }
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        there[j] = k0 + j < a.topk && at[j] >= 0 && at[j] < n_rows;
-        const T* from = rows + (there[j] ? at[j] : 0) * a.ld;
-#pragma unroll
-        for (int v = 0; v < kVectors; ++v) y[j][v] = load_few<T, N>(from + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
-      }
+      for (int j = 0; j < kRows; ++j)
+        if (at[j] >= n_rows) at[j] = -1;
+      load_rows<kRows, kVectors>(rows, a.ld, at, v0, step, vectors, y);
 #pragma unroll
       for (int j = 0; j < kRows; ++j) {
-        if (!there[j]) continue;
+        if (at[j] < 0) continue;
 #pragma unroll
         for (int v = 0; v < kVectors; ++v)
 #pragma unroll
           for (int n = 0; n < N; ++n) sum[v][n] = fmaf(w[j], widen(y[j][v].v[n]), sum[v][n]);
       }
-    }
+    };
+    int k = 0;
+    for (; k + 4 <= a.topk; k += 4) add(k, std::integral_constant<int, 4>{});
+    if (a.topk & 2) add(k, std::integral_constant<int, 2>{}), k += 2;
+    if (a.topk & 1) add(k, std::integral_constant<int, 1>{});
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
       Few<T, N> r;
@@ -292,11 +305,11 @@ __global__ void __launch_bounds__(256, 3) combine_rows_kernel(const CombineRows 
   }
 }
 
+// us, as above: 360, 104, 80 (5.5 TB/s at 8); with four rows at a time 353, 137, 116; by bulk copies 346, 180 and 153.
 template <typename T, int N>
-__global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const CombineRows a) {
+__global__ void __launch_bounds__(256, 4) combine_rows_backward_kernel(const CombineRows a) {
   constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
-  constexpr int kRows = 4;                        // of a token, at a time
-  __shared__ float part[kRows][8];
+  __shared__ float part[2][8];
   wait_predecessors();
   allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -307,54 +320,45 @@ __global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const Com
   const T* rows = static_cast<const T*>(a.rows);
   T* drows = static_cast<T*>(a.drows);
   const T* dout = static_cast<const T*>(a.dout) + token * a.dout_ld;
-  for (int k0 = 0; k0 < a.topk; k0 += kRows) {
-    int place[kRows];
+  auto choices = [&](int k0, auto count) {
+    constexpr int kRows = decltype(count)::value;
+    int64_t at[kRows];
     float w[kRows], dot[kRows];
     bool spare[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      const int k = min(k0 + j, a.topk - 1);
-      place[j] = a.place[token * a.topk + k];
-      w[j] = a.weights[token * a.topk + k];
-      spare[j] = drows != nullptr && a.source[token * a.topk + k] < 0;
+      at[j] = a.place[token * a.topk + k0 + j];
+      w[j] = a.weights[token * a.topk + k0 + j];
+      spare[j] = drows != nullptr && a.source[token * a.topk + k0 + j] < 0;
       dot[j] = 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      if (k0 + j >= a.topk) place[j] = -1, spare[j] = false;
-      if (place[j] >= n_rows) place[j] = -1;
-    }
+    for (int j = 0; j < kRows; ++j)
+      if (at[j] >= n_rows) at[j] = -1;
     for (int v0 = threadIdx.x; v0 < vectors; v0 += step * kVectors) {
-      Few<T, N> d[kVectors], y[kRows][kVectors];  // (nothing is asked between the loads, as above)
-#pragma unroll
-      for (int v = 0; v < kVectors; ++v) d[v] = load_few<T, N>(dout + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
-      if (a.dweights != nullptr) {
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-          const T* from = rows + (int64_t)max(place[j], 0) * a.ld;
-#pragma unroll
-          for (int v = 0; v < kVectors; ++v) y[j][v] = load_few<T, N>(from + (int64_t)(v0 + v * step < vectors ? v0 + v * step : 0) * N);
-        }
-      }
+      Few<T, N> d[1][kVectors], y[kRows][kVectors];
+      const int64_t first[1] = {0};
+      load_rows<1, kVectors>(dout, 0, first, v0, step, vectors, d);
+      if (a.dweights != nullptr) load_rows<kRows, kVectors>(rows, a.ld, at, v0, step, vectors, y);
 #pragma unroll
       for (int v = 0; v < kVectors; ++v) {
         if (v0 + v * step >= vectors) continue;
         const int64_t column = (int64_t)(v0 + v * step) * N;
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
-          if (place[j] >= 0) {
+          if (at[j] >= 0) {
             if (drows != nullptr) {
               Few<T, N> r;
 #pragma unroll
-              for (int n = 0; n < N; ++n) narrow(r.v[n], w[j] * widen(d[v].v[n]));
-              store_few(drows + (int64_t)place[j] * a.cols + column, r);
+              for (int n = 0; n < N; ++n) narrow(r.v[n], w[j] * widen(d[0][v].v[n]));
+              store_few(drows + at[j] * a.cols + column, r);
             }
             if (a.dweights != nullptr) {
 #pragma unroll
-              for (int n = 0; n < N; ++n) dot[j] = fmaf(widen(d[v].v[n]), widen(y[j][v].v[n]), dot[j]);
+              for (int n = 0; n < N; ++n) dot[j] = fmaf(widen(d[0][v].v[n]), widen(y[j][v].v[n]), dot[j]);
             }
           }
-          if (spare[j]) {
+          if (spare[j]) {  // a row that nobody has
             Few<T, N> zero;
 #pragma unroll
             for (int n = 0; n < N; ++n) narrow(zero.v[n], 0.f);
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const Com
         }
       }
     }
-    if (a.dweights == nullptr) continue;
+    if (a.dweights == nullptr) return;
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
 #pragma unroll
@@ -372,20 +376,23 @@ __global__ void __launch_bounds__(256, 3) combine_rows_backward_kernel(const Com
     if (warps == 1) {
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (lane == j && k0 + j < a.topk) a.dweights[token * a.topk + k0 + j] = dot[j];
-      continue;
+        if (lane == j) a.dweights[token * a.topk + k0 + j] = dot[j];
+      return;
     }
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
       if (lane == j) part[j][warp] = dot[j];
     __syncthreads();
-    if (warp == 0 && lane < kRows && k0 + lane < a.topk) {
+    if (warp == 0 && lane < kRows) {
       float sum = 0.f;
       for (int i = 0; i < warps; ++i) sum += part[lane][i];
       a.dweights[token * a.topk + k0 + lane] = sum;
     }
     __syncthreads();
-  }
+  };
+  int k = 0;
+  for (; k + 2 <= a.topk; k += 2) choices(k, std::integral_constant<int, 2>{});
+  if (a.topk & 1) choices(k, std::integral_constant<int, 1>{});
 }
 
 // The widest vector, in bytes of 16 or less, that divides all of these.
@@ -396,66 +403,12 @@ int widest(std::initializer_list<uint64_t> of) {
 }
 uint64_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
-// The shape of a pass by bulk copies: pieces of at most `most` bytes, `rows` of them to a slot, and so many that the SMs have
-// about two each.
-BulkArgs bulk_args(int64_t tokens, int64_t row_bytes, uint32_t most, uint32_t rows, int spare, int n_sms) {
-  BulkArgs a{};
-  int64_t pieces = (row_bytes + most - 1) / most;
-  while (tokens * pieces < 2 * n_sms && row_bytes / pieces > 1024) ++pieces;
-  a.piece = (uint32_t)(((row_bytes + pieces - 1) / pieces + 127) / 128 * 128);
-  a.pieces = (row_bytes + a.piece - 1) / a.piece;
-  a.slot = a.piece * rows;
-  a.slots = (int)(kBulkRing / a.slot) - spare;
-  if (a.slots > kBulkSlots) a.slots = kBulkSlots;
-  a.budget_ns = wait_budget_ns();
-  return a;
-}
-template <auto KERNEL>
-cudaError_t prepare_bulk(BulkArgs& a) {
-  int device = 0;
-  cudaError_t err = cudaGetDevice(&device);
-  if (err != cudaSuccess) return err;
-  if (device >= kMaxDevices) return cudaErrorInvalidDevice;
-  static std::atomic<bool> prepared[kMaxDevices];
-  if (!prepared[device].load(std::memory_order_relaxed)) {
-    if ((err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBulkSmem)) != cudaSuccess) return err;
-    prepared[device].store(true, std::memory_order_relaxed);
-  }
-  return ops_error_word(device, &a.status);
-}
-
-cudaError_t launch_take_bulk(const TakeRows& t, int n_sms, cudaStream_t stream) {
-  BulkArgs a = bulk_args(t.tokens, t.row_bytes, kTakeMostPiece, 1, 1, n_sms);
-  const cudaError_t err = prepare_bulk<take_rows_bulk_kernel>(a);
-  if (err != cudaSuccess) return err;
-  const int64_t items = t.tokens * a.pieces;
-  auto kernel = take_rows_bulk_kernel;
-  return launch_after(kernel, dim3((unsigned)(items < n_sms ? items : n_sms)), dim3(32), kBulkSmem, stream, t, a);
-}
-
-template <typename T, bool BACKWARD, int KEEP>
-cudaError_t launch_join(const CombineRows& c, int n_sms, cudaStream_t stream) {
-  const uint32_t rows = c.topk + (BACKWARD ? 1 : 0);
-  uint32_t most = kBulkRing / (4 * rows) / 128 * 128;  // four slots at least
-  if (most > kJoinMostPiece) most = kJoinMostPiece;
-  BulkArgs a = bulk_args(BACKWARD ? INT32_MAX : c.tokens, (int64_t)c.cols * sizeof(T), most, rows, 0, n_sms);
-  constexpr auto kernel = combine_rows_bulk_kernel<T, BACKWARD, KEEP>;
-  const cudaError_t err = prepare_bulk<kernel>(a);
-  if (err != cudaSuccess) return err;
-  a.whole = BACKWARD || c.tokens >= 4 * n_sms;
-  const int64_t units = a.whole ? c.tokens : c.tokens * a.pieces;
-  return launch_after(kernel, dim3((unsigned)(units < n_sms ? units : n_sms)), dim3(kJoinThreads), kBulkSmem, stream, c, a);
-}
-
 template <int N>
 cudaError_t launch_take(const TakeRows& t, int n_sms, cudaStream_t stream) {
   const Shape s = shape_of(t.tokens, t.row_bytes / N, kTakeVectors, n_sms, false);
   auto kernel = take_rows_kernel<N>;
   return launch_after(kernel, s.grid, s.block, 0, stream, t);
 }
-
-// Bytes of a token and its rows from which on bulk copies pay.
-constexpr uint64_t kBulkLeast = 16 * 1024;
 
 bool refused(const CombineRows& c) { return c.tokens < 0 || c.tokens > INT32_MAX || c.cols < 1 || c.topk < 1; }
 
@@ -476,14 +429,7 @@ cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaS
   const uint64_t size = sizeof(T);
   int wide = backward ? widest({address(c.rows), c.ld * size, c.cols * size, address(c.dout), c.dout_ld * size, address(c.drows)})
                       : widest({address(c.rows), c.ld * size, c.cols * size, address(c.out)});
-  if (wide == 16) {
-    if (c.cols * size * (c.topk + 1) >= kBulkLeast) {
-      if (!backward && c.topk <= kJoinMostTopk) return launch_join<T, false, 1>(c, n_sms, stream);
-      if (backward && c.topk <= 8) return launch_join<T, true, 8>(c, n_sms, stream);
-      if (backward && c.topk <= 16) return launch_join<T, true, 16>(c, n_sms, stream);
-    }
-    return launch_combine<T, 16 / sizeof(T)>(c, n_sms, backward, stream);
-  }
+  if (wide == 16) return launch_combine<T, 16 / sizeof(T)>(c, n_sms, backward, stream);
   if (wide >= 4) return launch_combine<T, 4 / sizeof(T)>(c, n_sms, backward, stream);
   if constexpr (sizeof(T) == 2) return launch_combine<T, 1>(c, n_sms, backward, stream);
   return cudaErrorMisalignedAddress;
@@ -496,6 +442,29 @@ cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaS
     case Type::kBf16: return launch_combine<__nv_bfloat16>(c, n_sms, backward, stream);
     default: return launch_combine<__half>(c, n_sms, backward, stream);
   }
+}
+
+// Whether a cluster of kOrderMaxCluster CTAs, which is more than every device promises, can run here.
+cudaError_t largest_cluster_fits(int device, int* fits) {
+  static std::atomic<int> known[kMaxDevices];  // 1: no, 2: yes
+  if (known[device].load(std::memory_order_relaxed) == 0) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kOrderMaxCluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(kOrderMaxCluster);
+    config.blockDim = dim3(kOrderThreads);
+    config.dynamicSmemBytes = order_smem(kOrderWarps, kOrderMaxExperts);
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    int clusters = 0;
+    const cudaError_t err = cudaOccupancyMaxActiveClusters(&clusters, order_kernel<int64_t>, &config);
+    if (err != cudaSuccess) return err;
+    known[device].store(clusters > 0 ? 2 : 1, std::memory_order_relaxed);
+  }
+  *fits = known[device].load(std::memory_order_relaxed) == 2;
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -514,10 +483,16 @@ cudaError_t launch_order(const Order& o, int device, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     prepared[device].store(true, std::memory_order_relaxed);
   }
-  // a CTA up to 64 chunks of 32 pairs, then as many as give each that many
+  // a CTA up to 64 chunks of 32 pairs, then as many as give each that many, where the device has room for such a cluster
   const int64_t chunks = (o.pairs + 31) / 32;
   int ctas = 1;
   while (ctas < kOrderMaxCluster && ctas * 64 < chunks) ctas *= 2;
+  if (ctas > 8) {
+    int fit = 0;
+    const cudaError_t err = largest_cluster_fits(device, &fit);
+    if (err != cudaSuccess) return err;
+    if (!fit) ctas = 8;
+  }
   int warps = (int)((chunks + ctas - 1) / ctas);
   if (warps > kOrderWarps) warps = kOrderWarps;
   if (warps < 1) warps = 1;
@@ -542,9 +517,7 @@ cudaError_t launch_take_rows(const TakeRows& t, int n_sms, cudaStream_t stream) 
   if (t.tokens < 0 || t.tokens > INT32_MAX || t.row_bytes < 1 || t.topk < 1) return cudaErrorInvalidValue;
   if (t.tokens == 0) return cudaSuccess;
   switch (widest({address(t.x), (uint64_t)t.ld_bytes, (uint64_t)t.row_bytes, address(t.rows)})) {
-    case 16:
-      if ((uint64_t)t.row_bytes * (t.topk + 1) >= kBulkLeast) return launch_take_bulk(t, n_sms, stream);
-      return launch_take<16>(t, n_sms, stream);
+    case 16: return launch_take<16>(t, n_sms, stream);
     case 8: return launch_take<8>(t, n_sms, stream);
     case 4: return launch_take<4>(t, n_sms, stream);
     case 2: return launch_take<2>(t, n_sms, stream);
