@@ -339,7 +339,8 @@ int few_stages(int cols, int blocks) {
   return stages < kFewStageMax ? stages < blocks ? stages : blocks : kFewStageMax < blocks ? kFewStageMax : blocks;
 }
 
-// How many CTAs share a tile's k blocks, and how many rows of a a CTA has: so that the cycles of block_cycles' kind are least.
+// How many CTAs share a tile's k blocks, and how many rows of a a CTA has: so that the cycles of block_cycles' kind are least.  cols is 0
+// where nothing fits.
 struct FewCost {
   int64_t cycles;
   int split, cols;
@@ -355,7 +356,8 @@ cudaError_t prepare_few(int device) {
 cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
   cudaError_t err = prepare_few(device);
   if (err != cudaSuccess) return err;
-  const int most_rows = p.out_type == Type::kF32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
+  const bool in_32 = p.out_type == Type::kF32;
+  const int most_rows = in_32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
   const int64_t tiles = (p.n + kFewTileRows - 1) / kFewTileRows, k_blocks = (p.k + kPairK - 1) / kPairK;
   *best = {INT64_MAX, 0, 0};
   for (int s = 1; s <= kFewMostSplit && s <= k_blocks; ++s) {
@@ -366,11 +368,12 @@ cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
     for (int64_t g = least_groups; g <= (p.m + 15) / 16 && g < least_groups + 16; ++g) {
       const int64_t cols = ((p.m + g - 1) / g + 15) / 16 * 16, groups = (p.m + cols - 1) / cols;
       const int64_t rounds = (tiles * groups + fit - 1) / fit, blocks = (k_blocks + s - 1) / s;
+      if (in_32 && few_chains((int)cols, (int)blocks, true) * kSumBlocks < blocks) continue;  // its parts would be longer than the pairs'
       const int64_t cycles = rounds * (blocks * (256 + 2 * cols) + 10 * cols + (s > 1 ? 1500 + 2 * cols : 0));
       if (cycles < best->cycles) *best = {cycles, s, (int)cols};
     }
   }
-  return best->cols > 0 ? cudaSuccess : cudaErrorInvalidConfiguration;
+  return cudaSuccess;
 }
 
 template <bool GATED>
@@ -505,7 +508,7 @@ cudaError_t launch_matmul(const Matmul& p, int device, cudaStream_t stream) {
     if (err == cudaSuccess) err = few_cost(p, device, &few);
     if (err != cudaSuccess) return err;
     const PairCost pairs = pair_cost(p.m, kRowStep, p.out_type == Type::kF32 ? kSumRows : kPairN, (p.n + kPairM - 1) / kPairM, (p.k + kPairK - 1) / kPairK, n_sm);
-    if (few.cycles <= pairs.cycles) return p.activation == kSwiglu ? launch_few<true>(p, few, device, stream) : launch_few<false>(p, few, device, stream);
+    if (few.cols > 0 && few.cycles <= pairs.cycles) return p.activation == kSwiglu ? launch_few<true>(p, few, device, stream) : launch_few<false>(p, few, device, stream);
   }
   return launch_forward(p, device, stream);
 }

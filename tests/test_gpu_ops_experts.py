@@ -325,3 +325,53 @@ def test_an_order_that_points_elsewhere_is_not_followed():
 @pytest.mark.parametrize("name", list(second_gradients("cpu")))
 def test_no_second_gradient(name):
     no_second_gradient(name, "cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.float64, torch.bool, torch.complex64, torch.int16])
+def test_rows_of_any_type(dtype):
+    order = ops.expert_order(ids_of(40, 3, 5, 4).cuda(), 5)
+    x = torch.randint(0, 2, (40, 9), generator=torch.Generator().manual_seed(0)).to(dtype)
+    got = ops.take_rows(x.cuda(), order)
+    assert got.dtype == dtype and torch.equal(got.cpu(), oracle.take(x, order.place.cpu()))
+
+
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_no_tokens(device):
+    idx = torch.empty(0, 3, dtype=torch.int64, device=device)
+    order = ops.expert_order(idx, 4)
+    assert order.counts.tolist() == [0] * 4 and order.source.shape == (0,)
+    x = torch.empty(0, 8, device=device).requires_grad_()
+    w = torch.empty(0, 3, device=device).requires_grad_()
+    out = ops.combine_rows(ops.take_rows(x, order), order, w)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    assert out.shape == dx.shape == (0, 8) and dw.shape == (0, 3)
+    logits = torch.empty(0, 5, device=device).requires_grad_()
+    weights, chosen = ops.gate_topk(logits, 2)
+    assert chosen.shape == (0, 2) and torch.autograd.grad(weights.sum(), logits)[0].shape == (0, 5)
+
+
+def test_many_choices_per_token():
+    idx = ids_of(6, 1024, 40, 2).cuda()
+    order = ops.expert_order(idx, 40)
+    for a, b in zip(order, ops.reference.expert_order_reference(idx, 40)):
+        assert torch.equal(a, b)
+    x = torch.randn(6, 24, device="cuda").requires_grad_()
+    rows = ops.take_rows(x, order)
+    assert torch.equal(rows, ops.reference.take_rows_reference(x, order.place, order.source))
+    w = torch.rand(6, 1024, device="cuda").requires_grad_()
+    d = torch.randn(6, 24, device="cuda")
+    dx, dw = torch.autograd.grad(ops.combine_rows(rows, order, w), (x, w), d)
+    want = (w.detach().double() * (order.place >= 0)).sum(1, keepdim=True) * d.double()
+    assert ((dx.double() - want).abs() <= 1026 * 2**-23 * want.abs()).all()
+    want = torch.where(order.place >= 0, (d.double() * x.detach().double()).sum(1, keepdim=True), 0.0)
+    size = (d.double() * x.detach().double()).abs().sum(1, keepdim=True)
+    assert ((dw.double() - want).abs() <= 32 * 2**-24 * size).all()
+
+
+def test_a_gate_without_a_gradient_of_its_weights():
+    """A loss that hangs on the choice's weights of some tokens only, and one that hangs on none."""
+    x = torch.randn(8, 16, device="cuda").requires_grad_()
+    weights, idx = ops.gate_topk(x, 3)
+    (dx,) = torch.autograd.grad(weights[2:4].sum(), x)
+    assert not dx[:2].any() and not dx[4:].any() and dx[2:4].any()
+    assert not idx.requires_grad
