@@ -236,6 +236,10 @@ __device__ __forceinline__ void narrow(float& p, float v) { p = v; }
 __device__ __forceinline__ void narrow(__nv_bfloat16& p, float v) { p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void narrow(__half& p, float v) { p = __float2half_rn(v); }
 
+// Vectors of a row per thread and round: 16 bytes, of rows off 4 bytes 8 (8192 x 8 rows of 2051 in bf16 back 102 us, with 16 bytes 124).
+template <typename T, int N>
+constexpr int kVectorsOf = N * sizeof(T) == 2 ? 4 : 16 / (N * sizeof(T));
+
 // ROWS of a token's rows at vectors v0, v0 + step, ... of their columns.  Nothing is asked between the loads (each would wait for the one
 // before): what is not there is read from the first row, or the row's first vector, and left out by the caller.
 template <int ROWS, int VECTORS, typename T, int N>
@@ -252,7 +256,7 @@ __device__ __forceinline__ void load_rows(const T* rows, int64_t ld, const int64
 // shared memory, 190 KB per SM under way, took 195, 104 and 84.
 template <typename T, int N>
 __global__ void __launch_bounds__(256, 4) combine_rows_kernel(const CombineRows a) {
-  constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
+  constexpr int kVectors = kVectorsOf<T, N>;
   wait_predecessors();
   allow_successor();
   const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(256, 4) combine_rows_kernel(const CombineRows 
 // us, as above: 360, 104, 80 (5.5 TB/s at 8); with four rows at a time 353, 137, 116; by bulk copies 346, 180 and 153.
 template <typename T, int N>
 __global__ void __launch_bounds__(256, 4) combine_rows_backward_kernel(const CombineRows a) {
-  constexpr int kVectors = 16 / (N * sizeof(T));  // of a row, per thread and round: 16 bytes
+  constexpr int kVectors = kVectorsOf<T, N>;
   __shared__ float part[2][8];
   wait_predecessors();
   allow_successor();
@@ -416,11 +420,11 @@ template <typename T, int N>
 cudaError_t launch_combine(const CombineRows& c, int n_sms, bool backward, cudaStream_t stream) {
   const int vectors = c.cols / N;
   if (backward) {
-    const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, true);
+    const Shape s = shape_of(c.tokens, vectors, kVectorsOf<T, N>, n_sms, true);
     auto kernel = combine_rows_backward_kernel<T, N>;
     return launch_after(kernel, s.grid, s.block, 0, stream, c);
   }
-  const Shape s = shape_of(c.tokens, vectors, 16 / (N * sizeof(T)), n_sms, false);
+  const Shape s = shape_of(c.tokens, vectors, kVectorsOf<T, N>, n_sms, false);
   auto kernel = combine_rows_kernel<T, N>;
   return launch_after(kernel, s.grid, s.block, 0, stream, c);
 }
