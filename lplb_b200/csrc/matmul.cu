@@ -358,19 +358,20 @@ cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
   if (err != cudaSuccess) return err;
   const bool in_32 = p.out_type == Type::kF32;
   const int most_rows = in_32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
-  const int64_t tiles = (p.n + kFewTileRows - 1) / kFewTileRows, k_blocks = (p.k + kPairK - 1) / kPairK;
+  // (32 bits and up to eight parts of the rows: the search is one of the call's five microseconds at most)
+  const int m = (int)p.m, tiles = (int)((p.n + kFewTileRows - 1) / kFewTileRows), k_blocks = (int)((p.k + kPairK - 1) / kPairK);
   *best = {INT64_MAX, 0, 0};
   for (int s = 1; s <= kFewMostSplit && s <= k_blocks; ++s) {
     int fit = 0;
     if ((err = resident_clusters(device, s, few_product_kernel<false>, &fit)) != cudaSuccess) return err;
     if (fit < 1) continue;
-    const int64_t least_groups = (p.m + most_rows - 1) / most_rows;
-    for (int64_t g = least_groups; g <= (p.m + 15) / 16 && g < least_groups + 16; ++g) {
-      const int64_t cols = ((p.m + g - 1) / g + 15) / 16 * 16, groups = (p.m + cols - 1) / cols;
-      const int64_t rounds = (tiles * groups + fit - 1) / fit, blocks = (k_blocks + s - 1) / s;
-      if (in_32 && few_chains((int)cols, (int)blocks, true) * kSumBlocks < blocks) continue;  // its parts would be longer than the pairs'
+    const int blocks = (k_blocks + s - 1) / s, least_groups = (m + most_rows - 1) / most_rows;
+    for (int g = least_groups; g <= (m + 15) / 16 && g < least_groups + 8; ++g) {
+      const int cols = ((m + g - 1) / g + 15) / 16 * 16, groups = (m + cols - 1) / cols;
+      if (in_32 && few_chains(cols, blocks, true) * kSumBlocks < blocks) continue;  // its parts would be longer than the pairs'
+      const int64_t rounds = ((int64_t)tiles * groups + fit - 1) / fit;
       const int64_t cycles = rounds * (blocks * (256 + 2 * cols) + 10 * cols + (s > 1 ? 1500 + 2 * cols : 0));
-      if (cycles < best->cycles) *best = {cycles, s, (int)cols};
+      if (cycles < best->cycles) *best = {cycles, s, cols};
     }
   }
   return cudaSuccess;

@@ -73,13 +73,15 @@ def matmul(
     kept, in 32 bits, and their gradients are rounded to ``a``'s type before they are multiplied; all sums are in 32 bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
     tensors on plain statements; calls and backward passes can be captured in a CUDA graph, and the same inputs give the same
     bits.  Wrong arguments raise ``ValueError``; :func:`~lplb_b200.ops.check` tells of waits that ran out."""
-    who = "matmul:"
-    _need(activation in MATMUL_ACTIVATIONS, f"{who} activation must be one of {MATMUL_ACTIVATIONS}, not {activation!r}")
-    out_dtype = a.dtype if out_dtype is None else out_dtype
-    _need(out_dtype in (a.dtype, torch.float32), f"{who} out_dtype must be a's type or float32, not {out_dtype}")
+    if activation not in MATMUL_ACTIVATIONS:  # (messages are put together where they are needed: the call is a few microseconds)
+        raise ValueError(f"lplb_b200.ops.matmul: activation must be one of {MATMUL_ACTIVATIONS}, not {activation!r}")
+    if out_dtype is None:
+        out_dtype = a.dtype
+    elif out_dtype is not torch.float32 and out_dtype is not a.dtype:
+        raise ValueError(f"lplb_b200.ops.matmul: out_dtype must be a's type or float32, not {out_dtype}")
     if a.is_cuda:
-        return _native().matmul(a, b, bias, MATMUL_ACTIVATIONS.index(activation), residual, rows, out_dtype == torch.float32)
-    _check(a, b, bias, activation, residual, rows, out_dtype, who)
+        return _native().matmul(a, b, bias, MATMUL_ACTIVATIONS.index(activation), residual, rows, out_dtype is torch.float32)
+    _check(a, b, bias, activation, residual, rows, out_dtype, "matmul:")
     if _wants_grad(a, b, bias, residual):
         return _Matmul.apply(a, b, bias, residual, rows, activation, out_dtype)
     return reference.matmul_reference(a, b, bias, activation, residual, rows)[0].to(out_dtype)

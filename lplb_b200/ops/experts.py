@@ -87,11 +87,11 @@ def gate_topk(
     A logit of -infinity is an expert that cannot be chosen: where fewer than ``topk`` are left, ``idx`` is -1, which the planner and
     :func:`expert_order` take for no choice, and the weight is 0.  A NaN counts as larger than any number and makes the weights that
     depend on it NaN.  Up to 1024 experts and 32 choices.  Differentiable with respect to ``logits``."""
-    who = "gate_topk:"
-    _need(score in ("softmax", "sigmoid"), f"{who} score must be 'softmax' or 'sigmoid', not {score!r}")
-    topk, renormalize, scale = int(topk), bool(renormalize), float(scale)
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"lplb_b200.ops.gate_topk: score must be 'softmax' or 'sigmoid', not {score!r}")
     if logits.is_cuda:
-        return _native().gate_topk(logits, topk, score == "sigmoid", renormalize, scale)
+        return _native().gate_topk(logits, int(topk), score == "sigmoid", bool(renormalize), float(scale))
+    who, topk, renormalize, scale = "gate_topk:", int(topk), bool(renormalize), float(scale)
     _check_type(logits, f"{who} logits")
     _need(logits.dim() == 2, f"{who} logits must be [tokens, experts]")
     _need(1 <= logits.shape[1] <= GATE_MAX_EXPERTS, f"{who} 1 to {GATE_MAX_EXPERTS} experts")
