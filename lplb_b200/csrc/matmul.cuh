@@ -114,12 +114,20 @@ __device__ __forceinline__ void store4(void* p, Type type, int64_t i, int limit,
 __device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 // (of a third of normcdff's instructions; off by 2^-24, not of the value, below zero)
 __device__ __forceinline__ float normal_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678f), 0.5f); }
-__device__ __forceinline__ float activated(float z, int activation) {
-  // (rounded by itself, not fused with what is added to it: every path of a product has the same bits)
-  if (activation == kSilu) return __fmul_rn(z, sigmoid_of(z));
-  if (activation == kGelu) return __fmul_rn(z, normal_cdf(z));
-  if (activation == kRelu) return z < 0.f ? 0.f : z;  // NaN stays
-  return z;
+// (Which activation is asked once for all values: asked for each, 4096 x 4096 x 1024 with silu took 65 us, without an activation 25.  Values are
+// rounded by themselves, not fused with what is added to them: every path of a product has the same bits.)
+template <int N>
+__device__ __forceinline__ void activate(float (&z)[N], int activation) {
+  if (activation == kSilu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = __fmul_rn(z[j], sigmoid_of(z[j]));
+  } else if (activation == kGelu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = __fmul_rn(z[j], normal_cdf(z[j]));
+  } else if (activation == kRelu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = z[j] < 0.f ? 0.f : z[j];  // NaN stays
+  }
 }
 
 // One CTA's 128 weight rows as columns of the result.  Four columns of a thread: `column`, and S apart.
@@ -153,9 +161,8 @@ struct Columns {
     if (GATED) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) z[j] = __fmul_rn(__fmul_rn(z[j], sigmoid_of(z[j])), up[j]);
-    } else if (e.activation != kNoActivation) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) z[j] = activated(z[j], e.activation);
+    } else {
+      activate(z, e.activation);
     }
     if (e.residual != nullptr) {
 #pragma unroll
@@ -536,11 +543,9 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           if constexpr (kGated) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[0][j] = __fmul_rn(__fmul_rn(v[0][j], sigmoid_of(v[0][j])), v[1][j]);
-          } else if (MODE == kForward && e.activation != kNoActivation) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[h][j] = activated(v[h][j], e.activation);
+          } else if (MODE == kForward) {
+            activate(v[0], e.activation);
+            activate(v[1], e.activation);
           }
           __syncwarp();  // the rows before have been read
           if (MODE <= kForwardGated && e.residual != nullptr) {
