@@ -244,7 +244,7 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   if (a.q_chunks == 0) a.q_chunks = 1;
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
   const int out_cols = MODE == kForwardGated ? a.features / 2 : a.features;
-  a.plain = a.e.type != Type::kF32 && a.e.residual_ld % 8 == 0 && address(a.e.residual) % 16 == 0 && a.e.pre == nullptr && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
+  a.plain = a.e.type != Type::kF32 && a.e.residual_ld % 8 == 0 && address(a.e.residual) % 16 == 0 && address(a.e.pre) % 32 == 0 && a.e.pre_ld % 8 == 0 && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
   const int most_rows = IN_32 ? kSumRows : kPairN;
   a.tile_steps = most_rows / PairTile<MODE>::kStep;
   if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm);
