@@ -380,6 +380,8 @@ class PlannerEngine {
                  "out must match idx in shape and dtype and be contiguous");
       LPLB_CHECK((out.is_cuda() && out.get_device() == device_) || (!out.is_cuda() && out.is_pinned()),
                  "out must live on this device or in pinned host memory");
+      // what autograd has saved of `out`, a gate's choices among them, is no longer what it was
+      if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     } else {
       LPLB_CHECK(!host_idx, "pass a pinned `out` tensor together with pinned host indices");
       out = torch::empty_like(idx);

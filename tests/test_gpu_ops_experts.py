@@ -7,7 +7,7 @@ import pytest
 import torch
 from test_ops_experts import SCORES, ids_of, logits_of, no_second_gradient, second_gradients
 
-from lplb_b200 import ops
+from lplb_b200 import Planner, cube, ops
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -375,3 +375,19 @@ def test_a_gate_without_a_gradient_of_its_weights():
     (dx,) = torch.autograd.grad(weights[2:4].sum(), x)
     assert not dx[:2].any() and not dx[4:].any() and dx[2:4].any()
     assert not idx.requires_grad
+
+
+def test_a_gate_whose_choices_were_overwritten_has_no_gradient():
+    """The planner may write the physical experts over the gate's; the gradient, which needs the gate's, is then refused, as behind
+    any other write in place, and not taken of other experts."""
+    planner = Planner(cube(), 48, 32, 8, device="cuda", n_nodes=1)
+    planner.update_redundancy_mapping(torch.arange(32, 0, -1).long().cuda())
+    avail = torch.zeros(1, dtype=torch.int32, device="cuda")
+    logits = torch.randn(64, 32, device="cuda", requires_grad=True)
+    weights, idx = ops.gate_topk(logits, 4)
+    kept = planner.run(idx, avail, out=torch.empty_like(idx))
+    torch.autograd.grad(weights.sum(), logits, retain_graph=True)
+    planner.run(idx, avail, out=idx)
+    assert kept.shape == idx.shape
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(weights.sum(), logits)
