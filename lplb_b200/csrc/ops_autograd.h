@@ -3,11 +3,14 @@
 
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <initializer_list>
 #include <memory>
+#include <unordered_set>
+#include <vector>
 
 #include "ops_check.h"
 
@@ -24,13 +27,31 @@ inline bool wants_grad(std::initializer_list<const Tensor*> tensors, const char*
   bool wanted = false;
   for (const Tensor* t : tensors) wanted = wanted || (t->defined() && t->requires_grad());
   if (!wanted || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return wanted;
+  // leaves behind a weight's cast, a view or earlier operators too
+  std::vector<std::shared_ptr<torch::autograd::Node>> held;  // leaves' own nodes, which nobody else may hold
+  std::vector<torch::autograd::Node*> next;
   for (const Tensor* t : tensors) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto collects = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = collects ? collects->stream() : std::nullopt;
-    if (stream && *stream == c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap())
-      throw std::runtime_error(std::string("lplb_b200.ops.") + who +
-                               ": a graph recorded on the default stream still holds this leaf; delete its outputs before a backward pass is captured");
+    if (!t->defined() || !t->requires_grad()) continue;
+    if (!t->is_leaf()) {
+      next.push_back(t->grad_fn().get());
+    } else if (auto collects = torch::autograd::impl::try_get_grad_accumulator(*t)) {
+      next.push_back(collects.get());
+      held.push_back(std::move(collects));
+    }
+  }
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!next.empty()) {
+    torch::autograd::Node* node = next.back();
+    next.pop_back();
+    if (!seen.insert(node).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) != nullptr) {
+      const auto stream = node->stream();
+      if (stream && *stream == c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap())
+        throw std::runtime_error(std::string("lplb_b200.ops.") + who +
+                                 ": a graph recorded on the default stream still holds this leaf; delete its outputs before a backward pass is captured");
+    }
+    for (const auto& edge : node->next_edges())
+      if (edge.function) next.push_back(edge.function.get());
   }
   return true;
 }

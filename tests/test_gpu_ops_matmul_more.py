@@ -173,3 +173,31 @@ def test_infinities_and_what_is_no_number_stay_in_their_rows(groups):
     rows = torch.ones(64, dtype=torch.bool, device="cuda")
     rows[7] = rows[50] = False
     assert torch.equal(out[rows], clean[rows]) and out[50].isnan().all()
+
+
+def test_a_capture_beside_a_living_graph_of_a_leaf_behind_other_operators():
+    """As for a leaf itself: a weight that is cast inside the capture, logits of a router's product."""
+    master = torch.randn(64, 64, device="cuda", requires_grad=True)
+    x = torch.randn(32, 64, device="cuda").bfloat16()
+    dout = torch.ones(32, 64, device="cuda").bfloat16()
+    living = master * 2
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still holds this leaf"):
+        with torch.cuda.graph(graph):
+            ops.matmul(x, master.bfloat16())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still holds this leaf"):
+        with torch.cuda.graph(graph):
+            ops.gate_topk(ops.matmul(x, master.detach().bfloat16(), out_dtype=torch.float32) + master[:32], 4)
+    with torch.no_grad():  # nothing is recorded
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.matmul(x, master.bfloat16())
+    assert living.requires_grad
+    del living
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(ops.matmul(x, master.bfloat16()), master, dout)
+    graph.replay()
+    (want,) = torch.autograd.grad(ops.matmul(x, master.bfloat16()), master, dout)
+    assert torch.equal(got, want)
