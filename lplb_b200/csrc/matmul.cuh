@@ -42,6 +42,7 @@ struct Epilogue {
   const void* residual;
   void* out;
   void* pre;
+  const uint32_t* most;  // of the gradients: magnitudes that say which part of a power of two a result row's sums are, or null
   int64_t residual_ld, out_ld, pre_ld;
   int n;            // features: weight rows, the length of a bias row
   int activation;
@@ -58,6 +59,17 @@ __device__ __forceinline__ void store_float(void* p, Type type, int64_t i, float
   else if (type == Type::kBf16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
+// dz in float16: values up to 2^127 and down to 2^-149 would be infinite and zero there, and with them a gradient that is neither.  So they
+// are stored times 2^(14 - e) for a largest finite magnitude of 2^e (the products see 2^14 to 2^15 at most), and the sums multiplied by
+// 2^(e - 14) before they are rounded.  Both are exact; what lies 2^28 below the largest has fewer bits, an error of 2^-39 of the largest.
+__device__ __forceinline__ uint32_t part_exponent(uint32_t most) { return max(most >> 23, 15u); }  // both factors are normal numbers
+__device__ __forceinline__ float part_of(uint32_t most) { return __uint_as_float((268u - part_exponent(most)) << 23); }
+__device__ __forceinline__ float whole_of(uint32_t most) { return __uint_as_float((part_exponent(most) - 14u) << 23); }
+__device__ __forceinline__ uint32_t finite_magnitude(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+
 // Four values that are `S` apart; next to one another (S = 1) they start on a boundary of their size and go in one piece.
 template <int S>
 __device__ __forceinline__ void load4(const void* p, Type type, int64_t i, int limit, float (&v)[4]) {
@@ -583,6 +595,14 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[h][j] = __uint_as_float(raw[h][j]) + (MODE <= kForwardGated ? bias[2 * h + (j >> 1 & 1)] : 0.f);
+          if (MODE > kForwardGated && e.most != nullptr) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {  // (what is not there is not stored)
+              const float whole = whole_of(e.most[row0 + min(c0 + 8 * (r >> 1) + 2 * (lane & 3) + (r & 1), n - 1)]);
+#pragma unroll
+              for (int h = 0; h < 4; ++h) v[h >> 1][4 * (r >> 1) + 2 * (h & 1) + (r & 1)] *= whole;
+            }
+          }
           if (MODE <= kForwardGated && e.pre != nullptr) keep(c0, v);
           if constexpr (kGated) {
 #pragma unroll
@@ -683,6 +703,11 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
             for (int j = 0; j < 4; ++j) {
               z[j] = from[j * S];
               up[j] = kGated ? from[16 + j * S] : 0.f;
+            }
+            if (MODE > kForwardGated && e.most != nullptr) {
+              const float whole = whole_of(e.most[row0 + at]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) z[j] *= whole;
             }
             mine.finish(e, row0 + at, z, up, r[q]);
           }

@@ -31,9 +31,14 @@ struct Matmul {
 };
 cudaError_t launch_matmul(const Matmul& p, int device, cudaStream_t stream);
 
+// dz of float16 operands, whose type has no more than five bits of an exponent, is stored in parts of a power of two: of a row for da, of a
+// column (and group) for db, so that its largest finite magnitude there is at least 2^14 and below 2^15.  `most` is that magnitude
+// before, as a float's bits; 0 has the factor of the smallest.  Null: dz as it is.
+
 // da = dz @ b: [m, k] of the type, row stride da_ld; rows behind the last group are zero
 struct MatmulInput {
   const void* dz;  // [m, n], row stride dz_ld
+  const uint32_t* most;  // [m], or null
   const void* b;   // [groups, n, k]
   const int* rows;
   void* da;
@@ -46,6 +51,7 @@ cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t s
 // db[e] = dz_e^T @ a_e over the rows of group e: [groups, n, k] of the type
 struct MatmulWeight {
   const void* dz;  // [m, n], row stride dz_ld
+  const uint32_t* most;  // [groups, n], or null
   const void* a;   // [m, k], row stride a_ld
   const int* rows;
   void* db;
@@ -63,6 +69,9 @@ struct MatmulPre {
   const float* pre;  // [m, n], row stride pre_ld; null without an activation
   const int* rows;
   void* dz;          // [m, n] of `type`, row stride dz_ld, or null: not wanted
+  void* dz_weight;   // with `column_most`: dz by columns for db, as dz
+  uint32_t* row_most;     // [m], taken and used here, or null: dz is not stored in parts
+  uint32_t* column_most;  // [groups, n], the same
   void* dbias;       // [groups, n] of bias_type, or null
   float* parts;      // matmul_pre_parts(): sums of a part of a group's rows
   int64_t m, n, dout_ld, pre_ld, dz_ld;

@@ -132,14 +132,29 @@ variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b,
   } else {
     // without an activation dz is dout, where the products can read it
     const bool same = act == lplb::ops::kNoActivation && !out_f32;
-    Tensor dz = same ? rows_for_tma(dout) : Tensor();
+    Tensor dz = same ? rows_for_tma(dout) : Tensor(), dz_weight = dz;
+    Tensor row_most, column_most;  // of dz in float16, which is stored in parts of a power of two
     if (!same || need_bias) {
       const Tensor d = rows_together(dout);
       lplb::ops::MatmulPre p{};
       if (!same && (need_a || need_b)) {
-        dz = make({s.m, up_to(s.n, 8)}, a.scalar_type(), a);
-        p.dz = dz.data_ptr();
-        p.dz_ld = dz.size(1);
+        const bool in_parts = type == Type::kF16;
+        if (need_a || !in_parts) {
+          dz = make({s.m, up_to(s.n, 8)}, a.scalar_type(), a);
+          p.dz = dz.data_ptr();
+        }
+        dz_weight = dz;
+        p.dz_ld = up_to(s.n, 8);
+        if (in_parts && need_a) {
+          row_most = make({s.m}, torch::kInt32, a);
+          p.row_most = reinterpret_cast<uint32_t*>(row_most.data_ptr<int>());
+        }
+        if (in_parts && need_b) {
+          dz_weight = make({s.m, up_to(s.n, 8)}, a.scalar_type(), a);
+          p.dz_weight = dz_weight.data_ptr();
+          column_most = make({s.groups, s.n}, torch::kInt32, a);
+          p.column_most = reinterpret_cast<uint32_t*>(column_most.data_ptr<int>());
+        }
       }
       p.dout = d.data_ptr();
       p.dout_ld = d.stride(0);
@@ -171,6 +186,7 @@ variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b,
     if (need_a) {
       lplb::ops::MatmulInput p{};
       p.dz = dz.data_ptr();
+      p.most = row_most.defined() ? reinterpret_cast<const uint32_t*>(row_most.data_ptr<int>()) : nullptr;
       p.b = b.data_ptr();
       p.rows = rows_of(rows);
       p.da = da.data_ptr();
@@ -186,14 +202,15 @@ variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b,
     if (need_b) {
       const Tensor from = rows_for_tma(a);
       lplb::ops::MatmulWeight p{};
-      p.dz = dz.data_ptr();
+      p.dz = dz_weight.data_ptr();
+      p.most = column_most.defined() ? reinterpret_cast<const uint32_t*>(column_most.data_ptr<int>()) : nullptr;
       p.a = from.data_ptr();
       p.rows = rows_of(rows);
       p.db = db.data_ptr();
       p.m = s.m;
       p.n = s.n;
       p.k = s.k;
-      p.dz_ld = ld_of(dz);
+      p.dz_ld = ld_of(dz_weight);
       p.a_ld = ld_of(from);
       p.groups = (int)s.groups;
       p.type = type;

@@ -70,7 +70,9 @@ def matmul(
     on a 16-byte boundary; rows of ``a`` that do not are copied first.
 
     Differentiable with respect to ``a``, ``b``, ``bias`` and ``residual``.  For the backward pass the sums before an activation are
-    kept, in 32 bits, and their gradients are rounded to ``a``'s type before they are multiplied; all sums are in 32 bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
+    kept, in 32 bits, and their gradients are rounded to ``a``'s bits before they are multiplied: to bfloat16, or to the 11 bits of
+    float16 in parts of a power of two, so that what float16 does not hold on the way, large or small, is not lost.  All sums are in 32
+    bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
     tensors on plain statements; calls and backward passes can be captured in a CUDA graph, and the same inputs give the same
     bits.  Wrong arguments raise ``ValueError``; :func:`~lplb_b200.ops.check` tells of waits that ran out."""
     if activation not in MATMUL_ACTIVATIONS:  # (messages are put together where they are needed: the call is a few microseconds)

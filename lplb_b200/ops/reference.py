@@ -392,6 +392,16 @@ def matmul_reference(
     return (out if residual is None else out + _wide(residual).to(out.dtype)), z
 
 
+def _as_operand(dz: torch.Tensor, dtype: torch.dtype, dim: int) -> torch.Tensor:
+    """``dz`` as a product's operand holds it.  In float16 it is held in parts of a power of two of its largest finite magnitude along ``dim``
+    (``part_of`` in ``csrc/matmul.cuh``): its own numbers would end at 65504 and 2**-24."""
+    if dtype != torch.float16 or dz.numel() == 0:
+        return dz.to(dtype).to(dz.dtype)
+    most = torch.where(dz.isfinite(), dz.abs(), torch.zeros_like(dz)).amax(dim, keepdim=True)
+    exponent = torch.frexp(most).exponent.clamp_min(-111) - 15
+    return torch.ldexp(torch.ldexp(dz, -exponent).to(dtype).to(dz.dtype), exponent)
+
+
 def matmul_backward_reference(
     dout: torch.Tensor, a: torch.Tensor, b: torch.Tensor, z: torch.Tensor | None, activation: str | None = None, rows: torch.Tensor | None = None
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -404,6 +414,5 @@ def matmul_backward_reference(
             dz = _through_activation(dz, _wide(z[part]).to(af.dtype), activation)
         at = slice(None) if e is None else e
         dbias[at] = dz.sum(0)
-        dz = dz.to(a.dtype).to(af.dtype)  # as the products behind it take it
-        da[part], db[at] = dz @ bf[at], dz.T @ af[part]
+        da[part], db[at] = _as_operand(dz, a.dtype, 1) @ bf[at], _as_operand(dz, a.dtype, 0).T @ af[part]
     return da, db, dbias
