@@ -316,8 +316,8 @@ PairCost pair_cost(int64_t rows, int step, int most_rows, int64_t tiles_p, int64
 }
 
 // Of a weight's gradient: the groups' rows are what is summed, here as if they were equal.
-int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm) {
-  return pair_cost(result_rows, kWeightStep, kPairN, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
+int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm, int most_rows) {
+  return pair_cost(result_rows, kWeightStep, most_rows, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
 }
 
 template <Mode MODE, bool IN_32 = false>
@@ -341,7 +341,7 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   a.plain = a.e.type != Type::kF32 && a.e.residual_ld % 8 == 0 && address(a.e.residual) % 16 == 0 && address(a.e.pre) % 32 == 0 && a.e.pre_ld % 8 == 0 && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
   const int most_rows = IN_32 ? kSumRows : kPairN;
   a.tile_steps = most_rows / PairTile<MODE>::kStep;
-  if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm);
+  if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm, most_rows);
   else if (a.rows == nullptr) a.tile_steps = pair_cost(a.n_rows, PairTile<MODE>::kStep, most_rows, a.tiles_p, a.k_blocks, n_sm).steps;
   return launch_after(kernel, dim3(n_sm & ~1), dim3(kPairThreads), kPairSmem, stream, maps, a);
 }
@@ -366,9 +366,9 @@ int is_wide(const Matmul& p) {
          fours(p.bias, p.n, p.bias_type);
 }
 
-// A result in 32 bits whose sum is longer than one part.  us, sums of one part in tiles of up to 256 rows and in registers: 600 x 4096 x 512 9.7,
-// 13.1; 8192 x 1000 x 512 18.0, 24.2.
-bool sums_in_parts(const Matmul& p) { return p.out_type == Type::kF32 && p.k > kSumBlocks * kPairK; }
+// Whether the sum is longer than one part.  us, sums of one part in tiles of up to 256 rows and in registers, results in 32 bits: 600 x 4096 x 512
+// 9.7, 13.1; 8192 x 1000 x 512 18.0, 24.2.
+bool sums_in_parts(const Matmul& p) { return p.k > longest_part(p.out_type); }
 
 cudaError_t launch_forward(const Matmul& p, int device, cudaStream_t stream) {
   PairMaps maps{};
@@ -427,10 +427,10 @@ cudaError_t resident_clusters(int device, int split, Kernel kernel, int* cluster
   if (err == cudaSuccess) known[device][split].store(*clusters, std::memory_order_relaxed);
   return err;
 }
-// Accumulators, and stages of the ring, of CTAs with `cols` rows of a and `blocks` k blocks.
-int few_chains(int cols, int blocks, bool in_32) {
+// Accumulators, and stages of the ring, of CTAs with `cols` rows of a and `blocks` k blocks, at most `part` of them to an accumulator.
+int few_chains(int cols, int blocks, int part) {
   int chains = 1;
-  while (in_32 && chains * kSumBlocks < blocks && (chains + 1) * cols <= kFewMostRows) ++chains;
+  while (chains * part < blocks && (chains + 1) * cols <= kFewMostRows) ++chains;
   return chains;
 }
 int few_stages(int cols, int blocks) {
@@ -459,6 +459,7 @@ cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
   const int most_rows = in_32 ? kFewMostRows / 2 : kFewMostRows;  // two accumulators at least
   // (32 bits and up to eight parts of the rows: the search is one of the call's five microseconds at most)
   const int m = (int)p.m, tiles = (int)((p.n + kFewTileRows - 1) / kFewTileRows), k_blocks = (int)((p.k + kPairK - 1) / kPairK);
+  const int part = longest_part(p.out_type) / kPairK;
   *best = {INT64_MAX, 0, 0};
   for (int s = 1; s <= kFewMostSplit && s <= k_blocks; ++s) {
     int fit = 0;
@@ -467,7 +468,7 @@ cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
     const int blocks = (k_blocks + s - 1) / s, least_groups = (m + most_rows - 1) / most_rows;
     for (int g = least_groups; g <= (m + 15) / 16 && g < least_groups + 8; ++g) {
       const int cols = ((m + g - 1) / g + 15) / 16 * 16, groups = (m + cols - 1) / cols;
-      if (in_32 && few_chains(cols, blocks, true) * kSumBlocks < blocks) continue;  // its parts would be longer than the pairs'
+      if ((int64_t)few_chains(cols, blocks, part) * part < blocks) continue;  // its parts would be longer than the pairs'
       const int64_t rounds = ((int64_t)tiles * groups + fit - 1) / fit;
       const int64_t cycles = rounds * (blocks * (256 + 2 * cols) + 10 * cols + (s > 1 ? 1500 + 2 * cols : 0));
       if (cycles < best->cycles) *best = {cycles, s, cols};
@@ -492,7 +493,7 @@ cudaError_t launch_few(const Matmul& p, const FewCost& how, int device, cudaStre
   a.cols = how.cols;
   const int split = how.split, groups = (a.m + a.cols - 1) / a.cols, blocks = (a.k_blocks + split - 1) / split;
   a.stages = few_stages(a.cols, blocks);
-  a.chains = few_chains(a.cols, blocks, p.out_type == Type::kF32);
+  a.chains = few_chains(a.cols, blocks, longest_part(p.out_type) / kPairK);
   CUtensorMap map_b, map_a;
   if ((err = map_2d(&map_b, p.b, p.n, p.k, p.k, GATED ? kFewTileRows / 2 : kFewTileRows)) != cudaSuccess) return err;
   if ((err = map_2d(&map_a, p.a, p.m, p.k, p.a_ld, a.cols)) != cudaSuccess) return err;
@@ -636,7 +637,8 @@ cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t s
   cudaError_t err = maps_of_rows(&maps, p.dz, p.m, p.n, p.dz_ld);
   a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
   if (err == cudaSuccess) err = a.p_chunks == 2 ? map_chunks(&maps.p[0], p.b, a.groups, p.n, p.k) : map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kPairK);
-  return err != cudaSuccess ? err : launch_pairs<kInput>(maps, a, device, stream);
+  if (err != cudaSuccess) return err;
+  return p.n > longest_part(p.type) ? launch_pairs<kInput, true>(maps, a, device, stream) : launch_pairs<kInput>(maps, a, device, stream);
 }
 
 int64_t matmul_weight_copies(const MatmulWeight& p) { return p.rows != nullptr ? weight_copies(p).bytes : 0; }
@@ -657,24 +659,30 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
   a.e.n = (int)p.k;
   a.e.type = p.type;
   PairMaps maps{};
+  const WeightCopies c = weight_copies(p);
+  uint8_t* of_dz = static_cast<uint8_t*>(p.copies) + c.a_bytes;
+  auto map = [](CUtensorMap* m, int chunks, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+    return chunks == 2 ? map_chunks(m, base, rows, cols, ld, kPairK) : map_2d(m, base, rows, cols, ld, kPairK);
+  };
+  auto map_q = [&](int chunks) {
+    a.q_chunks = chunks;
+    const cudaError_t err = map(&maps.q[0], chunks, p.dz, p.m, p.n, p.dz_ld);
+    return err != cudaSuccess || p.rows == nullptr ? err : map(&maps.q[1], chunks, of_dz, (int64_t)a.groups * kPairK, p.n, c.dz_ld);
+  };
+  // One group: its length is known.  Several: a launch for those of up to `longest` rows, and where there may be longer ones, one for them.
+  const int longest = longest_part(p.type);
+  const bool may_be_long = p.m > longest, all_long = may_be_long && p.rows == nullptr;
   if (p.m > 0) {  // (without a row there is nothing to load: every matrix is cleared)
     int n_sm = 0;
     cudaError_t err = multiprocessors(device, &n_sm);
-    const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm);
+    const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm, kPairN);
     a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
-    a.q_chunks = p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1;  // every tile has 256 result rows
-    auto map = [](CUtensorMap* m, int chunks, const void* base, int64_t rows, int64_t cols, int64_t ld) {
-      return chunks == 2 ? map_chunks(m, base, rows, cols, ld, kPairK) : map_2d(m, base, rows, cols, ld, kPairK);
-    };
     if (err == cudaSuccess) err = map(&maps.p[0], a.p_chunks, p.a, p.m, p.k, p.a_ld);
-    if (err == cudaSuccess) err = map(&maps.q[0], a.q_chunks, p.dz, p.m, p.n, p.dz_ld);
+    if (err == cudaSuccess) err = map_q(!all_long && p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1);  // 2: every tile has 256 result rows
     if (p.rows != nullptr) {
       if (p.copies == nullptr) return cudaErrorInvalidValue;
       a.copies = 1;
-      const WeightCopies c = weight_copies(p);
-      uint8_t* of_dz = static_cast<uint8_t*>(p.copies) + c.a_bytes;
       if (err == cudaSuccess) err = map(&maps.p[1], a.p_chunks, p.copies, (int64_t)a.groups * kPairK, p.k, c.a_ld);
-      if (err == cudaSuccess) err = map(&maps.q[1], a.q_chunks, of_dz, (int64_t)a.groups * kPairK, p.n, c.dz_ld);
       LastBlocks l{};
       l.from[0] = p.a, l.from[1] = p.dz;
       l.to[0] = p.copies, l.to[1] = of_dz;
@@ -691,7 +699,12 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
     }
     if (err != cudaSuccess) return err;
   }
-  return launch_pairs<kWeight>(maps, a, device, stream);
+  if (all_long) return launch_pairs<kWeight, true>(maps, a, device, stream);
+  a.long_sum = may_be_long ? longest : 0;
+  cudaError_t err = launch_pairs<kWeight>(maps, a, device, stream);
+  if (err != cudaSuccess || !may_be_long) return err;
+  if ((err = map_q(1)) != cudaSuccess) return err;
+  return launch_pairs<kWeight, true>(maps, a, device, stream);
 }
 
 cudaError_t matmul_pre_parts(const MatmulPre& p, int device, int64_t* floats, int* splits) {

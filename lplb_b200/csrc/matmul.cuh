@@ -211,12 +211,17 @@ constexpr uint32_t kTurn = 2048;   // of one such warp: 32 features x 32 result 
 constexpr uint32_t kPairBars = 256;
 constexpr size_t kPairSmem = 1024 + kPairRing + kPairBars + kStoreWarps * kTurn;
 constexpr int kPairThreads = 64 + 32 * kStoreWarps, kPairColumns = 512;
-// The tensor cores cut an accumulator's last bits off at every addition, which makes a long sum too small: by 1.6e-8 of it per 16
-// products, 7e-6 over 7168, where sums in 32 bits that are rounded are off by 1e-6.  A result in 32 bits shows that, so its sum is
-// taken over `kSumBlocks` blocks at a time in tensor memory, and these sums are added in registers (off by 5e-7 whatever the length).
+// The tensor cores cut an accumulator's last bits off at every addition, which makes a long sum too small: one of products of the same sign by
+// 6e-9 of it per product (3e-6 over 512, 1.0e-4 over 16,384, 6.7e-3 over 2^20, measured), one of either sign less, 7e-6 over 7168, where sums in 32
+// bits that are rounded are off by 1e-6.  A result in 32 bits shows that, so its sum is taken over `kSumBlocks` blocks at a time in tensor
+// memory, and these sums are added in registers (either sign: off by 5e-7 whatever the length).  A result in 16 bits hides it behind its
+// rounding up to `longest_part` products; longer sums go the same way as a result in 32 bits.
 // Tiles of at most `kSumRows` result rows: a thread holds half of them.  8192 x 4096 x 7168 in 450-500 us (16 bits 340-370),
 // 1001 x 4100 x 2064 in 24.3 (20.7); blocks of 4 541 and 25.9; 192 rows, whose sums do not fit the registers, 612 and 37.8.
 constexpr int kSumBlocks = 8, kSumRows = 128;
+// Products of one accumulator for a result of the type: what is cut off is at most a fifth of half a step (2^-11 and 2^-8).  It also keeps the
+// epilogue's wait for a sum far below its limit.
+constexpr int longest_part(Type type) { return type == Type::kF32 ? kSumBlocks * kPairK : type == Type::kF16 ? 16384 : 131072; }
 
 struct PairMaps {
   CUtensorMap p[2], q[kBoxes];  // P: the first only, but for kWeight
@@ -232,6 +237,7 @@ struct PairArgs {
   int tile_steps;   // result rows of a tile at most, in steps
   int p_chunks, q_chunks;  // chunks of an MN-major operand that a box holds: 2 where columns come in whole chunks (q: and a CTA has two)
   int copies;       // kWeight: the last blocks of groups have been copied
+  int long_sum;     // kWeight: groups of more rows are left to the launch that sums in parts, and it has them alone; 0: all groups are this launch's
   int wide;         // four neighbouring values of everything in the epilogue start on a boundary of their size
   int plain;        // a result in 16 bits, rows (the residual's too) of whole 16-byte words on boundaries
   uint32_t idesc;
@@ -268,7 +274,7 @@ struct PairTile {
 // it turns 32 features x 32 result rows round in shared memory of its own.  Two accumulators: the epilogue of a tile runs beside the
 // sums of the next.  (With four warps that met at a barrier every 16 rows a weight's gradient of 32 experts, 512 rows each on average,
 // 4096 x 7168, took 3070 us: its tiles have 8 blocks to sum, and 1750 cycles went into every 16 rows.)
-// IN_32: a result in 32 bits, summed in parts.
+// IN_32: summed in parts, as a result in 32 bits is.
 template <Mode MODE, bool IN_32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
@@ -317,7 +323,8 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
       }
       if (e < a.groups) {
         const int from = (int)min((long long)a.n_rows, before + scan - mine), to = (int)min((long long)a.n_rows, before + scan);
-        s_rows[e] = to - from;
+        const bool others = MODE == kWeight && a.long_sum > 0 && (to - from > a.long_sum) != IN_32;
+        s_rows[e] = others ? -1 : to - from;  // (neither summed nor cleared)
         s_start[e] = from;
         s_start[e + 1] = to;  // (also written, the same, by the next lane)
       }
@@ -715,7 +722,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
         if constexpr (IN_32) {
           constexpr int kBlocks = kSumRows / 64;
           float sum[kBlocks][2][16];  // this warp's 32 result rows of every 64
-          const int parts = (a.k_blocks + kSumBlocks - 1) / kSumBlocks;
+          const int parts = (blocks_of() + kSumBlocks - 1) / kSumBlocks;
           bool ok = true;
           for (int p = 0; p < parts; ++p) {
             if (!(ok = await())) break;
