@@ -2,6 +2,7 @@
 #pragma once
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
@@ -50,7 +51,13 @@ inline lplb::ops::Type type_of(const Tensor& t, const char* who) {
   return lplb::ops::Type::kF32;
 }
 
+// A dual tensor of forward-mode differentiation goes through a kernel without its tangent: the derivative would be zero, with no error.
+inline void check_no_tangent(const Tensor& t, const char* who) {
+  OPS_CHECK(!t.defined() || !t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+            who + std::string(" has a forward-mode tangent: these operators are differentiated backwards alone"));
+}
 inline void check_no_grad(const Tensor& t, const char* who) {
+  check_no_tangent(t, who);
   OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who + std::string(" requires a gradient: these operators have no backward pass (use torch.no_grad())"));
 }
 

@@ -14,8 +14,8 @@ bits, ``matmul_fp8``)::
     act = ops.matmul(rows, w13, activation="swiglu", rows=order.counts)
     y = ops.combine_rows(ops.matmul(act, w2, rows=order.counts), order, weights)
 
-Every one but :func:`expert_order`, which has whole numbers alone, has a gradient; a gradient's gradient is refused.  CUDA tensors
-run on the native kernels, on the current stream of their device; CPU tensors on the plain statements in
+Every one but :func:`expert_order`, which has whole numbers alone, has a gradient; a gradient's gradient is refused, and so is a CUDA
+tensor with a forward-mode tangent.  CUDA tensors run on the native kernels, on the current stream of their device; CPU tensors on the plain statements in
 :mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph, backward passes too.  The same inputs give the same
 bits.  Wrong arguments raise ``ValueError``.
 

@@ -303,7 +303,8 @@ def take_rows_reference(x: torch.Tensor, place: torch.Tensor, source: torch.Tens
     if raw.shape[0] == 0:
         return x.new_empty(0, x.shape[1])
     rows = raw[source.clamp_min(0).long() // place.shape[1]]
-    return torch.where((source >= 0).unsqueeze(1), rows, torch.zeros_like(rows)).view(x.dtype)
+    rows = torch.where((source >= 0).unsqueeze(1), rows, torch.zeros_like(rows))
+    return rows if rows.dtype == x.dtype else rows.view(x.dtype)  # (a view by type has no forward-mode derivative)
 
 
 def combine_rows_reference(rows: torch.Tensor, place: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
