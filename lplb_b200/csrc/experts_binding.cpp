@@ -45,7 +45,7 @@ variable_list gate_forward(const Tensor& logits, int64_t topk, bool sigmoid, boo
 
 Tensor gate_backward(const Tensor& logits, const Tensor& idx, const Tensor& dweights, bool sigmoid, bool renormalize, double scale) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
-  const Tensor x = rows_together(logits), d = dweights.contiguous();
+  const Tensor x = rows_together(logits), d = as_stored(dweights).contiguous();
   auto g = gate_args(x, idx.size(1), sigmoid, renormalize, scale);
   OPS_CHECK(idx.device() == x.device() && d.device() == x.device() && idx.scalar_type() == torch::kInt64 && idx.is_contiguous() &&
                 idx.size(0) == g.tokens && d.scalar_type() == torch::kFloat32 && d.sizes() == idx.sizes(),
@@ -78,7 +78,8 @@ struct GateTopk : torch::autograd::Function<GateTopk> {
   }
 };
 
-py::tuple gate_topk(const Tensor& logits, int64_t topk, bool sigmoid, bool renormalize, double scale) {
+py::tuple gate_topk(const Tensor& given, int64_t topk, bool sigmoid, bool renormalize, double scale) {
+  const Tensor logits = as_stored(given);
   const auto out = wants_grad({&logits}, "gate_topk") ? GateTopk::apply(logits, topk, sigmoid, renormalize, scale) : gate_forward(logits, topk, sigmoid, renormalize, scale);
   return py::make_tuple(out[0], out[1]);
 }
@@ -169,7 +170,7 @@ Tensor combine_forward(const Tensor& rows, const Tensor& place, const Tensor& so
 variable_list combine_backward(const Tensor& dout, const Tensor& rows, const Tensor& place, const Tensor& source, const Tensor& weights,
                                 bool need_rows, bool need_weights) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(rows));
-  const Tensor from = rows_together(rows), d = rows_together(dout);
+  const Tensor from = rows_together(rows), d = rows_together(as_stored(dout));
   auto c = combine_args(from, place, source, weights, "combine_rows");
   OPS_CHECK(d.device() == rows.device() && d.dim() == 2 && d.size(0) == c.tokens && d.size(1) == c.cols && d.scalar_type() == rows.scalar_type(),
             "combine_rows: the gradient must be of the output's shape, type and device");
@@ -195,7 +196,7 @@ struct TakeRows : torch::autograd::Function<TakeRows> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    return first_order({combine_forward(grads[0], saved[0], saved[1], std::nullopt), Tensor(), Tensor()}, "take_rows");
+    return first_order({combine_forward(as_stored(grads[0]), saved[0], saved[1], std::nullopt), Tensor(), Tensor()}, "take_rows");
   }
 };
 
@@ -218,20 +219,22 @@ struct Gather : torch::autograd::Function<Gather> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    return first_order({take_forward(grads[0], saved[0], saved[1]), Tensor(), Tensor()}, "combine_rows");
+    return first_order({take_forward(as_stored(grads[0]), saved[0], saved[1]), Tensor(), Tensor()}, "combine_rows");
   }
 };
 
-Tensor take_rows(const Tensor& x, const Tensor& place, const Tensor& source) {
+Tensor take_rows(const Tensor& given, const Tensor& place, const Tensor& source) {
+  const Tensor x = as_stored(given);
   if (!wants_grad({&x}, "take_rows")) return take_forward(x, place, source);
   type_of(x, "take_rows: x that requires a gradient");
   return TakeRows::apply(x, place, source);
 }
 
-Tensor combine_rows(const Tensor& rows, const Tensor& place, const Tensor& source, const OptTensor& weights) {
+Tensor combine_rows(const Tensor& given, const Tensor& place, const Tensor& source, const OptTensor& weights) {
+  const Tensor rows = as_stored(given);
   if (!weights) return wants_grad({&rows}, "combine_rows") ? Gather::apply(rows, place, source) : combine_forward(rows, place, source, std::nullopt);
   OPS_CHECK(weights->is_floating_point(), "combine_rows: weights must be floating point [tokens, topk] on the rows' device");
-  const Tensor w = weights->to(torch::kFloat32).contiguous();
+  const Tensor w = as_stored(*weights).to(torch::kFloat32).contiguous();
   return wants_grad({&rows, &w}, "combine_rows") ? Combine::apply(rows, place, source, w) : combine_forward(rows, place, source, w);
 }
 

@@ -105,10 +105,11 @@ variable_list run_forward(const Tensor& a, const Tensor& b, const OptTensor& bia
 }
 
 // (da, db, dbias), each where it is needed.  bias: its type, float32 or a's.
-variable_list run_backward(const Tensor& dout, const Tensor& a, const Tensor& b, const OptTensor& pre, int64_t activation, const OptTensor& rows, bool out_f32,
+variable_list run_backward(const Tensor& given, const Tensor& a, const Tensor& b, const OptTensor& pre, int64_t activation, const OptTensor& rows, bool out_f32,
                        bool bias_f32, bool need_a, bool need_b, bool need_bias) {
   const Shape s = check_operands(a, b, rows);
   const auto act = activation_of(activation, s);
+  const Tensor dout = as_stored(given);
   const int64_t cols = act == lplb::ops::kSwiglu ? s.n / 2 : s.n;
   const auto out_type = out_f32 ? torch::kFloat32 : a.scalar_type();
   OPS_CHECK(dout.device() == a.device() && dout.scalar_type() == out_type && dout.dim() == 2 && dout.size(0) == s.m && dout.size(1) == cols,
@@ -252,7 +253,10 @@ struct Product : torch::autograd::Function<Product> {
   }
 };
 
-Tensor matmul(const Tensor& a, const Tensor& b, const OptTensor& bias, int64_t activation, const OptTensor& residual, const OptTensor& rows, bool out_f32) {
+Tensor matmul(const Tensor& given_a, const Tensor& given_b, const OptTensor& given_bias, int64_t activation, const OptTensor& given_residual,
+              const OptTensor& rows, bool out_f32) {
+  const Tensor a = as_stored(given_a), b = as_stored(given_b);
+  const OptTensor bias = as_stored(given_bias), residual = as_stored(given_residual);
   const Tensor added = or_none(bias), carried = or_none(residual);
   if (wants_grad({&a, &b, &added, &carried}, "matmul")) return Product::apply(a, b, bias, residual, rows, activation, out_f32);
   return run_forward(a, b, bias, activation, residual, rows, out_f32, false)[0];

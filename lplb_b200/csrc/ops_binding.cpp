@@ -41,7 +41,8 @@ lplb::ops::RowFp8 row_args(const Tensor& x, const RowsOut& out, const char* who)
   return a;
 }
 
-py::tuple quantize_fp8(const Tensor& x) {
+py::tuple quantize_fp8(const Tensor& given) {
+  const Tensor x = as_stored(given);
   check_rows(x, "quantize_fp8: x");
   c10::cuda::CUDAGuard guard(x.device());
   const auto out = make_rows(x);
@@ -50,7 +51,9 @@ py::tuple quantize_fp8(const Tensor& x) {
   return py::make_tuple(out.q, out.scale);
 }
 
-py::tuple rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, bool return_normed) {
+py::tuple rms_norm_fp8(const Tensor& given, const Tensor& given_weight, const OptTensor& given_residual, double eps, bool return_normed) {
+  const Tensor x = as_stored(given), weight = as_stored(given_weight);
+  const OptTensor residual = as_stored(given_residual);
   check_rows(x, "rms_norm_fp8: x");
   check_no_grad(weight, "rms_norm_fp8: weight");
   OPS_CHECK(weight.is_cuda() && weight.device() == x.device() && weight.dim() == 1 && weight.size(0) == x.size(-1) && weight.is_contiguous(),
@@ -84,7 +87,8 @@ py::tuple rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& r
   return py::make_tuple(out.q, out.scale, sum);
 }
 
-py::tuple quantize_weight_fp8(const Tensor& w) {
+py::tuple quantize_weight_fp8(const Tensor& given) {
+  const Tensor w = as_stored(given);
   OPS_CHECK(w.is_cuda() && (w.dim() == 2 || w.dim() == 3) && w.is_contiguous(), "quantize_weight_fp8: w must be a contiguous CUDA tensor [rows, cols] or [matrices, rows, cols]");
   check_no_grad(w, "quantize_weight_fp8: w");
   const auto type = type_of(w, "quantize_weight_fp8: w");
@@ -140,6 +144,7 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
     OPS_CHECK(out->device() == device && out->scalar_type() == type && out->dim() == 2 && out->size(0) == m && out->size(1) == n &&
                   (out->stride(1) == 1 || n == 1) && (m < 2 || out->stride(0) >= n),
               "matmul_fp8: out must be [rows, n] of the output type on a's device, rows contiguous and apart from one another");
+    OPS_CHECK(!out->is_neg(), "matmul_fp8: out must not be a lazily negated view");
     check_no_grad(*out, "matmul_fp8: out");
     result = *out;
     // what autograd has saved of `out` is no longer what it was
@@ -167,10 +172,11 @@ Tensor matmul_fp8(const Tensor& a, const Tensor& a_scale, const Tensor& b, const
   return result;
 }
 
-Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& weights, const Tensor& w13, const Tensor& w2, const OptTensor& x_scale,
+Tensor moe_few_tokens(const Tensor& x, const Tensor& idx, const Tensor& given_weights, const Tensor& w13, const Tensor& w2, const OptTensor& x_scale,
                       const OptTensor& w13_scale, const OptTensor& w2_scale, const OptTensor& status) {
   const auto device = x.device();
   const bool fp8 = w13_scale.has_value();
+  const Tensor weights = as_stored(given_weights);
   OPS_CHECK(x.is_cuda() && x.dim() == 2, "moe_few_tokens: x must be a CUDA tensor [tokens, hidden]");
   const int64_t tokens = x.size(0), hidden = x.size(1);
   OPS_CHECK(tokens <= lplb::ops::kMoeFewMaxTokens, "moe_few_tokens: at most " + text(lplb::ops::kMoeFewMaxTokens) + " tokens, not " + text(tokens));

@@ -61,6 +61,11 @@ inline void check_no_grad(const Tensor& t, const char* who) {
   OPS_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), who + std::string(" requires a gradient: these operators have no backward pass (use torch.no_grad())"));
 }
 
+// A lazily conjugated or negated view (z.conj(), z.conj().imag) stands for other values than its memory holds: what a kernel reads is written
+// out first.  A recorded call does this before it is recorded, so that the gradient goes back through it.
+inline Tensor as_stored(const Tensor& t) { return t.defined() && (t.is_conj() || t.is_neg()) ? t.resolve_conj().resolve_neg() : t; }
+inline OptTensor as_stored(const OptTensor& t) { return t ? OptTensor(as_stored(*t)) : std::nullopt; }
+
 inline int sm_count(int device) {
   int n = 0;
   OPS_CUDA(lplb::ops::multiprocessors(device, &n));

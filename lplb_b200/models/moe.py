@@ -220,7 +220,7 @@ class MoELayer:
                 raise RuntimeError("expert placement changed: call place_weights() first")
             self._placed_version = version
         fuse = self.fuse_dispatch if fuse_dispatch is None else fuse_dispatch
-        phys_idx, weights = phys_idx.contiguous(), weights.float().contiguous()
+        phys_idx, weights = phys_idx.contiguous(), weights.float().contiguous().resolve_neg()
         if self._few_fits and self.few_tokens and not fuse_dispatch and upto == 5 and x.shape[0] <= ops.MOE_FEW_MAX_TOKENS:
             x = _rows_apart(x)
             if x_scale is not None and x_scale.stride(-1) != 1:
