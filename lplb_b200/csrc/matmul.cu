@@ -31,7 +31,9 @@ __device__ __forceinline__ void through(float (&d)[2][4], const float (&z)[2][4]
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float u = z[i / 4][i % 4];
-      d[i / 4][i % 4] *= normal_cdf(u) + u * 0.3989422804f * __expf(-0.5f * u * u);  // 1 / sqrt(2 pi)
+      float bell;
+      const float cdf = normal_cdf(u, bell);
+      d[i / 4][i % 4] *= cdf + u * 0.3989422804f * bell;  // 1 / sqrt(2 pi)
     }
   } else if (activation == kRelu) {
 #pragma unroll

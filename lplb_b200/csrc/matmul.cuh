@@ -121,11 +121,24 @@ __device__ __forceinline__ void store4(void* p, Type type, int64_t i, int limit,
   }
 }
 
-// (__expf is off by 2 + 1.2 |x| units in the last place, the quotient by two: 2^-20 of the value where it matters, and the
-// result, of up to 24 bits, is mostly rounded to 8 or 11)
+// (__expf is off by 2 + 1.2 |z| units in the last place, the quotient by two: some |z| units come from z's own last bit, too.  Below z = -87, where
+// silu is 1e-36, it is 0.)
 __device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-// (of a third of normcdff's instructions; off by 2^-24, not of the value, below zero)
-__device__ __forceinline__ float normal_cdf(float z) { return fmaf(0.5f, erff(z * 0.70710678f), 0.5f); }
+// The normal distribution's function, and e^(-z^2 / 2), in few instructions and good to some 2^-20 of the value on either side: for u >= 0
+// Phi(-u) e^(u^2 / 2) is smooth and falls slowly, here as a polynomial in 1 / (1 + 0.4 u), fitted to 0 <= u <= 14 by least squares of the relative error
+// with weights that level it (8e-8; in 32 bits 3.5e-7).  us, 4096 x 4096 x 1024 in bf16 with gelu: this 38, 0.5 erfc(-z / sqrt 2) 55, 0.5 + 0.5 erf(z / sqrt 2)
+// 39, but that is off by 2^-24, not of the value: 4 % at z = -5.
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  constexpr float kCoefficients[] = {-0.0396009646f, 0.20060125f,  -0.373683333f, 0.250973463f,    -0.0123857474f,
+                                     0.158416525f,   0.155786633f, 0.159904182f,  -1.19874376e-05f};
+  const float t = __fdividef(1.f, fmaf(0.4f, fabsf(z), 1.f));
+  bell = __expf(__fmul_rn(-0.5f, __fmul_rn(z, z)));
+  float q = kCoefficients[0];
+#pragma unroll
+  for (int i = 1; i < 9; ++i) q = fmaf(q, t, kCoefficients[i]);
+  q = __fmul_rn(q, bell);
+  return z > 0.f ? __fsub_rn(1.f, q) : q;
+}
 // (Which activation is asked once for all values: asked for each, 4096 x 4096 x 1024 with silu took 65 us, without an activation 25.  Values are
 // rounded by themselves, not fused with what is added to them: every path of a product has the same bits.)
 template <int N>
@@ -135,7 +148,10 @@ __device__ __forceinline__ void activate(float (&z)[N], int activation) {
     for (int j = 0; j < N; ++j) z[j] = __fmul_rn(z[j], sigmoid_of(z[j]));
   } else if (activation == kGelu) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = __fmul_rn(z[j], normal_cdf(z[j]));
+    for (int j = 0; j < N; ++j) {
+      float bell;
+      z[j] = __fmul_rn(z[j], normal_cdf(z[j], bell));
+    }
   } else if (activation == kRelu) {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = z[j] < 0.f ? 0.f : z[j];  // NaN stays
