@@ -4,6 +4,7 @@
 #include <atomic>
 
 #include "matmul.cuh"
+#include "matmul_cost.h"
 #include "matmul_few.cuh"
 #include "tensor_map.h"
 
@@ -297,26 +298,6 @@ cudaError_t maps_of_rows(PairMaps* maps, const void* base, uint64_t rows, uint64
 }
 
 // ---- CTA pairs --------------------------------------------------------------------------------------------
-// What a product takes, in cycles beside the launch: an SM is fed by some 64 bytes a cycle from the L2 and computes a block of 64 of 256
-// features x n rows (a pair) in 2 n cycles; then the last tile's way out.
-int64_t block_cycles(int64_t n) { return n < 256 ? 256 + n : 2 * n; }
-// One group: result rows in tiles of equal height, so high that this is least over the rounds of CTA pairs.  Several groups: their
-// rows are only known on the device.
-struct PairCost {
-  int64_t cycles;
-  int steps;  // of a tile
-};
-PairCost pair_cost(int64_t rows, int step, int most_rows, int64_t tiles_p, int64_t k_blocks, int n_sm) {
-  const int64_t steps = (rows + step - 1) / step;
-  PairCost best{INT64_MAX, most_rows / step};
-  for (int s = most_rows / step; s >= 1; --s) {
-    const int64_t tiles = (steps + s - 1) / s, high = (steps + tiles - 1) / tiles, n = high * step;
-    const int64_t rounds = (tiles * tiles_p + n_sm / 2 - 1) / (n_sm / 2), cycles = rounds * (k_blocks * block_cycles(n) + 100) + 8 * n;
-    if (cycles < best.cycles) best = {cycles, (int)high};
-  }
-  return best;
-}
-
 // Of a weight's gradient: the groups' rows are what is summed, here as if they were equal.
 int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm, int most_rows) {
   return pair_cost(result_rows, kWeightStep, most_rows, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
@@ -471,8 +452,7 @@ cudaError_t few_cost(const Matmul& p, int device, FewCost* best) {
     for (int g = least_groups; g <= (m + 15) / 16 && g < least_groups + 8; ++g) {
       const int cols = ((m + g - 1) / g + 15) / 16 * 16, groups = (m + cols - 1) / cols;
       if ((int64_t)few_chains(cols, blocks, part) * part < blocks) continue;  // its parts would be longer than the pairs'
-      const int64_t rounds = ((int64_t)tiles * groups + fit - 1) / fit;
-      const int64_t cycles = rounds * (blocks * (256 + 2 * cols) + 10 * cols + (s > 1 ? 1500 + 2 * cols : 0));
+      const int64_t cycles = few_cycles((int64_t)tiles * groups, fit, blocks, cols, s);
       if (cycles < best->cycles) *best = {cycles, s, cols};
     }
   }
