@@ -25,9 +25,14 @@ using torch::autograd::variable_list;
 inline bool wants_grad(std::initializer_list<const Tensor*> tensors, const char* who) {
   for (const Tensor* t : tensors) check_no_tangent(*t, who);
   if (!at::GradMode::is_enabled()) return false;
-  bool wanted = false;
-  for (const Tensor* t : tensors) wanted = wanted || (t->defined() && t->requires_grad());
-  if (!wanted || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return wanted;
+  const Tensor* wanted = nullptr;
+  for (const Tensor* t : tensors)
+    if (wanted == nullptr && t->defined() && t->requires_grad()) wanted = t;
+  if (wanted == nullptr) return false;
+  {
+    c10::cuda::OptionalCUDAGuard guard(at::device_of(*wanted));  // the stream that the call will run on, whatever device is current
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return true;
+  }
   // leaves behind a weight's cast, a view or earlier operators too
   std::vector<std::shared_ptr<torch::autograd::Node>> held;  // leaves' own nodes, which nobody else may hold
   std::vector<torch::autograd::Node*> next;

@@ -16,7 +16,8 @@ bits, ``matmul_fp8``)::
 
 Every one but :func:`expert_order`, which has whole numbers alone, has a gradient; a gradient's gradient is refused, and so is a CUDA
 tensor with a forward-mode tangent.  CUDA tensors run on the native kernels, on the current stream of their device; CPU tensors on the plain statements in
-:mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph, backward passes too.  The same inputs give the same
+:mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph, backward passes too; inside a capture a call that is recorded is
+refused (``RuntimeError``) while a graph recorded on the default stream still holds one of its leaves.  The same inputs give the same
 bits.  Wrong arguments raise ``ValueError``.
 
 The reference has no operators of this kind.
