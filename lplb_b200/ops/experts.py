@@ -38,6 +38,19 @@ GATE_MAX_EXPERTS, GATE_MAX_TOPK = 1024, 32  #: experts and choices that gate_top
 ORDER_MAX_EXPERTS = 1024  #: experts that expert_order takes
 
 
+def _whole(n, who: str) -> int:
+    """``n`` as a whole number, which nothing is cut off to make."""
+    if type(n) is int and -(2**62) < n < 2**62:
+        return n
+    try:
+        whole = int(n)
+        if whole == n and -(2**63) <= whole < 2**63:
+            return whole
+    except (TypeError, ValueError, OverflowError):
+        pass
+    raise ValueError(f"lplb_b200.ops.{who} must be a whole number, not {n!r}")
+
+
 def _wants_grad(*tensors: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -90,9 +103,10 @@ def gate_topk(
     depend on it NaN.  Up to 1024 experts and 32 choices.  Differentiable with respect to ``logits``."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"lplb_b200.ops.gate_topk: score must be 'softmax' or 'sigmoid', not {score!r}")
+    topk = _whole(topk, "gate_topk: topk")
     if logits.is_cuda:
-        return _native().gate_topk(logits, int(topk), score == "sigmoid", bool(renormalize), float(scale))
-    who, topk, renormalize, scale = "gate_topk:", int(topk), bool(renormalize), float(scale)
+        return _native().gate_topk(logits, topk, score == "sigmoid", bool(renormalize), float(scale))
+    who, renormalize, scale = "gate_topk:", bool(renormalize), float(scale)
     _check_type(logits, f"{who} logits")
     _need(logits.dim() == 2, f"{who} logits must be [tokens, experts]")
     _need(1 <= logits.shape[1] <= GATE_MAX_EXPERTS, f"{who} 1 to {GATE_MAX_EXPERTS} experts")
@@ -116,7 +130,7 @@ def expert_order(idx: torch.Tensor, n_experts: int) -> ExpertOrder:
     gate's experts, or physical ones as the planner gives them).  Numbers outside ``[0, n_experts)``, -1 among them, choose
     nothing.  Up to 1024 experts and 1024 choices per token, fewer than 2**31 choices in all.  Nothing waits for the device:
     there are as many rows as choices, and those behind the last expert's are nobody's."""
-    n_experts = int(n_experts)
+    n_experts = _whole(n_experts, "expert_order: n_experts")
     if idx.is_cuda:
         return ExpertOrder(*_native().expert_order(idx, n_experts))
     who = "expert_order:"
