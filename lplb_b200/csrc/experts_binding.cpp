@@ -223,15 +223,15 @@ struct Gather : torch::autograd::Function<Gather> {
   }
 };
 
-Tensor take_rows(const Tensor& given, const Tensor& place, const Tensor& source) {
-  const Tensor x = as_stored(given);
+Tensor take_rows(const Tensor& given, const Tensor& given_place, const Tensor& given_source) {
+  const Tensor x = as_stored(given), place = in_a_row(given_place), source = in_a_row(given_source);
   if (!wants_grad({&x}, "take_rows")) return take_forward(x, place, source);
   type_of(x, "take_rows: x that requires a gradient");
   return TakeRows::apply(x, place, source);
 }
 
-Tensor combine_rows(const Tensor& given, const Tensor& place, const Tensor& source, const OptTensor& weights) {
-  const Tensor rows = as_stored(given);
+Tensor combine_rows(const Tensor& given, const Tensor& given_place, const Tensor& given_source, const OptTensor& weights) {
+  const Tensor rows = as_stored(given), place = in_a_row(given_place), source = in_a_row(given_source);
   if (!weights) return wants_grad({&rows}, "combine_rows") ? Gather::apply(rows, place, source) : combine_forward(rows, place, source, std::nullopt);
   OPS_CHECK(weights->is_floating_point(), "combine_rows: weights must be floating point [tokens, topk] on the rows' device");
   const Tensor w = as_stored(*weights).to(torch::kFloat32).contiguous();

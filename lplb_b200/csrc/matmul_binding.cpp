@@ -254,8 +254,9 @@ struct Product : torch::autograd::Function<Product> {
 };
 
 Tensor matmul(const Tensor& given_a, const Tensor& given_b, const OptTensor& given_bias, int64_t activation, const OptTensor& given_residual,
-              const OptTensor& rows, bool out_f32) {
+              const OptTensor& given_rows, bool out_f32) {
   const Tensor a = as_stored(given_a), b = as_stored(given_b);
+  const OptTensor rows = given_rows ? OptTensor(in_a_row(*given_rows)) : std::nullopt;
   const OptTensor bias = as_stored(given_bias), residual = as_stored(given_residual);
   const Tensor added = or_none(bias), carried = or_none(residual);
   if (wants_grad({&a, &b, &added, &carried}, "matmul")) return Product::apply(a, b, bias, residual, rows, activation, out_f32);

@@ -66,6 +66,9 @@ inline void check_no_grad(const Tensor& t, const char* who) {
 inline Tensor as_stored(const Tensor& t) { return t.defined() && (t.is_conj() || t.is_neg()) ? t.resolve_conj().resolve_neg() : t; }
 inline OptTensor as_stored(const OptTensor& t) { return t ? OptTensor(as_stored(*t)) : std::nullopt; }
 
+// Whole numbers that a kernel reads one after the other, as an order's and a call's counts are.
+inline Tensor in_a_row(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+
 inline int sm_count(int device) {
   int n = 0;
   OPS_CUDA(lplb::ops::multiprocessors(device, &n));

@@ -19,3 +19,27 @@ def test_numbers_that_are_not_whole(device):
     for good in (2, 2.0, torch.tensor(2), torch.tensor(2.0)):
         assert torch.equal(ops.gate_topk(x, good)[1], ops.gate_topk(x, 2)[1])
         assert torch.equal(ops.expert_order(idx, good).place, ops.expert_order(idx, 2).place)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_orders_and_counts_of_any_strides(device):
+    idx = torch.tensor([[0, 1], [2, -1], [1, 0]], device=device)
+    order = ops.expert_order(idx, 3)
+    apart = lambda t: torch.stack([t, torch.full_like(t, -7)], -1)[..., 0]  # noqa: E731
+    other = ops.ExpertOrder(*(apart(t) for t in order))
+    turned = ops.ExpertOrder(apart(order.counts), order.place.T.contiguous().T, order.source)
+    assert not any(t.is_contiguous() for t in (*other, turned.counts, turned.place))
+    g = torch.Generator().manual_seed(0)
+    normal = lambda *shape: torch.randn(*shape, generator=g).to(device)  # noqa: E731
+    x, w, b = normal(3, 16).bfloat16().requires_grad_(), normal(3, 2).requires_grad_(), normal(3, 24, 16).bfloat16()
+
+    def run(order, weights):
+        rows = ops.take_rows(x, order)
+        out = ops.combine_rows(ops.matmul(rows, b, rows=order.counts), order, weights)
+        return [out, *torch.autograd.grad(out.float().square().sum(), (x, w) if weights is not None else (x,))]
+
+    for weights in (w, None):
+        want = run(order, weights)
+        for these in (other, turned):
+            for got, right in zip(run(these, weights), want):
+                assert torch.equal(got, right)
