@@ -102,7 +102,7 @@ def _check(a, b, bias, activation, residual, rows, out_dtype, who):
     _need(m <= _MOST_ROWS and groups * n <= _MOST_ROWS, f"{who} at most {_MOST_ROWS} rows of a, and of all matrices of b together")
     _need(8 <= k <= 2**28 and k % 8 == 0 and b.shape[-1] == k, f"{who} a and b must have the same k, a multiple of 8")
     _need(1 <= n <= 2**28, f"{who} b has no rows, or too many")
-    _need(b.is_contiguous(), f"{who} b must be contiguous")
+    _need(b.is_contiguous() and b.data_ptr() % 16 == 0, f"{who} b must be contiguous and start on a 16-byte boundary")
     _need(activation != "swiglu" or n % 256 == 0, f"{who} 'swiglu' needs blocks of 128 gate rows and their 128 up rows: n must be a multiple of 256")
     _need(
         bias is None or (bias.dtype in (a.dtype, torch.float32) and bias.shape == b.shape[:-1]),

@@ -37,6 +37,8 @@ __all__ = ["GATE_MAX_EXPERTS", "GATE_MAX_TOPK", "ORDER_MAX_EXPERTS", "ExpertOrde
 GATE_MAX_EXPERTS, GATE_MAX_TOPK = 1024, 32  #: experts and choices that gate_topk takes
 ORDER_MAX_EXPERTS = 1024  #: experts that expert_order takes
 
+_MOST_VALUES = (2**31 - 1) // 16  # of a row
+
 
 def _whole(n, who: str) -> int:
     """``n`` as a whole number, which nothing is cut off to make."""
@@ -110,6 +112,7 @@ def gate_topk(
     _check_type(logits, f"{who} logits")
     _need(logits.dim() == 2, f"{who} logits must be [tokens, experts]")
     _need(1 <= logits.shape[1] <= GATE_MAX_EXPERTS, f"{who} 1 to {GATE_MAX_EXPERTS} experts")
+    _need(logits.shape[0] < 2**31, f"{who} fewer than 2^31 tokens")
     _need(1 <= topk <= min(GATE_MAX_TOPK, logits.shape[1]), f"{who} topk must be 1 to {GATE_MAX_TOPK}, and no more than there are experts")
     if _wants_grad(logits):
         return _GateTopk.apply(logits, topk, score, renormalize, scale)
@@ -137,6 +140,7 @@ def expert_order(idx: torch.Tensor, n_experts: int) -> ExpertOrder:
     _need(idx.dim() == 2 and idx.dtype in (torch.int64, torch.int32), f"{who} idx must be [tokens, topk] of int64 or int32")
     _need(1 <= n_experts <= ORDER_MAX_EXPERTS, f"{who} 1 to {ORDER_MAX_EXPERTS} experts")
     _need(1 <= idx.shape[1] <= 1024, f"{who} 1 to 1024 choices per token")
+    _need(idx.numel() < 2**31, f"{who} fewer than 2^31 choices in all")
     return ExpertOrder(*reference.expert_order_reference(idx, n_experts))
 
 
@@ -184,11 +188,12 @@ class _CombineRows(torch.autograd.Function):
 
 def take_rows(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """``rows`` ``[tokens * topk, values]``, contiguous: ``rows[order.place[t, k]] = x[t]``; rows behind the last
-    expert's are zero.  ``x`` is ``[tokens, values]`` of any type, values in 8 bits and their scales among them; rows may be apart
-    from one another.  Differentiable for float32, bfloat16 and float16: ``dx[t]`` is the sum of its rows' gradients, in 32 bits."""
+    expert's are zero.  ``x`` is ``[tokens, values]`` of any type, values in 8 bits and their scales among them, of up to (2**31 - 1) //
+    16 values; rows may be apart from one another.  Differentiable for float32, bfloat16 and float16: ``dx[t]`` is the sum of its rows' gradients, in 32 bits."""
     if x.is_cuda:
         return _native().take_rows(x, order.place, order.source)
-    _need(x.dim() == 2 and x.shape[1] >= 1, "take_rows: x must be [tokens, values]")
+    _need(x.dim() == 2, "take_rows: x must be [tokens, values]")
+    _need(1 <= x.shape[1] <= _MOST_VALUES, "take_rows: rows without values, or too long")
     _check_order(x, order, "take_rows:")
     _need(order.place.shape[0] == x.shape[0], "take_rows: x must have a row for each of the order's tokens")
     if _wants_grad(x):
@@ -207,7 +212,8 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: torch.Tensor |
         return _native().combine_rows(rows, order.place, order.source, weights)
     who = "combine_rows:"
     _check_type(rows, f"{who} rows")
-    _need(rows.dim() == 2 and rows.shape[1] >= 1, f"{who} rows must be [tokens * topk, values]")
+    _need(rows.dim() == 2, f"{who} rows must be [tokens * topk, values]")
+    _need(1 <= rows.shape[1] <= _MOST_VALUES, f"{who} rows without values, or too long")
     _check_device(who, rows, weights)
     _check_order(rows, order, who)
     _need(rows.shape[0] == order.place.numel(), f"{who} rows must have one for each of the order's choices")

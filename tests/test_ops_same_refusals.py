@@ -43,3 +43,21 @@ def test_orders_and_counts_of_any_strides(device):
         for these in (other, turned):
             for got, right in zip(run(these, weights), want):
                 assert torch.equal(got, right)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_boundaries_and_lengths(device):
+    a = torch.zeros(4, 16, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError, match="16-byte"):
+        ops.matmul(a, torch.zeros(129, dtype=torch.bfloat16, device=device)[1:].view(8, 16))
+    order = ops.expert_order(torch.tensor([[0]], device=device), 1)
+    long = torch.zeros(1, 1, device=device).expand(1, 2**27)
+    with pytest.raises(ValueError, match="too long"):
+        ops.take_rows(long, order)
+    with pytest.raises(ValueError, match="too long"):
+        ops.combine_rows(long, order)
+    many = torch.zeros(1, 1, device=device)
+    with pytest.raises(ValueError, match="fewer than"):
+        ops.gate_topk(many.expand(2**31, 1), 1)
+    with pytest.raises(ValueError, match="fewer than"):
+        ops.expert_order(many.long().expand(2**21, 1024), 1)
