@@ -322,6 +322,7 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
   const int out_cols = MODE == kForwardGated ? a.features / 2 : a.features;
   a.plain = a.e.type != Type::kF32 && a.e.residual_ld % 8 == 0 && address(a.e.residual) % 16 == 0 && address(a.e.pre) % 32 == 0 && a.e.pre_ld % 8 == 0 && out_cols % 8 == 0 && a.e.out_ld % 8 == 0 && address(a.e.out) % 16 == 0;
+  if (MODE > kForwardGated && !(a.wide && a.plain)) return cudaErrorMisalignedAddress;
   const int most_rows = IN_32 ? kSumRows : kPairN;
   a.tile_steps = most_rows / PairTile<MODE>::kStep;
   if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm, most_rows);
@@ -626,7 +627,7 @@ cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t s
 int64_t matmul_weight_copies(const MatmulWeight& p) { return p.rows != nullptr ? weight_copies(p).bytes : 0; }
 
 cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t stream) {
-  if (refused(p.m, p.n, p.k, p.groups, device) || p.k % 8 || p.dz_ld % 8) return cudaErrorInvalidValue;
+  if (refused(p.m, p.n, p.k, p.groups, device) || p.m < 1 || p.k % 8 || p.dz_ld % 8) return cudaErrorInvalidValue;
   PairArgs a{};
   a.rows = p.rows;
   a.groups = p.rows ? p.groups : 1;
@@ -654,36 +655,35 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
   // One group: its length is known.  Several: a launch for those of up to `longest` rows, and where there may be longer ones, one for them.
   const int longest = longest_part(p.type);
   const bool may_be_long = p.m > longest, all_long = may_be_long && p.rows == nullptr;
-  if (p.m > 0) {  // (without a row there is nothing to load: every matrix is cleared)
-    int n_sm = 0;
-    cudaError_t err = multiprocessors(device, &n_sm);
-    const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm, kPairN);
-    a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
-    if (err == cudaSuccess) err = map(&maps.p[0], a.p_chunks, p.a, p.m, p.k, p.a_ld);
-    if (err == cudaSuccess) err = map_q(!all_long && p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1);  // 2: every tile has 256 result rows
-    if (p.rows != nullptr) {
-      if (p.copies == nullptr) return cudaErrorInvalidValue;
-      a.copies = 1;
-      if (err == cudaSuccess) err = map(&maps.p[1], a.p_chunks, p.copies, (int64_t)a.groups * kPairK, p.k, c.a_ld);
-      LastBlocks l{};
-      l.from[0] = p.a, l.from[1] = p.dz;
-      l.to[0] = p.copies, l.to[1] = of_dz;
-      l.from_ld[0] = p.a_ld * 2, l.from_ld[1] = p.dz_ld * 2;
-      l.to_ld[0] = c.a_ld * 2, l.to_ld[1] = c.dz_ld * 2;
-      l.words[0] = (int)(c.a_ld / 8), l.words[1] = (int)(c.dz_ld / 8);
-      l.bytes[0] = p.k * 2, l.bytes[1] = p.n * 2;
-      l.rows = p.rows;
-      l.groups = a.groups;
-      l.m = (int)p.m;
-      const int words = l.words[0] + l.words[1];
-      auto kernel = last_blocks_kernel;
-      if (err == cudaSuccess) err = launch_after(kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
-    }
-    if (err != cudaSuccess) return err;
+  int n_sm = 0;
+  cudaError_t err = multiprocessors(device, &n_sm);
+  if (err != cudaSuccess) return err;
+  const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm, kPairN);
+  a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
+  err = map(&maps.p[0], a.p_chunks, p.a, p.m, p.k, p.a_ld);
+  if (err == cudaSuccess) err = map_q(!all_long && p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1);  // 2: every tile has 256 result rows
+  if (p.rows != nullptr) {
+    if (p.copies == nullptr) return cudaErrorInvalidValue;
+    a.copies = 1;
+    if (err == cudaSuccess) err = map(&maps.p[1], a.p_chunks, p.copies, (int64_t)a.groups * kPairK, p.k, c.a_ld);
+    LastBlocks l{};
+    l.from[0] = p.a, l.from[1] = p.dz;
+    l.to[0] = p.copies, l.to[1] = of_dz;
+    l.from_ld[0] = p.a_ld * 2, l.from_ld[1] = p.dz_ld * 2;
+    l.to_ld[0] = c.a_ld * 2, l.to_ld[1] = c.dz_ld * 2;
+    l.words[0] = (int)(c.a_ld / 8), l.words[1] = (int)(c.dz_ld / 8);
+    l.bytes[0] = p.k * 2, l.bytes[1] = p.n * 2;
+    l.rows = p.rows;
+    l.groups = a.groups;
+    l.m = (int)p.m;
+    const int words = l.words[0] + l.words[1];
+    auto kernel = last_blocks_kernel;
+    if (err == cudaSuccess) err = launch_after(kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
   }
+  if (err != cudaSuccess) return err;
   if (all_long) return launch_pairs<kWeight, true>(maps, a, device, stream);
   a.long_sum = may_be_long ? longest : 0;
-  cudaError_t err = launch_pairs<kWeight>(maps, a, device, stream);
+  err = launch_pairs<kWeight>(maps, a, device, stream);
   if (err != cudaSuccess || !may_be_long) return err;
   if ((err = map_q(1)) != cudaSuccess) return err;
   return launch_pairs<kWeight, true>(maps, a, device, stream);

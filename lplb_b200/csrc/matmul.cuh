@@ -479,7 +479,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     const int64_t cta = blockIdx.x, ctas = gridDim.x;
     const int out_cols = kGated ? a.features / 2 : a.features;
     auto clear_row = [&](int64_t row) {
-      if (a.wide) {
+      if (MODE > kForwardGated || a.wide) {
         for (int c = 4 * et; c < out_cols; c += 4 * 32 * kStoreWarps) {
           float v[4] = {0.f, 0.f, 0.f, 0.f};
           if (e.residual != nullptr) load4<1>(e.residual, e.type, row * e.residual_ld + c, 4, v);
@@ -784,13 +784,15 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
         }
       }
     };
-    if (!IN_32 && a.plain) {
+    // (The gradients' rows are always of whole words on boundaries.)
+    if (!IN_32 && (MODE > kForwardGated || a.plain)) {
       if (e.type == Type::kBf16) plain(std::true_type{});
       else plain(std::false_type{});
-    } else if (a.wide) {
-      full(std::true_type{});
-    } else {
-      full(std::false_type{});
+    } else if (IN_32 || MODE <= kForwardGated) {
+      if constexpr (IN_32 || MODE <= kForwardGated) {
+        if (MODE > kForwardGated || a.wide) full(std::true_type{});
+        else if constexpr (MODE <= kForwardGated) full(std::false_type{});
+      }
     }
   }
 

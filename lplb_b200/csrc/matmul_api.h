@@ -48,7 +48,7 @@ struct MatmulInput {
 };
 cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t stream);
 
-// db[e] = dz_e^T @ a_e over the rows of group e: [groups, n, k] of the type
+// db[e] = dz_e^T @ a_e over the rows of group e: [groups, n, k] of the type; there is a row at least
 struct MatmulWeight {
   const void* dz;  // [m, n], row stride dz_ld
   const uint32_t* most;  // [groups, n], or null

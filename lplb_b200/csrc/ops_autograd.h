@@ -63,7 +63,6 @@ inline bool wants_grad(std::initializer_list<const Tensor*> tensors, const char*
 }
 inline Tensor or_none(const OptTensor& t) { return t ? *t : Tensor(); }
 inline OptTensor or_none(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
-inline py::object given(const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); }
 
 // Gradients as a backward pass returns them.  A pass that is itself recorded (create_graph=True) gets ones that refuse to be
 // differentiated: these operators' gradients have none.

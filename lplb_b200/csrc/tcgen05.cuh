@@ -200,9 +200,7 @@ __device__ __forceinline__ void mbar_arrive_remote_fenced(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // An arrival that hands nothing in memory over: it says that this thread's tcgen05.ld have returned (tcgen05.wait::ld).
-__device__ __forceinline__ void mbar_arrive_remote_read(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
+__device__ __forceinline__ void mbar_arrive_remote_read(uint32_t bar) { mbar_arrive_remote_fenced(bar); }
 
 // ---- tensor memory -----------------------------------------------------------------------------
 // Whole-warp calls, one warp in each CTA of the pair.  `slot` is a shared-memory word that
