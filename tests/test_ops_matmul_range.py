@@ -140,3 +140,55 @@ def test_the_ends_of_32_bits(dout, device):
     want[0, 0], want[1, 0] = d[0, 0].half(), 1.0
     assert torch.equal(got["a"], want)
     assert torch.equal(got["b"], (d[0, 0].double() + 1).half().expand(5, 8).to(device))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [None, [100, 0, 1, 150, 40]])
+def test_captured_and_on_several_streams(groups):
+    """What the parts are taken of is found anew by every replay, and shared by no two calls."""
+    names = ("a", "b", "bias")
+
+    def make(seed, by):
+        args, dout = _make("rows", 300, 512, 136, groups, seed)
+        lead = () if groups is None else (len(groups),)
+        args = {**args, "activation": "silu", "bias": torch.zeros(*lead, 512)}
+        return {name: t.cuda() if isinstance(t, torch.Tensor) else t for name, t in args.items()}, by * dout.cuda()
+
+    args, dout = make(1, 1.0)
+    _gradients(args, dout, names)
+    leaves = {name: args[name].clone().requires_grad_() for name in names}
+    held = dout.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(ops.matmul(**{**args, **leaves}), tuple(leaves.values()), held)
+    cases = [make(seed, by) for seed, by in ((2, 2.0**-8), (3, 2.0**8), (4, 0.0), (5, 2.0**-8))]
+    alone = [_gradients(*case, names) for case in cases]
+    for (fresh, d), want in zip(cases, alone):
+        with torch.no_grad():
+            for name in names:
+                leaves[name].copy_(fresh[name])
+            held.copy_(d)
+        graph.replay()
+        for got, name in zip(grads, names):
+            assert torch.equal(got, want[name]), name
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        together = []
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                together.append(_gradients(*case, names))
+        torch.cuda.synchronize()
+        for got, want in zip(together, alone):
+            assert all(torch.equal(got[name], want[name]) for name in names)
+    assert ops.check() == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_bias_alone(device):
+    args, dout = _make("large", 70, 256, 64, None, 1)
+    args = {name: t.to(device) if isinstance(t, torch.Tensor) else t for name, t in args.items()} | {"bias": torch.zeros(256, device=device)}
+    both, alone = _gradients(args, dout.to(device), ("a", "b", "bias")), _gradients(args, dout.to(device), ("bias",))
+    assert torch.equal(alone["bias"], both["bias"])
+    off = (alone["bias"].double() - dout.to(device).double().sum(0)).abs()
+    assert (off <= 70 * 2.0**-24 * dout.to(device).double().abs().sum(0)).all()
