@@ -308,8 +308,8 @@ cudaError_t maps_of_rows(PairMaps* maps, const void* base, uint64_t rows, uint64
 
 // ---- CTA pairs --------------------------------------------------------------------------------------------
 // Of a weight's gradient: the groups' rows are what is summed, here as if they were equal.
-int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm, int most_rows) {
-  return pair_cost(result_rows, kWeightStep, most_rows, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
+int weight_steps(int64_t result_rows, int64_t rows, int groups, int64_t tiles_p, int n_sm) {
+  return pair_cost(result_rows, kWeightStep, kPairN, tiles_p * groups, (rows / groups + kPairK - 1) / kPairK, n_sm).steps;
 }
 
 template <Mode MODE, bool IN_32 = false>
@@ -326,6 +326,7 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   }
   if ((err = ops_error_word(device, &a.status)) != cudaSuccess) return err;
   a.budget_ns = wait_budget_ns();
+  a.part_blocks = longest_part(a.e.type) / kPairK;
   if (a.p_chunks == 0) a.p_chunks = 1;
   if (a.q_chunks == 0) a.q_chunks = 1;
   a.tiles_p = (a.features + kPairM - 1) / kPairM;
@@ -334,7 +335,7 @@ cudaError_t launch_pairs(const PairMaps& maps, PairArgs& a, int device, cudaStre
   if (MODE > kForwardGated && !(a.wide && a.plain)) return cudaErrorMisalignedAddress;
   const int most_rows = IN_32 ? kSumRows : kPairN;
   a.tile_steps = most_rows / PairTile<MODE>::kStep;
-  if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm, most_rows);
+  if (MODE == kWeight) a.tile_steps = weight_steps(a.result_rows, a.n_rows, a.groups, a.tiles_p, n_sm);
   else if (a.rows == nullptr) a.tile_steps = pair_cost(a.n_rows, PairTile<MODE>::kStep, most_rows, a.tiles_p, a.k_blocks, n_sm).steps;
   return launch_after(kernel, dim3(n_sm & ~1), dim3(kPairThreads), kPairSmem, stream, maps, a);
 }
@@ -359,9 +360,9 @@ int is_wide(const Matmul& p) {
          fours(p.bias, p.n, p.bias_type);
 }
 
-// Whether the sum is longer than one part.  us, sums of one part in tiles of up to 256 rows and in registers, results in 32 bits: 600 x 4096 x 512
-// 9.7, 13.1; 8192 x 1000 x 512 18.0, 24.2.
-bool sums_in_parts(const Matmul& p) { return p.k > longest_part(p.out_type); }
+// A result in 32 bits whose sum is longer than one part.  us, sums of one part in tiles of up to 256 rows and in registers: 600 x 4096 x 512 9.7,
+// 13.1; 8192 x 1000 x 512 18.0, 24.2.
+bool sums_in_parts(const Matmul& p) { return p.out_type == Type::kF32 && p.k > longest_part(p.out_type); }
 
 cudaError_t launch_forward(const Matmul& p, int device, cudaStream_t stream) {
   PairMaps maps{};
@@ -629,8 +630,7 @@ cudaError_t launch_matmul_input(const MatmulInput& p, int device, cudaStream_t s
   cudaError_t err = maps_of_rows(&maps, p.dz, p.m, p.n, p.dz_ld);
   a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
   if (err == cudaSuccess) err = a.p_chunks == 2 ? map_chunks(&maps.p[0], p.b, a.groups, p.n, p.k) : map_3d(&maps.p[0], p.b, a.groups, p.n, p.k, kPairK);
-  if (err != cudaSuccess) return err;
-  return p.n > longest_part(p.type) ? launch_pairs<kInput, true>(maps, a, device, stream) : launch_pairs<kInput>(maps, a, device, stream);
+  return err != cudaSuccess ? err : launch_pairs<kInput>(maps, a, device, stream);
 }
 
 int64_t matmul_weight_copies(const MatmulWeight& p) { return p.rows != nullptr ? weight_copies(p).bytes : 0; }
@@ -656,25 +656,19 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
   auto map = [](CUtensorMap* m, int chunks, const void* base, int64_t rows, int64_t cols, int64_t ld) {
     return chunks == 2 ? map_chunks(m, base, rows, cols, ld, kPairK) : map_2d(m, base, rows, cols, ld, kPairK);
   };
-  auto map_q = [&](int chunks) {
-    a.q_chunks = chunks;
-    const cudaError_t err = map(&maps.q[0], chunks, p.dz, p.m, p.n, p.dz_ld);
-    return err != cudaSuccess || p.rows == nullptr ? err : map(&maps.q[1], chunks, of_dz, (int64_t)a.groups * kPairK, p.n, c.dz_ld);
-  };
-  // One group: its length is known.  Several: a launch for those of up to `longest` rows, and where there may be longer ones, one for them.
-  const int longest = longest_part(p.type);
-  const bool may_be_long = p.m > longest, all_long = may_be_long && p.rows == nullptr;
   int n_sm = 0;
   cudaError_t err = multiprocessors(device, &n_sm);
   if (err != cudaSuccess) return err;
-  const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm, kPairN);
+  const int steps = weight_steps(p.n, p.m, a.groups, (p.k + kPairM - 1) / kPairM, n_sm);
   a.p_chunks = p.k % kChunk == 0 && p.k > kChunk ? 2 : 1;
+  a.q_chunks = p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1;  // every tile has 256 result rows
   err = map(&maps.p[0], a.p_chunks, p.a, p.m, p.k, p.a_ld);
-  if (err == cudaSuccess) err = map_q(!all_long && p.n % kPairN == 0 && steps == kPairN / kWeightStep ? 2 : 1);  // 2: every tile has 256 result rows
+  if (err == cudaSuccess) err = map(&maps.q[0], a.q_chunks, p.dz, p.m, p.n, p.dz_ld);
   if (p.rows != nullptr) {
     if (p.copies == nullptr) return cudaErrorInvalidValue;
     a.copies = 1;
     if (err == cudaSuccess) err = map(&maps.p[1], a.p_chunks, p.copies, (int64_t)a.groups * kPairK, p.k, c.a_ld);
+    if (err == cudaSuccess) err = map(&maps.q[1], a.q_chunks, of_dz, (int64_t)a.groups * kPairK, p.n, c.dz_ld);
     LastBlocks l{};
     l.from[0] = p.a, l.from[1] = p.dz;
     l.to[0] = p.copies, l.to[1] = of_dz;
@@ -689,13 +683,7 @@ cudaError_t launch_matmul_weight(const MatmulWeight& p, int device, cudaStream_t
     auto kernel = last_blocks_kernel;
     if (err == cudaSuccess) err = launch_after(kernel, dim3((words + 255) / 256, a.groups, 4), dim3(256), 0, stream, l);
   }
-  if (err != cudaSuccess) return err;
-  if (all_long) return launch_pairs<kWeight, true>(maps, a, device, stream);
-  a.long_sum = may_be_long ? longest : 0;
-  err = launch_pairs<kWeight>(maps, a, device, stream);
-  if (err != cudaSuccess || !may_be_long) return err;
-  if ((err = map_q(1)) != cudaSuccess) return err;
-  return launch_pairs<kWeight, true>(maps, a, device, stream);
+  return err != cudaSuccess ? err : launch_pairs<kWeight>(maps, a, device, stream);
 }
 
 cudaError_t matmul_pre_parts(const MatmulPre& p, int device, int64_t* floats, int* splits) {

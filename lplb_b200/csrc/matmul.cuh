@@ -231,13 +231,13 @@ constexpr int kPairThreads = 64 + 32 * kStoreWarps, kPairColumns = 512;
 // 6e-9 of it per product (3e-6 over 512, 1.0e-4 over 16,384, 6.7e-3 over 2^20, measured), one of either sign less, 7e-6 over 7168, where sums in 32
 // bits that are rounded are off by 1e-6.  A result in 32 bits shows that, so its sum is taken over `kSumBlocks` blocks at a time in tensor
 // memory, and these sums are added in registers (either sign: off by 5e-7 whatever the length).  A result in 16 bits hides it behind its
-// rounding up to `longest_part` products; longer sums go the same way as a result in 32 bits.
+// rounding up to `longest_part` products; of longer sums the parts are added in tensor memory, in the accumulator that is not summed into.
 // Tiles of at most `kSumRows` result rows: a thread holds half of them.  8192 x 4096 x 7168 in 450-500 us (16 bits 340-370),
 // 1001 x 4100 x 2064 in 24.3 (20.7); blocks of 4 541 and 25.9; 192 rows, whose sums do not fit the registers, 612 and 37.8.
 constexpr int kSumBlocks = 8, kSumRows = 128;
-// Products of one accumulator for a result of the type: what is cut off is at most a fifth of half a step (2^-11 and 2^-8).  It also keeps the
+// Products of one accumulator for a result of the type: what is cut off is at most a tenth of half a step (2^-11 and 2^-8).  It also keeps the
 // epilogue's wait for a sum far below its limit.
-constexpr int longest_part(Type type) { return type == Type::kF32 ? kSumBlocks * kPairK : type == Type::kF16 ? 16384 : 131072; }
+constexpr int longest_part(Type type) { return type == Type::kF32 ? kSumBlocks * kPairK : type == Type::kF16 ? 8192 : 65536; }
 
 struct PairMaps {
   CUtensorMap p[2], q[kBoxes];  // P: the first only, but for kWeight
@@ -253,7 +253,7 @@ struct PairArgs {
   int tile_steps;   // result rows of a tile at most, in steps
   int p_chunks, q_chunks;  // chunks of an MN-major operand that a box holds: 2 where columns come in whole chunks (q: and a CTA has two)
   int copies;       // kWeight: the last blocks of groups have been copied
-  int long_sum;     // kWeight: groups of more rows are left to the launch that sums in parts, and it has them alone; 0: all groups are this launch's
+  int part_blocks;  // of a sum, for one accumulator
   int wide;         // four neighbouring values of everything in the epilogue start on a boundary of their size
   int plain;        // a result in 16 bits, rows (the residual's too) of whole 16-byte words on boundaries
   uint32_t idesc;
@@ -290,7 +290,10 @@ struct PairTile {
 // it turns 32 features x 32 result rows round in shared memory of its own.  Two accumulators: the epilogue of a tile runs beside the
 // sums of the next.  (With four warps that met at a barrier every 16 rows a weight's gradient of 32 experts, 512 rows each on average,
 // 4096 x 7168, took 3070 us: its tiles have 8 blocks to sum, and 1750 cycles went into every 16 rows.)
-// IN_32: summed in parts, as a result in 32 bits is.
+// Of a sum that is longer than one part the parts come one after the other in the tile's accumulator, and their sum stays in the other one, of
+// which every epilogue warp reads and writes what is its own alone.  So the tiles keep their height: the input's gradient of 1024 x 151936 x 4096
+// takes 847 us in three parts, 844 in one, and in IN_32's way 1.5 times that.  IN_32, a result in 32 bits: parts so short
+// that they alternate between the accumulators, and are added in registers.
 template <Mode MODE, bool IN_32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
@@ -339,8 +342,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
       }
       if (e < a.groups) {
         const int from = (int)min((long long)a.n_rows, before + scan - mine), to = (int)min((long long)a.n_rows, before + scan);
-        const bool others = MODE == kWeight && a.long_sum > 0 && (to - from > a.long_sum) != IN_32;
-        s_rows[e] = others ? -1 : to - from;  // (neither summed nor cleared)
+        s_rows[e] = to - from;
         s_start[e] = from;
         s_start[e + 1] = to;  // (also written, the same, by the next lane)
       }
@@ -429,17 +431,18 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   } else if (warp == 1) {
     // ---------------- matrix instructions, for both CTAs ----------------
     if (half == 0 && elect_one()) {
-      uint32_t s = 0, ph = 0, part = 0;  // part: sums handed to the epilogue, one per tile but for IN_32
+      uint32_t s = 0, ph = 0, acc = 0, used = 0;  // used: a bit per accumulator, turned over by every sum that is handed to the epilogue
+      const int part_blocks = IN_32 ? kSumBlocks : a.part_blocks;
       for (uint32_t i = 0; find(i) && !*abort; ++i) {
         const uint32_t idesc = a.idesc | umma_idesc_size(kPairM, cur.n);
         const int blocks = blocks_of();
         bool ok = true;
         uint32_t tmem_d = 0;
-        for (int kb = 0; kb < blocks; ++kb) {
-          const bool first = kb == 0 || (IN_32 && kb % kSumBlocks == 0), last = kb == blocks - 1 || (IN_32 && kb % kSumBlocks == kSumBlocks - 1);
-          const uint32_t acc = part & 1;
+        for (int kb = 0, in_part = 0; kb < blocks; ++kb) {
+          const bool first = in_part == 0, last = kb == blocks - 1 || in_part == part_blocks - 1;
+          in_part = last ? 0 : in_part + 1;
           if (first) {
-            if (!mbar_wait(bar_tempty + 8 * acc, ((part >> 1) & 1) ^ 1, abort, budget)) {
+            if (!mbar_wait(bar_tempty + 8 * acc, ((used >> acc) & 1) ^ 1, abort, budget)) {
               ok = false;
               break;
             }
@@ -462,10 +465,13 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           if (++s == stages) s = 0, ph ^= 1;
           if (last) {
             umma_pair_commit(bar_tfull + 8 * acc);
-            ++part;
+            used ^= 1u << acc;
+            if (IN_32) acc ^= 1;
           }
         }
         if (!ok) break;
+        // (Behind a long sum its accumulator is next again: it is given back once the sum of the parts has been read, too.)
+        if (!IN_32 && blocks <= part_blocks) acc ^= 1;
       }
     }
   } else {
@@ -497,20 +503,21 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     } else {
       for (int64_t r = s_start[a.groups] + cta; r < a.n_rows; r += ctas) clear_row(r);
     }
-    uint32_t part = 0;  // as the matrix instructions' side counts
+    uint32_t acc = 0, used = 0;  // as the matrix instructions' side counts
     const uint32_t lead_tempty = map_to_rank(bar_tempty, 0);
     auto await = [&]() {  // the next accumulator's sums, all of the warp together
-      if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * (part & 1), (part >> 1) & 1, abort, budget))) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, (used >> acc) & 1, abort, budget))) return false;
       tc_fence_after_sync();
       return true;
     };
     // The accumulator has been read: tcgen05.wait::ld has returned, and nothing else is handed over.  So the arrival does not release: at
     // cluster scope that waits for the thread's loads and stores under way, some 1500 cycles each time.
-    auto release = [&]() {
+    auto release = [&](bool to_other) {  // to_other: the next sum is the other accumulator's
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote_read(lead_tempty + 8 * (part & 1));
-      ++part;
+      if (lane == 0) mbar_arrive_remote_read(lead_tempty + 8 * acc);
+      used ^= 1u << acc;
+      acc ^= to_other;
     };
     const uint32_t tmem_mine = tmem_base + ((uint32_t)(quarter * 32) << 16);
     int n = 0;           // result rows of the tile that are there
@@ -520,6 +527,31 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
       n = min(cur.n, (MODE == kWeight ? a.result_rows : s_rows[cur.group]) - cur.row0);
       row0 = (MODE == kWeight ? (int64_t)cur.group * a.result_rows : (int64_t)s_start[cur.group]) + cur.row0;
       return true;
+    };
+
+    // The next accumulator's sums; before the last part of a long sum those of the parts before are added up beside it.
+    bool is_long = false;
+    auto await_last = [&]() {
+      const int blocks = blocks_of();
+      is_long = blocks > a.part_blocks;
+      for (int done = 0; done + a.part_blocks < blocks; done += a.part_blocks) {
+        if (!await()) return false;
+        for (int c = 32 * which; c < n; c += (c & 16) ? 48 : 16) {
+          float v[16], before[16];
+          __syncwarp();
+          tmem_ld_32x16(tmem_mine + acc * kPairN + c, v);
+          if (done > 0) tmem_ld_32x16(tmem_mine + (acc ^ 1) * kPairN + c, before);
+          tmem_ld_wait();
+          if (done > 0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += before[j];
+          }
+          tmem_st_32x16(tmem_mine + (acc ^ 1) * kPairN + c, v);
+        }
+        tmem_st_wait();
+        release(false);
+      }
+      return await();
     };
 
     // A result in 16 bits: bias, activation and residual on the matrix fragments, turned round by stmatrix, stored by 16 bytes.  The residual
@@ -605,14 +637,24 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
           }
         };
         fetch(32 * which);
-        if (!await()) break;
+        if (!await_last()) break;
         for (int c0 = 32 * which; c0 < n; c0 += 64) {
           // fragments: lanes l/4 and l/4 + 8 of a 16-lane half, result rows 8j + 2(l%4) and the next
           uint32_t raw[2][16];
           __syncwarp();
-          tmem_ld_16x32(tmem_mine + (part & 1) * kPairN + c0, raw[0]);
-          tmem_ld_16x32(tmem_mine + (16u << 16) + (part & 1) * kPairN + c0, raw[1]);
+          tmem_ld_16x32(tmem_mine + acc * kPairN + c0, raw[0]);
+          tmem_ld_16x32(tmem_mine + (16u << 16) + acc * kPairN + c0, raw[1]);
           tmem_ld_wait();
+          if (is_long) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t before[16];
+              tmem_ld_16x32(tmem_mine + (h * 16u << 16) + (acc ^ 1) * kPairN + c0, before);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) raw[h][j] = __float_as_uint(__uint_as_float(raw[h][j]) + __uint_as_float(before[j]));
+            }
+          }
           float v[2][16];
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -668,7 +710,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
             if (c0 + r < n && inside) *reinterpret_cast<uint4*>(out + (row0 + c0 + r) * e.out_ld) = w;
           }
         }
-        release();
+        release(!is_long);
       }
     };
 
@@ -727,18 +769,13 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
               z[j] = from[j * S];
               up[j] = kGated ? from[16 + j * S] : 0.f;
             }
-            if (MODE > kForwardGated && e.most != nullptr) {
-              const float whole = whole_of(e.most[row0 + at]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) z[j] *= whole;
-            }
             mine.finish(e, row0 + at, z, up, r[q]);
           }
         };
         if constexpr (IN_32) {
           constexpr int kBlocks = kSumRows / 64;
           float sum[kBlocks][2][16];  // this warp's 32 result rows of every 64
-          const int parts = (blocks_of() + kSumBlocks - 1) / kSumBlocks;
+          const int parts = (a.k_blocks + kSumBlocks - 1) / kSumBlocks;
           bool ok = true;
           for (int p = 0; p < parts; ++p) {
             if (!(ok = await())) break;
@@ -749,13 +786,13 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
               for (int h = 0; h < 2; ++h) {
                 float v[16];
                 __syncwarp();
-                tmem_ld_32x16(tmem_mine + (part & 1) * kPairN + 32 * which + 64 * c + 16 * h, v);
+                tmem_ld_32x16(tmem_mine + acc * kPairN + 32 * which + 64 * c + 16 * h, v);
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) sum[c][h][j] = p == 0 ? v[j] : sum[c][h][j] + v[j];
               }
             }
-            release();
+            release(true);
           }
           if (!ok) break;
 #pragma unroll 1
@@ -769,18 +806,25 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
             });
           }
         } else {
-          if (!await()) break;
+          if (!await_last()) break;
           for (int c0 = 32 * which; c0 < n; c0 += 64)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (c0 + 16 * h >= n) continue;
               float v[16];
               __syncwarp();
-              tmem_ld_32x16(tmem_mine + (part & 1) * kPairN + c0 + 16 * h, v);
+              tmem_ld_32x16(tmem_mine + acc * kPairN + c0 + 16 * h, v);
               tmem_ld_wait();
+              if (is_long) {
+                float before[16];
+                tmem_ld_32x16(tmem_mine + (acc ^ 1) * kPairN + c0 + 16 * h, before);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += before[j];
+              }
               finish16(c0 + 16 * h, [&] { turn16(v); });
             }
-          release();
+          release(!is_long);
         }
       }
     };
@@ -788,11 +832,9 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     if (!IN_32 && (MODE > kForwardGated || a.plain)) {
       if (e.type == Type::kBf16) plain(std::true_type{});
       else plain(std::false_type{});
-    } else if (IN_32 || MODE <= kForwardGated) {
-      if constexpr (IN_32 || MODE <= kForwardGated) {
-        if (MODE > kForwardGated || a.wide) full(std::true_type{});
-        else if constexpr (MODE <= kForwardGated) full(std::false_type{});
-      }
+    } else if constexpr (MODE <= kForwardGated) {
+      if (a.wide) full(std::true_type{});
+      else full(std::false_type{});
     }
   }
 

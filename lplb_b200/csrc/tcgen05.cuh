@@ -344,6 +344,17 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
       : "memory");
 }
 
+// The way back: thread l's values to lane l.
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]),
+        "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // 16 TMEM lanes x 32 fp32 columns (warp w may only touch lanes 32*(w%4) .. 32*(w%4)+31; the lane
 // field of `taddr` selects the first 16 or the last 16 of them).  Thread l receives, for j = 0..3,
 // v[4j], v[4j+1] = lane l/4, columns 8j + 2(l%4) and the next; v[4j+2], v[4j+3] = lane l/4 + 8.

@@ -9,8 +9,8 @@ from lplb_b200 import ops
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
 # A result is off by half a step of its type, and by what its sum is off: 6e-9 of it per product that the tensor cores add up, products of
-# one sign, so 1.0e-4 for the parts of 16384 that a result in float16 is taken in, 7.9e-4 for 131072 in bfloat16; or 3e-6 for parts of 512
-# that are added in registers, each addition by 2^-25 on average in either direction.  Here 1.8e-4 and 9.8e-4 are allowed.
+# one sign, so 4.9e-5 for the parts of 8192 that a result in float16 is taken in, 3.9e-4 for 65536 in bfloat16, and 2^-24 at most for each of
+# up to 512 parts, 3e-5.  Here 1.8e-4 and 9.8e-4 are allowed.
 OFF = {F16: 2.0**-11 * 9 / 8 + 2.0**-13, BF16: 2.0**-8 * 9 / 8 + 2.0**-11}
 
 
@@ -95,6 +95,49 @@ def test_weight_gradient(n, dtype, length):
 def test_weight_gradient_of_groups(dtype, groups):
     """Long ones beside short and empty ones: every matrix is written, once."""
     _weight_gradient(groups, dtype)
+
+
+@pytest.mark.parametrize("dtype,part", [(F16, 8192), (BF16, 65536)])
+def test_lengths_around_a_part(dtype, part):
+    """One block more or less than whole parts, long tiles beside short ones and behind one another, on few and many tiles per SM."""
+    _weight_gradient([part - 1, part, part + 1, 5, 2 * part, 2 * part + 1, 64, 3 * part - 63], dtype)
+    _weight_gradient([2 * part + 65, 100, part + 64, part + 64, 7], dtype, n=1024)
+    _weight_gradient([part + 1], dtype, n=1029)
+
+
+@pytest.mark.parametrize("activation,n,off", [("silu", 264, False), ("silu", 264, True), ("swiglu", 512, False), ("swiglu", 512, True)])
+@pytest.mark.parametrize("groups", [None, [700, 0, 1, 299, 300]])
+def test_long_sums_with_everything_behind_them(groups, activation, n, off):
+    """Bias, activation, residual and what backward needs, results that leave by whole words or not, several long tiles for every pair; against the
+    sums of a result in 32 bits, which are taken in parts of 512."""
+    m, k = 1300, 3 * 8192 + 200
+    g = torch.Generator(device="cuda").manual_seed(n)
+    normal = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
+    lead = () if groups is None else (len(groups),)
+    cols = n // 2 if activation == "swiglu" else n
+    residual = normal(m, cols + 1).half()
+    args = {
+        "a": normal(m, k).half(),
+        "b": (normal(*lead, n, k) * k**-0.5).half(),
+        "bias": normal(*lead, n),
+        "residual": residual[:, 1:] if off else residual[:, 1:].contiguous(),
+        "activation": activation,
+        "rows": None if groups is None else torch.tensor(groups, dtype=torch.int32, device="cuda"),
+    }
+    want = ops.matmul(**{**args, "residual": args["residual"].float()}, out_dtype=torch.float32)
+    bias = args["bias"].requires_grad_()
+    got = ops.matmul(**args)
+    # random signs: a sum is off by far less than its half step here, 2^-11 of what is summed at the end
+    size = want.abs() + args["residual"].float().abs() + 1
+    assert ((got.float() - want).abs() <= size * (2.0**-11 + 2.0**-13)).all()
+    d = normal(m, cols)
+    (kept,) = torch.autograd.grad(got, bias, d.half())
+    whole = ops.matmul(**{**args, "residual": args["residual"].float()}, out_dtype=torch.float32)
+    (right,) = torch.autograd.grad(whole, bias, d.half().float())
+    # z is off by what its sum is: 7e-6 of its magnitudes' norm and more, and as much the slopes, summed over up to 1300 rows
+    assert ((kept - right).norm() / right.norm()).item() <= 2.0**-13
+    with torch.no_grad():
+        assert torch.equal(ops.matmul(**args), got) and ops.check() == 0
 
 
 def test_weight_gradient_of_results_in_32_bits():
