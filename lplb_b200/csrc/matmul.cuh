@@ -326,6 +326,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
     tma_prefetch_desc(&maps.p[0]);
     tma_prefetch_desc(&maps.q[0]);
   }
+  cluster_sync();  // both CTAs have begun
   if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), kPairColumns);
   wait_predecessors();
   allow_successor();
@@ -353,6 +354,7 @@ pair_matmul_kernel(const __grid_constant__ PairMaps maps, const PairArgs a) {
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync();  // the peer's barriers are initialised and its tensor memory is allocated
+  if (warp == 1) tmem_relinquish();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort = &abort_flag;

@@ -318,6 +318,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     tma_prefetch_desc(&tmap_w);
     for (int b = 0; b < kRowBoxes; ++b) tma_prefetch_desc(&rows.box[b]);
   }
+  cluster_sync();  // both CTAs have begun
   if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), kTmemCols);
   wait_predecessors();
   if (threadIdx.x == 0) {
@@ -357,6 +358,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync();  // the peer's barriers are initialised and its tensor memory is allocated
+  if (warp == 1) tmem_relinquish();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
   volatile int* abort = &abort_flag;

@@ -205,10 +205,12 @@ __device__ __forceinline__ void mbar_arrive_remote_read(uint32_t bar) { mbar_arr
 // ---- tensor memory -----------------------------------------------------------------------------
 // Whole-warp calls, one warp in each CTA of the pair.  `slot` is a shared-memory word that
 // receives the base address.
+// The allocation acts on the tensor memory of both: the cluster meets before it (a CTA that asks while its peer has not begun may leave
+// the peer waiting for good), and again before the right to allocate is given up.
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t columns) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
