@@ -17,7 +17,7 @@ namespace {
 // dz = dout * act'(z), rounded to the operands' type for the products behind it, and the sum of dz (before the rounding) over
 // parts of a group's rows.  A CTA has 256 columns of z, a part of a group's rows, eight of them at a time; bound by DRAM.
 // 8192 x 4096 in bf16 through silu with the bias's gradient: 49 us, 5.5 TB/s (one row at a time for each warp 53, four 60, two converted
-// as they come 56); 16384 x 4096 of 32 experts through swiglu 80 us, 5.8 TB/s; gelu of 32-bit results 65, by its instructions.
+// as they come 56); 16384 x 4096 of 32 experts through swiglu 80 us, 5.8 TB/s; gelu of 32-bit results 61, by its instructions.
 constexpr int kPreColumns = 256, kPreRows = 8;
 
 // (which activation is asked once, not for each value)

@@ -124,10 +124,10 @@ __device__ __forceinline__ void store4(void* p, Type type, int64_t i, int limit,
 // (__expf is off by 2 + 1.2 |z| units in the last place, the quotient by two: some |z| units come from z's own last bit, too.  Below z = -87, where
 // silu is 1e-36, it is 0.)
 __device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-// The normal distribution's function, and e^(-z^2 / 2), in few instructions and good to some 2^-20 of the value on either side: for u >= 0
-// Phi(-u) e^(u^2 / 2) is smooth and falls slowly, here as a polynomial in 1 / (1 + 0.4 u), fitted to 0 <= u <= 14 by least squares of the relative error
-// with weights that level it (8e-8; in 32 bits 3.5e-7).  us, 4096 x 4096 x 1024 in bf16 with gelu: this 38, 0.5 erfc(-z / sqrt 2) 55, 0.5 + 0.5 erf(z / sqrt 2)
-// 39, but that is off by 2^-24, not of the value: 4 % at z = -5.
+// The normal distribution's function, and e^(-z^2 / 2), in few instructions and good to some 2^-20 of the value on either side: for
+// u >= 0 Phi(-u) e^(u^2 / 2) is smooth and falls slowly, here as a polynomial in 1 / (1 + 0.4 u), fitted to 0 <= u <= 14 by least
+// squares of the relative error with weights that level it (8e-8; in 32 bits 3.5e-7).  us, 4096 x 4096 x 1024 in bf16 with gelu: this
+// 38, 0.5 erfc(-z / sqrt 2) 55, 0.5 + 0.5 erf(z / sqrt 2) 39, but that is off by 2^-24, not of the value: 4 % at z = -5.
 __device__ __forceinline__ float normal_cdf(float z, float& bell) {
   constexpr float kCoefficients[] = {-0.0396009646f, 0.20060125f,  -0.373683333f, 0.250973463f,    -0.0123857474f,
                                      0.158416525f,   0.155786633f, 0.159904182f,  -1.19874376e-05f};

@@ -19,9 +19,9 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Whether the call is recorded; arguments with a forward-mode tangent are refused.  Inside a capture a leaf whose gradient is collected on the default stream, because a graph
-// that was recorded there still lives, is refused: the backward pass would make that stream wait for the captured one, which
-// breaks the capture off with an error that names neither.
+// Whether the call is recorded; arguments with a forward-mode tangent are refused.  Inside a capture a leaf whose gradient is
+// collected on the default stream, because a graph that was recorded there still lives, is refused: the backward pass would make that
+// stream wait for the captured one, which breaks the capture off with an error that names neither.
 inline bool wants_grad(std::initializer_list<const Tensor*> tensors, const char* who) {
   for (const Tensor* t : tensors) check_no_tangent(*t, who);
   if (!at::GradMode::is_enabled()) return false;

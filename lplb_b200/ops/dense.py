@@ -69,13 +69,16 @@ def matmul(
     ``K`` is a multiple of 8; ``a``, and all matrices of ``b`` together, have up to 2**31 - 256 rows.  ``b`` is contiguous and starts
     on a 16-byte boundary; rows of ``a`` that do not are copied first.
 
-    Differentiable with respect to ``a``, ``b``, ``bias`` and ``residual``.  For the backward pass the sums before an activation are
-    kept, in 32 bits, and their gradients are rounded to ``a``'s bits before they are multiplied: to bfloat16, or to the 11 bits of
-    float16 in parts of a power of two, so that what float16 does not hold on the way, large or small, is not lost.  All sums are in 32
-    bits.  A gradient's gradient is refused.  CUDA tensors run on the native kernels, on the current stream of their device, CPU
-    tensors on plain statements; calls and backward passes can be captured in a CUDA graph, and the same inputs give the same
-    bits.  Inside a capture a call that is recorded is refused (``RuntimeError``) while a graph recorded on the default stream still
-    holds one of its leaves: delete that graph's outputs first, or call under ``torch.no_grad()`` if there will be no backward pass.  Wrong arguments raise ``ValueError``; :func:`~lplb_b200.ops.check` tells of waits that ran out."""
+    Differentiable with respect to ``a``, ``b``, ``bias`` and ``residual``; a gradient's gradient is refused, and so is a CUDA tensor with
+    a forward-mode tangent.  For the backward pass the sums before an activation are kept, in 32 bits, and their gradients are rounded
+    to ``a``'s bits before they are multiplied: to bfloat16, or to the 11 bits of float16 in parts of a power of two, so that what
+    float16 does not hold on the way, large or small, is not lost.  All sums are in 32 bits.
+
+    CUDA tensors run on the native kernels, on the current stream of their device, CPU tensors on plain statements; calls and
+    backward passes can be captured in a CUDA graph, and the same inputs give the same bits.  Inside a capture a call that is
+    recorded is refused (``RuntimeError``) while a graph recorded on the default stream still holds one of its leaves: delete that
+    graph's outputs first, or call under ``torch.no_grad()`` if there will be no backward pass.  Wrong arguments raise
+    ``ValueError``; :func:`~lplb_b200.ops.check` tells of waits that ran out."""
     if activation not in MATMUL_ACTIVATIONS:  # (messages are put together where they are needed: the call is a few microseconds)
         raise ValueError(f"lplb_b200.ops.matmul: activation must be one of {MATMUL_ACTIVATIONS}, not {activation!r}")
     if out_dtype is None:

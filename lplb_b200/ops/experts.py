@@ -15,10 +15,10 @@ bits, ``matmul_fp8``)::
     y = ops.combine_rows(ops.matmul(act, w2, rows=order.counts), order, weights)
 
 Every one but :func:`expert_order`, which has whole numbers alone, has a gradient; a gradient's gradient is refused, and so is a CUDA
-tensor with a forward-mode tangent.  CUDA tensors run on the native kernels, on the current stream of their device; CPU tensors on the plain statements in
-:mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph, backward passes too; inside a capture a call that is recorded is
-refused (``RuntimeError``) while a graph recorded on the default stream still holds one of its leaves.  The same inputs give the same
-bits.  Wrong arguments raise ``ValueError``.
+tensor with a forward-mode tangent.  CUDA tensors run on the native kernels, on the current stream of their device; CPU tensors on
+the plain statements in :mod:`lplb_b200.ops.reference`.  Calls can be captured in a CUDA graph, backward passes too; inside a capture
+a call that is recorded is refused (``RuntimeError``) while a graph recorded on the default stream still holds one of its leaves.
+The same inputs give the same bits.  Wrong arguments raise ``ValueError``.
 
 The reference has no operators of this kind.
 """
@@ -189,7 +189,8 @@ class _CombineRows(torch.autograd.Function):
 def take_rows(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """``rows`` ``[tokens * topk, values]``, contiguous: ``rows[order.place[t, k]] = x[t]``; rows behind the last
     expert's are zero.  ``x`` is ``[tokens, values]`` of any type, values in 8 bits and their scales among them, of up to (2**31 - 1) //
-    16 values; rows may be apart from one another.  Differentiable for float32, bfloat16 and float16: ``dx[t]`` is the sum of its rows' gradients, in 32 bits."""
+    16 values; rows may be apart from one another.  Differentiable for float32, bfloat16 and float16: ``dx[t]`` is the sum of its
+    rows' gradients, in 32 bits."""
     if x.is_cuda:
         return _native().take_rows(x, order.place, order.source)
     _need(x.dim() == 2, "take_rows: x must be [tokens, values]")
